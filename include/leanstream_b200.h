@@ -419,6 +419,101 @@ uint64_t ls_b200_batch_scratch_bytes(uint32_t hidden, uint32_t group_size, uint3
 int ls_b200_batch_mlp(const ls_b200_batch_args* args, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* Paged key/value cache: attention of new tokens, eviction            */
+/* (new; the reference leaves attention to its applications).          */
+/* ------------------------------------------------------------------ */
+
+enum { LS_B200_FP16 = 0, LS_B200_BF16 = 1 };
+/* Bits that the kernels of this section set in a call's `error` word. What a
+ * flagged sequence or page would have touched is skipped. */
+enum {
+    LS_B200_ATTN_TIMEOUT = 1u << 0, /* a bounded wait gave up: the call's outputs are invalid */
+    LS_B200_ATTN_LENGTH = 1u << 1,  /* q_start / kv_len of a sequence do not fit the call: skipped */
+    LS_B200_ATTN_PAGE = 1u << 2     /* a page index of a visible slot is outside the pool */
+};
+
+/* Attention of the new tokens of `batch` sequences over their cache. Token t of
+ * sequence b is row q_start[b] + t of q; with n = kv_len[b] (new tokens
+ * included) and nq = q_start[b + 1] - q_start[b] it stands at cache slot
+ * p = n - nq + t and sees the slots k <= p, under a window only those with
+ * k > p - window or k < sinks. Slots are counted in the cache, so after an
+ * eviction the window is over the slots that are left. A row that sees nothing
+ * gives output 0 and lse -inf. Slots that no row of the call sees are not
+ * read, whatever their memory or their page index holds. Strides are in
+ * elements, non-negative multiples of 8 for 16-bit tensors, whose last
+ * dimension is contiguous and which start on 16 bytes. */
+typedef struct ls_b200_attention_args {
+    uint32_t dtype;                 /* LS_B200_FP16 / LS_B200_BF16: q, keys, values and output */
+    uint32_t q_heads, kv_heads;     /* q_heads a multiple of kv_heads: head i reads kv head i / group */
+    uint32_t head_dim;              /* 64 or 128 */
+    uint32_t page_size;             /* slots of a page: 16, 32, 64, 128 or 256 */
+    uint32_t pages;                 /* pages of the pool */
+    uint32_t batch;
+    uint32_t tokens;                /* rows of q */
+    uint32_t max_q;                 /* bound of one sequence's new tokens */
+    uint32_t table_pages;           /* columns of page_table */
+    uint32_t window;                /* 0: every earlier slot is visible */
+    uint32_t sinks;                 /* first slots that a window leaves visible */
+    float scale;                    /* of q . k, > 0 */
+    uint32_t weights_length;        /* columns of weights (0 without) */
+    const void* q;                  /* [tokens][q_heads][head_dim] */
+    const void* k_new;              /* optional [tokens][kv_heads][head_dim], both or none: written to the */
+    const void* v_new;              /* new tokens' slots by this call; without, the cache holds them */
+    void* k_pages;                  /* [pages][page_size][kv_heads][head_dim] */
+    void* v_pages;
+    const int32_t* page_table;      /* device [batch][table_pages] */
+    const int32_t* q_start;         /* device [batch + 1], ascending */
+    const int32_t* kv_len;          /* device [batch] */
+    void* output;                   /* [tokens][q_heads][head_dim] */
+    float* lse;                     /* optional [tokens][q_heads], natural logarithm */
+    float* weights;                 /* optional [batch][kv_heads][weights_length] */
+    int64_t q_token_stride, q_head_stride;
+    int64_t k_new_token_stride, k_new_head_stride, v_new_token_stride, v_new_head_stride;
+    int64_t k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;
+    int64_t output_token_stride, output_head_stride;
+    int64_t table_stride, weights_sequence_stride, weights_head_stride;
+    void* scratch;                  /* zeroed once before the first call; calls on one scratch must not
+                                     * overlap. After an error it is to be zeroed again */
+    uint64_t scratch_bytes;
+    uint32_t* error;                /* optional device word, LS_B200_ATTN_* bits are ORed in */
+    uint64_t timeout_ns;            /* bound of every wait (0 = 2 s, at most 60 s) */
+} ls_b200_attention_args;
+/* Scratch of a call of this shape (dtype, heads, sizes, batch, tokens, max_q,
+ * weights_length; pointers are not read); 0 when the shape is refused. */
+uint64_t ls_b200_attention_scratch_bytes(const ls_b200_attention_args* args);
+/* weights[b][h][k] += sum over the new tokens and the query heads of kv head h
+ * of the slot's softmax weight; the new tokens' own slots start at this call's
+ * sum. Returns 0, EINVAL, ENOSPC or a CUDA error code. */
+int ls_b200_paged_attention(const ls_b200_attention_args* args, void* stream);
+
+/* Keeps `budget` slots of each sequence and kv head: the first `sinks`, the
+ * last `recent`, and between them those of the largest weight (equal weights:
+ * the lower slot; NaN counts as -inf). A sequence of at most `budget` slots
+ * keeps all. Kept rows go, in order, to the slots 0 .. of the pages of
+ * new_table, which must be none of the batch's old pages; the old ones are left
+ * as they are. */
+typedef struct ls_b200_evict_args {
+    uint32_t kv_heads, head_dim, page_size, pages, batch;
+    uint32_t table_pages, new_table_pages;
+    uint32_t weights_length;        /* columns of weights */
+    uint32_t budget, sinks, recent; /* sinks + recent <= budget */
+    uint32_t reserved;
+    void* k_pages;                  /* 16-bit elements, as above */
+    void* v_pages;
+    const int32_t* page_table;
+    const int32_t* new_table;       /* device [batch][new_table_pages] */
+    const int32_t* kv_len;
+    const float* weights;           /* [batch][kv_heads][weights_length] */
+    int32_t* new_len;               /* device [batch]: slots kept */
+    int32_t* kept;                  /* device [batch][kv_heads][budget]: old slot of each new one, -1 past new_len */
+    float* new_weights;             /* optional [batch][kv_heads][budget]: their weights, 0 past new_len */
+    int64_t k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;
+    int64_t table_stride, new_table_stride, weights_sequence_stride, weights_head_stride;
+    uint32_t* error;
+} ls_b200_evict_args;
+int ls_b200_evict_cache(const ls_b200_evict_args* args, void* stream);
+
+/* ------------------------------------------------------------------ */
 /* Streaming IO: IOBackend (include/leanstream/weight_manager.h:8-24)  */
 /* over pinned host memory -> HBM staging copies.                      */
 /* ------------------------------------------------------------------ */

@@ -5,8 +5,9 @@ include/leanstream_b200.h). This package is the Python host-side mirror of
 the reference's native-backend API, plus the seeded synthetic data format.
 """
 from ._native import load as load_library, LIBRARY  # noqa: F401
+from .attention import PagedAttention, evict_cache  # noqa: F401
 from .backend import B200Backend, DeviceQueue, ExecutionQueue, quantize_io_load  # noqa: F401
 from .batch import BatchMLP, union_plan  # noqa: F401
 
-__all__ = ["B200Backend", "BatchMLP", "DeviceQueue", "ExecutionQueue", "quantize_io_load", "union_plan",
-           "load_library", "LIBRARY"]
+__all__ = ["B200Backend", "BatchMLP", "DeviceQueue", "ExecutionQueue", "PagedAttention", "evict_cache", "quantize_io_load",
+           "union_plan", "load_library", "LIBRARY"]

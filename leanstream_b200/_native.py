@@ -132,6 +132,41 @@ class BatchArgs(C.Structure):
                 ("rms_eps", C.c_float), ("norm_weight", C.c_void_p), ("error", C.c_void_p),
                 ("timeout_ns", C.c_uint64)]
 
+FP16, BF16 = 0, 1
+ATTN_TIMEOUT, ATTN_LENGTH, ATTN_PAGE = 1, 2, 4
+
+
+class AttentionArgs(C.Structure):
+    """ls_b200_attention_args: attention of new tokens over a paged cache."""
+    _fields_ = [(n, C.c_uint32) for n in ("dtype", "q_heads", "kv_heads", "head_dim", "page_size", "pages", "batch",
+                                          "tokens", "max_q", "table_pages", "window", "sinks")] + \
+               [("scale", C.c_float), ("weights_length", C.c_uint32)] + \
+               [(n, C.c_void_p) for n in ("q", "k_new", "v_new", "k_pages", "v_pages", "page_table", "q_start",
+                                          "kv_len", "output", "lse", "weights")] + \
+               [(n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "k_new_token_stride",
+                                         "k_new_head_stride", "v_new_token_stride", "v_new_head_stride",
+                                         "k_page_stride", "k_slot_stride", "k_head_stride", "v_page_stride",
+                                         "v_slot_stride", "v_head_stride", "output_token_stride",
+                                         "output_head_stride", "table_stride", "weights_sequence_stride",
+                                         "weights_head_stride")] + \
+               [("scratch", C.c_void_p), ("scratch_bytes", C.c_uint64), ("error", C.c_void_p),
+                ("timeout_ns", C.c_uint64)]
+
+
+class EvictArgs(C.Structure):
+    """ls_b200_evict_args: eviction from a paged cache by accumulated weight."""
+    _fields_ = [(n, C.c_uint32) for n in ("kv_heads", "head_dim", "page_size", "pages", "batch", "table_pages",
+                                          "new_table_pages", "weights_length", "budget", "sinks", "recent",
+                                          "reserved")] + \
+               [(n, C.c_void_p) for n in ("k_pages", "v_pages", "page_table", "new_table", "kv_len", "weights",
+                                          "new_len", "kept", "new_weights")] + \
+               [(n, C.c_int64) for n in ("k_page_stride", "k_slot_stride", "k_head_stride", "v_page_stride",
+                                         "v_slot_stride", "v_head_stride", "table_stride", "new_table_stride",
+                                         "weights_sequence_stride", "weights_head_stride")] + \
+               [("error", C.c_void_p)]
+
+
+assert C.sizeof(AttentionArgs) == 56 + 11 * 8 + 17 * 8 + 32 and C.sizeof(EvictArgs) == 48 + 9 * 8 + 10 * 8 + 8
 assert C.sizeof(IOCompletion) == 24 and C.sizeof(IOBackend) == 64 and C.sizeof(StreamConfig) == 104
 assert C.sizeof(ExecDesc) == 20 and C.sizeof(QueueControl) == 128 and C.sizeof(DeviceExecQueue) == 32
 
@@ -176,6 +211,9 @@ SIGNATURES = {
     "ls_b200_spin": (C.c_int, [C.c_uint64, C.c_void_p]),
     "ls_b200_batch_scratch_bytes": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint32]),
     "ls_b200_batch_mlp": (C.c_int, [C.POINTER(BatchArgs), C.c_void_p]),
+    "ls_b200_attention_scratch_bytes": (C.c_uint64, [C.POINTER(AttentionArgs)]),
+    "ls_b200_paged_attention": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
+    "ls_b200_evict_cache": (C.c_int, [C.POINTER(EvictArgs), C.c_void_p]),
     "ls_b200_stream_create": (C.c_void_p, [C.POINTER(StreamConfig)]),
     "ls_b200_stream_view": (C.c_int, [C.c_void_p, C.POINTER(IOBackend)]),
     "ls_b200_stream_stats": (C.c_int, [C.c_void_p, C.POINTER(StreamStats)]),

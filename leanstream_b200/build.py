@@ -17,7 +17,9 @@ PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 LIBRARY = PACKAGE / "libleanstream_b200.so"
-SOURCES = ("ls_kernel.cu", "ls_kernel_traced.cu", "ls_backend.cu", "ls_aux.cu", "ls_stream.cu", "ls_batch.cu")
+SOURCES = ("ls_kernel.cu", "ls_kernel_traced.cu", "ls_backend.cu", "ls_aux.cu", "ls_stream.cu", "ls_batch.cu",
+           "ls_attention.cu", "ls_evict.cu")
+HEADERS = ("ls_internal.h", "ls_attention.h")
 ARCH = ("-gencode", "arch=compute_100a,code=sm_100a")
 
 
@@ -32,7 +34,7 @@ def needs_build(target: Path = LIBRARY) -> bool:
     if not target.exists():
         return True
     stamp = target.stat().st_mtime
-    inputs = [CSRC / s for s in SOURCES] + [CSRC / "ls_internal.h", ROOT / "include" / "leanstream_b200.h"]
+    inputs = [CSRC / s for s in SOURCES] + [CSRC / h for h in HEADERS] + [ROOT / "include" / "leanstream_b200.h"]
     return any(p.stat().st_mtime > stamp for p in inputs)
 
 
@@ -51,7 +53,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
     objdir = PACKAGE / "_build"
     objdir.mkdir(exist_ok=True)
-    headers = [CSRC / "ls_internal.h", ROOT / "include" / "leanstream_b200.h", CSRC / "ls_kernel.cu"]
+    headers = [CSRC / h for h in HEADERS] + [ROOT / "include" / "leanstream_b200.h", CSRC / "ls_kernel.cu"]
     newest_header = max(h.stat().st_mtime for h in headers)
 
     def compile_one(src: str):

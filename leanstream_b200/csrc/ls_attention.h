@@ -1,0 +1,145 @@
+// Internal types of the paged-cache attention (ls_attention.cu) and of the
+// cache eviction (ls_evict.cu). Not part of the public ABI.
+#pragma once
+#include <stdint.h>
+#include <cuda_runtime.h>
+#include "../../include/leanstream_b200.h"
+
+namespace lsb {
+
+constexpr uint32_t kErrLength = 1u << 1;  // a sequence's lengths do not fit the call
+constexpr uint32_t kErrPage = 1u << 2;    // a visible slot's page index is outside the pool
+
+// ls_b200_attention_args in the kernels' units. Strides are in elements.
+struct AttnParams {
+    const uint16_t* q;
+    const uint16_t* k_new;
+    const uint16_t* v_new;
+    uint16_t* k_pages;
+    uint16_t* v_pages;
+    uint16_t* out;
+    const int32_t* table;
+    const int32_t* q_start;
+    const int32_t* kv_len;
+    float* lse;       // [tokens][Hq]: the caller's, or scratch where only the weights need it
+    float* weights;
+    float* part;      // partial results of split items
+    uint32_t* count;  // [grid] arrived pieces of the item that begins in a CTA (zero at rest)
+    float* logits;    // [B][Hkv][wlen][rows] base-2 logits of a call with weights
+    uint32_t* err;
+    int64_t q_ts, q_hs, kn_ts, kn_hs, vn_ts, vn_hs, o_ts, o_hs;
+    int64_t kp_ps, kp_ss, kp_hs, vp_ps, vp_ss, vp_hs;
+    int64_t table_s, w_ss, w_hs;
+    float c;  // scale * log2(e)
+    uint32_t B, Hq, Hkv, g, D, P, pshift, pages, tpages, tokens, max_q, window, sinks, wlen;
+    uint32_t rows;   // max_q * g: row capacity of `logits`
+    uint32_t fused;  // 1: the attention kernel appends the new keys and values
+};
+
+// A sequence of the call: its new tokens are rows q0 .. q0 + nq - 1 of q and
+// take cache slots f .. n - 1. Row t sees the slots k <= f + t that its window
+// leaves; f < 0 (more tokens than slots) leaves the first rows empty.
+struct SeqRange {
+    int32_t q0, nq, n, f;
+};
+
+__device__ __forceinline__ SeqRange load_seq(const AttnParams& p, uint32_t b) {
+    SeqRange s;
+    s.q0 = p.q_start[b];
+    s.nq = p.q_start[b + 1] - s.q0;
+    s.n = p.kv_len[b];
+    const bool ok = s.q0 >= 0 && s.nq >= 0 && uint32_t(s.nq) <= p.max_q && uint32_t(s.q0) <= p.tokens &&
+                    uint32_t(s.nq) <= p.tokens - uint32_t(s.q0) && s.n >= 0 &&
+                    uint64_t(s.n) <= uint64_t(p.tpages) << p.pshift && (!p.weights || uint32_t(s.n) <= p.wlen);
+    if (!ok) {
+        if (p.err) atomicOr(p.err, kErrLength);
+        s.q0 = s.nq = s.n = 0;
+    }
+    s.f = s.n - s.nq;
+    return s;
+}
+
+// The cache slots that the rows of tokens [t0, t1) see between them: [0, sink)
+// and [lo, hi), cut into tiles of TK slots: `ns` tiles of the first slots, then
+// the tiles from `first`. Rows without any visible slot keep one (empty) tile,
+// so that somebody writes their output.
+struct KeyRange {
+    int32_t lo, hi, sink, ns, first, tiles;
+};
+
+template <int TK>
+__device__ __forceinline__ KeyRange key_range(const AttnParams& p, const SeqRange& s, int32_t t0, int32_t t1) {
+    KeyRange r;
+    r.hi = max(0, s.f + t1);
+    r.lo = p.window ? max(0, int32_t(max(int64_t(s.f) + t0 + 1 - int64_t(p.window), int64_t(0)))) : 0;
+    r.lo = min(r.lo, r.hi);
+    r.sink = int32_t(min(p.window ? p.sinks : 0u, uint32_t(r.lo)));
+    r.ns = (r.sink + TK - 1) / TK;
+    r.first = max(r.lo / TK, r.ns);
+    r.tiles = max(1, r.ns + max(0, (r.hi + TK - 1) / TK - r.first));
+    return r;
+}
+
+__device__ __forceinline__ int32_t tile_at(const KeyRange& r, int32_t j) { return j < r.ns ? j : r.first + j - r.ns; }
+
+// Whether position pos sees slot k (pos < 0: nothing).
+__device__ __forceinline__ bool sees(const AttnParams& p, int32_t pos, int32_t k) {
+    return k <= pos && (!p.window || int64_t(k) > int64_t(pos) - int64_t(p.window) || uint32_t(k) < p.sinks);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kLog2e = 1.44269504088896341f;
+
+// The 16-bit element types: conversions and the pair forms the MMAs take.
+struct F16 {
+    static constexpr uint32_t kUmmaFormat = 0;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ void unpack(uint32_t v, float& lo, float& hi) {
+        asm("{.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;}"
+            : "=f"(lo), "=f"(hi) : "r"(v));
+    }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+struct BF16 {
+    static constexpr uint32_t kUmmaFormat = 1;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ void unpack(uint32_t v, float& lo, float& hi) {
+        lo = __uint_as_float(v << 16);
+        hi = __uint_as_float(v & 0xffff0000u);
+    }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+// First unit of CTA c when U units are cut evenly over G CTAs, and the CTA of a unit.
+__device__ __forceinline__ int64_t cut_begin(int64_t U, int64_t G, int64_t c) { return c * U / G; }
+__device__ __forceinline__ int64_t cut_owner(int64_t U, int64_t G, int64_t u) { return ((u + 1) * G - 1) / U; }
+
+}  // namespace lsb
