@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(256) attn_weights_kernel(const AttnParams p) {
 bool al16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 constexpr uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
 constexpr uint64_t kMaxTimeoutNs = 60000000000ull;
-constexpr uint32_t kMaxCtas = 512;  // CTAs of a launch, and counters in the scratch header
+constexpr uint64_t kTimeoutNs = 2000000000ull;
 
 uint32_t sm_count() {
     int dev = 0, sms = 0;
@@ -562,13 +562,29 @@ uint32_t dec_mt(const ls_b200_attention_args& a) {
     return uint64_t(a.max_q) * (a.q_heads / a.kv_heads) <= 16 ? 1 : 2;
 }
 
+// Rows of a sequence and kv head beyond which the call goes to the 128-row
+// tensor-core tiles of ls_attention_chunk.cu.
+constexpr uint64_t kChunkRows = 32;
+bool is_chunk(const ls_b200_attention_args& a) {
+    const uint32_t g = a.q_heads / a.kv_heads;
+    return uint64_t(a.max_q) * g > kChunkRows && g <= 128 && !a.weights_length;
+}
+
 struct ScratchPlan {
-    uint64_t count, part, lse, logits, total;
+    uint64_t count, part, lse, logits, plan, items, chunk_part, total;
 };
 ScratchPlan scratch_plan(const ls_b200_attention_args& a) {
     ScratchPlan s{};
     s.count = 0;
     s.part = up256(kMaxCtas * sizeof(uint32_t));
+    if (is_chunk(a)) {
+        const uint32_t g = a.q_heads / a.kv_heads;
+        s.plan = s.part;
+        s.items = s.plan + up256(sizeof(ChunkPlan));
+        s.chunk_part = s.items + up256(chunk_items(a.tokens, a.batch, g) * sizeof(ChunkItem));
+        s.total = s.chunk_part + up256(2ull * sm_count() * chunk_part_floats(a.head_dim) * sizeof(float));
+        return s;
+    }
     s.lse = s.part + up256(2ull * kMaxCtas * 16 * dec_mt(a) * (a.head_dim + 2) * sizeof(float));
     const bool w = a.weights_length != 0;
     s.logits = s.lse + (w ? up256(uint64_t(a.tokens) * a.q_heads * sizeof(float)) : 0);
@@ -676,7 +692,14 @@ int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
     while ((1u << p.pshift) < p.P) ++p.pshift;
     p.window = a->window, p.sinks = a->sinks, p.wlen = a->weights_length;
     p.rows = p.max_q * p.g;
+    p.timeout_ns = a->timeout_ns ? a->timeout_ns : kTimeoutNs;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (is_chunk(*a)) {
+        const ChunkScratch c{reinterpret_cast<ChunkPlan*>(scratch + plan.plan),
+                             reinterpret_cast<ChunkItem*>(scratch + plan.items),
+                             reinterpret_cast<float*>(scratch + plan.chunk_part)};
+        return launch_chunk(p, a->dtype, c, sm_count(), s);
+    }
     const uint32_t mt = dec_mt(*a);
     p.fused = p.k_new && p.rows <= 16 * mt;
     if (p.k_new && !p.fused) {

@@ -34,7 +34,34 @@ struct AttnParams {
     uint32_t B, Hq, Hkv, g, D, P, pshift, pages, tpages, tokens, max_q, window, sinks, wlen;
     uint32_t rows;   // max_q * g: row capacity of `logits`
     uint32_t fused;  // 1: the attention kernel appends the new keys and values
+    uint64_t timeout_ns;
 };
+
+// The tensor-core path of chunks (ls_attention_chunk.cu): one item is two
+// 128-row tiles of one kv head, a row being a (token, head of the group).
+constexpr uint32_t kMaxCtas = 512;  // CTAs of a launch, and counters in the scratch header
+struct ChunkItem {                  // tokens t0 .. of a sequence, written by the plan kernel
+    int32_t b, q0, nq, n;           // the sequence, as SeqRange
+    int32_t t0, tiles;              // first token, tiles of 128 slots
+    int64_t units;                  // tiles of the items before, over all kv heads
+};
+struct ChunkPlan {
+    int64_t units;                  // tiles of the call
+    int32_t items, ctas;            // items; CTAs that share the tiles
+    int32_t start[kMaxCtas];        // item in which each CTA begins
+    int2 open[kMaxCtas];            // item and kv head that begin in a CTA and go on in the next (x < 0: none)
+};
+struct ChunkScratch {
+    ChunkPlan* plan;
+    ChunkItem* items;
+    float* part;
+};
+__host__ __device__ inline uint32_t chunk_tokens(uint32_t g) { return 128 / g; }  // of one 128-row tile
+inline uint64_t chunk_items(uint64_t tokens, uint64_t batch, uint32_t g) {
+    return tokens / (2 * chunk_tokens(g)) + batch;
+}
+inline uint64_t chunk_part_floats(uint32_t D) { return 256ull * (D + 2); }  // one partial result
+int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream);
 
 // A sequence of the call: its new tokens are rows q0 .. q0 + nq - 1 of q and
 // take cache slots f .. n - 1. Row t sees the slots k <= f + t that its window

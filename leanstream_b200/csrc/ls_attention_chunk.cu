@@ -1,0 +1,713 @@
+// Attention of chunks (many new tokens per sequence) over a paged cache, on
+// the 5th-generation tensor cores. The formula is that of ls_attention.cu.
+//
+// Rows are (token, head of the group): all query heads of a kv head stand in
+// one 128-row MMA tile, so a key read serves the whole group. One item is two
+// such tiles (Q0, Q1) of one kv head; its slots go by in tiles of 128. Per tile
+// of slots and row tile i
+//     S_i = Q_i K^T            M 128, N 128, K head_dim, into tensor memory
+//     P_i = exp2(S_i c - m c)  by one thread per row, back into S_i's columns
+//     O_i += P_i V             A from tensor memory, V read as it lies (N-major)
+// While the warps of one row tile work on their exponentials the tensor cores
+// run the other's products. Roles of the warps: 0-3 and 4-7 the rows of Q0 and
+// Q1, 8 issues the MMAs, 9 the TMA loads (Q by item; K and V tiles through
+// one ring of 128-slot stages, one box per page and 64 elements), 10 lays out
+// the CTA's pieces of items for the others.
+//
+// The running maximum is only raised when a row's maximum grows by more than
+// 2^8 (probabilities then stay below 2^8, exact in either 16-bit type's
+// range); raising it rescales O_i in tensor memory, which is rare after the
+// first tiles. P is rounded once to the 16-bit type (the MMA's operand); sums
+// and maxima stay in 32 bits, the row sum over the unrounded P.
+//
+// The tiles of all items, in order, are cut evenly over one CTA per SM, so a
+// few long sequences fill the GPU as many short ones do. An item cut over
+// several CTAs leaves its parts in scratch, and a short kernel joins them in
+// order.
+#include <cuda.h>
+#include <stdint.h>
+
+#include <atomic>
+#include <cerrno>
+
+#include "ls_attention.h"
+#include "ls_tc.h"
+
+namespace lsb {
+namespace {
+
+using namespace tc;
+
+constexpr int kKeys = 128;  // slots of a tile
+constexpr int kThreads = 384;  // twelve warps, 168 registers per thread
+constexpr uint32_t kPanel = 128 * 128;  // 128 rows of 64 elements
+constexpr uint64_t kGraceNs = 1000000000ull;
+constexpr float kRaise = 8.f;  // base-2 growth of a row's maximum that raises the reference
+
+template <int D>
+struct Geo {
+    static constexpr uint32_t kPanels = D / 64, kTile = kPanels * kPanel;
+    static constexpr uint32_t kStages = D == 128 ? 5 : 8;
+    static constexpr uint32_t kRing = 2 * kTile, kBars = kRing + kStages * kTile;
+    static constexpr uint32_t kSegs = kBars + 288;
+    static constexpr uint32_t kSmem = kSegs + 256 + 1024;  // + alignment of the swizzled tiles
+};
+static_assert(Geo<128>::kSmem <= 227 * 1024 && Geo<64>::kSmem <= 227 * 1024, "shared memory of a CTA");
+
+// Barriers: ring full / empty, Q full / empty, S full, P ready, O full, the
+// last MMAs after a failure, pieces full / empty.
+struct Bars {
+    uint32_t base;
+    __device__ uint32_t full(uint32_t s) const { return base + 8 * s; }
+    __device__ uint32_t empty(uint32_t s) const { return base + 8 * (8 + s); }
+    __device__ uint32_t q_full() const { return base + 8 * 16; }
+    __device__ uint32_t q_empty() const { return base + 8 * 17; }
+    __device__ uint32_t s_full(uint32_t i) const { return base + 8 * (18 + i); }
+    __device__ uint32_t p_ready(uint32_t i) const { return base + 8 * (20 + i); }
+    __device__ uint32_t o_full(uint32_t i) const { return base + 8 * (22 + i); }
+    __device__ uint32_t drain() const { return base + 8 * 24; }
+    __device__ uint32_t seg_full(uint32_t s) const { return base + 8 * (25 + s); }
+    __device__ uint32_t seg_empty(uint32_t s) const { return base + 8 * (29 + s); }
+};
+
+// Appends the new keys and values (blocks 1 ..) and lays out the items (block 0).
+__global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, const ChunkScratch sc, uint32_t grid) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (blockIdx.x) {
+        // one warp per token
+        const uint32_t pieces = p.D / 8, per_token = p.Hkv * pieces;
+        const uint32_t per_seq = (p.max_q + 7) / 8, at = blockIdx.x - 1, b = at / per_seq;
+        const SeqRange s = load_seq(p, b);
+        const int32_t t = int32_t(at % per_seq * 8 + warp), slot = s.f + t;
+        if (t >= s.nq || slot < 0) return;
+        const int32_t id = p.table[int64_t(b) * p.table_s + (slot >> p.pshift)];
+        if (uint32_t(id) >= p.pages) {
+            if (p.err) atomicOr(p.err, kErrPage);
+            return;
+        }
+        const int64_t in = slot & int32_t(p.P - 1), tok = s.q0 + t;
+        for (uint32_t i = lane; i < per_token; i += 32) {
+            const int64_t h = i / pieces, e = (i % pieces) * 8;
+            *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + in * p.kp_ss + h * p.kp_hs + e) =
+                *reinterpret_cast<const uint4*>(p.k_new + tok * p.kn_ts + h * p.kn_hs + e);
+            *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + in * p.vp_ss + h * p.vp_hs + e) =
+                *reinterpret_cast<const uint4*>(p.v_new + tok * p.vn_ts + h * p.vn_hs + e);
+        }
+        return;
+    }
+    __shared__ int32_t first[257];  // items before each sequence of the batch piece
+    __shared__ int64_t wsum[8];
+    const int32_t per_item = 2 * int32_t(chunk_tokens(p.g));
+    const int32_t cap = int32_t(p.tokens / uint32_t(per_item) + p.B);
+    int32_t items = 0;
+    int64_t units = 0;
+    auto scan = [&](int64_t v, int64_t& before) {  // over the block
+        int64_t inc = v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+            if (int(lane) >= o) inc += x;
+        }
+        __syncthreads();
+        if (lane == 31) wsum[warp] = inc;
+        __syncthreads();
+        int64_t total = 0;
+        before = inc - v;
+        for (uint32_t w = 0; w < 8; ++w) {
+            if (w < warp) before += wsum[w];
+            total += wsum[w];
+        }
+        return total;
+    };
+    for (uint32_t b0 = 0; b0 < p.B; b0 += 256) {
+        SeqRange s{0, 0, 0, 0};
+        if (b0 + tid < p.B) s = load_seq(p, b0 + tid);
+        int64_t before;
+        const int32_t count = (s.nq + per_item - 1) / per_item;
+        int32_t total = int32_t(scan(count, before));
+        if (total > cap - items) {  // overlapping q_start ranges
+            total = max(0, cap - items);
+            if (tid == 0 && p.err) atomicOr(p.err, kErrLength);
+        }
+        first[tid] = int32_t(before);
+        if (tid == 0) first[256] = total;
+        __syncthreads();
+        for (int32_t i0 = 0; i0 < total; i0 += 256) {
+            const int32_t i = i0 + int32_t(tid);
+            ChunkItem it{};
+            if (i < total) {
+                uint32_t lo = 0, hi = 256;  // the sequence: first[lo] <= i < first[lo + 1]
+                while (hi - lo > 1) {
+                    const uint32_t mid = (lo + hi) / 2;
+                    if (first[mid] <= i) lo = mid;
+                    else hi = mid;
+                }
+                it.b = int32_t(b0 + lo);
+                const SeqRange q = load_seq(p, uint32_t(it.b));
+                it.q0 = q.q0, it.nq = q.nq, it.n = q.n;
+                it.t0 = (i - first[lo]) * per_item;
+                it.tiles = key_range<kKeys>(p, q, it.t0, min(q.nq, it.t0 + per_item)).tiles;
+            }
+            const int64_t sum = scan(int64_t(it.tiles) * p.Hkv, before);
+            it.units = units + before;
+            if (i < total) sc.items[items + i] = it;
+            units += sum;
+        }
+        items += total;
+        __syncthreads();
+    }
+    // CTAs take at least four tiles: below that the joining of parts costs
+    // more than the tiles it spreads.
+    const int64_t G = max(int64_t(1), min(int64_t(grid), (units + 3) / 4));
+    if (tid == 0) {
+        sc.plan->units = units;
+        sc.plan->items = items;
+        sc.plan->ctas = int32_t(G);
+    }
+    for (uint32_t c = tid; c < kMaxCtas; c += 256) sc.plan->open[c] = make_int2(-1, 0);
+    __syncthreads();
+    for (int32_t i = int32_t(tid); i < items; i += 256) {  // each thread reads what this block wrote
+        const int64_t u = sc.items[i].units, end = u + int64_t(sc.items[i].tiles) * p.Hkv;
+        for (int64_t c = (u * G + units - 1) / units; c < G && cut_begin(units, G, c) < end; ++c)
+            sc.plan->start[c] = i;
+    }
+}
+
+// The pieces of items that a CTA works on, in order.
+struct Walk {
+    int64_t U, G, u, u_begin, u_end;
+    int32_t i;  // item
+    ChunkItem it;
+    int32_t h, j0, steps;
+    int64_t item;  // first unit of (item, kv head)
+    KeyRange kr;
+    __device__ bool begin(const ChunkScratch& sc) {
+        U = sc.plan->units;
+        G = sc.plan->ctas;
+        if (int64_t(blockIdx.x) >= G || !U) return false;
+        u = u_begin = cut_begin(U, G, blockIdx.x);
+        u_end = cut_begin(U, G, blockIdx.x + 1);
+        i = sc.plan->start[blockIdx.x] - 1;
+        it.units = -1;
+        it.tiles = 0;
+        steps = 0;
+        return true;
+    }
+    __device__ bool next(const AttnParams& p, const ChunkScratch& sc) {
+        u += steps;
+        if (u >= u_end) return false;
+        if (it.units < 0 || u >= it.units + int64_t(it.tiles) * p.Hkv) {
+            it = sc.items[++i];
+            const SeqRange s{it.q0, it.nq, it.n, it.n - it.nq};
+            kr = key_range<kKeys>(p, s, it.t0, min(it.nq, it.t0 + 2 * int32_t(chunk_tokens(p.g))));
+        }
+        h = int32_t((u - it.units) / it.tiles);
+        item = it.units + int64_t(h) * it.tiles;
+        j0 = int32_t(u - item);
+        steps = int32_t(min(u_end, item + it.tiles) - u);
+        return true;
+    }
+};
+
+// One piece of an item in shared memory (four in flight): what the roles need.
+struct Seg {
+    int32_t steps;      // tiles; 0: no more pieces
+    int32_t row0;       // row of q of the item's first token
+    int32_t left;       // tokens of the sequence from there
+    int32_t pos0;       // their first cache slot
+    int32_t h, b, j0;   // kv head, sequence, first tile
+    int32_t ns, first;  // as KeyRange
+    int32_t lo, hi, sink;
+    int32_t whole;      // the item is all in this piece
+    int32_t part;       // which of the CTA's two partial results
+    int32_t pad[2];
+    __device__ int32_t slot0(int32_t step) const {
+        const int32_t j = j0 + step;
+        return (j < ns ? j : first + j - ns) * kKeys;
+    }
+};
+static_assert(sizeof(Seg) == 64, "four pieces fit");
+constexpr uint32_t kSegs = 4, kSegReaders = 10;
+
+template <class T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    chunk_attn_kernel(const AttnParams p, const ChunkScratch sc, const __grid_constant__ CUtensorMap qmap,
+                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using G = Geo<D>;
+    extern __shared__ uint8_t raw[];
+    const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
+    uint8_t* const base = raw + (smem - smem_u32(raw));
+    const Bars bar{smem + G::kBars};
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(base + G::kBars + 8 * 33);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int32_t per_tile = int32_t(chunk_tokens(p.g));  // tokens of a row tile
+
+    if (tid == 0) {
+        for (uint32_t s = 0; s < G::kStages; ++s) {
+            bar_init(bar.full(s), 1);
+            bar_init(bar.empty(s), 1);
+        }
+        bar_init(bar.q_full(), 1);
+        bar_init(bar.q_empty(), 1);
+        bar_init(bar.drain(), 1);
+        for (uint32_t i = 0; i < 2; ++i) {
+            bar_init(bar.s_full(i), 1);
+            bar_init(bar.p_ready(i), 4);  // the four warps of the row tile
+            bar_init(bar.o_full(i), 1);
+        }
+        for (uint32_t i = 0; i < kSegs; ++i) {
+            bar_init(bar.seg_full(i), 1);
+            bar_init(bar.seg_empty(i), kSegReaders);  // warps 0 .. 9
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) alloc<512>(smem_u32(tmem_slot));
+    if (warp == 9 && lane == 0) {
+        prefetch_map(&qmap);
+        prefetch_map(&kmap);
+        prefetch_map(&vmap);
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint64_t deadline = now() + p.timeout_ns;
+    constexpr uint32_t kS = 0, kO = 256;  // columns: S_0, S_1 (128 each), O_0, O_1 (D each)
+    bool ok = true;
+    const Seg* const segs = reinterpret_cast<const Seg*>(base + G::kSegs);
+
+    // the next piece; false when there is none (or at the deadline)
+    uint32_t sg = 0;
+    auto next = [&]() -> bool {
+        if (!warp_wait(bar.seg_full(sg % kSegs), (sg / kSegs) & 1u, deadline)) return ok = false;
+        return segs[sg % kSegs].steps != 0;
+    };
+    auto release = [&]() {
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar.seg_empty(sg % kSegs));
+        ++sg;
+    };
+
+    if (warp == 10) {
+        // ---- pieces
+        if (lane == 0) {
+            Walk w;
+            bool more = w.begin(sc);
+            for (; ok; ++sg) {
+                if (sg >= kSegs && !bar_wait(bar.seg_empty(sg % kSegs), (sg / kSegs - 1) & 1u, deadline)) {
+                    ok = false;
+                    break;
+                }
+                more = more && w.next(p, sc);
+                Seg x{};
+                if (more) {
+                    x.steps = w.steps, x.row0 = w.it.q0 + w.it.t0, x.left = w.it.nq - w.it.t0;
+                    x.pos0 = w.it.n - w.it.nq + w.it.t0, x.h = w.h, x.b = w.it.b, x.j0 = w.j0;
+                    x.ns = w.kr.ns, x.first = w.kr.first, x.lo = w.kr.lo, x.hi = w.kr.hi, x.sink = w.kr.sink;
+                    x.whole = w.j0 == 0 && w.steps == w.it.tiles;
+                    x.part = w.u != w.u_begin;
+                    if (!x.whole && !w.j0) sc.plan->open[blockIdx.x] = make_int2(w.i, w.h);
+                }
+                *reinterpret_cast<Seg*>(base + G::kSegs + (sg % kSegs) * sizeof(Seg)) = x;
+                bar_arrive(bar.seg_full(sg % kSegs));
+                if (!more) break;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // ---- loads
+        uint32_t slot = 0;  // ring slots filled
+        const uint32_t box = min(p.P, 128u), boxes = 128 / box;
+        while (ok && next()) {
+            const Seg w = segs[sg % kSegs];
+            const int32_t two = w.left > per_tile ? 2 : 1;
+            if (sg && !warp_wait(bar.q_empty(), (sg - 1) & 1u, deadline)) {
+                ok = false;
+                break;
+            }
+            if (lane == 0) {
+                bar_arrive_tx(bar.q_full(), uint32_t(two) * G::kPanels * uint32_t(per_tile) * p.g * 128);
+                for (int32_t i = 0; i < two; ++i)
+                    for (uint32_t c = 0; c < G::kPanels; ++c)
+                        tma3(smem + uint32_t(i) * G::kTile + c * kPanel, &qmap, bar.q_full(), int32_t(c * 64),
+                             w.h * int32_t(p.g), w.row0 + i * per_tile);
+            }
+            const int32_t* trow = p.table + int64_t(w.b) * p.table_s;
+            auto page_of = [&](int32_t step) -> int32_t {  // this lane's page of a step (outside the pool: zeros)
+                if (step >= w.steps || lane >= boxes) return int32_t(p.pages);
+                const int32_t k0 = w.slot0(step) + int32_t(lane * box), k1 = k0 + int32_t(box);
+                if (!((k0 < w.hi && k1 > w.lo) || k0 < w.sink)) return int32_t(p.pages);
+                const int32_t id = trow[k0 >> p.pshift];
+                if (uint32_t(id) < p.pages) return id;
+                if (p.err) atomicOr(p.err, kErrPage);
+                return int32_t(p.pages);
+            };
+            int32_t next_id = page_of(0);
+            for (int32_t j = 0; j < w.steps; ++j) {
+                const int32_t id = next_id;
+                next_id = page_of(j + 1);
+                const int32_t in = (w.slot0(j) + int32_t(lane * box)) & int32_t(p.P - 1);
+                for (int kv = 0; kv < 2; ++kv, ++slot) {
+                    const uint32_t s = slot % G::kStages, n = slot / G::kStages;
+                    if (n && !warp_wait(bar.empty(s), (n - 1) & 1u, deadline)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) bar_arrive_tx(bar.full(s), G::kTile);
+                    __syncwarp();
+                    if (lane < boxes)
+                        for (uint32_t c = 0; c < G::kPanels; ++c)
+                            tma4(smem + G::kRing + s * G::kTile + c * kPanel + lane * box * 128, kv ? &vmap : &kmap,
+                                 bar.full(s), int32_t(c * 64), in, w.h, id);
+                }
+                if (!ok) break;
+            }
+            release();
+        }
+        // every load has landed and every stage been released before the CTA ends
+        const uint64_t grace = ok ? deadline + kGraceNs : now() + kGraceNs;
+        const uint32_t last = min(slot, G::kStages);
+        for (uint32_t x = slot - last; x < slot; ++x) {
+            const uint32_t s = x % G::kStages, n = x / G::kStages;
+            warp_wait(bar.full(s), n & 1u, grace);
+            if (ok) warp_wait(bar.empty(s), n & 1u, grace);
+        }
+        if (sg) warp_wait(bar.q_full(), (sg - 1) & 1u, grace);
+    } else if (warp == 8) {
+        // ---- MMAs: one thread issues, the warp moves through the pieces together
+        constexpr uint32_t kIs = instr(T::kUmmaFormat, 128, kKeys, false);
+        constexpr uint32_t kIo = instr(T::kUmmaFormat, 128, D, true);
+        uint32_t slot = 0, pr[2] = {0, 0};
+        auto score = [&](uint32_t i, uint32_t s) {
+#pragma unroll
+            for (uint32_t k = 0; k < D / 16; ++k) {
+                const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
+                mma_ss(tmem + kS + i * 128, desc128(smem + i * G::kTile + off, 16, 1024),
+                       desc128(smem + G::kRing + s * G::kTile + off, 16, 1024), kIs, k > 0);
+            }
+            commit(bar.s_full(i));
+        };
+        while (ok && next()) {
+            const int32_t steps = segs[sg % kSegs].steps;
+            const uint32_t two = segs[sg % kSegs].left > per_tile ? 2 : 1;
+            if (lane == 0) {
+                ok = bar_wait(bar.q_full(), sg & 1u, deadline) &&
+                     bar_wait(bar.full(slot % G::kStages), (slot / G::kStages) & 1u, deadline);
+                if (ok) {
+                    fence_after();
+                    for (uint32_t i = 0; i < two; ++i) score(i, slot % G::kStages);
+                    commit(bar.empty(slot % G::kStages));
+                    if (steps == 1) commit(bar.q_empty());
+                }
+                uint32_t at = slot + 1;
+                for (int32_t j = 0; j < steps && ok; ++j, at += 2) {
+                    const uint32_t vs = at % G::kStages, ks = (at + 1) % G::kStages;
+                    const bool more = j + 1 < steps;
+                    if (!bar_wait(bar.full(vs), (at / G::kStages) & 1u, deadline) ||
+                        (more && !bar_wait(bar.full(ks), ((at + 1) / G::kStages) & 1u, deadline))) {
+                        ok = false;
+                        break;
+                    }
+                    for (uint32_t i = 0; i < two; ++i) {
+                        if (!bar_wait(bar.p_ready(i), pr[i] & 1u, deadline)) {
+                            ok = false;
+                            break;
+                        }
+                        ++pr[i];
+                        fence_after();
+#pragma unroll
+                        for (uint32_t k = 0; k < kKeys / 16; ++k)
+                            mma_ts(tmem + kO + i * D, tmem + kS + i * 128 + k * 8,
+                                   desc128(smem + G::kRing + vs * G::kTile + k * 2048, kPanel, 1024), kIo,
+                                   j > 0 || k > 0);
+                        if (more) score(i, ks);
+                        else commit(bar.o_full(i));
+                    }
+                    if (!ok) break;
+                    commit(bar.empty(vs));
+                    if (more) {
+                        commit(bar.empty(ks));
+                        if (j + 2 == steps) commit(bar.q_empty());
+                    }
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
+            slot += 2 * uint32_t(steps);
+            release();
+        }
+        if (!ok && lane == 0) {  // MMAs in flight end (bounded) before the tensor memory goes
+            commit(bar.drain());
+            bar_wait(bar.drain(), 0, now() + kGraceNs);
+        }
+        __syncwarp();
+    } else if (warp < 8) {
+        // ---- rows: thread r of row tile i
+        const uint32_t i = warp >> 2;
+        const uint32_t r = tid & 127u, quarter = (warp & 3u) << 21;  // lane 32 * (warp % 4) of tensor memory
+        const uint32_t ts = tmem + quarter + kS + i * 128, to = tmem + quarter + kO + i * D;
+        const int32_t lt = int32_t(r / p.g);
+        uint32_t ns = 0, no = 0, slot = 0;  // S tiles and O results seen, ring slots passed
+        while (ok && next()) {
+            const Seg& w = segs[sg % kSegs];
+            const int32_t steps = w.steps, t_tile = int32_t(i) * per_tile;  // first token of the tile, in the item
+            if (t_tile >= w.left) {  // the item has one row tile
+                slot += 2 * uint32_t(steps);
+                release();
+                continue;
+            }
+            const bool real = lt < per_tile && t_tile + lt < w.left;
+            const bool busy = __any_sync(0xffffffffu, real);
+            const int32_t pos = real ? max(w.pos0 + t_tile + lt, -1) : -1;
+            const int32_t pos_lo = w.pos0 + t_tile, pos_hi = w.pos0 + min(w.left, t_tile + per_tile) - 1;
+            float m = -INFINITY, l = 0.f;  // reference maximum and sum of the row
+            for (int32_t j = 0; j < steps; ++j, ++ns) {
+                const int32_t k0 = w.slot0(j);
+                if (!warp_wait(bar.s_full(i), ns & 1u, deadline)) {
+                    ok = false;
+                    break;
+                }
+                if (i == 0 && !(k0 >= w.lo && k0 + kKeys <= w.hi) && k0 + kKeys > w.sink) {
+                    // slots that no row sees: their values may be anything, and 0 * NaN is not 0
+                    const uint32_t vslot = slot + 2 * uint32_t(j) + 1, vs = vslot % G::kStages;
+                    if (!warp_wait(bar.full(vs), (vslot / G::kStages) & 1u, deadline)) {
+                        ok = false;
+                        break;
+                    }
+                    const int32_t k = k0 + int32_t(r);
+                    if (!((k >= w.lo && k < w.hi) || k < w.sink)) {
+                        uint8_t* v = base + G::kRing + vs * G::kTile + r * 128;
+#pragma unroll
+                        for (uint32_t c = 0; c < G::kPanels; ++c)
+#pragma unroll
+                            for (uint32_t e = 0; e < 8; ++e)
+                                *reinterpret_cast<uint4*>(v + c * kPanel + e * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    proxy_fence();
+                    __syncwarp();
+                }
+                if (busy) {
+                    fence_after();
+                    float x[128];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) ld32(ts + c * 32, x + c * 32);
+                    wait_ld();
+                    if (k0 + kKeys - 1 > pos_lo ||
+                        (p.window && int64_t(k0) <= int64_t(pos_hi) - int64_t(p.window))) {
+                        // columns [lo, hi) and those below s
+                        const int32_t hi = pos + 1 - k0, s = p.window ? int32_t(p.sinks) - k0 : 0;
+                        const int32_t lo = p.window ? pos + 1 - int32_t(p.window) - k0 : 0;
+#pragma unroll
+                        for (int c = 0; c < 128; ++c)
+                            if (c >= hi || (c < lo && c >= s)) x[c] = -INFINITY;
+                    }
+                    float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                    for (int c = 4; c < 128; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
+                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    const bool raise = m == -INFINITY ? mx > -INFINITY : (mx - m) * p.c > kRaise;
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float nm = raise ? mx : m;
+                        const float f2 = nm == -INFINITY ? 1.f : ex2((m - nm) * p.c);
+                        l *= f2;
+                        m = nm;
+                        if (j) {
+#pragma unroll
+                            for (int c = 0; c < D; c += 16) {
+                                float o[16];
+                                ld16(to + c, o);
+                                wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) o[e] *= f2;
+                                st16(to + c, o);
+                            }
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.f : -m * p.c;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float a = ex2(fmaf(x[c * 32 + 2 * e], p.c, ref));
+                            const float d = ex2(fmaf(x[c * 32 + 2 * e + 1], p.c, ref));
+                            sum[(2 * e) & 3] += a;
+                            sum[(2 * e + 1) & 3] += d;
+                            pk[e] = T::pack(a, d);
+                        }
+                        st16(ts + c * 16, pk);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    wait_st();
+                    fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar.p_ready(i));
+            }
+            if (!ok || !warp_wait(bar.o_full(i), no & 1u, deadline)) {
+                ok = false;
+                break;
+            }
+            slot += 2 * uint32_t(steps);
+            ++no;
+            if (busy) {
+                fence_after();
+                const bool whole = w.whole != 0;
+                const int64_t token = w.row0 + t_tile + lt;
+                const int32_t head = w.h * int32_t(p.g) + int32_t(r % p.g);
+                uint16_t* out = p.out + token * p.o_ts + int64_t(head) * p.o_hs;
+                float* part = sc.part + (2 * int64_t(blockIdx.x) + w.part) * (256 * (D + 2));
+                const uint32_t row = i * 128 + r;
+                const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    ld32(to + c, o);
+                    wait_ld();
+                    if (real && whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint4 v;
+                            v.x = T::pack(o[e] * inv, o[e + 1] * inv);
+                            v.y = T::pack(o[e + 2] * inv, o[e + 3] * inv);
+                            v.z = T::pack(o[e + 4] * inv, o[e + 5] * inv);
+                            v.w = T::pack(o[e + 6] * inv, o[e + 7] * inv);
+                            *reinterpret_cast<uint4*>(out + c + e) = v;
+                        }
+                    } else if (real) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<float4*>(part + row * D + c + e) =
+                                make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                    __syncwarp();
+                }
+                if (real) {
+                    if (whole) {
+                        if (p.lse) p.lse[token * p.Hq + head] = l == 0.f ? -INFINITY : (m * p.c + lg2(l)) * kLn2;
+                    } else {
+                        part[256 * D + row] = m * p.c;
+                        part[256 * D + 256 + row] = l;
+                    }
+                }
+                fence_before();  // O is read before the next item's first P V
+            }
+            release();
+        }
+    }
+    if (!ok && lane == 0 && p.err) atomicOr(p.err, uint32_t(LS_B200_ATTN_TIMEOUT));
+    fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        fence_after();
+        dealloc<512>(tmem);
+    }
+}
+
+// Joins the parts of one item cut over several CTAs: CTA (c, block of 32 rows),
+// for the item that begins in c and goes on.
+template <class T, int D>
+__global__ void __launch_bounds__(256) chunk_join_kernel(const AttnParams p, const ChunkScratch sc) {
+    const int64_t U = sc.plan->units, G = sc.plan->ctas;
+    if (int64_t(blockIdx.x) >= G || !U) return;
+    const int2 open = sc.plan->open[blockIdx.x];
+    if (open.x < 0) return;
+    const ChunkItem it = sc.items[open.x];
+    const int64_t item = it.units + int64_t(open.y) * it.tiles;
+    const int64_t c0 = blockIdx.x, c1 = cut_owner(U, G, item + it.tiles - 1);
+    const int32_t per_tile = int32_t(chunk_tokens(p.g));
+    for (uint32_t x = threadIdx.x; x < 32 * (D / 4); x += blockDim.x) {
+        const uint32_t row = blockIdx.y * 32 + x / (D / 4), d = x % (D / 4) * 4, r = row & 127u;
+        const int32_t lt = int32_t(r / p.g), t = it.t0 + int32_t(row >> 7) * per_tile + lt;
+        if (lt >= per_tile || t >= it.nq) continue;
+        auto part = [&](int64_t c) {
+            return sc.part + (2 * c + (c == c0 && cut_begin(U, G, c0) != item ? 1 : 0)) * (256 * (D + 2));
+        };
+        float mx = -INFINITY;
+        for (int64_t c = c0; c <= c1; ++c) mx = fmaxf(mx, part(c)[256 * D + row]);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+        for (int64_t c = c0; c <= c1; ++c) {
+            const float* ps = part(c);
+            const float f = mx == -INFINITY ? 0.f : ex2(ps[256 * D + row] - mx);
+            const float4 v = *reinterpret_cast<const float4*>(ps + row * D + d);
+            o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+            sum = fmaf(f, ps[256 * D + 256 + row], sum);
+        }
+        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+        const int64_t token = it.q0 + t;
+        const int32_t head = open.y * int32_t(p.g) + int32_t(r % p.g);
+        *reinterpret_cast<uint2*>(p.out + token * p.o_ts + int64_t(head) * p.o_hs + d) =
+            make_uint2(T::pack(o.x * inv, o.y * inv), T::pack(o.z * inv, o.w * inv));
+        if (d == 0 && p.lse) p.lse[token * p.Hq + head] = sum == 0.f ? -INFINITY : (mx + lg2(sum)) * kLn2;
+    }
+}
+
+using Encode = decltype(&cuTensorMapEncodeTiled);
+Encode encoder() {
+    static const Encode fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult res;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &res) !=
+                cudaSuccess ||
+            res != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<Encode>(f);
+    }();
+    return fn;
+}
+
+bool encode(CUtensorMap* map, bool bf16, const void* base, uint32_t rank, const cuuint64_t* dims, const int64_t* strides,
+            const cuuint32_t* box) {
+    cuuint64_t bytes[3];
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    for (uint32_t i = 0; i + 1 < rank; ++i)  // the stride of a dimension of one is never used
+        bytes[i] = dims[i + 1] > 1 ? cuuint64_t(strides[i]) * 2 : cuuint64_t(dims[0]) * 2;
+    return encoder()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                     const_cast<void*>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int D>
+int launch(const AttnParams& p, bool bf16, const ChunkScratch& s, uint32_t grid, cudaStream_t stream) {
+    if (!encoder()) return ENOSYS;
+    CUtensorMap qm, km, vm;
+    const cuuint64_t qd[3] = {D, p.Hq, p.tokens};
+    const int64_t qs[2] = {p.q_hs, p.q_ts};
+    const cuuint32_t qb[3] = {64, p.g, chunk_tokens(p.g)};
+    const cuuint64_t kd[4] = {D, p.P, p.Hkv, p.pages};
+    const int64_t ks[3] = {p.kp_ss, p.kp_hs, p.kp_ps}, vs[3] = {p.vp_ss, p.vp_hs, p.vp_ps};
+    const cuuint32_t kb[4] = {64, p.P < 128 ? p.P : 128, 1, 1};
+    if (!encode(&qm, bf16, p.q, 3, qd, qs, qb) || !encode(&km, bf16, p.k_pages, 4, kd, ks, kb) ||
+        !encode(&vm, bf16, p.v_pages, 4, kd, vs, kb))
+        return EINVAL;
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return int(e);
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(chunk_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 int(Geo<D>::kSmem));
+        if (e != cudaSuccess) return int(e);
+        done.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    const uint32_t append = p.k_new ? p.B * ((p.max_q + 7) / 8) : 0;
+    chunk_prepare_kernel<<<1 + append, 256, 0, stream>>>(p, s, grid);
+    chunk_attn_kernel<T, D><<<grid, kThreads, Geo<D>::kSmem, stream>>>(p, s, qm, km, vm);
+    chunk_join_kernel<T, D><<<dim3(grid, 8), 256, 0, stream>>>(p, s);
+    return int(cudaGetLastError());
+}
+
+}  // namespace
+
+int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream) {
+    const uint32_t grid = sms < kMaxCtas ? sms : kMaxCtas;
+    if (p.D == 64)
+        return dtype == LS_B200_BF16 ? launch<BF16, 64>(p, true, s, grid, stream)
+                                     : launch<F16, 64>(p, false, s, grid, stream);
+    return dtype == LS_B200_BF16 ? launch<BF16, 128>(p, true, s, grid, stream)
+                                 : launch<F16, 128>(p, false, s, grid, stream);
+}
+
+}  // namespace lsb

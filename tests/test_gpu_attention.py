@@ -2,7 +2,7 @@
 against the formula in 64 bits.
 
 Bounds, per element. Output: the result is rounded once to 16 bits (unit
-roundoff u = 2^-11 for float16, 2^-9 for bfloat16), and each probability may
+roundoff u = 2^-11 for float16, 2^-8 for bfloat16), and each probability may
 be rounded to 16 bits before it meets its value, which moves the sum by at most
 u * A, A = sum p |v|; the logits (up to about 40 here, a 128-term sum in 32
 bits times scale * log2 e, one rounding each) and the exponential are good to
@@ -16,7 +16,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -9}
+UNIT = {t: torch.finfo(t).eps / 2 for t in (torch.float16, torch.bfloat16)}
 
 
 class Call:
