@@ -567,14 +567,15 @@ uint32_t dec_mt(const ls_b200_attention_args& a) {
 constexpr uint64_t kChunkRows = 32;
 bool is_chunk(const ls_b200_attention_args& a) {
     const uint32_t g = a.q_heads / a.kv_heads;
-    return uint64_t(a.max_q) * g > kChunkRows && g <= 128 && !a.weights_length;
+    return uint64_t(a.max_q) * g > kChunkRows && g <= 128;
 }
 
 struct ScratchPlan {
-    uint64_t count, part, lse, logits, plan, items, chunk_part, total;
+    uint64_t count, part, lse, logits, plan, items, chunk_part, w_plan, w_items, w_part, total;
 };
 ScratchPlan scratch_plan(const ls_b200_attention_args& a) {
     ScratchPlan s{};
+    const bool w = a.weights_length != 0;
     s.count = 0;
     s.part = up256(kMaxCtas * sizeof(uint32_t));
     if (is_chunk(a)) {
@@ -582,11 +583,14 @@ ScratchPlan scratch_plan(const ls_b200_attention_args& a) {
         s.plan = s.part;
         s.items = s.plan + up256(sizeof(ChunkPlan));
         s.chunk_part = s.items + up256(chunk_items(a.tokens, a.batch, g) * sizeof(ChunkItem));
-        s.total = s.chunk_part + up256(2ull * sm_count() * chunk_part_floats(a.head_dim) * sizeof(float));
+        s.w_plan = s.chunk_part + up256(2ull * sm_count() * chunk_part_floats(a.head_dim) * sizeof(float));
+        s.w_items = s.w_plan + (w ? up256(sizeof(ChunkPlan)) : 0);
+        s.w_part = s.w_items + (w ? up256(chunk_weight_items(a.batch, a.weights_length) * sizeof(ChunkItem)) : 0);
+        s.lse = s.w_part + (w ? up256(2ull * sm_count() * 128 * sizeof(float)) : 0);
+        s.total = s.lse + (w ? up256(uint64_t(a.tokens) * a.q_heads * sizeof(float)) : 0);
         return s;
     }
     s.lse = s.part + up256(2ull * kMaxCtas * 16 * dec_mt(a) * (a.head_dim + 2) * sizeof(float));
-    const bool w = a.weights_length != 0;
     s.logits = s.lse + (w ? up256(uint64_t(a.tokens) * a.q_heads * sizeof(float)) : 0);
     s.total = s.logits + (w ? up256(uint64_t(a.batch) * a.q_heads * a.weights_length * a.max_q * sizeof(float)) : 0);
     return s;
@@ -697,7 +701,10 @@ int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
     if (is_chunk(*a)) {
         const ChunkScratch c{reinterpret_cast<ChunkPlan*>(scratch + plan.plan),
                              reinterpret_cast<ChunkItem*>(scratch + plan.items),
-                             reinterpret_cast<float*>(scratch + plan.chunk_part)};
+                             reinterpret_cast<float*>(scratch + plan.chunk_part),
+                             reinterpret_cast<ChunkPlan*>(scratch + plan.w_plan),
+                             reinterpret_cast<ChunkItem*>(scratch + plan.w_items),
+                             reinterpret_cast<float*>(scratch + plan.w_part)};
         return launch_chunk(p, a->dtype, c, sm_count(), s);
     }
     const uint32_t mt = dec_mt(*a);

@@ -40,9 +40,10 @@ struct AttnParams {
 // The tensor-core path of chunks (ls_attention_chunk.cu): one item is two
 // 128-row tiles of one kv head, a row being a (token, head of the group).
 constexpr uint32_t kMaxCtas = 512;  // CTAs of a launch, and counters in the scratch header
-struct ChunkItem {                  // tokens t0 .. of a sequence, written by the plan kernel
+constexpr int kChunkKeys = 128;     // slots of a tile
+struct ChunkItem {                  // written by the plan kernel
     int32_t b, q0, nq, n;           // the sequence, as SeqRange
-    int32_t t0, tiles;              // first token, tiles of 128 slots
+    int32_t t0, tiles;              // attention: first token, tiles of slots; weights: first slot, row tiles
     int64_t units;                  // tiles of the items before, over all kv heads
 };
 struct ChunkPlan {
@@ -55,10 +56,16 @@ struct ChunkScratch {
     ChunkPlan* plan;
     ChunkItem* items;
     float* part;
+    ChunkPlan* w_plan;  // of the weights
+    ChunkItem* w_items;
+    float* w_part;      // [2 * CTAs][128]
 };
 __host__ __device__ inline uint32_t chunk_tokens(uint32_t g) { return 128 / g; }  // of one 128-row tile
-inline uint64_t chunk_items(uint64_t tokens, uint64_t batch, uint32_t g) {
+__host__ __device__ inline uint64_t chunk_items(uint64_t tokens, uint64_t batch, uint32_t g) {
     return tokens / (2 * chunk_tokens(g)) + batch;
+}
+__host__ __device__ inline uint64_t chunk_weight_items(uint64_t batch, uint64_t wlen) {
+    return batch * (wlen / kChunkKeys + 2);
 }
 inline uint64_t chunk_part_floats(uint32_t D) { return 256ull * (D + 2); }  // one partial result
 int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream);
@@ -108,6 +115,20 @@ __device__ __forceinline__ KeyRange key_range(const AttnParams& p, const SeqRang
 }
 
 __device__ __forceinline__ int32_t tile_at(const KeyRange& r, int32_t j) { return j < r.ns ? j : r.first + j - r.ns; }
+
+// The row tiles (of chunk_tokens tokens) with a token that sees one of the 128
+// slots from k0.
+struct RowTiles {
+    int32_t begin, end;
+};
+__device__ __forceinline__ RowTiles row_tiles(const AttnParams& p, const SeqRange& s, int32_t k0) {
+    const int32_t T = int32_t(chunk_tokens(p.g)), t_lo = max(0, k0 - s.f);
+    int32_t t_hi = s.nq;
+    if (p.window && uint32_t(k0) >= p.sinks)
+        t_hi = int32_t(max(int64_t(0), min(int64_t(s.nq), int64_t(k0) + kChunkKeys - 1 + p.window - s.f)));
+    const int32_t begin = t_lo / T;
+    return {begin, t_lo < t_hi ? (t_hi + T - 1) / T : begin};
+}
 
 // Whether position pos sees slot k (pos < 0: nothing).
 __device__ __forceinline__ bool sees(const AttnParams& p, int32_t pos, int32_t k) {
@@ -168,5 +189,36 @@ struct BF16 {
 // First unit of CTA c when U units are cut evenly over G CTAs, and the CTA of a unit.
 __device__ __forceinline__ int64_t cut_begin(int64_t U, int64_t G, int64_t c) { return c * U / G; }
 __device__ __forceinline__ int64_t cut_owner(int64_t U, int64_t G, int64_t u) { return ((u + 1) * G - 1) / U; }
+
+// The pieces of items that a CTA works on, in order.
+struct Walk {
+    int64_t U, G, u, u_begin, u_end;
+    int64_t item;  // first unit of (item, kv head)
+    int32_t i, h, j0, steps;
+    ChunkItem it;
+    __device__ bool begin(const ChunkPlan* plan) {
+        U = plan->units;
+        G = plan->ctas;
+        if (int64_t(blockIdx.x) >= G || !U) return false;
+        u = u_begin = cut_begin(U, G, blockIdx.x);
+        u_end = cut_begin(U, G, blockIdx.x + 1);
+        i = plan->start[blockIdx.x] - 1;
+        it.units = it.tiles = steps = 0;
+        return true;
+    }
+    __device__ bool next(const AttnParams& p, const ChunkPlan* plan, const ChunkItem* items) {
+        u += steps;
+        if (u >= u_end) return false;
+        while (u >= it.units + int64_t(it.tiles) * p.Hkv || !it.tiles) {
+            if (++i >= plan->items) return false;
+            it = items[i];
+        }
+        h = int32_t((u - it.units) / it.tiles);
+        item = it.units + int64_t(h) * it.tiles;
+        j0 = int32_t(u - item);
+        steps = int32_t(min(u_end, item + it.tiles) - u);
+        return true;
+    }
+};
 
 }  // namespace lsb

@@ -38,7 +38,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kKeys = 128;  // slots of a tile
+constexpr int kKeys = kChunkKeys;
 constexpr int kThreads = 384;  // twelve warps, 168 registers per thread
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows of 64 elements
 constexpr uint64_t kGraceNs = 1000000000ull;
@@ -70,35 +70,15 @@ struct Bars {
     __device__ uint32_t seg_empty(uint32_t s) const { return base + 8 * (29 + s); }
 };
 
-// Appends the new keys and values (blocks 1 ..) and lays out the items (block 0).
-__global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, const ChunkScratch sc, uint32_t grid) {
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (blockIdx.x) {
-        // one warp per token
-        const uint32_t pieces = p.D / 8, per_token = p.Hkv * pieces;
-        const uint32_t per_seq = (p.max_q + 7) / 8, at = blockIdx.x - 1, b = at / per_seq;
-        const SeqRange s = load_seq(p, b);
-        const int32_t t = int32_t(at % per_seq * 8 + warp), slot = s.f + t;
-        if (t >= s.nq || slot < 0) return;
-        const int32_t id = p.table[int64_t(b) * p.table_s + (slot >> p.pshift)];
-        if (uint32_t(id) >= p.pages) {
-            if (p.err) atomicOr(p.err, kErrPage);
-            return;
-        }
-        const int64_t in = slot & int32_t(p.P - 1), tok = s.q0 + t;
-        for (uint32_t i = lane; i < per_token; i += 32) {
-            const int64_t h = i / pieces, e = (i % pieces) * 8;
-            *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + in * p.kp_ss + h * p.kp_hs + e) =
-                *reinterpret_cast<const uint4*>(p.k_new + tok * p.kn_ts + h * p.kn_hs + e);
-            *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + in * p.vp_ss + h * p.vp_hs + e) =
-                *reinterpret_cast<const uint4*>(p.v_new + tok * p.vn_ts + h * p.vn_hs + e);
-        }
-        return;
-    }
+// Lays out the items of a call in `plan` and `items`: for the attention
+// (WEIGHTS false) the pairs of row tiles of each sequence, counted in tiles of
+// 128 slots; for the weights the tiles of 128 slots, counted in row tiles.
+template <bool WEIGHTS>
+__device__ void lay_out(const AttnParams& p, ChunkPlan* plan, ChunkItem* list, int32_t cap, uint32_t grid) {
     __shared__ int32_t first[257];  // items before each sequence of the batch piece
     __shared__ int64_t wsum[8];
-    const int32_t per_item = 2 * int32_t(chunk_tokens(p.g));
-    const int32_t cap = int32_t(p.tokens / uint32_t(per_item) + p.B);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int32_t per_tile = int32_t(chunk_tokens(p.g));
     int32_t items = 0;
     int64_t units = 0;
     auto scan = [&](int64_t v, int64_t& before) {  // over the block
@@ -122,14 +102,14 @@ __global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, 
         SeqRange s{0, 0, 0, 0};
         if (b0 + tid < p.B) s = load_seq(p, b0 + tid);
         int64_t before;
-        const int32_t count = (s.nq + per_item - 1) / per_item;
+        const int32_t count = WEIGHTS ? (s.nq ? key_range<kKeys>(p, s, 0, s.nq).tiles : 0)
+                                      : (s.nq + 2 * per_tile - 1) / (2 * per_tile);
         int32_t total = int32_t(scan(count, before));
         if (total > cap - items) {  // overlapping q_start ranges
             total = max(0, cap - items);
             if (tid == 0 && p.err) atomicOr(p.err, kErrLength);
         }
         first[tid] = int32_t(before);
-        if (tid == 0) first[256] = total;
         __syncthreads();
         for (int32_t i0 = 0; i0 < total; i0 += 256) {
             const int32_t i = i0 + int32_t(tid);
@@ -144,12 +124,18 @@ __global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, 
                 it.b = int32_t(b0 + lo);
                 const SeqRange q = load_seq(p, uint32_t(it.b));
                 it.q0 = q.q0, it.nq = q.nq, it.n = q.n;
-                it.t0 = (i - first[lo]) * per_item;
-                it.tiles = key_range<kKeys>(p, q, it.t0, min(q.nq, it.t0 + per_item)).tiles;
+                if (WEIGHTS) {
+                    it.t0 = tile_at(key_range<kKeys>(p, q, 0, q.nq), i - first[lo]) * kKeys;
+                    const RowTiles r = row_tiles(p, q, it.t0);
+                    it.tiles = r.end - r.begin;
+                } else {
+                    it.t0 = (i - first[lo]) * 2 * per_tile;
+                    it.tiles = key_range<kKeys>(p, q, it.t0, min(q.nq, it.t0 + 2 * per_tile)).tiles;
+                }
             }
             const int64_t sum = scan(int64_t(it.tiles) * p.Hkv, before);
             it.units = units + before;
-            if (i < total) sc.items[items + i] = it;
+            if (i < total) list[items + i] = it;
             units += sum;
         }
         items += total;
@@ -159,54 +145,49 @@ __global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, 
     // more than the tiles it spreads.
     const int64_t G = max(int64_t(1), min(int64_t(grid), (units + 3) / 4));
     if (tid == 0) {
-        sc.plan->units = units;
-        sc.plan->items = items;
-        sc.plan->ctas = int32_t(G);
+        plan->units = units;
+        plan->items = items;
+        plan->ctas = int32_t(G);
     }
-    for (uint32_t c = tid; c < kMaxCtas; c += 256) sc.plan->open[c] = make_int2(-1, 0);
+    for (uint32_t c = tid; c < kMaxCtas; c += 256) plan->open[c] = make_int2(-1, 0);
     __syncthreads();
-    for (int32_t i = int32_t(tid); i < items; i += 256) {  // each thread reads what this block wrote
-        const int64_t u = sc.items[i].units, end = u + int64_t(sc.items[i].tiles) * p.Hkv;
-        for (int64_t c = (u * G + units - 1) / units; c < G && cut_begin(units, G, c) < end; ++c)
-            sc.plan->start[c] = i;
+    for (int32_t i = int32_t(tid); i < items; i += 256) {  // what this block wrote
+        const int64_t u = list[i].units, end = u + int64_t(list[i].tiles) * p.Hkv;
+        if (u < end)
+            for (int64_t c = (u * G + units - 1) / units; c < G && cut_begin(units, G, c) < end; ++c)
+                plan->start[c] = i;
     }
 }
 
-// The pieces of items that a CTA works on, in order.
-struct Walk {
-    int64_t U, G, u, u_begin, u_end;
-    int32_t i;  // item
-    ChunkItem it;
-    int32_t h, j0, steps;
-    int64_t item;  // first unit of (item, kv head)
-    KeyRange kr;
-    __device__ bool begin(const ChunkScratch& sc) {
-        U = sc.plan->units;
-        G = sc.plan->ctas;
-        if (int64_t(blockIdx.x) >= G || !U) return false;
-        u = u_begin = cut_begin(U, G, blockIdx.x);
-        u_end = cut_begin(U, G, blockIdx.x + 1);
-        i = sc.plan->start[blockIdx.x] - 1;
-        it.units = -1;
-        it.tiles = 0;
-        steps = 0;
-        return true;
-    }
-    __device__ bool next(const AttnParams& p, const ChunkScratch& sc) {
-        u += steps;
-        if (u >= u_end) return false;
-        if (it.units < 0 || u >= it.units + int64_t(it.tiles) * p.Hkv) {
-            it = sc.items[++i];
-            const SeqRange s{it.q0, it.nq, it.n, it.n - it.nq};
-            kr = key_range<kKeys>(p, s, it.t0, min(it.nq, it.t0 + 2 * int32_t(chunk_tokens(p.g))));
+// Lays out the attention's items (block 0) and the weights' (block 1), and
+// appends the new keys and values (blocks 2 .., a warp per token).
+__global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, const ChunkScratch sc, uint32_t grid) {
+    if (blockIdx.x == 0) {
+        lay_out<false>(p, sc.plan, sc.items, int32_t(chunk_items(p.tokens, p.B, p.g)), grid);
+    } else if (blockIdx.x == 1) {
+        if (p.weights) lay_out<true>(p, sc.w_plan, sc.w_items, int32_t(chunk_weight_items(p.B, p.wlen)), grid);
+    } else {
+        const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const uint32_t pieces = p.D / 8, per_token = p.Hkv * pieces;
+        const uint32_t per_seq = (p.max_q + 7) / 8, at = blockIdx.x - 2, b = at / per_seq;
+        const SeqRange s = load_seq(p, b);
+        const int32_t t = int32_t(at % per_seq * 8 + warp), slot = s.f + t;
+        if (t >= s.nq || slot < 0) return;
+        const int32_t id = p.table[int64_t(b) * p.table_s + (slot >> p.pshift)];
+        if (uint32_t(id) >= p.pages) {
+            if (p.err) atomicOr(p.err, kErrPage);
+            return;
         }
-        h = int32_t((u - it.units) / it.tiles);
-        item = it.units + int64_t(h) * it.tiles;
-        j0 = int32_t(u - item);
-        steps = int32_t(min(u_end, item + it.tiles) - u);
-        return true;
+        const int64_t in = slot & int32_t(p.P - 1), tok = s.q0 + t;
+        for (uint32_t i = lane; i < per_token; i += 32) {
+            const int64_t h = i / pieces, e = (i % pieces) * 8;
+            *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + in * p.kp_ss + h * p.kp_hs + e) =
+                *reinterpret_cast<const uint4*>(p.k_new + tok * p.kn_ts + h * p.kn_hs + e);
+            *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + in * p.vp_ss + h * p.vp_hs + e) =
+                *reinterpret_cast<const uint4*>(p.v_new + tok * p.vn_ts + h * p.vn_hs + e);
+        }
     }
-};
+}
 
 // One piece of an item in shared memory (four in flight): what the roles need.
 struct Seg {
@@ -291,18 +272,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- pieces
         if (lane == 0) {
             Walk w;
-            bool more = w.begin(sc);
+            KeyRange kr{};
+            bool more = w.begin(sc.plan);
             for (; ok; ++sg) {
                 if (sg >= kSegs && !bar_wait(bar.seg_empty(sg % kSegs), (sg / kSegs - 1) & 1u, deadline)) {
                     ok = false;
                     break;
                 }
-                more = more && w.next(p, sc);
+                more = more && w.next(p, sc.plan, sc.items);
                 Seg x{};
                 if (more) {
+                    const SeqRange q{w.it.q0, w.it.nq, w.it.n, w.it.n - w.it.nq};
+                    kr = key_range<kKeys>(p, q, w.it.t0, min(w.it.nq, w.it.t0 + 2 * per_tile));
                     x.steps = w.steps, x.row0 = w.it.q0 + w.it.t0, x.left = w.it.nq - w.it.t0;
                     x.pos0 = w.it.n - w.it.nq + w.it.t0, x.h = w.h, x.b = w.it.b, x.j0 = w.j0;
-                    x.ns = w.kr.ns, x.first = w.kr.first, x.lo = w.kr.lo, x.hi = w.kr.hi, x.sink = w.kr.sink;
+                    x.ns = kr.ns, x.first = kr.first, x.lo = kr.lo, x.hi = kr.hi, x.sink = kr.sink;
                     x.whole = w.j0 == 0 && w.steps == w.it.tiles;
                     x.part = w.u != w.u_begin;
                     if (!x.whole && !w.j0) sc.plan->open[blockIdx.x] = make_int2(w.i, w.h);
@@ -642,6 +626,311 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const AttnParams p, con
     }
 }
 
+// weights[b, h, slot] of a call, once the rows' lse are known: per tile of 128
+// slots and row tile S^T = K Q^T (M the slots, N the rows), then each thread
+// sums exp2(S c - lse) over the rows of its slot, with no exchange between
+// threads and in a fixed order. Warps 0-3 and 4-7 take the row tiles in turn; two score buffers each in
+// tensor memory let the MMAs run ahead. A slot tile cut over several CTAs is
+// summed, in order, by the one that arrives last. The exponentials bound it:
+// 128 x 128 of them per 2 * 128^2 * head_dim operations.
+template <int D>
+struct GeoW {
+    static constexpr uint32_t kPanels = D / 64, kTile = kPanels * kPanel, kStages = 4;
+    static constexpr uint32_t kRing = 2 * kTile, kBars = kRing + kStages * kTile;  // two K tiles, then Q tiles
+    static constexpr uint32_t kLse = kBars + 512;                                  // [2 groups][2][128] floats
+    static constexpr uint32_t kSmem = kLse + 2048 + 1024;
+};
+struct BarsW {
+    uint32_t base;
+    __device__ uint32_t k_full(uint32_t i) const { return base + 8 * i; }
+    __device__ uint32_t k_empty(uint32_t i) const { return base + 8 * (2 + i); }
+    __device__ uint32_t q_full(uint32_t i) const { return base + 8 * (4 + i); }
+    __device__ uint32_t q_empty(uint32_t i) const { return base + 8 * (8 + i); }
+    __device__ uint32_t s_full(uint32_t i) const { return base + 8 * (12 + i); }
+    __device__ uint32_t s_empty(uint32_t i) const { return base + 8 * (16 + i); }
+    __device__ uint32_t sums() const { return base + 8 * 20; }
+    __device__ uint32_t summed() const { return base + 8 * 21; }
+    __device__ uint32_t drain() const { return base + 8 * 22; }
+};
+
+__device__ __forceinline__ void group_sync(uint32_t group) {
+    asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory");
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    chunk_weights_kernel(const AttnParams p, const ChunkScratch sc, const __grid_constant__ CUtensorMap qmap,
+                         const __grid_constant__ CUtensorMap kmap) {
+    using G = GeoW<D>;
+    extern __shared__ uint8_t raw[];
+    const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
+    uint8_t* const base = raw + (smem - smem_u32(raw));
+    const BarsW bar{smem + G::kBars};
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(base + G::kBars + 8 * 23);
+    float* const lse_s = reinterpret_cast<float*>(base + G::kLse);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int32_t per_tile = int32_t(chunk_tokens(p.g));
+
+    if (tid == 0) {
+        for (uint32_t i = 0; i < 2; ++i) {
+            bar_init(bar.k_full(i), 1);
+            bar_init(bar.k_empty(i), 1);
+        }
+        for (uint32_t i = 0; i < 4; ++i) {
+            bar_init(bar.q_full(i), 1);
+            bar_init(bar.q_empty(i), 1);
+            bar_init(bar.s_full(i), 1);
+            bar_init(bar.s_empty(i), 4);
+        }
+        bar_init(bar.sums(), 128);
+        bar_init(bar.summed(), 128);
+        bar_init(bar.drain(), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) alloc<512>(smem_u32(tmem_slot));
+    if (warp == 9 && lane == 0) {
+        prefetch_map(&qmap);
+        prefetch_map(&kmap);
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint64_t deadline = now() + p.timeout_ns;
+    bool ok = true;
+    Walk w;
+    if (w.begin(sc.w_plan)) {
+        uint32_t seg = 0, n = 0;  // pieces begun, row tiles passed
+        if (warp == 9) {
+            const uint32_t box = min(p.P, 128u), boxes = 128 / box;
+            for (; ok && w.next(p, sc.w_plan, sc.w_items); ++seg) {
+                const SeqRange s{w.it.q0, w.it.nq, w.it.n, w.it.n - w.it.nq};
+                const int32_t tile0 = row_tiles(p, s, w.it.t0).begin + w.j0;
+                const uint32_t kb = seg & 1u;
+                if (seg >= 2 && !warp_wait(bar.k_empty(kb), (seg / 2 - 1) & 1u, deadline)) {
+                    ok = false;
+                    break;
+                }
+                int32_t id = int32_t(p.pages);
+                const int32_t k0 = w.it.t0 + int32_t(lane * box);
+                if (lane < boxes && k0 < w.it.n) {  // (slots that no row sees may be read: their sums are not kept)
+                    const KeyRange kr = key_range<kKeys>(p, s, 0, s.nq);
+                    if ((k0 < kr.hi && k0 + int32_t(box) > kr.lo) || k0 < kr.sink) {
+                        id = p.table[int64_t(w.it.b) * p.table_s + (k0 >> p.pshift)];
+                        if (uint32_t(id) >= p.pages) id = int32_t(p.pages);  // reported by the attention
+                    }
+                }
+                if (lane == 0) bar_arrive_tx(bar.k_full(kb), G::kTile);
+                __syncwarp();
+                if (lane < boxes)
+                    for (uint32_t c = 0; c < G::kPanels; ++c)
+                        tma4(smem + kb * G::kTile + c * kPanel + lane * box * 128, &kmap, bar.k_full(kb),
+                             int32_t(c * 64), k0 & int32_t(p.P - 1), w.h, id);
+                for (int32_t j = 0; j < w.steps; ++j, ++n) {
+                    const uint32_t st = n % G::kStages;
+                    if (n >= G::kStages && !warp_wait(bar.q_empty(st), (n / G::kStages - 1) & 1u, deadline)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) {
+                        bar_arrive_tx(bar.q_full(st), G::kPanels * uint32_t(per_tile) * p.g * 128);
+                        for (uint32_t c = 0; c < G::kPanels; ++c)
+                            tma3(smem + G::kRing + st * G::kTile + c * kPanel, &qmap, bar.q_full(st), int32_t(c * 64),
+                                 w.h * int32_t(p.g), w.it.q0 + (tile0 + j) * per_tile);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) {
+                    ++seg;
+                    break;
+                }
+            }
+            const uint64_t grace = ok ? deadline + kGraceNs : now() + kGraceNs;
+            for (uint32_t x = n - min(n, G::kStages); x < n; ++x) {
+                warp_wait(bar.q_full(x % G::kStages), (x / G::kStages) & 1u, grace);
+                if (ok) warp_wait(bar.q_empty(x % G::kStages), (x / G::kStages) & 1u, grace);
+            }
+            for (uint32_t x = seg - min(seg, 2u); x < seg; ++x) {
+                warp_wait(bar.k_full(x & 1u), (x / 2) & 1u, grace);
+                if (ok) warp_wait(bar.k_empty(x & 1u), (x / 2) & 1u, grace);
+            }
+        } else if (warp == 8) {
+            if (lane == 0) {
+                constexpr uint32_t kIs = instr(T::kUmmaFormat, 128, 128, false);
+                for (; ok && w.next(p, sc.w_plan, sc.w_items); ++seg) {
+                    const uint32_t kb = seg & 1u;
+                    ok = bar_wait(bar.k_full(kb), (seg / 2) & 1u, deadline);
+                    for (int32_t j = 0; j < w.steps && ok; ++j, ++n) {
+                        const uint32_t st = n % G::kStages, sb = n & 3u;
+                        if (!bar_wait(bar.q_full(st), (n / G::kStages) & 1u, deadline) ||
+                            (n >= 4 && !bar_wait(bar.s_empty(sb), (n / 4 - 1) & 1u, deadline))) {
+                            ok = false;
+                            break;
+                        }
+                        fence_after();
+#pragma unroll
+                        for (uint32_t k = 0; k < D / 16; ++k) {
+                            const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
+                            mma_ss(tmem + sb * 128, desc128(smem + kb * G::kTile + off, 16, 1024),
+                                   desc128(smem + G::kRing + st * G::kTile + off, 16, 1024), kIs, k > 0);
+                        }
+                        commit(bar.s_full(sb));
+                        commit(bar.q_empty(st));
+                    }
+                    if (ok) commit(bar.k_empty(kb));
+                }
+                if (!ok) {
+                    commit(bar.drain());
+                    bar_wait(bar.drain(), 0, now() + kGraceNs);
+                }
+            }
+            __syncwarp();
+        } else if (warp < 8) {
+            const uint32_t grp = warp >> 2, r = tid & 127u;
+            const uint32_t ts = tmem + ((warp & 3u) << 21);
+            const int32_t ct = int32_t(r / p.g), ch = int32_t(r % p.g);  // this thread's row when it fetches lse
+            float* const mine = lse_s + grp * 256;
+            uint32_t buf = 0;
+            // (after a wait that gave up the pieces still go by, without further
+            // waits, so that every thread meets its group's barriers)
+            for (; w.next(p, sc.w_plan, sc.w_items); ++seg) {
+                const SeqRange s{w.it.q0, w.it.nq, w.it.n, w.it.n - w.it.nq};
+                const int32_t tile0 = row_tiles(p, s, w.it.t0).begin + w.j0;
+                const int32_t k0 = w.it.t0, k = k0 + int32_t(r);
+                // -lse (base 2) of row r of a row tile
+                auto fetch = [&](int32_t j) -> float {
+                    const int32_t t = (tile0 + j) * per_tile + ct;
+                    if (j >= w.steps || ct >= per_tile || t >= s.nq) return 0.f;
+                    return -p.lse[int64_t(s.q0 + t) * p.Hq + w.h * p.g + ch] * kLog2e;
+                };
+                float acc = 0.f;
+                const int32_t odd = int32_t((grp ^ n) & 1u);  // this group's first row tile of the piece
+                float nxt = fetch(odd);
+                for (int32_t j = odd; j < w.steps; j += 2) {
+                    const uint32_t at = n + uint32_t(j), sb = at & 3u;
+                    mine[buf * 128 + r] = nxt;
+                    group_sync(grp);
+                    nxt = fetch(j + 2);
+                    if (!warp_wait(bar.s_full(sb), (at / 4) & 1u, deadline)) ok = false;
+                    const int32_t t0 = (tile0 + j) * per_tile, cols = min(per_tile, s.nq - t0) * int32_t(p.g);
+                    const int32_t p0 = s.f + t0, p1 = p0 + min(per_tile, s.nq - t0) - 1;
+                    const float4* ls = reinterpret_cast<const float4*>(mine + buf * 128);
+                    const bool full = cols == 128 && k0 + kKeys - 1 <= p0 &&
+                                      (!p.window || int64_t(p1) < int64_t(k0) + p.window);
+                    // columns [lo, hi): rows whose token sees slot k
+                    const int64_t last = p.window && uint32_t(k) >= p.sinks ? int64_t(k) + p.window - p0 : per_tile;
+                    const int32_t lo = max(k - p0, 0), hi = int32_t(max(int64_t(0), min(last, int64_t(per_tile))));
+                    const int32_t c_lo = min(lo, per_tile) * int32_t(p.g), c_hi = min(hi * int32_t(p.g), cols);
+                    fence_after();
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    float x[2][32];
+                    ld32(ts + sb * 128, x[0]);
+                    wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (c < 3) ld32(ts + sb * 128 + (c + 1) * 32, x[(c + 1) & 1]);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 v = ls[c * 8 + e / 4];
+                            float y[4] = {ex2(fmaf(x[c & 1][e], p.c, v.x)), ex2(fmaf(x[c & 1][e + 1], p.c, v.y)),
+                                          ex2(fmaf(x[c & 1][e + 2], p.c, v.z)), ex2(fmaf(x[c & 1][e + 3], p.c, v.w))};
+                            if (!full) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const int32_t col = c * 32 + e + i;
+                                    if (col < c_lo || col >= c_hi) y[i] = 0.f;
+                                }
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) sum[i] += y[i];
+                        }
+                        if (c < 3) wait_ld();
+                    }
+                    acc += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(bar.s_empty(sb));
+                    buf ^= 1u;
+                }
+                n += uint32_t(w.steps);
+                // the groups' sums meet in the second group's second lse buffer
+                float* const other = lse_s + 384;
+                if (grp == 1) {
+                    group_sync(1);
+                    other[r] = acc;
+                    buf = 0;  // the other buffer goes on
+                    bar_arrive(bar.sums());
+                    if (!bar_wait(bar.summed(), seg & 1u, deadline)) ok = false;
+                } else {
+                    if (!bar_wait(bar.sums(), seg & 1u, deadline)) ok = false;
+                    acc += other[r];
+                    bar_arrive(bar.summed());
+                    const bool whole = w.j0 == 0 && w.steps == w.it.tiles;
+                    bool write = whole;
+                    if (!whole) {
+                        const int64_t c0 = cut_owner(w.U, w.G, w.item);
+                        const int64_t c1 = cut_owner(w.U, w.G, w.item + w.it.tiles - 1);
+                        auto piece = [&](int64_t c) {
+                            return sc.w_part + (2 * c + (c == c0 && cut_begin(w.U, w.G, c0) != w.item ? 1 : 0)) * 128;
+                        };
+                        sc.w_part[(2 * int64_t(blockIdx.x) + (w.u == w.u_begin ? 0 : 1)) * 128 + r] = acc;
+                        __threadfence();
+                        group_sync(0);
+                        uint32_t* last_s = reinterpret_cast<uint32_t*>(base + G::kBars + 8 * 24);
+                        if (r == 0) {
+                            const bool last = atomicAdd(p.count + c0, 1u) == uint32_t(c1 - c0);
+                            if (last) p.count[c0] = 0;
+                            *last_s = last;
+                        }
+                        group_sync(0);
+                        write = *last_s != 0;
+                        if (write) {
+                            __threadfence();
+                            acc = 0.f;
+                            for (int64_t c = c0; c <= c1; ++c) acc += __ldcg(piece(c) + r);
+                        }
+                        group_sync(0);  // last_s is free again
+                    }
+                    if (write && k < s.n) {
+                        const bool seen = (!p.window || int64_t(k) > int64_t(s.f) - int64_t(p.window)) ||
+                                          uint32_t(k) < p.sinks;
+                        if (seen) {
+                            float* wt = p.weights + int64_t(w.it.b) * p.w_ss + int64_t(w.h) * p.w_hs + k;
+                            *wt = (k >= s.f ? 0.f : *wt) + acc;
+                        }
+                    }
+                }
+            }
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        if (!ok && lane == 0 && p.err) atomicOr(p.err, uint32_t(LS_B200_ATTN_TIMEOUT));
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        fence_after();
+        dealloc<512>(tmem);
+    }
+}
+
+template <class T, int D>
+int launch_chunk_weights(const AttnParams& p, const ChunkScratch& s, uint32_t grid, const CUtensorMap& qm,
+                         const CUtensorMap& km, cudaStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return int(e);
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(chunk_weights_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 int(GeoW<D>::kSmem));
+        if (e != cudaSuccess) return int(e);
+        done.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    chunk_weights_kernel<T, D><<<grid, kThreads, GeoW<D>::kSmem, stream>>>(p, s, qm, km);
+    return int(cudaGetLastError());
+}
+
 using Encode = decltype(&cuTensorMapEncodeTiled);
 Encode encoder() {
     static const Encode fn = [] {
@@ -693,10 +982,12 @@ int launch(const AttnParams& p, bool bf16, const ChunkScratch& s, uint32_t grid,
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
     const uint32_t append = p.k_new ? p.B * ((p.max_q + 7) / 8) : 0;
-    chunk_prepare_kernel<<<1 + append, 256, 0, stream>>>(p, s, grid);
+    chunk_prepare_kernel<<<2 + append, 256, 0, stream>>>(p, s, grid);
     chunk_attn_kernel<T, D><<<grid, kThreads, Geo<D>::kSmem, stream>>>(p, s, qm, km, vm);
     chunk_join_kernel<T, D><<<dim3(grid, 8), 256, 0, stream>>>(p, s);
-    return int(cudaGetLastError());
+    e = cudaGetLastError();
+    if (e != cudaSuccess || !p.weights) return int(e);
+    return launch_chunk_weights<T, D>(p, s, grid, qm, km, stream);
 }
 
 }  // namespace
