@@ -212,8 +212,8 @@ SIGNATURES = {
     "ls_b200_batch_scratch_bytes": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint32]),
     "ls_b200_batch_mlp": (C.c_int, [C.POINTER(BatchArgs), C.c_void_p]),
     "ls_b200_attention_scratch_bytes": (C.c_uint64, [C.POINTER(AttentionArgs)]),
-    "ls_b200_paged_attention": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
-    "ls_b200_evict_cache": (C.c_int, [C.POINTER(EvictArgs), C.c_void_p]),
+    "ls_b200_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "ls_b200_evict_cache": (C.c_int, [C.c_void_p, C.c_void_p]),
     "ls_b200_stream_create": (C.c_void_p, [C.POINTER(StreamConfig)]),
     "ls_b200_stream_view": (C.c_int, [C.c_void_p, C.POINTER(IOBackend)]),
     "ls_b200_stream_stats": (C.c_int, [C.c_void_p, C.POINTER(StreamStats)]),

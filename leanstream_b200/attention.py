@@ -15,33 +15,46 @@ The caller owns every buffer until the stream has run; nothing synchronises.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
+
+import torch
 
 from . import _native as N
 from .backend import _check
 
+# The argument structures as one pack each: a call a decode step is worth the
+# few microseconds that filling ctypes fields one by one would take.
+_ATTENTION = struct.Struct("=12IfI11Q17qQQQQ")
+_EVICT = struct.Struct("=12I9Q10qQ")
+assert _ATTENTION.size == C.sizeof(N.AttentionArgs) and _EVICT.size == C.sizeof(N.EvictArgs)
 
-def _dtype_code(dtype) -> int:
-    name = str(dtype).replace("torch.", "")
-    if name not in ("float16", "bfloat16"):
-        raise ValueError(f"float16 or bfloat16, got {name}")
-    return N.FP16 if name == "float16" else N.BF16
+_INT, _FLOAT = torch.int32, torch.float32
+_CODES = {torch.float16: N.FP16, torch.bfloat16: N.BF16}
+
+
+def _element(dtype) -> torch.dtype:
+    got = dtype if isinstance(dtype, torch.dtype) else getattr(torch, str(dtype), None)
+    if got not in _CODES:
+        raise ValueError(f"float16 or bfloat16, got {dtype}")
+    return got
 
 
 def _handle(stream) -> int:
     if stream is None:
-        import torch
-
         stream = torch.cuda.current_stream()
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-def _want(name, t, dtype, shape):
-    """Shape and type of a tensor; -1 in `shape` takes any size."""
-    if str(t.dtype) != dtype or t.dim() != len(shape) or any(w not in (-1, s) for w, s in zip(shape, t.shape)):
+def _want(name, t, dtype, shape, contiguous=False):
+    """Refuses a tensor of another type or shape (-1 in `shape` takes any
+    size), with a strided last dimension, or that is not on the GPU."""
+    if t.dtype is not dtype or t.dim() != len(shape) or any(w not in (-1, s) for w, s in zip(shape, t.shape)):
         raise ValueError(f"{name}: {dtype} {list(shape)} expected, got {t.dtype} {list(t.shape)}")
-    if t.numel() and t.stride(-1) != 1:
-        raise ValueError(f"{name}: the last dimension has to be contiguous")
+    if t.numel() and (t.stride(-1) != 1 or (contiguous and not t.is_contiguous())):
+        raise ValueError(f"{name}: {'a contiguous tensor' if contiguous else 'a contiguous last dimension'} expected")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: a tensor on the GPU is expected")
 
 
 class PagedAttention:
@@ -58,11 +71,11 @@ class PagedAttention:
                  scratch: Optional[tuple] = None, error: Optional[int] = None):
         self.lib = N.load()
         self.q_heads, self.kv_heads, self.head_dim, self.page_size = q_heads, kv_heads, head_dim, page_size
-        self.dtype = _dtype_code(dtype)
-        self.element = "torch.float16" if self.dtype == N.FP16 else "torch.bfloat16"
+        self.dtype = _element(dtype)
         self.max_sequences, self.max_tokens = max_sequences, max_tokens
         self.max_queries, self.max_weights_length = max_queries, max_weights_length
-        shape = N.AttentionArgs(dtype=self.dtype, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim,
+        self._code, self._scale = _CODES[self.dtype], head_dim ** -0.5 if head_dim > 0 else 1.0
+        shape = N.AttentionArgs(dtype=self._code, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim,
                                 page_size=page_size, batch=max_sequences, tokens=max_tokens, max_q=max_queries,
                                 weights_length=max_weights_length, scale=1.0)
         self.scratch_bytes = int(self.lib.ls_b200_attention_scratch_bytes(C.byref(shape)))
@@ -76,72 +89,99 @@ class PagedAttention:
                 raise ValueError(f"scratch of {have} B, {self.scratch_bytes} B needed")
             self.error_ptr = int(error or 0)
         else:
-            import torch
-
             self._scratch = torch.zeros(self.scratch_bytes, dtype=torch.uint8, device=device or "cuda")
             self.scratch_ptr = self._scratch.data_ptr()
             self._error = torch.zeros(1, dtype=torch.int32, device=device or "cuda")
             self.error_ptr = self._error.data_ptr()
 
-    def args(self, *, q, output, k_pages, v_pages, page_table, q_start, kv_len, max_q: int, k_new=None, v_new=None,
-             scale: Optional[float] = None, window: int = 0, sinks: int = 0, lse=None, weights=None,
-             timeout_ns: int = 0) -> N.AttentionArgs:
-        """q, output [tokens][q_heads][head_dim]; k_new, v_new [tokens]
-        [kv_heads][head_dim], written to their slots first (without them the
-        cache holds the new tokens already); page_table [sequences][columns],
-        q_start [sequences + 1], kv_len [sequences] int32 on the device, kv_len
-        with the new tokens; max_q: the most new tokens of one sequence. scale:
-        1 / sqrt(head_dim) unless given. lse [tokens][q_heads] and weights
-        [sequences][kv_heads][slots] float32, optional."""
-        tokens, batch = q.shape[0] if q.dim() else 0, kv_len.shape[0] if kv_len.dim() else 0
-        hq, hk, dim = self.q_heads, self.kv_heads, self.head_dim
-        _want("q", q, self.element, (-1, hq, dim))
-        _want("output", output, self.element, (tokens, hq, dim))
-        _want("k_pages", k_pages, self.element, (-1, self.page_size, hk, dim))
-        _want("v_pages", v_pages, self.element, (k_pages.shape[0], self.page_size, hk, dim))
-        _want("kv_len", kv_len, "torch.int32", (-1,))
-        _want("page_table", page_table, "torch.int32", (batch, -1))
-        _want("q_start", q_start, "torch.int32", (batch + 1,))
+    def _refuse(self, q, output, k_pages, v_pages, page_table, q_start, kv_len, max_q, k_new, v_new, lse, weights,
+                window, sinks):
+        """Names what is wrong with the arguments of a call."""
+        hq, hk, dim, size, e = self.q_heads, self.kv_heads, self.head_dim, self.page_size, self.dtype
+        _want("q", q, e, (-1, hq, dim))
+        _want("output", output, e, (q.shape[0], hq, dim))
+        _want("k_pages", k_pages, e, (-1, size, hk, dim))
+        _want("v_pages", v_pages, e, (k_pages.shape[0], size, hk, dim))
+        _want("kv_len", kv_len, _INT, (-1,))
+        _want("page_table", page_table, _INT, (kv_len.shape[0], -1))
+        _want("q_start", q_start, _INT, (kv_len.shape[0] + 1,))
         if (k_new is None) != (v_new is None):
             raise ValueError("k_new and v_new come together")
         if k_new is not None:
-            _want("k_new", k_new, self.element, (tokens, hk, dim))
-            _want("v_new", v_new, self.element, (tokens, hk, dim))
+            _want("k_new", k_new, e, (q.shape[0], hk, dim))
+            _want("v_new", v_new, e, (q.shape[0], hk, dim))
         if lse is not None:
-            _want("lse", lse, "torch.float32", (tokens, hq))
-            if not lse.is_contiguous():
-                raise ValueError("lse has to be contiguous")
-        length = 0
+            _want("lse", lse, _FLOAT, (q.shape[0], hq), contiguous=True)
         if weights is not None:
-            _want("weights", weights, "torch.float32", (batch, hk, -1))
-            length = weights.shape[2]
-        if batch > self.max_sequences or tokens > self.max_tokens or max_q > self.max_queries or \
-                length > self.max_weights_length:
-            raise ValueError(f"{batch} sequences, {tokens} tokens, {max_q} of one sequence, weights of {length} slots: "
-                             f"sized for {self.max_sequences}, {self.max_tokens}, {self.max_queries}, "
-                             f"{self.max_weights_length}")
-        if window < 0 or sinks < 0:
-            raise ValueError("window and sinks are not negative")
-        for name, t in (("q", q), ("output", output), ("k_pages", k_pages), ("v_pages", v_pages),
-                        ("page_table", page_table), ("q_start", q_start), ("kv_len", kv_len), ("k_new", k_new),
-                        ("v_new", v_new), ("lse", lse), ("weights", weights)):
-            if t is not None and not t.is_cuda:
-                raise ValueError(f"{name}: a tensor on the GPU is expected")
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        two = lambda t: (t.stride(0), t.stride(1)) if t is not None else (0, 0)  # noqa: E731
-        return N.AttentionArgs(
-            self.dtype, hq, hk, dim, self.page_size, k_pages.shape[0], batch, tokens, max_q, page_table.shape[1],
-            window, sinks, dim ** -0.5 if scale is None else scale, length, ptr(q), ptr(k_new), ptr(v_new),
-            ptr(k_pages), ptr(v_pages), ptr(page_table), ptr(q_start), ptr(kv_len), ptr(output), ptr(lse),
-            ptr(weights), *two(q), *two(k_new), *two(v_new), *k_pages.stride()[:3], *v_pages.stride()[:3],
-            *two(output), page_table.stride(0), *two(weights), self.scratch_ptr, self.scratch_bytes, self.error_ptr,
-            int(timeout_ns))
+            _want("weights", weights, _FLOAT, (kv_len.shape[0], hk, -1))
+        raise ValueError(f"{kv_len.shape[0]} sequences, {q.shape[0]} tokens, {max_q} of one sequence, weights of "
+                         f"{0 if weights is None else weights.shape[2]} slots, window {window}, {sinks} first slots: "
+                         f"sized for {self.max_sequences}, {self.max_tokens}, {self.max_queries}, "
+                         f"{self.max_weights_length}, and none is negative")
 
-    def run(self, stream=None, **kw) -> None:
+    def run(self, stream=None, *, q, output, k_pages, v_pages, page_table, q_start, kv_len, max_q: int, k_new=None,
+            v_new=None, scale: Optional[float] = None, window: int = 0, sinks: int = 0, lse=None, weights=None,
+            timeout_ns: int = 0) -> None:
         """Enqueues one call on `stream` (a torch stream, a raw cudaStream_t as
-        int, or None for torch's current stream). Keyword arguments as `args`."""
-        a = self.args(**kw)
-        _check(self.lib.ls_b200_paged_attention(C.byref(a), _handle(stream)), "ls_b200_paged_attention")
+        int, or None for torch's current stream). q, output [tokens][q_heads]
+        [head_dim]; k_new, v_new [tokens][kv_heads][head_dim], written to their
+        slots by the call (without them the cache holds the new tokens
+        already); page_table [sequences][columns], q_start [sequences + 1],
+        kv_len [sequences] int32 on the device, kv_len with the new tokens;
+        max_q: the most new tokens of one sequence. scale: 1 / sqrt(head_dim)
+        unless given. lse [tokens][q_heads] and weights [sequences][kv_heads]
+        [slots] float32, optional."""
+        e, hq, hk, dim = self.dtype, self.q_heads, self.kv_heads, self.head_dim
+        tokens, batch, pages = len(q) if q.dim() else 0, len(kv_len) if kv_len.dim() else 0, len(k_pages)
+        pool, table_shape = (pages, self.page_size, hk, dim), page_table.shape
+        kn = vn = ls = ws = length = 0
+        kn0 = kn1 = vn0 = vn1 = ws0 = ws1 = 0
+        good = (q.dtype is e and output.dtype is e and k_pages.dtype is e and v_pages.dtype is e and
+                q.shape == (tokens, hq, dim) and output.shape == q.shape and k_pages.shape == pool and
+                v_pages.shape == pool and kv_len.dtype is _INT and page_table.dtype is _INT and
+                q_start.dtype is _INT and kv_len.dim() == 1 and len(table_shape) == 2 and
+                table_shape[0] == batch and q_start.shape == (batch + 1,) and q.is_cuda and output.is_cuda and
+                k_pages.is_cuda and v_pages.is_cuda and page_table.is_cuda and q_start.is_cuda and kv_len.is_cuda and
+                tokens <= self.max_tokens and batch <= self.max_sequences and max_q <= self.max_queries and
+                max_q >= 0 and window >= 0 and sinks >= 0 and (k_new is None) == (v_new is None))
+        if good and k_new is not None:
+            kn, vn = k_new.data_ptr(), v_new.data_ptr()
+            kn0, kn1, last = k_new.stride()
+            vn0, vn1, last2 = v_new.stride()
+            good = (k_new.dtype is e and v_new.dtype is e and k_new.shape == (tokens, hk, dim) and
+                    v_new.shape == (tokens, hk, dim) and k_new.is_cuda and v_new.is_cuda and
+                    (last == last2 == 1 or not tokens))
+        if good and lse is not None:
+            ls = lse.data_ptr()
+            good = lse.dtype is _FLOAT and lse.shape == (tokens, hq) and lse.is_contiguous() and lse.is_cuda
+        if good and weights is not None:
+            ws, shape = weights.data_ptr(), weights.shape
+            good = weights.dtype is _FLOAT and len(shape) == 3 and shape[0] == batch and shape[1] == hk and \
+                shape[2] <= self.max_weights_length and weights.is_cuda
+            if good:
+                length = shape[2]
+                ws0, ws1, last = weights.stride()
+                good = last == 1 or not weights.numel()
+        if good:
+            q0, q1, a = q.stride()
+            o0, o1, b = output.stride()
+            k0, k1, k2, c = k_pages.stride()
+            v0, v1, v2, d = v_pages.stride()
+            t0, f = page_table.stride()
+            good = (a == b == 1 or not tokens) and (c == d == 1 or not pages) and \
+                (f == 1 or not page_table.numel()) and kv_len.is_contiguous() and q_start.is_contiguous()
+        if not good:
+            self._refuse(q, output, k_pages, v_pages, page_table, q_start, kv_len, max_q, k_new, v_new, lse, weights,
+                         window, sinks)
+        a = _ATTENTION.pack(
+            self._code, hq, hk, dim, self.page_size, pages, batch, tokens, max_q, table_shape[1], window, sinks,
+            self._scale if scale is None else scale, length, q.data_ptr(), kn, vn, k_pages.data_ptr(),
+            v_pages.data_ptr(), page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), output.data_ptr(), ls, ws,
+            q0, q1, kn0, kn1, vn0, vn1, k0, k1, k2, v0, v1, v2, o0, o1, t0, ws0, ws1, self.scratch_ptr,
+            self.scratch_bytes, self.error_ptr, timeout_ns)
+        rc = self.lib.ls_b200_paged_attention(a, _handle(stream))
+        if rc:
+            _check(rc, "ls_b200_paged_attention")
 
     def error(self) -> int:
         """The sticky N.ATTN_* bits of the calls so far; reads a device word."""
@@ -158,6 +198,25 @@ class PagedAttention:
         self._scratch.zero_()
 
 
+def _refuse_evict(k_pages, v_pages, page_table, kv_len, weights, budget, new_table, new_len, kept, sinks, recent,
+                  new_weights, error):
+    e = _element(k_pages.dtype)
+    _want("k_pages", k_pages, e, (-1, -1, -1, -1))
+    _want("v_pages", v_pages, e, tuple(k_pages.shape))
+    _want("kv_len", kv_len, _INT, (-1,))
+    batch, hk = kv_len.shape[0], k_pages.shape[2]
+    _want("page_table", page_table, _INT, (batch, -1))
+    _want("new_table", new_table, _INT, (batch, -1))
+    _want("weights", weights, _FLOAT, (batch, hk, -1))
+    _want("new_len", new_len, _INT, (batch,), contiguous=True)
+    _want("kept", kept, _INT, (batch, hk, budget), contiguous=True)
+    if new_weights is not None:
+        _want("new_weights", new_weights, _FLOAT, (batch, hk, budget), contiguous=True)
+    if error is not None:
+        _want("error", error, _INT, (1,))
+    raise ValueError(f"a budget of {budget} slots does not hold {sinks} first and {recent} last ones")
+
+
 def evict_cache(*, k_pages, v_pages, page_table, kv_len, weights, budget: int, new_table, new_len, kept,
                 sinks: int = 0, recent: int = 0, new_weights=None, error=None, stream=None) -> None:
     """Keeps `budget` slots of each sequence and kv head by their weights
@@ -166,35 +225,42 @@ def evict_cache(*, k_pages, v_pages, page_table, kv_len, weights, budget: int, n
     none of which may be a page of `page_table`; new_len [sequences], kept
     [sequences][kv_heads][budget] (each new slot's old one, -1 past new_len) and
     new_weights (the same shape, float32, optional) are written. error: an
-    optional int32 device tensor, N.ATTN_* bits are ORed in."""
-    batch, hk = kv_len.shape[0] if kv_len.dim() else 0, k_pages.shape[2] if k_pages.dim() == 4 else 0
-    element = str(k_pages.dtype)
-    _dtype_code(element)
-    _want("k_pages", k_pages, element, (-1, -1, -1, -1))
-    _want("v_pages", v_pages, element, tuple(k_pages.shape))
-    _want("kv_len", kv_len, "torch.int32", (-1,))
-    _want("page_table", page_table, "torch.int32", (batch, -1))
-    _want("new_table", new_table, "torch.int32", (batch, -1))
-    _want("weights", weights, "torch.float32", (batch, hk, -1))
-    _want("new_len", new_len, "torch.int32", (batch,))
-    _want("kept", kept, "torch.int32", (batch, hk, budget))
-    if new_weights is not None:
-        _want("new_weights", new_weights, "torch.float32", (batch, hk, budget))
-    if error is not None:
-        _want("error", error, "torch.int32", (1,))
-    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
-        raise ValueError(f"a budget of {budget} slots holds {sinks} first and {recent} last ones?")
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("new_table", new_table),
-                    ("kv_len", kv_len), ("weights", weights), ("new_len", new_len), ("kept", kept),
-                    ("new_weights", new_weights), ("error", error)):
-        if t is not None and not t.is_cuda:
-            raise ValueError(f"{name}: a tensor on the GPU is expected")
-    if not kept.is_contiguous() or (new_weights is not None and not new_weights.is_contiguous()):
-        raise ValueError("kept and new_weights have to be contiguous")
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    a = N.EvictArgs(hk, k_pages.shape[3], k_pages.shape[1], k_pages.shape[0], batch, page_table.shape[1],
-                    new_table.shape[1], weights.shape[2], budget, sinks, recent, 0, ptr(k_pages), ptr(v_pages),
-                    ptr(page_table), ptr(new_table), ptr(kv_len), ptr(weights), ptr(new_len), ptr(kept),
-                    ptr(new_weights), *k_pages.stride()[:3], *v_pages.stride()[:3], page_table.stride(0),
-                    new_table.stride(0), weights.stride(0), weights.stride(1), ptr(error))
-    _check(N.load().ls_b200_evict_cache(C.byref(a), _handle(stream)), "ls_b200_evict_cache")
+    optional int32 device tensor, N.ATTN_* bits are ORed in. `stream` as in
+    PagedAttention.run."""
+    pool, table, new, wide = k_pages.shape, page_table.shape, new_table.shape, weights.shape
+    batch = len(kv_len) if kv_len.dim() else 0
+    good = (len(pool) == 4 and len(table) == len(new) == 2 and len(wide) == 3 and k_pages.dtype in _CODES and
+            v_pages.dtype is k_pages.dtype and v_pages.shape == pool and kv_len.dim() == 1 and
+            kv_len.dtype is _INT and page_table.dtype is _INT and new_table.dtype is _INT and
+            weights.dtype is _FLOAT and new_len.dtype is _INT and kept.dtype is _INT and table[0] == batch and
+            new[0] == batch and wide[0] == batch and wide[1] == pool[2] and new_len.shape == (batch,) and
+            kept.shape == (batch, pool[2], budget) and budget >= 1 and sinks >= 0 and recent >= 0 and
+            sinks + recent <= budget and k_pages.is_cuda and v_pages.is_cuda and page_table.is_cuda and
+            new_table.is_cuda and kv_len.is_cuda and weights.is_cuda and new_len.is_cuda and kept.is_cuda and
+            kept.is_contiguous() and new_len.is_contiguous() and kv_len.is_contiguous())
+    nw = er = 0
+    if good and new_weights is not None:
+        nw = new_weights.data_ptr()
+        good = new_weights.dtype is _FLOAT and new_weights.shape == kept.shape and new_weights.is_contiguous() and \
+            new_weights.is_cuda
+    if good and error is not None:
+        er = error.data_ptr()
+        good = error.dtype is _INT and error.shape == (1,) and error.is_cuda
+    if good:
+        k0, k1, k2, a = k_pages.stride()
+        v0, v1, v2, b = v_pages.stride()
+        t0, c = page_table.stride()
+        n0, d = new_table.stride()
+        w0, w1, f = weights.stride()
+        good = (a == b == 1 or not k_pages.numel()) and (c == 1 or not page_table.numel()) and \
+            (d == 1 or not new_table.numel()) and (f == 1 or not weights.numel())
+    if not good:
+        _refuse_evict(k_pages, v_pages, page_table, kv_len, weights, budget, new_table, new_len, kept, sinks, recent,
+                      new_weights, error)
+    args = _EVICT.pack(pool[2], pool[3], pool[1], pool[0], batch, table[1], new[1], wide[2], budget, sinks, recent, 0,
+                       k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), new_table.data_ptr(),
+                       kv_len.data_ptr(), weights.data_ptr(), new_len.data_ptr(), kept.data_ptr(), nw, k0, k1, k2, v0,
+                       v1, v2, t0, n0, w0, w1, er)
+    rc = N.load().ls_b200_evict_cache(args, _handle(stream))
+    if rc:
+        _check(rc, "ls_b200_evict_cache")
