@@ -444,7 +444,7 @@ enum {
  * dimension is contiguous and which start on 16 bytes. */
 typedef struct ls_b200_attention_args {
     uint32_t dtype;                 /* LS_B200_FP16 / LS_B200_BF16: q, keys, values and output */
-    uint32_t q_heads, kv_heads;     /* q_heads a multiple of kv_heads: head i reads kv head i / group */
+    uint32_t q_heads, kv_heads;     /* head i reads kv head i / group; group = q_heads / kv_heads, whole, <= 128 */
     uint32_t head_dim;              /* 64 or 128 */
     uint32_t page_size;             /* slots of a page: 16, 32, 64, 128 or 256 */
     uint32_t pages;                 /* pages of the pool */

@@ -21,28 +21,55 @@
 #include <cmath>
 
 #include "ls_attention.h"
+#include "ls_tc.h"
 
 namespace lsb {
 namespace {
 
+using namespace tc;
+
 constexpr int kDecWarps = 4, kDecThreads = 32 * kDecWarps;
-constexpr int kDecKeys = 16;                     // keys of one warp's step
-constexpr int kDecTile = kDecKeys * kDecWarps;   // slots of one unit of work
-constexpr int kDecStages = 3;
-constexpr int kDecCtasPerSm = 2;
+constexpr int kDecKeys = 16;                    // slots of one warp's step
+constexpr int kDecTile = kDecKeys * kDecWarps;  // slots of one unit of work
+constexpr uint32_t kDecSegs = 12;               // pieces of items listed at a time
+constexpr int64_t kDecItemCost = 2;             // units that beginning and joining an item counts as
+constexpr int64_t kDecMinUnits = 2 + kDecItemCost;  // units that a CTA takes at least
+constexpr uint64_t kGraceNs = 1000000000ull;
 
-__host__ __device__ constexpr uint32_t dec_ring(int D) { return uint32_t(kDecWarps * kDecStages * kDecKeys * D * 2 * 2); }
-__host__ __device__ constexpr uint32_t dec_smem(int D, int MT) { return dec_ring(D) + uint32_t(16 * MT * D * 2) + 1024; }
+// One 16-row MMA tile of rows keeps its registers within three CTAs per SM,
+// two tiles within two; the ring takes the shared memory that leaves.
+template <int D, int MT>
+struct GeoD {
+    static constexpr int kCtas = MT == 1 ? 3 : 2, kRows = 16 * MT;
+    static constexpr uint32_t kHalf = kDecKeys * D * 2, kStage = 2 * kHalf;  // a step's keys, and its values
+    static constexpr int kStages = 2 * (128 / D);
+    static constexpr uint32_t kRing = kDecWarps * kStages * kStage;
+    static constexpr uint32_t kJoin = kRing, kJoinBytes = kRows * D * 4;  // sums of the warps; queries before
+    static constexpr uint32_t kSegs = kJoin + kJoinBytes, kBars = kSegs + kDecSegs * 64;
+    static constexpr uint32_t kStat = kBars + 8 * kDecWarps * kStages;  // scan words, flags; row maxima and sums
+    static constexpr uint32_t kSmem = kStat + 128 + 2 * kDecWarps * kRows * 4;
+    static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
+};
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
-// 16 bytes from global memory, or zeros where `on` is false (src is then not read)
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+// A piece of an item: `steps` tiles from tile j0 of a sequence and kv head.
+struct DecSeg {
+    int32_t b, h, q0, rows;
+    int32_t f, hi, lo, sink;  // as SeqRange, KeyRange
+    int32_t ns, first, j0, steps;
+    int32_t tiles, own;       // tiles of the item; own: it does not begin the CTA's range
+    int64_t item;             // first unit of the item
+    __device__ __forceinline__ int32_t slot0(int32_t step, uint32_t warp) const {
+        const int32_t j = j0 + step;
+        return (j < ns ? j : first + j - ns) * kDecTile + int32_t(warp) * kDecKeys;
+    }
+};
+static_assert(sizeof(DecSeg) == 64, "list entries");
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {  // zeros where off (src is not read)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void cp_arrive(uint32_t bar) {  // one arrival, when this thread's copies have landed
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -52,457 +79,561 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
-
-// Row r of a tile of D-element rows: 16-byte pieces XORed with the row's low
-// bits, so that the eight rows of an ldmatrix lie in different banks.
-template <int D>
+// 16-byte piece of a row in a tile of ROWS rows: panels of 64 elements, each
+// row's pieces XORed with its low bits (the 128-byte swizzle of the TMA), so
+// that the eight rows of an ldmatrix lie in different banks.
+template <int ROWS>
 __device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t piece) {
-    return row * (D * 2) + ((piece ^ (row & 7u)) << 4);
+    return (piece >> 3) * (ROWS * 128) + row * 128 + (((piece ^ row) & 7u) << 4);
 }
 
-// Units of work of one sequence: tiles of its row tiles, over the kv heads.
-template <int MR>
-__device__ int64_t seq_units(const AttnParams& p, const SeqRange& s) {
-    int64_t tiles = 0;
-    const int32_t rows = s.nq * int32_t(p.g);
-    for (int32_t r = 0; r < rows; r += MR)
-        tiles += key_range<kDecTile>(p, s, r / int32_t(p.g), (min(rows, r + MR) - 1) / int32_t(p.g) + 1).tiles;
-    return tiles * p.Hkv;
-}
-
-// Sum over the block, and the sum over the threads before this one.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& before) {
+// Sums of (x, y) over the block, and over the threads before this one.
+struct Pair {
+    int64_t x;
+    int32_t y;
+};
+__device__ __forceinline__ Pair block_scan(Pair v, Pair* sh, Pair& before) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t inc = v;
+    Pair inc = v;
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (int(lane) >= o) inc += x;
+        const int64_t x = __shfl_up_sync(0xffffffffu, inc.x, o);
+        const int32_t y = __shfl_up_sync(0xffffffffu, inc.y, o);
+        if (int(lane) >= o) inc.x += x, inc.y += y;
     }
     __syncthreads();
     if (lane == 31) sh[warp] = inc;
     __syncthreads();
-    int64_t total = 0;
-    before = inc - v;
+    Pair total{0, 0};
+    before = Pair{inc.x - v.x, inc.y - v.y};
     for (uint32_t w = 0; w < kDecWarps; ++w) {
-        if (w < warp) before += sh[w];
-        total += sh[w];
+        if (w < warp) before.x += sh[w].x, before.y += sh[w].y;
+        total.x += sh[w].x, total.y += sh[w].y;
     }
     return total;
 }
 
-// Writes one row's results: out = o / l and lse (base 2: m2 + log2 l).
-template <class T>
-__device__ __forceinline__ void store_pair(const AttnParams& p, int32_t token, uint32_t head, uint32_t d, float x,
-                                           float y) {
-    *reinterpret_cast<uint32_t*>(p.out + int64_t(token) * p.o_ts + int64_t(head) * p.o_hs + d) = T::pack(x, y);
-}
-
-// The kernel. Items are (sequence, tile of 16 * MT rows, kv head); rows are
-// (token, head of the group), so that all heads that share a key read it once.
-// Each item's slots are cut into units of 64; the units of all items, in
-// order, are cut evenly over the CTAs, so that long and short sequences fill
-// the GPU alike. A CTA's four warps take 16 slots of a unit each, with rings,
-// sums and maxima of their own (no barrier in the loop), and join at the end of
-// the item. An item cut over several CTAs is joined, in the order of its
-// pieces, by the CTA that arrives last.
+// The kernel for few rows per sequence and kv head (decoding, drafts): bound
+// by the read of the cache. An item is a sequence and kv head; its rows are
+// (token, head of the group), so all heads that share a key read it once. The
+// units (64 slots) of all items, in order, are cut evenly over the CTAs. A
+// CTA's four warps take 16 slots of a unit each, with rings, maxima and sums
+// of their own, and meet only at the end of a piece; the loads run on into the
+// next piece meanwhile. A step's keys and values are one TMA box each; steps
+// with new tokens or with slots that no row sees come by 16-byte copies
+// instead, row by row, with zeros for those. An item cut over several CTAs is
+// joined, in the order of its pieces, by the CTA that arrives last.
 template <class T, int D, int MT>
-__global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) attn_decode_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kDecThreads, GeoD<D, MT>::kCtas)
+    attn_decode_kernel(const AttnParams p, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap) {
+    using G = GeoD<D, MT>;
     constexpr int MR = 16 * MT, KS = D / 16, PIECES = D / 8, RPI = 32 / PIECES, ITERS = kDecKeys / RPI;
-    constexpr uint32_t kStage = kDecKeys * D * 2 * 2;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* ring = smem;
-    uint8_t* qs = smem + dec_ring(D);
-    int64_t* scan = reinterpret_cast<int64_t*>(qs + MR * D * 2);
-    int64_t* pick = scan + 8;
+    const uint32_t sbase = smem_u32(smem);
+    DecSeg* const segs = reinterpret_cast<DecSeg*>(smem + G::kSegs);
+    float* const join = reinterpret_cast<float*>(smem + G::kJoin);
+    Pair* const scan = reinterpret_cast<Pair*>(smem + G::kStat);
+    volatile uint32_t* const flag = reinterpret_cast<uint32_t*>(scan + kDecWarps);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t g = int32_t(p.g);
+    const uint32_t bar0 = sbase + G::kBars + 8 * warp * G::kStages;  // this warp's stages
+    const uint32_t ring = sbase + warp * (G::kStages * G::kStage);
 
-    // total units, and the sequence in which this CTA begins
-    int64_t U = 0;
-    for (uint32_t b0 = 0; b0 < p.B; b0 += kDecThreads) {
-        const uint32_t b = b0 + tid;
-        int64_t before;
-        U += block_scan(b < p.B ? seq_units<MR>(p, load_seq(p, b)) : 0, scan, before);
+    if (lane == 0) {
+        for (int i = 0; i < G::kStages; ++i) bar_init(bar0 + 8 * i, 32);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // units of this thread's sequence (of the first 128), and of the call; y: 1
+    // where the sequence has rows
+    auto units_of = [&](uint32_t b, SeqRange& s) -> Pair {
+        s = SeqRange{0, 0, 0, 0};
+        if (b < p.B) s = load_seq(p, b);
+        if (!s.nq) return Pair{0, 0};
+        return Pair{(key_range<kDecTile>(p, s, 0, s.nq).tiles + kDecItemCost) * p.Hkv, 1};
+    };
+    SeqRange seq0;
+    const Pair v0 = units_of(tid, seq0);
+    Pair before0;
+    const Pair total0 = block_scan(v0, scan, before0);
+    int64_t U = total0.x;
+    for (uint32_t b0 = kDecThreads; b0 < p.B; b0 += kDecThreads) {
+        SeqRange s;
+        Pair before;
+        U += block_scan(units_of(b0 + tid, s), scan, before).x;
     }
     if (!U) return;
-    const int64_t G = min(int64_t(gridDim.x), U);
-    if (int64_t(blockIdx.x) >= G) return;
-    const int64_t cta = blockIdx.x, u_end = cut_begin(U, G, cta + 1);
-    int64_t u = cut_begin(U, G, cta), seq_base = 0;
-    const int64_t u_begin = u;
-    uint32_t b = 0;
-    {
+    const int64_t NC = max(int64_t(1), min(int64_t(gridDim.x), (U + kDecMinUnits - 1) / kDecMinUnits));
+    if (int64_t(blockIdx.x) >= NC) return;
+    const int64_t cta = blockIdx.x, u_begin = cut_begin(U, NC, cta), u_end = cut_begin(U, NC, cta + 1);
+    const uint64_t deadline = now() + p.timeout_ns;
+    bool ok = true;
+    uint32_t used = 0, filled = 0;  // steps of this warp: computed, loaded
+
+    for (int64_t u = u_begin; u < u_end;) {
+        // the next pieces, listed by the threads of their sequences: items (y
+        // counts sequences with rows) from the one that holds unit u
+        if (tid == 0) flag[0] = flag[1] = 0;
+        __syncthreads();
         int64_t base = 0;
-        for (uint32_t b0 = 0; b0 < p.B; b0 += kDecThreads) {
-            const uint32_t bb = b0 + tid;
-            const int64_t v = bb < p.B ? seq_units<MR>(p, load_seq(p, bb)) : 0;
-            int64_t before;
-            const int64_t total = block_scan(v, scan, before);
-            if (u < base + total) {
-                if (u >= base + before && u < base + before + v) {
-                    pick[0] = bb;
-                    pick[1] = base + before;
+        int32_t seqs = 0;
+        for (uint32_t b0 = 0; b0 < p.B && base < u_end; b0 += kDecThreads) {
+            SeqRange s = seq0;
+            Pair v = v0, before = before0, total = total0;
+            if (b0) {
+                v = units_of(b0 + tid, s);
+                total = block_scan(v, scan, before);
+            }
+            const int64_t at = base + before.x, item_units = v.y ? v.x / p.Hkv : 1;
+            const int32_t seq = seqs + before.y;
+            if (v.y && u >= at && u < at + v.x) flag[1] = uint32_t(seq * int32_t(p.Hkv) + int32_t((u - at) / item_units));
+            __syncthreads();
+            const int64_t from = max(u, at), to = min(u_end, at + v.x);
+            if (from < to) {
+                const KeyRange kr = key_range<kDecTile>(p, s, 0, s.nq);
+                int32_t h = int32_t((from - at) / item_units);
+                int32_t idx = seq * int32_t(p.Hkv) + h - int32_t(flag[1]);
+                for (; h < int32_t(p.Hkv) && idx < int32_t(kDecSegs); ++h, ++idx) {
+                    DecSeg x;
+                    x.item = at + h * item_units + kDecItemCost;
+                    const int64_t a = max(x.item, u), e = min(x.item + kr.tiles, u_end);
+                    if (a >= e) break;  // only the item's cost lies in the range
+                    x.b = int32_t(b0 + tid), x.h = h, x.q0 = s.q0, x.rows = s.nq * g;
+                    x.f = s.f, x.hi = kr.hi, x.lo = kr.lo, x.sink = kr.sink, x.ns = kr.ns, x.first = kr.first;
+                    x.tiles = kr.tiles;
+                    x.j0 = int32_t(a - x.item), x.steps = int32_t(e - a);
+                    x.own = a != u_begin;
+                    segs[idx] = x;
+                    atomicMax(const_cast<uint32_t*>(flag), uint32_t(idx + 1));
+                }
+            }
+            base += total.x;
+            seqs += total.y;
+        }
+        __syncthreads();
+        const uint32_t count = flag[0];
+        if (!count) break;  // what is left of the range is the cost of an item
+
+        // Steps in blocks of 32, laid out by the lanes side by side: lane i holds
+        // step base + i, its first slot (a multiple of 16) with flags below.
+        constexpr int32_t kSeen = 1, kEdge = 2, kMasked = 4;
+        auto lay_out = [&](uint32_t c, int32_t step) -> int32_t {
+            if (c >= count) return 0;
+            const DecSeg& x = segs[c];
+            if (step >= x.steps) return 0;
+            const int32_t k0 = x.slot0(step, warp), k1 = k0 + kDecKeys;
+            if (!((k0 < x.hi && k1 > x.lo) || k0 < x.sink)) return 0;
+            // edge: new tokens, or slots that no row sees; masked: a row does not see all
+            const bool edge = (p.fused && k1 > x.f) || k1 > x.hi || (k0 < x.lo && k1 > x.sink);
+            const bool masked = k1 - 1 > x.f || (p.window && int64_t(k0) <= int64_t(x.hi) - 1 - int64_t(p.window));
+            return k0 | kSeen | (edge ? kEdge : 0) | (masked ? kMasked : 0);
+        };
+        // ---- loads of this warp, ahead of its computation: the block
+        // of piece l_seg, and the one after it, whose page indices are under way
+        uint32_t l_seg = 0, n_seg = 0;
+        int32_t n_base = 0;
+        auto after = [&](uint32_t& c, int32_t& b) {
+            b += 32;
+            if (c < count && b >= segs[c].steps) ++c, b = 0;
+        };
+        auto page_of = [&](uint32_t c, int32_t k) -> int32_t {
+            if (!(k & kSeen)) return 0;
+            const int32_t id = p.table[int64_t(segs[c].b) * p.table_s + (k >> p.pshift)];
+            if (uint32_t(id) < p.pages) return id;
+            if (p.err) atomicOr(p.err, kErrPage);
+            return int32_t(p.pages);
+        };
+        int32_t l_k = lay_out(0, int32_t(lane)), l_id = page_of(0, l_k), n_k, n_id;
+        after(n_seg, n_base);
+        n_k = lay_out(n_seg, n_base + int32_t(lane));
+        n_id = page_of(n_seg, n_k);
+        uint32_t l_todo = __ballot_sync(0xffffffffu, l_k & kSeen);  // steps of the block to load
+        auto load = [&]() {  // the next step that some row sees
+            while (!l_todo) {
+                l_seg = n_seg;
+                if (l_seg >= count) return;
+                l_k = n_k, l_id = n_id;
+                l_todo = __ballot_sync(0xffffffffu, l_k & kSeen);
+                after(n_seg, n_base);
+                n_k = lay_out(n_seg, n_base + int32_t(lane));
+                n_id = page_of(n_seg, n_k);
+            }
+            const int32_t i = __ffs(int(l_todo)) - 1;
+            l_todo &= l_todo - 1;
+            const int32_t kf = __shfl_sync(0xffffffffu, l_k, i), id = __shfl_sync(0xffffffffu, l_id, i);
+            const int32_t k0 = kf & ~15, in = k0 & int32_t(p.P - 1);
+            const uint32_t st = filled % G::kStages, dst = ring + st * G::kStage, bar = bar0 + 8 * st;
+            ++filled;
+            if (!(kf & kEdge)) {
+                if (lane == 0) {
+                    const int32_t h = segs[l_seg].h;
+                    bar_arrive_tx(bar, G::kStage);
+                    tma5(dst, &kmap, bar, 0, in, 0, h, id);
+                    tma5(dst + G::kHalf, &vmap, bar, 0, in, 0, h, id);
+                } else {
+                    bar_arrive(bar);
+                }
+                return;
+            }
+            const DecSeg& x = segs[l_seg];
+            const bool there = uint32_t(id) < p.pages;
+            const uint16_t* kb = p.k_pages + (there ? int64_t(id) * p.kp_ps : 0) + int64_t(x.h) * p.kp_hs;
+            const uint16_t* vb = p.v_pages + (there ? int64_t(id) * p.vp_ps : 0) + int64_t(x.h) * p.vp_hs;
+            const uint32_t piece = lane % PIECES;
+#pragma unroll 1
+            for (int i = 0; i < ITERS; ++i) {
+                const int32_t row = i * RPI + int32_t(lane / PIECES), key = k0 + row;
+                const bool fresh = p.fused && key >= x.f;
+                const bool on = ((key < x.hi && key >= x.lo) || key < x.sink) && (fresh || there);
+                const int64_t tok = int64_t(x.q0) + key - x.f;
+                const uint16_t* ks = !on ? p.k_pages
+                                     : fresh ? p.k_new + tok * p.kn_ts + int64_t(x.h) * p.kn_hs
+                                             : kb + int64_t(in + row) * p.kp_ss;
+                const uint16_t* vs = !on ? p.v_pages
+                                     : fresh ? p.v_new + tok * p.vn_ts + int64_t(x.h) * p.vn_hs
+                                             : vb + int64_t(in + row) * p.vp_ss;
+                cp16(dst + swz<kDecKeys>(row, piece), ks + piece * 8, on);
+                cp16(dst + G::kHalf + swz<kDecKeys>(row, piece), vs + piece * 8, on);
+            }
+            cp_arrive(bar);
+        };
+        uint32_t qf[MT == 1 ? KS : 1][4];
+        auto queries = [&](const DecSeg& x) {  // as A fragments; zero past the rows
+            const uint16_t* q[2];
+            bool on[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int32_t r = int32_t(lane >> 2) + 8 * i;
+                on[i] = r < x.rows;
+                q[i] = p.q + int64_t(x.q0 + (on[i] ? r / g : 0)) * p.q_ts +
+                       int64_t(x.h * g + (on[i] ? r % g : 0)) * p.q_hs + (lane & 3u) * 2;
+            }
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    qf[kk][i] = on[i & 1] ? *reinterpret_cast<const uint32_t*>(q[i & 1] + kk * 16 + (i >> 1) * 8) : 0u;
+        };
+        if constexpr (MT == 1) queries(segs[0]);  // ahead of the cache's stream
+#pragma unroll 1
+        for (int i = 0; i < G::kStages; ++i) load();
+
+        for (uint32_t c = 0; c < count; ++c) {
+            const DecSeg& x = segs[c];
+            const int32_t R = x.rows, steps = x.steps, h = x.h;
+            if constexpr (MT > 1) {
+                for (uint32_t i = tid; i < uint32_t(MR * PIECES); i += kDecThreads) {
+                    const uint32_t row = i / PIECES, piece = i % PIECES;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (int32_t(row) < R)
+                        v = *reinterpret_cast<const uint4*>(p.q + int64_t(x.q0 + int32_t(row) / g) * p.q_ts +
+                                                            int64_t(h * g + int32_t(row) % g) * p.q_hs + piece * 8);
+                    *reinterpret_cast<uint4*>(smem + G::kJoin + swz<MR>(row, piece)) = v;
                 }
                 __syncthreads();
-                b = uint32_t(pick[0]);
-                seq_base = pick[1];
-                break;
             }
-            base += total;
-        }
-    }
-    SeqRange s = load_seq(p, b);
-    int32_t r0 = 0, rows = s.nq * g;
-    int64_t tile_base = seq_base;  // first unit of row tile r0
-    KeyRange kr = key_range<kDecTile>(p, s, 0, (min(rows, MR) - 1) / g + 1);
-
-    while (u < u_end) {
-        // the item of unit u
-        while (u >= tile_base + int64_t(kr.tiles) * p.Hkv || r0 >= rows) {
-            if (r0 < rows) {
-                tile_base += int64_t(kr.tiles) * p.Hkv;
-                r0 += MR;
-            }
-            while (r0 >= rows) {  // u < U: a later sequence has rows
-                s = load_seq(p, ++b);
-                r0 = 0;
-                rows = s.nq * g;
-            }
-            kr = key_range<kDecTile>(p, s, r0 / g, (min(rows, r0 + MR) - 1) / g + 1);
-        }
-        const int32_t h = int32_t((u - tile_base) / kr.tiles);
-        const int64_t item = tile_base + int64_t(h) * kr.tiles;
-        const int32_t j0 = int32_t(u - item);
-        const int32_t steps = int32_t(min(u_end, item + kr.tiles) - u);
-        const int32_t R = min(MR, rows - r0);
-
-        // queries to shared memory, zero rows past R
-        __syncthreads();  // earlier item's shared memory is no longer read
-        for (uint32_t i = tid; i < uint32_t(MR * PIECES); i += kDecThreads) {
-            const uint32_t row = i / PIECES, piece = i % PIECES;
-            const int32_t rr = r0 + int32_t(row);
-            const bool on = int32_t(row) < R;
-            const int32_t t = on ? rr / g : 0, hh = on ? h * g + rr % g : 0;
-            cp16(smem_u32(qs) + swz<D>(row, piece), p.q + int64_t(s.q0 + t) * p.q_ts + int64_t(hh) * p.q_hs + piece * 8,
-                 on);
-        }
-        cp_commit();
-
-        int32_t pos[MT][2];  // slot of the token of this lane's rows (-1: no row)
+            int32_t pos[MT][2];  // slot of the token of this lane's rows (-1: no row)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int32_t row = mt * 16 + int32_t(lane >> 2) + 8 * i;
-                pos[mt][i] = row < R ? s.f + (r0 + row) / g : -1;
-            }
-        const int32_t pos_lo = s.f + r0 / g, pos_hi = s.f + (r0 + R - 1) / g;
-
-        // page indices: lane i holds the page of step base + i
-        const int32_t* trow = p.table + int64_t(b) * p.table_s;
-        auto page_of = [&](int32_t step) -> int32_t {
-            if (step >= steps) return 0;
-            const int32_t k0 = tile_at(kr, j0 + step) * kDecTile + int32_t(warp) * kDecKeys;
-            if (!((k0 < kr.hi && k0 + kDecKeys > kr.lo) || k0 < kr.sink)) return 0;
-            const int32_t id = trow[k0 >> p.pshift];
-            if (uint32_t(id) >= p.pages) {
-                if (p.err) atomicOr(p.err, kErrPage);
-                return -1;
-            }
-            return id;
-        };
-        int32_t ids = page_of(int32_t(lane)), ids_next = page_of(int32_t(lane) + 32);
-        const uint32_t wring = smem_u32(ring) + warp * (kDecStages * kStage);
-        const uint32_t my_piece = lane % PIECES, my_row = lane / PIECES;
-        int32_t id_base = 0;
-        auto id_at = [&](int32_t step) -> int32_t {
-            if (step >= id_base + 32) {
-                id_base += 32;
-                ids = ids_next;
-                ids_next = page_of(id_base + 32 + int32_t(lane));
-            }
-            return __shfl_sync(0xffffffffu, ids, step - id_base);
-        };
-        auto load = [&](int32_t step) {
-            if (step < steps) {
-                const int32_t id = id_at(step);
-                const int32_t k0 = tile_at(kr, j0 + step) * kDecTile + int32_t(warp) * kDecKeys;
-                const uint32_t dst = wring + uint32_t(step % kDecStages) * kStage;
-                const int64_t off = int64_t(k0 & int32_t(p.P - 1));
-                const uint16_t* kb = p.k_pages + int64_t(max(id, 0)) * p.kp_ps + off * p.kp_ss + int64_t(h) * p.kp_hs;
-                const uint16_t* vb = p.v_pages + int64_t(max(id, 0)) * p.vp_ps + off * p.vp_ss + int64_t(h) * p.vp_hs;
-#pragma unroll
-                for (int i = 0; i < ITERS; ++i) {
-                    const int32_t row = i * RPI + int32_t(my_row), key = k0 + row;
-                    const bool fresh = p.fused && key >= s.f;
-                    const bool on = ((key < kr.hi && key >= kr.lo) || key < kr.sink) && (fresh || id >= 0);
-                    const int64_t tok = int64_t(s.q0) + key - s.f;
-                    const uint16_t* ks = fresh && on ? p.k_new + tok * p.kn_ts + int64_t(h) * p.kn_hs
-                                                     : on ? kb + row * p.kp_ss : p.k_pages;
-                    const uint16_t* vs = fresh && on ? p.v_new + tok * p.vn_ts + int64_t(h) * p.vn_hs
-                                                     : on ? vb + row * p.vp_ss : p.v_pages;
-                    cp16(dst + swz<D>(row, my_piece), ks + my_piece * 8, on);
-                    cp16(dst + kDecKeys * D * 2 + swz<D>(row, my_piece), vs + my_piece * 8, on);
-                }
-            }
-            cp_commit();
-        };
-#pragma unroll
-        for (int i = 0; i < kDecStages - 1; ++i) load(i);
-        cp_wait<kDecStages - 1>();
-        __syncthreads();  // queries in shared memory
-
-        float o[MT][2 * KS][4], m[MT][2], l[MT][2];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int n = 0; n < 2 * KS; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
-            m[mt][0] = m[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.f;
-        }
-
-        for (int32_t step = 0; step < steps; ++step) {
-            cp_wait<kDecStages - 2>();
-            __syncwarp();
-            const int32_t k0 = tile_at(kr, j0 + step) * kDecTile + int32_t(warp) * kDecKeys;
-            const uint32_t ks = wring + uint32_t(step % kDecStages) * kStage, vs = ks + kDecKeys * D * 2;
-            // S = Q K^T
-            float sc[MT][2][4] = {};
-#pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                uint32_t bf[4];
-                ldsm4(bf, ks + swz<D>((lane & 7u) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1u)));
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    uint32_t af[4];
-                    ldsm4(af, smem_u32(qs) + swz<D>(mt * 16 + (lane & 15u), kk * 2 + (lane >> 4)));
-                    T::mma(sc[mt][0], af, bf[0], bf[1]);
-                    T::mma(sc[mt][1], af, bf[2], bf[3]);
-                }
-            }
-            const bool full = k0 + kDecKeys - 1 <= pos_lo && R == MR &&
-                              (!p.window || int64_t(k0) > int64_t(pos_hi) - int64_t(p.window));
-            if (!full) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!sees(p, pos[mt][e >> 1], k0 + nt * 8 + int32_t(lane & 3u) * 2 + (e & 1)))
-                                sc[mt][nt][e] = -INFINITY;
-            }
-            if (p.logits) {
-                float* lg = p.logits + ((int64_t(b) * p.Hkv + h) * p.wlen) * p.rows;
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int32_t row = mt * 16 + int32_t(lane >> 2) + 8 * (e >> 1);
-                            const int32_t key = k0 + nt * 8 + int32_t(lane & 3u) * 2 + (e & 1);
-                            if (row < R && key < kr.hi) lg[int64_t(key) * p.rows + r0 + row] = sc[mt][nt][e] * p.c;
-                        }
-            }
-            // running maximum, probabilities and sums
-            uint32_t ph[MT][4], pl[MT][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                float nm[2], base[2], al[2];
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float x = fmaxf(fmaxf(sc[mt][0][2 * i], sc[mt][0][2 * i + 1]),
-                                    fmaxf(sc[mt][1][2 * i], sc[mt][1][2 * i + 1]));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                    nm[i] = fmaxf(m[mt][i], x);
-                    base[i] = nm[i] == -INFINITY ? 0.f : nm[i] * p.c;
-                    al[i] = ex2(m[mt][i] * p.c - base[i]);
+                    const int32_t row = mt * 16 + int32_t(lane >> 2) + 8 * i;
+                    pos[mt][i] = row < R ? max(x.f + row / g, -1) : -1;
                 }
-                if (__any_sync(0xffffffffu, nm[0] > m[mt][0] || nm[1] > m[mt][1])) {
+            float o[MT][2 * KS][4], m[MT][2], l[MT][2];
 #pragma unroll
-                    for (int n = 0; n < 2 * KS; ++n)
+            for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[mt][n][e] *= al[e >> 1];
-                    l[mt][0] *= al[0];
-                    l[mt][1] *= al[1];
-                    m[mt][0] = nm[0];
-                    m[mt][1] = nm[1];
-                }
+                for (int n = 0; n < 2 * KS; ++n)
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float a = ex2(fmaf(sc[mt][nt][2 * i], p.c, -base[i]));
-                        const float c = ex2(fmaf(sc[mt][nt][2 * i + 1], p.c, -base[i]));
-                        l[mt][i] += a + c;
-                        // A fragment: registers (row, row + 8) x (keys 0-7, 8-15)
-                        ph[mt][nt * 2 + i] = T::pack(a, c);
-                        float ha, hc;
-                        T::unpack(ph[mt][nt * 2 + i], ha, hc);
-                        pl[mt][nt * 2 + i] = T::pack(a - ha, c - hc);
-                    }
+                    for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+                m[mt][0] = m[mt][1] = -INFINITY;
+                l[mt][0] = l[mt][1] = 0.f;
             }
-            // O += P V. P enters as its 16-bit rounding plus the 16-bit rounding
-            // of what that leaves: the tensor cores are far from busy here, and
-            // the sum keeps about twice the bits.
+
+            for (int32_t block = 0; block < steps; block += 32) {
+              const int32_t c_k = lay_out(c, block + int32_t(lane));
+              for (uint32_t todo = __ballot_sync(0xffffffffu, c_k & kSeen); todo; todo &= todo - 1) {
+                const int32_t kf = __shfl_sync(0xffffffffu, c_k, __ffs(int(todo)) - 1), k0 = kf & ~15;
+                const uint32_t st = used % G::kStages, ks = ring + st * G::kStage, vs = ks + G::kHalf;
+                if (!warp_wait(bar0 + 8 * st, (used / G::kStages) & 1u, deadline)) ok = false;
+                ++used;
+                // S = Q K^T
+                float sc[MT][2][4] = {};
 #pragma unroll
-            for (int n = 0; n < KS; ++n) {
-                uint32_t vf[4];
-                ldsm4t(vf, vs + swz<D>((lane & 7u) + (((lane >> 3) & 1u) << 3), n * 2 + (lane >> 4)));
+                for (int kk = 0; kk < KS; ++kk) {
+                    uint32_t bf[4];
+                    ldsm4(bf, ks + swz<kDecKeys>((lane & 7u) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1u)));
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    T::mma(o[mt][2 * n], ph[mt], vf[0], vf[1]);
-                    T::mma(o[mt][2 * n + 1], ph[mt], vf[2], vf[3]);
-                    T::mma(o[mt][2 * n], pl[mt], vf[0], vf[1]);
-                    T::mma(o[mt][2 * n + 1], pl[mt], vf[2], vf[3]);
-                }
-            }
-            // the new tokens' keys and values go to their slots
-            if (p.fused && k0 + kDecKeys > s.f && k0 < s.n) {
-                const int32_t id = trow[k0 >> p.pshift];
-                if (uint32_t(id) < p.pages) {
-#pragma unroll
-                    for (int i = 0; i < ITERS; ++i) {
-                        const int32_t row = i * RPI + int32_t(my_row), key = k0 + row;
-                        if (key >= s.f && key < s.n) {
-                            const int64_t at = key & int32_t(p.P - 1);
-                            const uint32_t o16 = swz<D>(row, my_piece);
-                            const uint8_t* kk = ring + (ks - smem_u32(ring)) + o16;
-                            const uint8_t* vv = ring + (vs - smem_u32(ring)) + o16;
-                            *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + at * p.kp_ss +
-                                                      int64_t(h) * p.kp_hs + my_piece * 8) =
-                                *reinterpret_cast<const uint4*>(kk);
-                            *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + at * p.vp_ss +
-                                                      int64_t(h) * p.vp_hs + my_piece * 8) =
-                                *reinterpret_cast<const uint4*>(vv);
+                    for (int mt = 0; mt < MT; ++mt) {
+                        if constexpr (MT == 1) {
+                            T::mma(sc[mt][0], qf[kk], bf[0], bf[1]);
+                            T::mma(sc[mt][1], qf[kk], bf[2], bf[3]);
+                        } else {
+                            uint32_t af[4];
+                            ldsm4(af, sbase + G::kJoin + swz<MR>(mt * 16 + (lane & 15u), kk * 2 + (lane >> 4)));
+                            T::mma(sc[mt][0], af, bf[0], bf[1]);
+                            T::mma(sc[mt][1], af, bf[2], bf[3]);
                         }
                     }
                 }
-            }
-            __syncwarp();
-            load(step + kDecStages - 1);
-        }
-        cp_wait<0>();
-        __syncthreads();
-
-        // join the warps through the ring's shared memory
-        float* so = reinterpret_cast<float*>(ring);  // [4][MR][D]
-        float* sm = so + kDecWarps * MR * D;          // [4][MR] maxima, base 2
-        float* sl = sm + kDecWarps * MR;              // [4][MR] sums
-        static_assert(kDecWarps * MR * (D + 2) * 4 <= int(dec_ring(D)), "the join fits the ring");
+                if (kf & kMasked) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float x = l[mt][i];
-                x += __shfl_xor_sync(0xffffffffu, x, 1);
-                x += __shfl_xor_sync(0xffffffffu, x, 2);
-                const uint32_t row = mt * 16 + (lane >> 2) + 8 * i;
-                if ((lane & 3u) == 0) {
-                    sm[warp * MR + row] = m[mt][i] * p.c;
-                    sl[warp * MR + row] = x;
+                        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (!sees(p, pos[mt][e >> 1], k0 + nt * 8 + int32_t(lane & 3u) * 2 + (e & 1)))
+                                    sc[mt][nt][e] = -INFINITY;
                 }
+                if (p.logits) {
+                    float* lg = p.logits + ((int64_t(x.b) * p.Hkv + h) * p.wlen) * p.rows;
 #pragma unroll
-                for (int n = 0; n < 2 * KS; ++n)
-                    *reinterpret_cast<float2*>(so + (warp * MR + row) * D + n * 8 + (lane & 3u) * 2) =
-                        make_float2(o[mt][n][2 * i], o[mt][n][2 * i + 1]);
-            }
-        __syncthreads();
-        const bool whole = j0 == 0 && steps == kr.tiles;
-        float* slot = p.part + (2 * cta + (u == u_begin ? 0 : 1)) * int64_t(MR * (D + 2));
-        for (uint32_t i = tid; i < uint32_t(R * (D / 2)); i += kDecThreads) {
-            const uint32_t row = i / (D / 2), d = (i % (D / 2)) * 2;
-            float mx = -INFINITY;
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, sm[w * MR + row]);
-            float x = 0.f, y = 0.f, sum = 0.f;
+                        for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-            for (int w = 0; w < kDecWarps; ++w) {
-                const float f = mx == -INFINITY ? 0.f : ex2(sm[w * MR + row] - mx);
-                const float2 v = *reinterpret_cast<const float2*>(so + (w * MR + row) * D + d);
-                x = fmaf(f, v.x, x);
-                y = fmaf(f, v.y, y);
-                sum = fmaf(f, sl[w * MR + row], sum);
-            }
-            if (whole) {
-                const int32_t rr = r0 + int32_t(row), token = s.q0 + rr / g;
-                const uint32_t head = uint32_t(h * g + rr % g);
-                const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
-                store_pair<T>(p, token, head, d, x * inv, y * inv);
-                if (d == 0 && p.lse)
-                    p.lse[int64_t(token) * p.Hq + head] = sum == 0.f ? -INFINITY : (mx + lg2(sum)) * kLn2;
-            } else {
-                *reinterpret_cast<float2*>(slot + row * D + d) = make_float2(x, y);
-                if (d == 0) {
-                    slot[MR * D + row] = mx;
-                    slot[MR * D + MR + row] = sum;
+                            for (int e = 0; e < 4; ++e) {
+                                const int32_t row = mt * 16 + int32_t(lane >> 2) + 8 * (e >> 1);
+                                const int32_t key = k0 + nt * 8 + int32_t(lane & 3u) * 2 + (e & 1);
+                                if (row < R && key < x.hi) lg[int64_t(key) * p.rows + row] = sc[mt][nt][e] * p.c;
+                            }
                 }
-            }
-        }
-        if (!whole) {
-            const int64_t c0 = cut_owner(U, G, item), c1 = cut_owner(U, G, item + kr.tiles - 1);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) pick[0] = atomicAdd(p.count + c0, 1u) == uint32_t(c1 - c0);
-            __syncthreads();
-            if (pick[0]) {
-                __threadfence();
-                if (tid == 0) p.count[c0] = 0;
-                auto piece = [&](int64_t c) {
-                    return p.part + (2 * c + (c == c0 && cut_begin(U, G, c0) != item ? 1 : 0)) * int64_t(MR * (D + 2));
-                };
-                for (uint32_t i = tid; i < uint32_t(R * (D / 2)); i += kDecThreads) {
-                    const uint32_t row = i / (D / 2), d = (i % (D / 2)) * 2;
-                    float mx = -INFINITY;
-                    for (int64_t c = c0; c <= c1; ++c) mx = fmaxf(mx, __ldcg(piece(c) + MR * D + row));
-                    float x = 0.f, y = 0.f, sum = 0.f;
-                    for (int64_t c = c0; c <= c1; ++c) {
-                        const float* ps = piece(c);
-                        const float f = mx == -INFINITY ? 0.f : ex2(__ldcg(ps + MR * D + row) - mx);
-                        const float2 v = __ldcg(reinterpret_cast<const float2*>(ps + row * D + d));
-                        x = fmaf(f, v.x, x);
-                        y = fmaf(f, v.y, y);
-                        sum = fmaf(f, __ldcg(ps + MR * D + MR + row), sum);
+                // running maximum, probabilities and sums
+                uint32_t ph[MT][4], pl[MT][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    float nm[2], bs[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float y = fmaxf(fmaxf(sc[mt][0][2 * i], sc[mt][0][2 * i + 1]),
+                                        fmaxf(sc[mt][1][2 * i], sc[mt][1][2 * i + 1]));
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+                        nm[i] = fmaxf(m[mt][i], y);
+                        bs[i] = nm[i] == -INFINITY ? 0.f : nm[i] * p.c;
                     }
-                    const int32_t rr = r0 + int32_t(row), token = s.q0 + rr / g;
-                    const uint32_t head = uint32_t(h * g + rr % g);
-                    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
-                    store_pair<T>(p, token, head, d, x * inv, y * inv);
-                    if (d == 0 && p.lse)
-                        p.lse[int64_t(token) * p.Hq + head] = sum == 0.f ? -INFINITY : (mx + lg2(sum)) * kLn2;
+                    if (__any_sync(0xffffffffu, nm[0] > m[mt][0] || nm[1] > m[mt][1])) {
+                        const float al[2] = {ex2(m[mt][0] * p.c - bs[0]), ex2(m[mt][1] * p.c - bs[1])};
+#pragma unroll
+                        for (int n = 0; n < 2 * KS; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[mt][n][e] *= al[e >> 1];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) l[mt][i] *= al[i], m[mt][i] = nm[i];
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float a = ex2(fmaf(sc[mt][nt][2 * i], p.c, -bs[i]));
+                            const float d = ex2(fmaf(sc[mt][nt][2 * i + 1], p.c, -bs[i]));
+                            l[mt][i] += a + d;
+                            // A fragment: registers (row, row + 8) x (keys 0-7, 8-15)
+                            ph[mt][nt * 2 + i] = T::pack(a, d);
+                            float ha, hd;
+                            T::unpack(ph[mt][nt * 2 + i], ha, hd);
+                            pl[mt][nt * 2 + i] = T::pack(a - ha, d - hd);
+                        }
+                }
+                // O += P V. P enters as its 16-bit rounding plus the 16-bit
+                // rounding of what that leaves: the tensor cores are far from
+                // busy here, and the sum keeps about twice the bits.
+#pragma unroll
+                for (int n = 0; n < KS; ++n) {
+                    uint32_t vf[4];
+                    ldsm4t(vf, vs + swz<kDecKeys>((lane & 7u) + (((lane >> 3) & 1u) << 3), n * 2 + (lane >> 4)));
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        T::mma(o[mt][2 * n], ph[mt], vf[0], vf[1]);
+                        T::mma(o[mt][2 * n + 1], ph[mt], vf[2], vf[3]);
+                        T::mma(o[mt][2 * n], pl[mt], vf[0], vf[1]);
+                        T::mma(o[mt][2 * n + 1], pl[mt], vf[2], vf[3]);
+                    }
+                }
+                // the new tokens' keys and values go to their slots
+                if (p.fused && (kf & kEdge) && k0 + kDecKeys > x.f) {
+                    const int32_t id = p.table[int64_t(x.b) * p.table_s + (k0 >> p.pshift)];
+                    const uint32_t piece = lane % PIECES;
+                    if (uint32_t(id) < p.pages) {
+#pragma unroll 2
+                        for (int i = 0; i < ITERS; ++i) {
+                            const int32_t row = i * RPI + int32_t(lane / PIECES), key = k0 + row;
+                            if (key >= x.f && key < x.hi) {
+                                const int64_t at = key & int32_t(p.P - 1);
+                                const uint8_t* kk = smem + (ks - sbase) + swz<kDecKeys>(row, piece);
+                                *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + at * p.kp_ss +
+                                                          int64_t(h) * p.kp_hs + piece * 8) =
+                                    *reinterpret_cast<const uint4*>(kk);
+                                *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + at * p.vp_ss +
+                                                          int64_t(h) * p.vp_hs + piece * 8) =
+                                    *reinterpret_cast<const uint4*>(kk + G::kHalf);
+                            }
+                        }
+                    }
+                }
+                // the stage's next contents come through the TMA's proxy: what the
+                // copies wrote is ordered before
+                if (kf & kEdge) proxy_fence();
+                __syncwarp();
+                load();
+              }
+            }
+
+            // The warps' sums meet: maxima first, then the rows, those of several
+            // warps at a time where they fit beside one another.
+            float* const sm = reinterpret_cast<float*>(smem + G::kStat) + 32;  // [4][MR]
+            float* const sl = sm + kDecWarps * MR;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float y = l[mt][i];
+                    y += __shfl_xor_sync(0xffffffffu, y, 1);
+                    y += __shfl_xor_sync(0xffffffffu, y, 2);
+                    if ((lane & 3u) == 0) {
+                        const uint32_t row = mt * 16 + (lane >> 2) + 8 * i;
+                        sm[warp * MR + row] = m[mt][i] * p.c;
+                        sl[warp * MR + row] = y;
+                    }
+                }
+            __syncthreads();  // (and the queries of MT 2 have been read)
+            const uint32_t side = R * 4 <= MR ? 4 : R * 2 <= MR ? 2 : 1;
+            for (uint32_t turn = 0; turn < kDecWarps / side; ++turn) {
+                if (warp / side == turn) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t row = mt * 16 + (lane >> 2) + 8 * i, at = warp % side * uint32_t(R) + row;
+                            if (int32_t(row) >= R) continue;
+                            float mx = sm[row];
+#pragma unroll
+                            for (int w = 1; w < kDecWarps; ++w) mx = fmaxf(mx, sm[w * MR + row]);
+                            const float f = mx == -INFINITY ? 0.f : ex2(m[mt][i] * p.c - mx);
+                            float* to = join + at * D + (lane & 3u) * 2;
+#pragma unroll
+                            for (int n = 0; n < 2 * KS; ++n) {
+                                float2* cell = reinterpret_cast<float2*>(to + ((n * 8) ^ (at & 7u) * 8));
+                                float2 v = make_float2(o[mt][n][2 * i] * f, o[mt][n][2 * i + 1] * f);
+                                if (turn) v.x += cell->x, v.y += cell->y;
+                                *cell = v;
+                            }
+                        }
+                }
+                __syncthreads();
+            }
+            if constexpr (MT == 1)
+                if (c + 1 < count) queries(segs[c + 1]);
+            // rows by warps, D / 32 elements of a row per lane
+            constexpr int E = D / 32;
+            const bool whole = x.j0 == 0 && steps == x.tiles;
+            constexpr int64_t kPart = MR * (D + 2);
+            float* const slot = p.part + (2 * cta + x.own) * kPart;
+            auto finish = [&](int32_t row, const float (&v)[E], float mx, float sum) {
+                const int32_t token = x.q0 + row / g;
+                const int64_t head = h * g + row % g;
+                const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+                uint16_t* out = p.out + int64_t(token) * p.o_ts + head * p.o_hs + lane * E;
+                if constexpr (E == 4)
+                    *reinterpret_cast<uint2*>(out) =
+                        make_uint2(T::pack(v[0] * inv, v[1] * inv), T::pack(v[2] * inv, v[3] * inv));
+                else
+                    *reinterpret_cast<uint32_t*>(out) = T::pack(v[0] * inv, v[1] * inv);
+                if (lane == 0 && p.lse)
+                    p.lse[int64_t(token) * p.Hq + head] = sum == 0.f ? -INFINITY : (mx + lg2(sum)) * kLn2;
+            };
+            for (int32_t row = int32_t(warp); row < R; row += kDecWarps) {
+                float mx = sm[row], sum = 0.f, v[E];
+#pragma unroll
+                for (int w = 1; w < kDecWarps; ++w) mx = fmaxf(mx, sm[w * MR + row]);
+#pragma unroll
+                for (int w = 0; w < kDecWarps; ++w)
+                    sum = fmaf(mx == -INFINITY ? 0.f : ex2(sm[w * MR + row] - mx), sl[w * MR + row], sum);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = 0.f;
+                for (uint32_t w = 0; w < side; ++w) {
+                    const uint32_t at = w * uint32_t(R) + uint32_t(row);
+                    const float* from = join + at * D + ((lane * E) ^ (at & 7u) * 8);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[e] += from[e];
+                }
+                if (whole) {
+                    finish(row, v, mx, sum);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) slot[row * D + lane * E + e] = v[e];
+                    if (lane == 0) slot[MR * D + row] = mx, slot[MR * D + MR + row] = sum;
                 }
             }
+            if (!whole) {
+                const int64_t c0 = cut_owner(U, NC, x.item), c1 = cut_owner(U, NC, x.item + x.tiles - 1);
+                __threadfence();
+                __syncthreads();
+                if (tid == 0) {
+                    const bool last = atomicAdd(p.count + c0, 1u) == uint32_t(c1 - c0);
+                    if (last) p.count[c0] = 0;
+                    *flag = last;
+                }
+                __syncthreads();
+                if (*flag) {
+                    __threadfence();
+                    const int32_t pieces = int32_t(c1 - c0) + 1;
+                    const float* const p0 = p.part + (2 * c0 + (cut_begin(U, NC, c0) != x.item)) * kPart;
+                    auto piece = [&](int32_t i) { return i ? p.part + 2 * (c0 + i) * kPart : p0; };
+                    for (int32_t row = int32_t(warp); row < R; row += kDecWarps) {
+                        float mx = -INFINITY, sum = 0.f, v[E] = {};
+                        for (int32_t i0 = 0; i0 < pieces; i0 += 32) {
+                            const int32_t i = i0 + int32_t(lane), n = min(32, pieces - i0);
+                            const float pm = i < pieces ? __ldcg(piece(i) + MR * D + row) : -INFINITY;
+                            const float ps = i < pieces ? __ldcg(piece(i) + MR * D + MR + row) : 0.f;
+                            float f = 0.f;
+                            for (int32_t k0 = 0; k0 < n; k0 += 8) {
+                                float y[8][E];
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) {
+                                    const float* from = piece(min(i0 + k0 + k, pieces - 1)) + row * D + lane * E;
+                                    if constexpr (E == 4)
+                                        *reinterpret_cast<float4*>(y[k]) = __ldcg(reinterpret_cast<const float4*>(from));
+                                    else
+                                        *reinterpret_cast<float2*>(y[k]) = __ldcg(reinterpret_cast<const float2*>(from));
+                                }
+                                if (!k0) {  // the maximum may grow with each 32 pieces
+                                    float nm = pm;
+#pragma unroll
+                                    for (int d = 16; d; d >>= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, d));
+                                    nm = fmaxf(nm, mx);
+                                    const float ref = nm == -INFINITY ? 0.f : nm, old = ex2(mx - ref);
+                                    f = ex2(pm - ref);
+                                    sum = fmaf(f, ps, sum * old);
+#pragma unroll
+                                    for (int e = 0; e < E; ++e) v[e] *= old;
+                                    mx = nm;
+                                }
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) {
+                                    const float fk = __shfl_sync(0xffffffffu, f, (k0 + k) & 31);
+                                    if (k0 + k < n)
+#pragma unroll
+                                        for (int e = 0; e < E; ++e) v[e] = fmaf(fk, y[k][e], v[e]);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                        finish(row, v, mx, sum);
+                    }
+                }
+            }
+            __syncthreads();  // the joined sums and maxima have been read
         }
-        u += steps;
+        u = segs[count - 1].item + segs[count - 1].j0 + segs[count - 1].steps;
     }
-}
-
-// New keys and values to their slots, for calls whose rows need several tiles.
-__global__ void __launch_bounds__(256) attn_append_kernel(const AttnParams p) {
-    const SeqRange s = load_seq(p, blockIdx.x);
-    const uint32_t pieces = p.D / 8, per_token = p.Hkv * pieces;
-    const int32_t t_end = min(s.nq, int32_t(blockIdx.y + 1) * 16);
-    for (int32_t t = int32_t(blockIdx.y) * 16; t < t_end; ++t) {
-        const int32_t slot = s.f + t;
-        if (slot < 0) continue;
-        const int32_t id = p.table[int64_t(blockIdx.x) * p.table_s + (slot >> p.pshift)];
-        if (uint32_t(id) >= p.pages) {
-            if (p.err) atomicOr(p.err, kErrPage);
-            continue;
-        }
-        const int64_t at = slot & int32_t(p.P - 1), tok = s.q0 + t;
-        for (uint32_t i = threadIdx.x; i < per_token; i += blockDim.x) {
-            const int64_t h = i / pieces, e = (i % pieces) * 8;
-            *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + at * p.kp_ss + h * p.kp_hs + e) =
-                *reinterpret_cast<const uint4*>(p.k_new + tok * p.kn_ts + h * p.kn_hs + e);
-            *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + at * p.vp_ss + h * p.vp_hs + e) =
-                *reinterpret_cast<const uint4*>(p.v_new + tok * p.vn_ts + h * p.vn_hs + e);
-        }
-    }
+    // every load has landed before the CTA ends (they all have, unless a wait gave up)
+    for (uint32_t i = filled - min(filled, uint32_t(G::kStages)); i < filled; ++i)
+        warp_wait(bar0 + 8 * (i % G::kStages), (i / G::kStages) & 1u, deadline + kGraceNs);
+    if (!ok && lane == 0 && p.err) atomicOr(p.err, uint32_t(LS_B200_ATTN_TIMEOUT));
 }
 
 // weights[b, h, slot] from the stored logits, once the rows' lse are known.
@@ -552,12 +683,7 @@ uint32_t sm_count() {
     }
     return uint32_t(sms);
 }
-uint32_t dec_grid() {
-    const uint32_t g = sm_count() * kDecCtasPerSm;
-    return g < kMaxCtas ? g : kMaxCtas;
-}
-// rows that one item of the decode kernel takes (two 16-row MMA tiles hold
-// more rows per key read; one keeps twice the registers for latency)
+// 16-row MMA tiles that hold the rows of an item of the decode kernel
 uint32_t dec_mt(const ls_b200_attention_args& a) {
     return uint64_t(a.max_q) * (a.q_heads / a.kv_heads) <= 16 ? 1 : 2;
 }
@@ -567,7 +693,7 @@ uint32_t dec_mt(const ls_b200_attention_args& a) {
 constexpr uint64_t kChunkRows = 32;
 bool is_chunk(const ls_b200_attention_args& a) {
     const uint32_t g = a.q_heads / a.kv_heads;
-    return uint64_t(a.max_q) * g > kChunkRows && g <= 128;
+    return uint64_t(a.max_q) * g > kChunkRows;
 }
 
 struct ScratchPlan {
@@ -600,7 +726,7 @@ bool stride8(int64_t v) { return v % 8 == 0 && v >= 0; }
 
 // The call's shape: everything that does not depend on pointers.
 int check_shape(const ls_b200_attention_args& a) {
-    if (a.dtype > LS_B200_BF16 || !a.kv_heads || !a.q_heads || a.q_heads % a.kv_heads || a.q_heads > 65536 ||
+    if (a.dtype > LS_B200_BF16 || !a.kv_heads || !a.q_heads || a.q_heads % a.kv_heads || a.q_heads / a.kv_heads > 128 || a.q_heads > 65536 ||
         (a.head_dim != 64 && a.head_dim != 128))
         return EINVAL;
     if (a.page_size < 16 || a.page_size > 256 || (a.page_size & (a.page_size - 1))) return EINVAL;
@@ -613,7 +739,14 @@ int check_shape(const ls_b200_attention_args& a) {
 }
 
 template <class T, int D, int MT>
-int launch_decode(const AttnParams& p, cudaStream_t s) {
+int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
+    using G = GeoD<D, MT>;
+    CUtensorMap km, vm;
+    const uint64_t dims[5] = {64, p.P, D / 64, p.Hkv, p.pages};
+    const int64_t ks[4] = {p.kp_ss, 64, p.kp_hs, p.kp_ps}, vs[4] = {p.vp_ss, 64, p.vp_hs, p.vp_ps};
+    const uint32_t box[5] = {64, uint32_t(kDecKeys), D / 64, 1, 1};
+    if (!encode_map(&km, bf16, p.k_pages, 5, dims, ks, box) || !encode_map(&vm, bf16, p.v_pages, 5, dims, vs, box))
+        return EINVAL;
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -621,20 +754,21 @@ int launch_decode(const AttnParams& p, cudaStream_t s) {
     const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
     if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
         e = cudaFuncSetAttribute(attn_decode_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 int(dec_smem(D, MT)));
+                                 int(G::kSmem));
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(attn_decode_kernel<T, D, MT>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                      int(cudaSharedmemCarveoutMaxShared));
         if (e != cudaSuccess) return int(e);
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
-    attn_decode_kernel<T, D, MT><<<dec_grid(), kDecThreads, dec_smem(D, MT), s>>>(p);
+    const uint32_t grid = sm_count() * uint32_t(G::kCtas);
+    attn_decode_kernel<T, D, MT><<<grid < kMaxCtas ? grid : kMaxCtas, kDecThreads, G::kSmem, s>>>(p, km, vm);
     return int(cudaGetLastError());
 }
 template <class T>
-int launch_decode(const AttnParams& p, uint32_t mt, cudaStream_t s) {
-    if (p.D == 64) return mt == 1 ? launch_decode<T, 64, 1>(p, s) : launch_decode<T, 64, 2>(p, s);
-    return mt == 1 ? launch_decode<T, 128, 1>(p, s) : launch_decode<T, 128, 2>(p, s);
+int launch_decode(const AttnParams& p, bool bf16, uint32_t mt, cudaStream_t s) {
+    if (p.D == 64) return mt == 1 ? launch_decode<T, 64, 1>(p, bf16, s) : launch_decode<T, 64, 2>(p, bf16, s);
+    return mt == 1 ? launch_decode<T, 128, 1>(p, bf16, s) : launch_decode<T, 128, 2>(p, bf16, s);
 }
 
 }  // namespace
@@ -708,12 +842,9 @@ int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
         return launch_chunk(p, a->dtype, c, sm_count(), s);
     }
     const uint32_t mt = dec_mt(*a);
-    p.fused = p.k_new && p.rows <= 16 * mt;
-    if (p.k_new && !p.fused) {
-        attn_append_kernel<<<dim3(p.B, (p.max_q + 15) / 16), 256, 0, s>>>(p);
-        if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return int(e);
-    }
-    const int rc = a->dtype == LS_B200_FP16 ? launch_decode<F16>(p, mt, s) : launch_decode<BF16>(p, mt, s);
+    p.fused = p.k_new != nullptr;
+    const int rc =
+        a->dtype == LS_B200_FP16 ? launch_decode<F16>(p, false, mt, s) : launch_decode<BF16>(p, true, mt, s);
     if (rc || !p.weights) return rc;
     attn_weights_kernel<<<p.B * p.Hkv * ((p.wlen + 255) / 256), 256, 0, s>>>(p);
     return int(cudaGetLastError());

@@ -1,6 +1,7 @@
 // Internal types of the paged-cache attention (ls_attention.cu) and of the
 // cache eviction (ls_evict.cu). Not part of the public ABI.
 #pragma once
+#include <cuda.h>
 #include <stdint.h>
 #include <cuda_runtime.h>
 #include "../../include/leanstream_b200.h"
@@ -68,6 +69,10 @@ __host__ __device__ inline uint64_t chunk_weight_items(uint64_t batch, uint64_t 
     return batch * (wlen / kChunkKeys + 2);
 }
 inline uint64_t chunk_part_floats(uint32_t D) { return 256ull * (D + 2); }  // one partial result
+// A tensor map of 16-bit elements with 128-byte swizzle; strides in elements,
+// from the second dimension on. False when the driver refuses it.
+bool encode_map(CUtensorMap* map, bool bf16, const void* base, uint32_t rank, const uint64_t* dims,
+                const int64_t* strides, const uint32_t* box);
 int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream);
 
 // A sequence of the call: its new tokens are rows q0 .. q0 + nq - 1 of q and

@@ -931,44 +931,17 @@ int launch_chunk_weights(const AttnParams& p, const ChunkScratch& s, uint32_t gr
     return int(cudaGetLastError());
 }
 
-using Encode = decltype(&cuTensorMapEncodeTiled);
-Encode encoder() {
-    static const Encode fn = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult res;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &res) !=
-                cudaSuccess ||
-            res != cudaDriverEntryPointSuccess)
-            f = nullptr;
-        return reinterpret_cast<Encode>(f);
-    }();
-    return fn;
-}
-
-bool encode(CUtensorMap* map, bool bf16, const void* base, uint32_t rank, const cuuint64_t* dims, const int64_t* strides,
-            const cuuint32_t* box) {
-    cuuint64_t bytes[3];
-    const cuuint32_t ones[4] = {1, 1, 1, 1};
-    for (uint32_t i = 0; i + 1 < rank; ++i)  // the stride of a dimension of one is never used
-        bytes[i] = dims[i + 1] > 1 ? cuuint64_t(strides[i]) * 2 : cuuint64_t(dims[0]) * 2;
-    return encoder()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
-                     const_cast<void*>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <class T, int D>
 int launch(const AttnParams& p, bool bf16, const ChunkScratch& s, uint32_t grid, cudaStream_t stream) {
-    if (!encoder()) return ENOSYS;
     CUtensorMap qm, km, vm;
-    const cuuint64_t qd[3] = {D, p.Hq, p.tokens};
+    const uint64_t qd[3] = {D, p.Hq, p.tokens};
     const int64_t qs[2] = {p.q_hs, p.q_ts};
-    const cuuint32_t qb[3] = {64, p.g, chunk_tokens(p.g)};
-    const cuuint64_t kd[4] = {D, p.P, p.Hkv, p.pages};
+    const uint32_t qb[3] = {64, p.g, chunk_tokens(p.g)};
+    const uint64_t kd[4] = {D, p.P, p.Hkv, p.pages};
     const int64_t ks[3] = {p.kp_ss, p.kp_hs, p.kp_ps}, vs[3] = {p.vp_ss, p.vp_hs, p.vp_ps};
-    const cuuint32_t kb[4] = {64, p.P < 128 ? p.P : 128, 1, 1};
-    if (!encode(&qm, bf16, p.q, 3, qd, qs, qb) || !encode(&km, bf16, p.k_pages, 4, kd, ks, kb) ||
-        !encode(&vm, bf16, p.v_pages, 4, kd, vs, kb))
+    const uint32_t kb[4] = {64, p.P < 128 ? p.P : 128, 1, 1};
+    if (!encode_map(&qm, bf16, p.q, 3, qd, qs, qb) || !encode_map(&km, bf16, p.k_pages, 4, kd, ks, kb) ||
+        !encode_map(&vm, bf16, p.v_pages, 4, kd, vs, kb))
         return EINVAL;
     static std::atomic<uint64_t> done{0};
     int dev = 0;
@@ -990,7 +963,39 @@ int launch(const AttnParams& p, bool bf16, const ChunkScratch& s, uint32_t grid,
     return launch_chunk_weights<T, D>(p, s, grid, qm, km, stream);
 }
 
+using Encode = decltype(&cuTensorMapEncodeTiled);
+Encode encoder() {
+    static const Encode fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult res;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &res) !=
+                cudaSuccess ||
+            res != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<Encode>(f);
+    }();
+    return fn;
+}
+
 }  // namespace
+
+bool encode_map(CUtensorMap* map, bool bf16, const void* base, uint32_t rank, const uint64_t* dims,
+                const int64_t* strides, const uint32_t* box) {
+    cuuint64_t size[5], bytes[4];
+    cuuint32_t part[5];
+    const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+    for (uint32_t i = 0; i < rank; ++i) {
+        size[i] = dims[i];
+        part[i] = box[i];
+        if (i)  // the stride of a dimension of one is never used
+            bytes[i - 1] = dims[i] > 1 ? cuuint64_t(strides[i - 1]) * 2 : 128;
+    }
+    return encoder() &&
+           encoder()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                     const_cast<void*>(base), size, bytes, part, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream) {
     const uint32_t grid = sms < kMaxCtas ? sms : kMaxCtas;

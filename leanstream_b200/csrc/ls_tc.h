@@ -25,7 +25,7 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, uint64_t deadline) {
+static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, uint64_t deadline) {
     for (;;) {
         for (int i = 0; i < 16; ++i)
             if (bar_try(bar, parity)) return true;
@@ -56,6 +56,12 @@ __device__ __forceinline__ void tma4(uint32_t dst, const void* map, uint32_t bar
                                      int32_t w) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
                  "%4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+                 : "memory");
+}
+__device__ __forceinline__ void tma5(uint32_t dst, const void* map, uint32_t bar, int32_t x, int32_t y, int32_t z,
+                                     int32_t w, int32_t v) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+                 "%4, %5, %6, %7}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
                  : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const void* map) {
