@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, MT>::kCtas)
     const uint32_t bar0 = sbase + G::kBars + 8 * warp * G::kStages;  // this warp's stages
     const uint32_t ring = sbase + warp * (G::kStages * G::kStage);
 
+    after_start();
     if (lane == 0) {
         for (int i = 0; i < G::kStages; ++i) bar_init(bar0 + 8 * i, 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -642,6 +643,7 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, MT>::kCtas)
 __global__ void __launch_bounds__(256) attn_weights_kernel(const AttnParams p) {
     __shared__ float lse2[256];
     __shared__ int32_t pos[256];
+    after_wait();
     const uint32_t chunks = (p.wlen + 255) / 256;
     const uint32_t chunk = blockIdx.x % chunks, bh = blockIdx.x / chunks, h = bh % p.Hkv, b = bh / p.Hkv;
     const SeqRange s = load_seq(p, b);
@@ -846,8 +848,7 @@ int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
     const int rc =
         a->dtype == LS_B200_FP16 ? launch_decode<F16>(p, false, mt, s) : launch_decode<BF16>(p, true, mt, s);
     if (rc || !p.weights) return rc;
-    attn_weights_kernel<<<p.B * p.Hkv * ((p.wlen + 255) / 256), 256, 0, s>>>(p);
-    return int(cudaGetLastError());
+    return int(launch_after(attn_weights_kernel, p.B * p.Hkv * ((p.wlen + 255) / 256), 256, 0, s, p));
 }
 
 }  // extern "C"

@@ -3,14 +3,17 @@
 //
 // Rows are (token, head of the group): all query heads of a kv head stand in
 // one 128-row MMA tile, so a key read serves the whole group. One item is two
-// such tiles (Q0, Q1) of one kv head; its slots go by in tiles of 128. Per tile
-// of slots and row tile i
-//     S_i = Q_i K^T            M 128, N 128, K head_dim, into tensor memory
+// such tiles (Q0, Q1) of one kv head; its slots go by in tiles of 128, each
+// worked on in two halves of 64. Per half and row tile i
+//     S_i = Q_i K^T            M 128, N 64, K head_dim, into tensor memory
 //     P_i = exp2(S_i c - m c)  by one thread per row, back into S_i's columns
 //     O_i += P_i V             A from tensor memory, V read as it lies (N-major)
-// While the warps of one row tile work on their exponentials the tensor cores
-// run the other's products. Roles of the warps: 0-3 and 4-7 the rows of Q0 and
-// Q1, 8 issues the MMAs, 9 the TMA loads (Q by item; K and V tiles through
+// Each row tile has two S buffers of a half, so that the next S is there when
+// its warps end with one: they go from exponentials to exponentials, and the
+// tensor cores run beside them. (With one buffer of 128 slots per row tile the
+// warps waited for P V and the next S in turn: 882 us for a 4096-token chunk
+// over 16384 slots.) Roles of the warps: 0-3 and 4-7 the rows of Q0 and
+// Q1, 8 and 11 issue their MMAs, 9 the TMA loads (Q by item; K and V tiles through
 // one ring of 128-slot stages, one box per page and 64 elements), 10 lays out
 // the CTA's pieces of items for the others.
 //
@@ -38,7 +41,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kKeys = kChunkKeys;
+constexpr int kKeys = kChunkKeys, kHalf = kKeys / 2;
 constexpr int kThreads = 384;  // twelve warps, 168 registers per thread
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows of 64 elements
 constexpr uint64_t kGraceNs = 1000000000ull;
@@ -49,25 +52,25 @@ struct Geo {
     static constexpr uint32_t kPanels = D / 64, kTile = kPanels * kPanel;
     static constexpr uint32_t kStages = D == 128 ? 5 : 8;
     static constexpr uint32_t kRing = 2 * kTile, kBars = kRing + kStages * kTile;
-    static constexpr uint32_t kSegs = kBars + 288;
+    static constexpr uint32_t kSegs = kBars + 336;
     static constexpr uint32_t kSmem = kSegs + 256 + 1024;  // + alignment of the swizzled tiles
 };
 static_assert(Geo<128>::kSmem <= 227 * 1024 && Geo<64>::kSmem <= 227 * 1024, "shared memory of a CTA");
 
-// Barriers: ring full / empty, Q full / empty, S full, P ready, O full, the
-// last MMAs after a failure, pieces full / empty.
+// Barriers: ring full / empty, Q full / empty; S full, P ready and P V done by
+// row tile and buffer; the last MMAs after a failure, pieces full / empty.
 struct Bars {
     uint32_t base;
     __device__ uint32_t full(uint32_t s) const { return base + 8 * s; }
     __device__ uint32_t empty(uint32_t s) const { return base + 8 * (8 + s); }
     __device__ uint32_t q_full() const { return base + 8 * 16; }
     __device__ uint32_t q_empty() const { return base + 8 * 17; }
-    __device__ uint32_t s_full(uint32_t i) const { return base + 8 * (18 + i); }
-    __device__ uint32_t p_ready(uint32_t i) const { return base + 8 * (20 + i); }
-    __device__ uint32_t o_full(uint32_t i) const { return base + 8 * (22 + i); }
-    __device__ uint32_t drain() const { return base + 8 * 24; }
-    __device__ uint32_t seg_full(uint32_t s) const { return base + 8 * (25 + s); }
-    __device__ uint32_t seg_empty(uint32_t s) const { return base + 8 * (29 + s); }
+    __device__ uint32_t s_full(uint32_t i, uint32_t b) const { return base + 8 * (18 + 2 * i + b); }
+    __device__ uint32_t p_ready(uint32_t i, uint32_t b) const { return base + 8 * (22 + 2 * i + b); }
+    __device__ uint32_t o_done(uint32_t i, uint32_t b) const { return base + 8 * (26 + 2 * i + b); }
+    __device__ uint32_t drain(uint32_t i) const { return base + 8 * (30 + i); }
+    __device__ uint32_t seg_full(uint32_t s) const { return base + 8 * (32 + s); }
+    __device__ uint32_t seg_empty(uint32_t s) const { return base + 8 * (36 + s); }
 };
 
 // Lays out the items of a call in `plan` and `items`: for the attention
@@ -162,6 +165,7 @@ __device__ void lay_out(const AttnParams& p, ChunkPlan* plan, ChunkItem* list, i
 // Lays out the attention's items (block 0) and the weights' (block 1), and
 // appends the new keys and values (blocks 2 .., a warp per token).
 __global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, const ChunkScratch sc, uint32_t grid) {
+    after_start();
     if (blockIdx.x == 0) {
         lay_out<false>(p, sc.plan, sc.items, int32_t(chunk_items(p.tokens, p.B, p.g)), grid);
     } else if (blockIdx.x == 1) {
@@ -179,12 +183,24 @@ __global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, 
             return;
         }
         const int64_t in = slot & int32_t(p.P - 1), tok = s.q0 + t;
-        for (uint32_t i = lane; i < per_token; i += 32) {
-            const int64_t h = i / pieces, e = (i % pieces) * 8;
-            *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + in * p.kp_ss + h * p.kp_hs + e) =
-                *reinterpret_cast<const uint4*>(p.k_new + tok * p.kn_ts + h * p.kn_hs + e);
-            *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + in * p.vp_ss + h * p.vp_hs + e) =
-                *reinterpret_cast<const uint4*>(p.v_new + tok * p.vn_ts + h * p.vn_hs + e);
+        for (uint32_t i0 = lane; i0 < per_token; i0 += 128) {  // four pieces of each under way at a time
+            uint4 k[4], v[4];
+#pragma unroll
+            for (uint32_t x = 0; x < 4; ++x) {
+                const uint32_t i = i0 + 32 * x;
+                if (i >= per_token) break;
+                const int64_t h = i / pieces, e = (i % pieces) * 8;
+                k[x] = *reinterpret_cast<const uint4*>(p.k_new + tok * p.kn_ts + h * p.kn_hs + e);
+                v[x] = *reinterpret_cast<const uint4*>(p.v_new + tok * p.vn_ts + h * p.vn_hs + e);
+            }
+#pragma unroll
+            for (uint32_t x = 0; x < 4; ++x) {
+                const uint32_t i = i0 + 32 * x;
+                if (i >= per_token) break;
+                const int64_t h = i / pieces, e = (i % pieces) * 8;
+                *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + in * p.kp_ss + h * p.kp_hs + e) = k[x];
+                *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + in * p.vp_ss + h * p.vp_hs + e) = v[x];
+            }
         }
     }
 }
@@ -205,9 +221,14 @@ struct Seg {
         const int32_t j = j0 + step;
         return (j < ns ? j : first + j - ns) * kKeys;
     }
+    // halves of a tile with a slot that some row sees: bits 0 and 1
+    __device__ uint32_t halves(int32_t step) const {
+        const int32_t k0 = slot0(step), k1 = k0 + kHalf;
+        return uint32_t((k0 < hi && k1 > lo) || k0 < sink) | uint32_t((k1 < hi && k1 + kHalf > lo) || k1 < sink) << 1;
+    }
 };
 static_assert(sizeof(Seg) == 64, "four pieces fit");
-constexpr uint32_t kSegs = 4, kSegReaders = 10;
+constexpr uint32_t kSegs = 4, kSegReaders = 11;
 
 template <class T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -218,26 +239,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t* const base = raw + (smem - smem_u32(raw));
     const Bars bar{smem + G::kBars};
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(base + G::kBars + 8 * 33);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(base + G::kBars + 8 * 40);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t per_tile = int32_t(chunk_tokens(p.g));  // tokens of a row tile
 
     if (tid == 0) {
         for (uint32_t s = 0; s < G::kStages; ++s) {
             bar_init(bar.full(s), 1);
-            bar_init(bar.empty(s), 1);
+            bar_init(bar.empty(s), 2);  // the two MMA warps
         }
         bar_init(bar.q_full(), 1);
-        bar_init(bar.q_empty(), 1);
-        bar_init(bar.drain(), 1);
+        bar_init(bar.q_empty(), 2);
         for (uint32_t i = 0; i < 2; ++i) {
-            bar_init(bar.s_full(i), 1);
-            bar_init(bar.p_ready(i), 4);  // the four warps of the row tile
-            bar_init(bar.o_full(i), 1);
+            for (uint32_t b = 0; b < 2; ++b) {
+                bar_init(bar.s_full(i, b), 1);
+                bar_init(bar.p_ready(i, b), 4);  // the four warps of the row tile
+                bar_init(bar.o_done(i, b), 1);
+            }
+            bar_init(bar.drain(i), 1);
         }
         for (uint32_t i = 0; i < kSegs; ++i) {
             bar_init(bar.seg_full(i), 1);
-            bar_init(bar.seg_empty(i), kSegReaders);  // warps 0 .. 9
+            bar_init(bar.seg_empty(i), kSegReaders);  // all but warp 10
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -251,6 +274,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_slot;
+    after_start();
+    after_wait();
     const uint64_t deadline = now() + p.timeout_ns;
     constexpr uint32_t kS = 0, kO = 256;  // columns: S_0, S_1 (128 each), O_0, O_1 (D each)
     bool ok = true;
@@ -260,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t sg = 0;
     auto next = [&]() -> bool {
         if (!warp_wait(bar.seg_full(sg % kSegs), (sg / kSegs) & 1u, deadline)) return ok = false;
-        return segs[sg % kSegs].steps != 0;
+        return uniform(segs[sg % kSegs].steps) != 0;
     };
     auto release = [&]() {
         __syncwarp();
@@ -356,80 +381,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok) warp_wait(bar.empty(s), n & 1u, grace);
         }
         if (sg) warp_wait(bar.q_full(), (sg - 1) & 1u, grace);
-    } else if (warp == 8) {
-        // ---- MMAs: one thread issues, the warp moves through the pieces together
-        constexpr uint32_t kIs = instr(T::kUmmaFormat, 128, kKeys, false);
-        constexpr uint32_t kIo = instr(T::kUmmaFormat, 128, D, true);
-        uint32_t slot = 0, pr[2] = {0, 0};
-        auto score = [&](uint32_t i, uint32_t s) {
-#pragma unroll
-            for (uint32_t k = 0; k < D / 16; ++k) {
-                const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
-                mma_ss(tmem + kS + i * 128, desc128(smem + i * G::kTile + off, 16, 1024),
-                       desc128(smem + G::kRing + s * G::kTile + off, 16, 1024), kIs, k > 0);
-            }
-            commit(bar.s_full(i));
-        };
-        while (ok && next()) {
-            const int32_t steps = segs[sg % kSegs].steps;
-            const uint32_t two = segs[sg % kSegs].left > per_tile ? 2 : 1;
-            if (lane == 0) {
-                ok = bar_wait(bar.q_full(), sg & 1u, deadline) &&
-                     bar_wait(bar.full(slot % G::kStages), (slot / G::kStages) & 1u, deadline);
-                if (ok) {
-                    fence_after();
-                    for (uint32_t i = 0; i < two; ++i) score(i, slot % G::kStages);
-                    commit(bar.empty(slot % G::kStages));
-                    if (steps == 1) commit(bar.q_empty());
-                }
-                uint32_t at = slot + 1;
-                for (int32_t j = 0; j < steps && ok; ++j, at += 2) {
-                    const uint32_t vs = at % G::kStages, ks = (at + 1) % G::kStages;
-                    const bool more = j + 1 < steps;
-                    if (!bar_wait(bar.full(vs), (at / G::kStages) & 1u, deadline) ||
-                        (more && !bar_wait(bar.full(ks), ((at + 1) / G::kStages) & 1u, deadline))) {
-                        ok = false;
-                        break;
-                    }
-                    for (uint32_t i = 0; i < two; ++i) {
-                        if (!bar_wait(bar.p_ready(i), pr[i] & 1u, deadline)) {
-                            ok = false;
-                            break;
-                        }
-                        ++pr[i];
-                        fence_after();
-#pragma unroll
-                        for (uint32_t k = 0; k < kKeys / 16; ++k)
-                            mma_ts(tmem + kO + i * D, tmem + kS + i * 128 + k * 8,
-                                   desc128(smem + G::kRing + vs * G::kTile + k * 2048, kPanel, 1024), kIo,
-                                   j > 0 || k > 0);
-                        if (more) score(i, ks);
-                        else commit(bar.o_full(i));
-                    }
-                    if (!ok) break;
-                    commit(bar.empty(vs));
-                    if (more) {
-                        commit(bar.empty(ks));
-                        if (j + 2 == steps) commit(bar.q_empty());
-                    }
-                }
-            }
-            ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
-            slot += 2 * uint32_t(steps);
-            release();
-        }
-        if (!ok && lane == 0) {  // MMAs in flight end (bounded) before the tensor memory goes
-            commit(bar.drain());
-            bar_wait(bar.drain(), 0, now() + kGraceNs);
-        }
-        __syncwarp();
     } else if (warp < 8) {
         // ---- rows: thread r of row tile i
         const uint32_t i = warp >> 2;
         const uint32_t r = tid & 127u, quarter = (warp & 3u) << 21;  // lane 32 * (warp % 4) of tensor memory
         const uint32_t ts = tmem + quarter + kS + i * 128, to = tmem + quarter + kO + i * D;
         const int32_t lt = int32_t(r / p.g);
-        uint32_t ns = 0, no = 0, slot = 0;  // S tiles and O results seen, ring slots passed
+        uint32_t n = 0, slot = 0;  // halves and ring slots passed
         while (ok && next()) {
             const Seg& w = segs[sg % kSegs];
             const int32_t steps = w.steps, t_tile = int32_t(i) * per_tile;  // first token of the tile, in the item
@@ -442,50 +400,60 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool busy = __any_sync(0xffffffffu, real);
             const int32_t pos = real ? max(w.pos0 + t_tile + lt, -1) : -1;
             const int32_t pos_lo = w.pos0 + t_tile, pos_hi = w.pos0 + min(w.left, t_tile + per_tile) - 1;
+            const uint32_t n0 = n;
             float m = -INFINITY, l = 0.f;  // reference maximum and sum of the row
-            for (int32_t j = 0; j < steps; ++j, ++ns) {
-                const int32_t k0 = w.slot0(j);
-                if (!warp_wait(bar.s_full(i), ns & 1u, deadline)) {
+            for (int32_t half = 0; half < 2 * steps && ok; ++half) {
+                if (!(w.halves(half >> 1) >> (half & 1) & 1u)) continue;
+                const int32_t k0 = w.slot0(half >> 1) + (half & 1) * kHalf;
+                const uint32_t b = n & 1u, tb = ts + b * kHalf;
+                // (every phase of P V is waited for before the next can come: a parity
+                // tells only two apart)
+                if (!warp_wait(bar.s_full(i, b), (n >> 1) & 1u, deadline) ||
+                    (n - n0 > 1 && !warp_wait(bar.o_done(i, b), ((n >> 1) - 1) & 1u, deadline))) {
                     ok = false;
                     break;
                 }
-                if (i == 0 && !(k0 >= w.lo && k0 + kKeys <= w.hi) && k0 + kKeys > w.sink) {
-                    // slots that no row sees: their values may be anything, and 0 * NaN is not 0
-                    const uint32_t vslot = slot + 2 * uint32_t(j) + 1, vs = vslot % G::kStages;
-                    if (!warp_wait(bar.full(vs), (vslot / G::kStages) & 1u, deadline)) {
+                if (!(k0 >= w.lo && k0 + kHalf <= w.hi) && k0 + kHalf > w.sink) {
+                    // slots that no row sees: their values may be anything, and 0 * NaN is
+                    // not 0 (the other row tile's warps write the same zeros)
+                    const uint32_t at = slot + 2 * uint32_t(half >> 1) + 1, vs = at % G::kStages;
+                    if (!warp_wait(bar.full(vs), (at / G::kStages) & 1u, deadline)) {
                         ok = false;
                         break;
                     }
-                    const int32_t k = k0 + int32_t(r);
-                    if (!((k >= w.lo && k < w.hi) || k < w.sink)) {
-                        uint8_t* v = base + G::kRing + vs * G::kTile + r * 128;
+                    const int32_t k = k0 + int32_t(r & 63u);
+                    if ((r >> 6) < G::kPanels && !((k >= w.lo && k < w.hi) || k < w.sink)) {
+                        uint8_t* v = base + G::kRing + vs * G::kTile + (r >> 6) * kPanel +
+                                     (uint32_t(half & 1) * kHalf + (r & 63u)) * 128;
 #pragma unroll
-                        for (uint32_t c = 0; c < G::kPanels; ++c)
-#pragma unroll
-                            for (uint32_t e = 0; e < 8; ++e)
-                                *reinterpret_cast<uint4*>(v + c * kPanel + e * 16) = make_uint4(0, 0, 0, 0);
+                        for (uint32_t e = 0; e < 8; ++e)
+                            *reinterpret_cast<uint4*>(v + e * 16) = make_uint4(0, 0, 0, 0);
                     }
                     proxy_fence();
                     __syncwarp();
                 }
                 if (busy) {
                     fence_after();
-                    float x[128];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) ld32(ts + c * 32, x + c * 32);
+                    float x[kHalf];
+                    ld32(tb, x);
+                    ld32(tb + 32, x + 32);
                     wait_ld();
-                    if (k0 + kKeys - 1 > pos_lo ||
+                    if (k0 + kHalf - 1 > pos_lo ||
                         (p.window && int64_t(k0) <= int64_t(pos_hi) - int64_t(p.window))) {
                         // columns [lo, hi) and those below s
                         const int32_t hi = pos + 1 - k0, s = p.window ? int32_t(p.sinks) - k0 : 0;
                         const int32_t lo = p.window ? pos + 1 - int32_t(p.window) - k0 : 0;
 #pragma unroll
-                        for (int c = 0; c < 128; ++c)
+                        for (int c = 0; c < kHalf; ++c)
                             if (c >= hi || (c < lo && c >= s)) x[c] = -INFINITY;
                     }
                     float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                    for (int c = 4; c < 128; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
+                    for (int c = 4; c < kHalf - 4; c += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top[e] = max3(top[e], x[c + e], x[c + 4 + e]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], x[kHalf - 4 + e]);
                     const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                     const bool raise = m == -INFINITY ? mx > -INFINITY : (mx - m) * p.c > kRaise;
                     if (__any_sync(0xffffffffu, raise)) {
@@ -493,7 +461,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float f2 = nm == -INFINITY ? 1.f : ex2((m - nm) * p.c);
                         l *= f2;
                         m = nm;
-                        if (j) {
+                        if (n != n0) {  // the P V before has to be in O
+                            if (!warp_wait(bar.o_done(i, b ^ 1u), ((n - 1) >> 1) & 1u, deadline)) ok = false;
+                            fence_after();
 #pragma unroll
                             for (int c = 0; c < D; c += 16) {
                                 float o[16];
@@ -506,33 +476,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     const float ref = m == -INFINITY ? 0.f : -m * p.c;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const uint64_t c2 = pack2(p.c, p.c), ref2 = pack2(ref, ref);
+                    uint64_t sum[2] = {0, 0};
+                    uint32_t pk[kHalf / 2];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float a = ex2(fmaf(x[c * 32 + 2 * e], p.c, ref));
-                            const float d = ex2(fmaf(x[c * 32 + 2 * e + 1], p.c, ref));
-                            sum[(2 * e) & 3] += a;
-                            sum[(2 * e + 1) & 3] += d;
-                            pk[e] = T::pack(a, d);
-                        }
-                        st16(ts + c * 16, pk);
+                    for (int e = 0; e < kHalf / 2; ++e) {
+                        float a, d;
+                        unpack2(fma2(pack2(x[2 * e], x[2 * e + 1]), c2, ref2), a, d);
+                        a = ex2(a);
+                        d = ex2(d);
+                        sum[e & 1] = add2(sum[e & 1], pack2(a, d));
+                        pk[e] = T::pack(a, d);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    st32(tb, pk);
+                    float s0, s1;
+                    unpack2(add2(sum[0], sum[1]), s0, s1);
+                    l += s0 + s1;
                     wait_st();
                     fence_before();
                 }
+                ++n;
                 __syncwarp();
-                if (lane == 0) bar_arrive(bar.p_ready(i));
+                if (lane == 0) bar_arrive(bar.p_ready(i, b));
             }
-            if (!ok || !warp_wait(bar.o_full(i), no & 1u, deadline)) {
-                ok = false;
-                break;
+            const bool any = n != n0;  // (otherwise O is not written)
+            if (any && ok) {
+                if (n - n0 > 1) ok = warp_wait(bar.o_done(i, n & 1u), ((n >> 1) - 1) & 1u, deadline);
+                ok = warp_wait(bar.o_done(i, (n - 1) & 1u), ((n - 1) >> 1) & 1u, deadline) && ok;
             }
+            if (!ok) break;
             slot += 2 * uint32_t(steps);
-            ++no;
             if (busy) {
                 fence_after();
                 const bool whole = w.whole != 0;
@@ -547,6 +520,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     float o[32];
                     ld32(to + c, o);
                     wait_ld();
+                    if (!any)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
                     if (real && whole) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 8) {
@@ -577,6 +553,106 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             release();
         }
+    } else {
+        // ---- MMAs of row tile i: the warp goes through the pieces together, one
+        // lane issues. A warp per row tile, so that one's waits and counting
+        // pass beside the other's MMAs.
+        const uint32_t i = warp == 8 ? 0 : 1;
+        constexpr uint32_t kIs = instr(T::kUmmaFormat, 128, kHalf, false);
+        constexpr uint32_t kIo = instr(T::kUmmaFormat, 128, D, true);
+        const uint32_t q_lo = desc_lo(smem + i * G::kTile, 16), k_lo = desc_lo(smem + G::kRing, 16);
+        const uint32_t v_lo = desc_lo(smem + G::kRing, kPanel);
+        const uint32_t t_s = tmem + kS + i * 128, t_o = tmem + kO + i * D;
+        const bool lead = elect();
+        uint32_t n = 0;  // halves passed
+        // The halves that are seen, twice: for S, and two halves behind for P V.
+        struct Cursor {
+            int32_t j;            // tile of the piece
+            uint32_t left;        // its halves still to come
+            uint32_t stage, odd;  // ring stage of its keys (values), and how often the ring has gone round
+            bool there;           // the stage has landed
+        };
+        Cursor cs{0, 0, 0, 0, false}, cp{0, 0, 1, 0, false};
+        while (ok && next()) {
+            Seg w;
+            w.ns = uniform(segs[sg % kSegs].ns), w.first = uniform(segs[sg % kSegs].first);
+            w.j0 = uniform(segs[sg % kSegs].j0), w.lo = uniform(segs[sg % kSegs].lo);
+            w.hi = uniform(segs[sg % kSegs].hi), w.sink = uniform(segs[sg % kSegs].sink);
+            const int32_t steps = uniform(segs[sg % kSegs].steps);
+            const bool here = int32_t(i) * per_tile < uniform(segs[sg % kSegs].left);  // the item has this row tile
+            cs.j = cp.j = 0;
+            cs.left = cp.left = w.halves(0);
+            cs.there = cp.there = false;
+            ok = warp_wait(bar.q_full(), sg & 1u, deadline);
+            auto landed = [&](Cursor& c) {
+                if (!c.there) c.there = warp_wait(bar.full(c.stage), c.odd & 1u, deadline);
+                return c.there;
+            };
+            auto advance = [&](Cursor& c) {  // a tile's last half releases its stage
+                c.left &= c.left - 1;
+                if (c.left) return;
+                if (lead) commit(bar.empty(c.stage));
+                c.stage += 2;
+                if (c.stage >= G::kStages) c.stage -= G::kStages, ++c.odd;
+                c.there = false;
+                if (++c.j < steps) c.left = w.halves(c.j);
+            };
+            auto step_s = [&](uint32_t b) {  // S of the next half, into buffer b
+                const uint32_t k = k_lo + cs.stage * (G::kTile / 16) + ((cs.left & 1u) ? 0 : kHalf * 128 / 16);
+                if (lead) {
+#pragma unroll
+                    for (uint32_t x = 0; x < D / 16; ++x) {
+                        const uint32_t off = ((x / 4) * kPanel + (x % 4) * 32) / 16;
+                        mma_ss(t_s + b * kHalf, desc_of<1024>(q_lo + off), desc_of<1024>(k + off), kIs, x > 0);
+                    }
+                    commit(bar.s_full(i, b));
+                }
+            };
+            if (!here || !cs.left) {  // no such row tile, or no slot is seen: the tiles go by
+                while (ok && cs.j < steps) {
+                    ok = landed(cs) && landed(cp);
+                    cs.left = cp.left = 0;
+                    advance(cs);
+                    advance(cp);
+                }
+                if (lead) commit(bar.q_empty());
+                release();
+                continue;
+            }
+            bool more = true;
+            for (uint32_t t = 0; t < 2 && ok && more; ++t) {
+                if (!(ok = landed(cs))) break;
+                step_s((n + t) & 1u);
+                advance(cs);
+                more = cs.j < steps;
+                if (!more && lead) commit(bar.q_empty());
+            }
+            for (bool first = true; ok && cp.j < steps; first = false, ++n) {
+                const uint32_t b = n & 1u;
+                if (!(ok = landed(cp) && (!more || landed(cs)) &&
+                           warp_wait(bar.p_ready(i, b), (n >> 1) & 1u, deadline)))
+                    break;
+                fence_after();
+                const uint32_t v = v_lo + cp.stage * (G::kTile / 16) + ((cp.left & 1u) ? 0 : kHalf * 128 / 16);
+                if (lead) {
+#pragma unroll
+                    for (uint32_t x = 0; x < kHalf / 16; ++x)
+                        mma_ts(t_o, t_s + b * kHalf + x * 8, desc_of<1024>(v + x * 128), kIo, x > 0 || !first);
+                    commit(bar.o_done(i, b));
+                }
+                if (more) step_s(b);
+                advance(cp);
+                if (more) {
+                    advance(cs);
+                    more = cs.j < steps;
+                    if (!more && lead) commit(bar.q_empty());
+                }
+            }
+            release();
+        }
+        // MMAs in flight end (bounded) before the tensor memory goes
+        if (lead) commit(bar.drain(i));
+        warp_wait(bar.drain(i), 0, now() + kGraceNs);
     }
     if (!ok && lane == 0 && p.err) atomicOr(p.err, uint32_t(LS_B200_ATTN_TIMEOUT));
     fence_before();
@@ -588,41 +664,98 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the parts of one item cut over several CTAs: CTA (c, block of 32 rows),
-// for the item that begins in c and goes on.
+// for the item that begins in c and goes on; a warp takes four rows, a lane
+// D / 32 elements of each (lane k the statistics of part k).
 template <class T, int D>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const AttnParams p, const ChunkScratch sc) {
-    const int64_t U = sc.plan->units, G = sc.plan->ctas;
-    if (int64_t(blockIdx.x) >= G || !U) return;
+    constexpr int E = D / 32, kRowsPerWarp = 4;
+    after_start();
+    after_wait();
     const int2 open = sc.plan->open[blockIdx.x];
     if (open.x < 0) return;
+    const int64_t U = sc.plan->units, G = sc.plan->ctas;
     const ChunkItem it = sc.items[open.x];
+    const uint32_t lane = threadIdx.x & 31, row0 = blockIdx.y * 32 + (threadIdx.x >> 5) * kRowsPerWarp;
+    const int32_t per_tile = int32_t(chunk_tokens(p.g));
     const int64_t item = it.units + int64_t(open.y) * it.tiles;
     const int64_t c0 = blockIdx.x, c1 = cut_owner(U, G, item + it.tiles - 1);
-    const int32_t per_tile = int32_t(chunk_tokens(p.g));
-    for (uint32_t x = threadIdx.x; x < 32 * (D / 4); x += blockDim.x) {
-        const uint32_t row = blockIdx.y * 32 + x / (D / 4), d = x % (D / 4) * 4, r = row & 127u;
+    const int32_t parts = int32_t(c1 - c0) + 1;
+    constexpr int64_t kPart = 256 * (D + 2);
+    const float* const p0 = sc.part + (2 * c0 + (cut_begin(U, G, c0) != item)) * kPart;
+    auto part = [&](int32_t i) { return i ? sc.part + 2 * (c0 + i) * kPart : p0; };
+    float mx[kRowsPerWarp], sum[kRowsPerWarp], v[kRowsPerWarp][E];
+    bool real[kRowsPerWarp], any = false;
+    int32_t token[kRowsPerWarp], head[kRowsPerWarp];
+#pragma unroll
+    for (int x = 0; x < kRowsPerWarp; ++x) {
+        const uint32_t row = row0 + x, r = row & 127u;
         const int32_t lt = int32_t(r / p.g), t = it.t0 + int32_t(row >> 7) * per_tile + lt;
-        if (lt >= per_tile || t >= it.nq) continue;
-        auto part = [&](int64_t c) {
-            return sc.part + (2 * c + (c == c0 && cut_begin(U, G, c0) != item ? 1 : 0)) * (256 * (D + 2));
-        };
-        float mx = -INFINITY;
-        for (int64_t c = c0; c <= c1; ++c) mx = fmaxf(mx, part(c)[256 * D + row]);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f;
-        for (int64_t c = c0; c <= c1; ++c) {
-            const float* ps = part(c);
-            const float f = mx == -INFINITY ? 0.f : ex2(ps[256 * D + row] - mx);
-            const float4 v = *reinterpret_cast<const float4*>(ps + row * D + d);
-            o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
-            sum = fmaf(f, ps[256 * D + 256 + row], sum);
+        real[x] = lt < per_tile && t < it.nq;
+        any = any || real[x];
+        token[x] = it.q0 + t;
+        head[x] = open.y * int32_t(p.g) + int32_t(r % p.g);
+        mx[x] = -INFINITY;
+        sum[x] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[x][e] = 0.f;
+    }
+    if (!any) return;
+    for (int32_t i0 = 0; i0 < parts; i0 += 32) {
+        const int32_t i = i0 + int32_t(lane), n = min(32, parts - i0);
+        float f[kRowsPerWarp];
+#pragma unroll
+        for (int x = 0; x < kRowsPerWarp; ++x) {
+            const bool on = i < parts && real[x];
+            const float pm = on ? part(i)[256 * D + row0 + x] : -INFINITY;
+            const float ps = on ? part(i)[256 * D + 256 + row0 + x] : 0.f;
+            float nm = pm;
+#pragma unroll
+            for (int d = 16; d; d >>= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, d));
+            nm = fmaxf(nm, mx[x]);
+            const float ref = nm == -INFINITY ? 0.f : nm, old = ex2(mx[x] - ref);
+            f[x] = ex2(pm - ref);
+            sum[x] = fmaf(f[x], ps, sum[x] * old);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[x][e] *= old;
+            mx[x] = nm;
         }
-        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
-        const int64_t token = it.q0 + t;
-        const int32_t head = open.y * int32_t(p.g) + int32_t(r % p.g);
-        *reinterpret_cast<uint2*>(p.out + token * p.o_ts + int64_t(head) * p.o_hs + d) =
-            make_uint2(T::pack(o.x * inv, o.y * inv), T::pack(o.z * inv, o.w * inv));
-        if (d == 0 && p.lse) p.lse[token * p.Hq + head] = sum == 0.f ? -INFINITY : (mx + lg2(sum)) * kLn2;
+#pragma unroll 2
+        for (int32_t k = 0; k < n; ++k) {
+            const float* from = part(i0 + k) + row0 * D + lane * E;
+            float y[kRowsPerWarp][E];
+#pragma unroll
+            for (int x = 0; x < kRowsPerWarp; ++x) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[x][e] = 0.f;
+                if (!real[x]) continue;
+                if constexpr (E == 4)
+                    *reinterpret_cast<float4*>(y[x]) = *reinterpret_cast<const float4*>(from + x * D);
+                else
+                    *reinterpret_cast<float2*>(y[x]) = *reinterpret_cast<const float2*>(from + x * D);
+            }
+#pragma unroll
+            for (int x = 0; x < kRowsPerWarp; ++x) {
+                const float fk = __shfl_sync(0xffffffffu, f[x], k);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[x][e] = fmaf(fk, y[x][e], v[x][e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < kRowsPerWarp; ++x) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], d);
+        if (!real[x]) continue;
+        const float inv = sum[x] > 0.f ? 1.f / sum[x] : sum[x] == 0.f ? 0.f : NAN;
+        uint16_t* out = p.out + int64_t(token[x]) * p.o_ts + int64_t(head[x]) * p.o_hs + lane * E;
+        if constexpr (E == 4)
+            *reinterpret_cast<uint2*>(out) =
+                make_uint2(T::pack(v[x][0] * inv, v[x][1] * inv), T::pack(v[x][2] * inv, v[x][3] * inv));
+        else
+            *reinterpret_cast<uint32_t*>(out) = T::pack(v[x][0] * inv, v[x][1] * inv);
+        if (lane == 0 && p.lse)
+            p.lse[int64_t(token[x]) * p.Hq + head[x]] =
+                sum[x] == 0.f ? -INFINITY : (mx[x] + lg2(sum[x])) * kLn2;
     }
 }
 
@@ -696,6 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_slot;
+    after_wait();
     const uint64_t deadline = now() + p.timeout_ns;
     bool ok = true;
     Walk w;
@@ -755,35 +889,37 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (ok) warp_wait(bar.k_empty(x & 1u), (x / 2) & 1u, grace);
             }
         } else if (warp == 8) {
-            if (lane == 0) {
-                constexpr uint32_t kIs = instr(T::kUmmaFormat, 128, 128, false);
-                for (; ok && w.next(p, sc.w_plan, sc.w_items); ++seg) {
-                    const uint32_t kb = seg & 1u;
-                    ok = bar_wait(bar.k_full(kb), (seg / 2) & 1u, deadline);
-                    for (int32_t j = 0; j < w.steps && ok; ++j, ++n) {
-                        const uint32_t st = n % G::kStages, sb = n & 3u;
-                        if (!bar_wait(bar.q_full(st), (n / G::kStages) & 1u, deadline) ||
-                            (n >= 4 && !bar_wait(bar.s_empty(sb), (n / 4 - 1) & 1u, deadline))) {
-                            ok = false;
-                            break;
-                        }
-                        fence_after();
+            constexpr uint32_t kIs = instr(T::kUmmaFormat, 128, 128, false);
+            const uint32_t k_lo = desc_lo(smem, 16), q_lo = desc_lo(smem + G::kRing, 16);
+            const bool lead = elect();
+            while (ok && w.next(p, sc.w_plan, sc.w_items)) {
+                const int32_t steps = uniform(w.steps);
+                const uint32_t kb = seg & 1u;
+                ok = warp_wait(bar.k_full(kb), (seg / 2) & 1u, deadline);
+                for (int32_t j = 0; j < steps && ok; ++j, ++n) {
+                    const uint32_t st = n % G::kStages, sb = n & 3u;
+                    if (!warp_wait(bar.q_full(st), (n / G::kStages) & 1u, deadline) ||
+                        (n >= 4 && !warp_wait(bar.s_empty(sb), (n / 4 - 1) & 1u, deadline))) {
+                        ok = false;
+                        break;
+                    }
+                    fence_after();
+                    const uint32_t a = k_lo + kb * (G::kTile / 16), b = q_lo + st * (G::kTile / 16);
+                    if (lead) {
 #pragma unroll
-                        for (uint32_t k = 0; k < D / 16; ++k) {
-                            const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
-                            mma_ss(tmem + sb * 128, desc128(smem + kb * G::kTile + off, 16, 1024),
-                                   desc128(smem + G::kRing + st * G::kTile + off, 16, 1024), kIs, k > 0);
+                        for (uint32_t x = 0; x < D / 16; ++x) {
+                            const uint32_t off = ((x / 4) * kPanel + (x % 4) * 32) / 16;
+                            mma_ss(tmem + sb * 128, desc_of<1024>(a + off), desc_of<1024>(b + off), kIs, x > 0);
                         }
                         commit(bar.s_full(sb));
                         commit(bar.q_empty(st));
                     }
-                    if (ok) commit(bar.k_empty(kb));
                 }
-                if (!ok) {
-                    commit(bar.drain());
-                    bar_wait(bar.drain(), 0, now() + kGraceNs);
-                }
+                if (ok && lead) commit(bar.k_empty(kb));
+                ++seg;
             }
+            if (lead) commit(bar.drain());
+            warp_wait(bar.drain(), 0, now() + kGraceNs);
             __syncwarp();
         } else if (warp < 8) {
             const uint32_t grp = warp >> 2, r = tid & 127u;
@@ -927,8 +1063,7 @@ int launch_chunk_weights(const AttnParams& p, const ChunkScratch& s, uint32_t gr
         if (e != cudaSuccess) return int(e);
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
-    chunk_weights_kernel<T, D><<<grid, kThreads, GeoW<D>::kSmem, stream>>>(p, s, qm, km);
-    return int(cudaGetLastError());
+    return int(launch_after(chunk_weights_kernel<T, D>, grid, kThreads, GeoW<D>::kSmem, stream, p, s, qm, km));
 }
 
 template <class T, int D>
@@ -956,9 +1091,10 @@ int launch(const AttnParams& p, bool bf16, const ChunkScratch& s, uint32_t grid,
     }
     const uint32_t append = p.k_new ? p.B * ((p.max_q + 7) / 8) : 0;
     chunk_prepare_kernel<<<2 + append, 256, 0, stream>>>(p, s, grid);
-    chunk_attn_kernel<T, D><<<grid, kThreads, Geo<D>::kSmem, stream>>>(p, s, qm, km, vm);
-    chunk_join_kernel<T, D><<<dim3(grid, 8), 256, 0, stream>>>(p, s);
     e = cudaGetLastError();
+    if (e == cudaSuccess)
+        e = launch_after(chunk_attn_kernel<T, D>, grid, kThreads, Geo<D>::kSmem, stream, p, s, qm, km, vm);
+    if (e == cudaSuccess) e = launch_after(chunk_join_kernel<T, D>, dim3(grid, 8), 256, 0, stream, p, s);
     if (e != cudaSuccess || !p.weights) return int(e);
     return launch_chunk_weights<T, D>(p, s, grid, qm, km, stream);
 }

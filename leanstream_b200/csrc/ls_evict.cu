@@ -15,6 +15,7 @@
 #include <cerrno>
 
 #include "ls_attention.h"
+#include "ls_tc.h"
 
 namespace lsb {
 namespace {
@@ -56,6 +57,7 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 // bits found so far), then the kept slots are written in order.
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams p) {
     __shared__ uint32_t hist[256], warp_gt[32], warp_eq[32], found[2];
+    tc::after_start();
     const uint32_t b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t n = evict_len(p, b);
     const float* w = p.weights + int64_t(b) * p.w_ss + int64_t(h) * p.w_hs;
@@ -151,6 +153,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
 
 // Kept rows to the new pages: 16 bytes of a key and of a value per thread.
 __global__ void __launch_bounds__(256) evict_copy_kernel(const EvictParams p) {
+    tc::after_wait();
     const uint32_t pieces = p.D / 8, per_block = 256 / pieces;
     const uint32_t chunks = (p.budget + per_block - 1) / per_block;
     const uint32_t bh = blockIdx.x / chunks, b = bh / p.Hkv, h = bh % p.Hkv;
@@ -209,6 +212,6 @@ extern "C" int ls_b200_evict_cache(const ls_b200_evict_args* a, void* stream) {
     if (uint64_t(p.B) * p.Hkv * chunks > 0x7fffffffull) return EINVAL;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     evict_select_kernel<<<p.B * p.Hkv, kSelThreads, 0, s>>>(p);
-    evict_copy_kernel<<<p.B * p.Hkv * chunks, 256, 0, s>>>(p);
-    return int(cudaGetLastError());
+    if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return int(e);
+    return int(tc::launch_after(evict_copy_kernel, p.B * p.Hkv * chunks, 256, 0, s, p));
 }
