@@ -830,7 +830,9 @@ int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
     p.B = a->batch, p.Hq = a->q_heads, p.Hkv = a->kv_heads, p.g = a->q_heads / a->kv_heads, p.D = a->head_dim;
     p.P = a->page_size, p.pages = a->pages, p.tpages = a->table_pages, p.tokens = a->tokens, p.max_q = a->max_q;
     while ((1u << p.pshift) < p.P) ++p.pshift;
-    p.window = a->window, p.sinks = a->sinks, p.wlen = a->weights_length;
+    // (a window that no cache of this table fills is none)
+    p.window = uint64_t(a->window) < uint64_t(a->table_pages) * a->page_size ? a->window : 0;
+    p.sinks = a->sinks, p.wlen = a->weights_length;
     p.rows = p.max_q * p.g;
     p.timeout_ns = a->timeout_ns ? a->timeout_ns : kTimeoutNs;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

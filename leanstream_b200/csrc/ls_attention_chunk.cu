@@ -53,12 +53,13 @@ struct Geo {
     static constexpr uint32_t kStages = D == 128 ? 5 : 8;
     static constexpr uint32_t kRing = 2 * kTile, kBars = kRing + kStages * kTile;
     static constexpr uint32_t kSegs = kBars + 336;
-    static constexpr uint32_t kSmem = kSegs + 256 + 1024;  // + alignment of the swizzled tiles
+    static constexpr uint32_t kSmem = kSegs + 320 + 1024;  // + alignment of the swizzled tiles
 };
 static_assert(Geo<128>::kSmem <= 227 * 1024 && Geo<64>::kSmem <= 227 * 1024, "shared memory of a CTA");
 
-// Barriers: ring full / empty, Q full / empty; S full, P ready and P V done by
-// row tile and buffer; the last MMAs after a failure, pieces full / empty.
+// Barriers: ring full / empty, Q full / empty; S full and P ready by row tile
+// and buffer, the last two P V of a piece by row tile; the last MMAs of the
+// CTA, pieces full / empty.
 struct Bars {
     uint32_t base;
     __device__ uint32_t full(uint32_t s) const { return base + 8 * s; }
@@ -67,10 +68,10 @@ struct Bars {
     __device__ uint32_t q_empty() const { return base + 8 * 17; }
     __device__ uint32_t s_full(uint32_t i, uint32_t b) const { return base + 8 * (18 + 2 * i + b); }
     __device__ uint32_t p_ready(uint32_t i, uint32_t b) const { return base + 8 * (22 + 2 * i + b); }
-    __device__ uint32_t o_done(uint32_t i, uint32_t b) const { return base + 8 * (26 + 2 * i + b); }
-    __device__ uint32_t drain(uint32_t i) const { return base + 8 * (30 + i); }
-    __device__ uint32_t seg_full(uint32_t s) const { return base + 8 * (32 + s); }
-    __device__ uint32_t seg_empty(uint32_t s) const { return base + 8 * (36 + s); }
+    __device__ uint32_t o_done(uint32_t i) const { return base + 8 * (26 + i); }
+    __device__ uint32_t drain(uint32_t i) const { return base + 8 * (28 + i); }
+    __device__ uint32_t seg_full(uint32_t s) const { return base + 8 * (30 + s); }
+    __device__ uint32_t seg_empty(uint32_t s) const { return base + 8 * (34 + s); }
 };
 
 // Lays out the items of a call in `plan` and `items`: for the attention
@@ -206,29 +207,64 @@ __global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, 
 }
 
 // One piece of an item in shared memory (four in flight): what the roles need.
+// Its halves that some row sees are na halves from ha on (of the first slots),
+// then those from hb on; each of its tiles has one at least, unless the item
+// sees nothing.
 struct Seg {
-    int32_t steps;      // tiles; 0: no more pieces
-    int32_t row0;       // row of q of the item's first token
-    int32_t left;       // tokens of the sequence from there
-    int32_t pos0;       // their first cache slot
-    int32_t h, b, j0;   // kv head, sequence, first tile
-    int32_t ns, first;  // as KeyRange
+    int32_t steps;       // tiles; 0: no more pieces
+    int32_t row0;        // row of q of the item's first token
+    int32_t left;        // tokens of the sequence from there
+    int32_t pos0;        // their first cache slot
+    int32_t h, b, j0;    // kv head, sequence, first tile
+    int32_t ns, first;   // as KeyRange
     int32_t lo, hi, sink;
-    int32_t whole;      // the item is all in this piece
-    int32_t part;       // which of the CTA's two partial results
+    int32_t whole;       // the item is all in this piece
+    int32_t part;        // which of the CTA's two partial results
+    int32_t halves;      // of all tiles
+    int32_t na, ha, hb;
     int32_t pad[2];
     __device__ int32_t slot0(int32_t step) const {
         const int32_t j = j0 + step;
         return (j < ns ? j : first + j - ns) * kKeys;
     }
-    // halves of a tile with a slot that some row sees: bits 0 and 1
-    __device__ uint32_t halves(int32_t step) const {
-        const int32_t k0 = slot0(step), k1 = k0 + kHalf;
-        return uint32_t((k0 < hi && k1 > lo) || k0 < sink) | uint32_t((k1 < hi && k1 + kHalf > lo) || k1 < sink) << 1;
+    __device__ void set_halves() {
+        const int32_t a = (sink + kHalf - 1) / kHalf, w = max(lo / kHalf, a), end = (hi + kHalf - 1) / kHalf;
+        const int32_t j1 = j0 + steps;
+        ha = 2 * j0;
+        na = j0 < ns ? max(0, min(a, 2 * min(j1, ns)) - ha) : 0;
+        hb = j0 < ns ? w : max(w, 2 * (first + j0 - ns));
+        const int32_t last = j1 > ns ? min(end, 2 * (first + j1 - ns)) : j1 == ns ? min(end, 2 * ns) : hb;
+        halves = na + max(0, last - hb);
     }
 };
-static_assert(sizeof(Seg) == 64, "four pieces fit");
+static_assert(sizeof(Seg) == 80, "four pieces fit");
 constexpr uint32_t kSegs = 4, kSegReaders = 11;
+
+// Goes through the halves of a piece, and through the ring stages of their keys
+// (values) from piece to piece.
+struct Halves {
+    uint32_t stage, odd;  // ring stage, and how often the ring has gone round
+    int32_t t, h;         // half of the piece, and of the sequence
+    bool fresh;           // the first half of its tile
+    __device__ void begin(int32_t na, int32_t ha, int32_t hb) {
+        t = 0;
+        h = na ? ha : hb;
+        fresh = true;
+    }
+    // To the next half; true when it leaves its tile.
+    __device__ bool next(int32_t count, int32_t na, int32_t hb) {
+        const int32_t tile = h >> 1;
+        ++t;
+        h = t == na ? hb : h + 1;
+        fresh = t == count || (h >> 1) != tile;
+        return fresh;
+    }
+    template <uint32_t kStages>
+    __device__ void next_stage() {
+        stage += 2;
+        if (stage >= kStages) stage -= kStages, ++odd;
+    }
+};
 
 template <class T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -239,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t* const base = raw + (smem - smem_u32(raw));
     const Bars bar{smem + G::kBars};
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(base + G::kBars + 8 * 40);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(base + G::kBars + 8 * 38);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t per_tile = int32_t(chunk_tokens(p.g));  // tokens of a row tile
 
@@ -254,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (uint32_t b = 0; b < 2; ++b) {
                 bar_init(bar.s_full(i, b), 1);
                 bar_init(bar.p_ready(i, b), 4);  // the four warps of the row tile
-                bar_init(bar.o_done(i, b), 1);
             }
+            bar_init(bar.o_done(i), 1);
             bar_init(bar.drain(i), 1);
         }
         for (uint32_t i = 0; i < kSegs; ++i) {
@@ -312,6 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     x.steps = w.steps, x.row0 = w.it.q0 + w.it.t0, x.left = w.it.nq - w.it.t0;
                     x.pos0 = w.it.n - w.it.nq + w.it.t0, x.h = w.h, x.b = w.it.b, x.j0 = w.j0;
                     x.ns = kr.ns, x.first = kr.first, x.lo = kr.lo, x.hi = kr.hi, x.sink = kr.sink;
+                    x.set_halves();
                     x.whole = w.j0 == 0 && w.steps == w.it.tiles;
                     x.part = w.u != w.u_begin;
                     if (!x.whole && !w.j0) sc.plan->open[blockIdx.x] = make_int2(w.i, w.h);
@@ -387,44 +424,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t r = tid & 127u, quarter = (warp & 3u) << 21;  // lane 32 * (warp % 4) of tensor memory
         const uint32_t ts = tmem + quarter + kS + i * 128, to = tmem + quarter + kO + i * D;
         const int32_t lt = int32_t(r / p.g);
-        uint32_t n = 0, slot = 0;  // halves and ring slots passed
+        uint32_t n = 0, no = 0;  // halves passed, results of P V waited for
+        Halves at{1, 0, 0, 0, false};
         while (ok && next()) {
             const Seg& w = segs[sg % kSegs];
-            const int32_t steps = w.steps, t_tile = int32_t(i) * per_tile;  // first token of the tile, in the item
+            const int32_t count = w.halves, na = w.na, hb = w.hb, t_tile = int32_t(i) * per_tile;
             if (t_tile >= w.left) {  // the item has one row tile
-                slot += 2 * uint32_t(steps);
+                for (int32_t j = w.steps; j; --j) at.next_stage<G::kStages>();
                 release();
                 continue;
             }
             const bool real = lt < per_tile && t_tile + lt < w.left;
             const bool busy = __any_sync(0xffffffffu, real);
             const int32_t pos = real ? max(w.pos0 + t_tile + lt, -1) : -1;
-            const int32_t pos_lo = w.pos0 + t_tile, pos_hi = w.pos0 + min(w.left, t_tile + per_tile) - 1;
-            const uint32_t n0 = n;
+            // slots [all_lo, all_hi) are seen by every row of the tile, [seen_lo, seen_hi) by some row of the item
+            const int32_t all_hi = w.pos0 + t_tile + 1, seen_lo = w.lo, seen_hi = w.hi, sink = w.sink;
+            const int32_t all_lo =
+                p.window ? int32_t(max(int64_t(0), int64_t(w.pos0) + min(w.left, t_tile + per_tile) - p.window)) : 0;
             float m = -INFINITY, l = 0.f;  // reference maximum and sum of the row
-            for (int32_t half = 0; half < 2 * steps && ok; ++half) {
-                if (!(w.halves(half >> 1) >> (half & 1) & 1u)) continue;
-                const int32_t k0 = w.slot0(half >> 1) + (half & 1) * kHalf;
+            at.begin(na, w.ha, hb);
+            for (; at.t < count; ++n) {
+                const int32_t k0 = at.h * kHalf;
                 const uint32_t b = n & 1u, tb = ts + b * kHalf;
-                // (every phase of P V is waited for before the next can come: a parity
-                // tells only two apart)
-                if (!warp_wait(bar.s_full(i, b), (n >> 1) & 1u, deadline) ||
-                    (n - n0 > 1 && !warp_wait(bar.o_done(i, b), ((n >> 1) - 1) & 1u, deadline))) {
-                    ok = false;
-                    break;
-                }
-                if (!(k0 >= w.lo && k0 + kHalf <= w.hi) && k0 + kHalf > w.sink) {
+                const bool last = at.t + 1 == count;
+                ok = warp_wait(bar.s_full(i, b), (n >> 1) & 1u, deadline);
+                if (last && at.t) ok = warp_wait(bar.o_done(i), no++ & 1u, deadline) && ok;  // the P V before
+                if (!ok) break;
+                if (!(k0 >= seen_lo && k0 + kHalf <= seen_hi) && k0 + kHalf > sink) {
                     // slots that no row sees: their values may be anything, and 0 * NaN is
                     // not 0 (the other row tile's warps write the same zeros)
-                    const uint32_t at = slot + 2 * uint32_t(half >> 1) + 1, vs = at % G::kStages;
-                    if (!warp_wait(bar.full(vs), (at / G::kStages) & 1u, deadline)) {
-                        ok = false;
-                        break;
-                    }
+                    if (!(ok = warp_wait(bar.full(at.stage), at.odd & 1u, deadline))) break;
                     const int32_t k = k0 + int32_t(r & 63u);
-                    if ((r >> 6) < G::kPanels && !((k >= w.lo && k < w.hi) || k < w.sink)) {
-                        uint8_t* v = base + G::kRing + vs * G::kTile + (r >> 6) * kPanel +
-                                     (uint32_t(half & 1) * kHalf + (r & 63u)) * 128;
+                    if ((r >> 6) < G::kPanels && !((k >= seen_lo && k < seen_hi) || k < sink)) {
+                        uint8_t* v = base + G::kRing + at.stage * G::kTile + (r >> 6) * kPanel +
+                                     (uint32_t(at.h & 1) * kHalf + (r & 63u)) * 128;
 #pragma unroll
                         for (uint32_t e = 0; e < 8; ++e)
                             *reinterpret_cast<uint4*>(v + e * 16) = make_uint4(0, 0, 0, 0);
@@ -438,8 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ld32(tb, x);
                     ld32(tb + 32, x + 32);
                     wait_ld();
-                    if (k0 + kHalf - 1 > pos_lo ||
-                        (p.window && int64_t(k0) <= int64_t(pos_hi) - int64_t(p.window))) {
+                    if (k0 + kHalf > all_hi || k0 < all_lo) {
                         // columns [lo, hi) and those below s
                         const int32_t hi = pos + 1 - k0, s = p.window ? int32_t(p.sinks) - k0 : 0;
                         const int32_t lo = p.window ? pos + 1 - int32_t(p.window) - k0 : 0;
@@ -461,8 +493,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float f2 = nm == -INFINITY ? 1.f : ex2((m - nm) * p.c);
                         l *= f2;
                         m = nm;
-                        if (n != n0) {  // the P V before has to be in O
-                            if (!warp_wait(bar.o_done(i, b ^ 1u), ((n - 1) >> 1) & 1u, deadline)) ok = false;
+                        if (at.t) {  // the P V before has to be in O: it is when the next S is there
+                            if (!last && !warp_wait(bar.s_full(i, b ^ 1u), ((n + 1) >> 1) & 1u, deadline)) ok = false;
                             fence_after();
 #pragma unroll
                             for (int c = 0; c < D; c += 16) {
@@ -495,17 +527,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     wait_st();
                     fence_before();
                 }
-                ++n;
                 __syncwarp();
                 if (lane == 0) bar_arrive(bar.p_ready(i, b));
+                if (at.next(count, na, hb)) at.next_stage<G::kStages>();
             }
-            const bool any = n != n0;  // (otherwise O is not written)
-            if (any && ok) {
-                if (n - n0 > 1) ok = warp_wait(bar.o_done(i, n & 1u), ((n >> 1) - 1) & 1u, deadline);
-                ok = warp_wait(bar.o_done(i, (n - 1) & 1u), ((n - 1) >> 1) & 1u, deadline) && ok;
-            }
+            const bool any = count != 0;  // (otherwise O is not written)
+            if (any && ok) ok = warp_wait(bar.o_done(i), no++ & 1u, deadline);
             if (!ok) break;
-            slot += 2 * uint32_t(steps);
+            if (!any)
+                for (int32_t j = w.steps; j; --j) at.next_stage<G::kStages>();
             if (busy) {
                 fence_after();
                 const bool whole = w.whole != 0;
@@ -565,40 +595,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t t_s = tmem + kS + i * 128, t_o = tmem + kO + i * D;
         const bool lead = elect();
         uint32_t n = 0;  // halves passed
-        // The halves that are seen, twice: for S, and two halves behind for P V.
-        struct Cursor {
-            int32_t j;            // tile of the piece
-            uint32_t left;        // its halves still to come
-            uint32_t stage, odd;  // ring stage of its keys (values), and how often the ring has gone round
-            bool there;           // the stage has landed
-        };
-        Cursor cs{0, 0, 0, 0, false}, cp{0, 0, 1, 0, false};
+        Halves cs{0, 0, 0, 0, false}, cp{1, 0, 0, 0, false};  // for S, and two halves behind for P V
         while (ok && next()) {
-            Seg w;
-            w.ns = uniform(segs[sg % kSegs].ns), w.first = uniform(segs[sg % kSegs].first);
-            w.j0 = uniform(segs[sg % kSegs].j0), w.lo = uniform(segs[sg % kSegs].lo);
-            w.hi = uniform(segs[sg % kSegs].hi), w.sink = uniform(segs[sg % kSegs].sink);
-            const int32_t steps = uniform(segs[sg % kSegs].steps);
-            const bool here = int32_t(i) * per_tile < uniform(segs[sg % kSegs].left);  // the item has this row tile
-            cs.j = cp.j = 0;
-            cs.left = cp.left = w.halves(0);
-            cs.there = cp.there = false;
+            const Seg& w = segs[sg % kSegs];
+            const int32_t count = uniform(w.halves), na = uniform(w.na), ha = uniform(w.ha), hb = uniform(w.hb);
             ok = warp_wait(bar.q_full(), sg & 1u, deadline);
-            auto landed = [&](Cursor& c) {
-                if (!c.there) c.there = warp_wait(bar.full(c.stage), c.odd & 1u, deadline);
-                return c.there;
+            if (int32_t(i) * per_tile >= uniform(w.left) || !count) {  // no such row tile, or nothing seen
+                for (int32_t j = uniform(w.steps); j && ok; --j)
+                    for (Halves* c : {&cs, &cp}) {
+                        ok = ok && warp_wait(bar.full(c->stage), c->odd & 1u, deadline);
+                        if (lead) commit(bar.empty(c->stage));
+                        c->next_stage<G::kStages>();
+                    }
+                if (lead) commit(bar.q_empty());
+                release();
+                continue;
+            }
+            cs.begin(na, ha, hb);
+            cp.begin(na, ha, hb);
+            auto landed = [&](const Halves& c) {
+                return !c.fresh || warp_wait(bar.full(c.stage), c.odd & 1u, deadline);
             };
-            auto advance = [&](Cursor& c) {  // a tile's last half releases its stage
-                c.left &= c.left - 1;
-                if (c.left) return;
-                if (lead) commit(bar.empty(c.stage));
-                c.stage += 2;
-                if (c.stage >= G::kStages) c.stage -= G::kStages, ++c.odd;
-                c.there = false;
-                if (++c.j < steps) c.left = w.halves(c.j);
+            auto advance = [&](Halves& c) {  // a tile's last half releases its stage
+                const uint32_t stage = c.stage;
+                if (!c.next(count, na, hb)) return;
+                if (lead) commit(bar.empty(stage));
+                c.next_stage<G::kStages>();
             };
             auto step_s = [&](uint32_t b) {  // S of the next half, into buffer b
-                const uint32_t k = k_lo + cs.stage * (G::kTile / 16) + ((cs.left & 1u) ? 0 : kHalf * 128 / 16);
+                const uint32_t k = k_lo + cs.stage * (G::kTile / 16) + (cs.h & 1) * (kHalf * 128 / 16);
                 if (lead) {
 #pragma unroll
                     for (uint32_t x = 0; x < D / 16; ++x) {
@@ -607,46 +632,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     commit(bar.s_full(i, b));
                 }
+                advance(cs);
+                if (cs.t == count && lead) commit(bar.q_empty());
             };
-            if (!here || !cs.left) {  // no such row tile, or no slot is seen: the tiles go by
-                while (ok && cs.j < steps) {
-                    ok = landed(cs) && landed(cp);
-                    cs.left = cp.left = 0;
-                    advance(cs);
-                    advance(cp);
-                }
-                if (lead) commit(bar.q_empty());
-                release();
-                continue;
-            }
-            bool more = true;
-            for (uint32_t t = 0; t < 2 && ok && more; ++t) {
+            for (uint32_t t = 0; t < 2 && ok && cs.t < count; ++t) {
                 if (!(ok = landed(cs))) break;
                 step_s((n + t) & 1u);
-                advance(cs);
-                more = cs.j < steps;
-                if (!more && lead) commit(bar.q_empty());
             }
-            for (bool first = true; ok && cp.j < steps; first = false, ++n) {
+            for (; ok && cp.t < count; ++n) {
                 const uint32_t b = n & 1u;
+                const bool more = cs.t < count;
                 if (!(ok = landed(cp) && (!more || landed(cs)) &&
                            warp_wait(bar.p_ready(i, b), (n >> 1) & 1u, deadline)))
                     break;
                 fence_after();
-                const uint32_t v = v_lo + cp.stage * (G::kTile / 16) + ((cp.left & 1u) ? 0 : kHalf * 128 / 16);
+                const uint32_t v = v_lo + cp.stage * (G::kTile / 16) + (cp.h & 1) * (kHalf * 128 / 16);
                 if (lead) {
 #pragma unroll
                     for (uint32_t x = 0; x < kHalf / 16; ++x)
-                        mma_ts(t_o, t_s + b * kHalf + x * 8, desc_of<1024>(v + x * 128), kIo, x > 0 || !first);
-                    commit(bar.o_done(i, b));
+                        mma_ts(t_o, t_s + b * kHalf + x * 8, desc_of<1024>(v + x * 128), kIo, x > 0 || cp.t > 0);
+                    if (!more) commit(bar.o_done(i));
                 }
                 if (more) step_s(b);
                 advance(cp);
-                if (more) {
-                    advance(cs);
-                    more = cs.j < steps;
-                    if (!more && lead) commit(bar.q_empty());
-                }
             }
             release();
         }
