@@ -19,6 +19,7 @@
 #include <atomic>
 #include <cerrno>
 #include <cmath>
+#include <type_traits>
 
 #include "ls_attention.h"
 #include "ls_tc.h"
@@ -36,11 +37,10 @@ constexpr int64_t kDecItemCost = 2;             // units that beginning and join
 constexpr int64_t kDecMinUnits = 2 + kDecItemCost;  // units that a CTA takes at least
 constexpr uint64_t kGraceNs = 1000000000ull;
 
-// One 16-row MMA tile of rows keeps its registers within three CTAs per SM,
-// two tiles within two; the ring takes the shared memory that leaves.
-template <int D, int MT>
+// Three CTAs per SM by registers; the ring takes the shared memory that leaves.
+template <int D>
 struct GeoD {
-    static constexpr int kCtas = MT == 1 ? 3 : 2, kRows = 16 * MT;
+    static constexpr int kCtas = 3, kRows = 16;
     static constexpr uint32_t kHalf = kDecKeys * D * 2, kStage = 2 * kHalf;  // a step's keys, and its values
     static constexpr int kStages = 2 * (128 / D);
     static constexpr uint32_t kRing = kDecWarps * kStages * kStage;
@@ -123,12 +123,12 @@ __device__ __forceinline__ Pair block_scan(Pair v, Pair* sh, Pair& before) {
 // with new tokens or with slots that no row sees come by 16-byte copies
 // instead, row by row, with zeros for those. An item cut over several CTAs is
 // joined, in the order of its pieces, by the CTA that arrives last.
-template <class T, int D, int MT>
-__global__ void __launch_bounds__(kDecThreads, GeoD<D, MT>::kCtas)
+template <class T, int D>
+__global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
     attn_decode_kernel(const AttnParams p, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
-    using G = GeoD<D, MT>;
-    constexpr int MR = 16 * MT, KS = D / 16, PIECES = D / 8, RPI = 32 / PIECES, ITERS = kDecKeys / RPI;
+    using G = GeoD<D>;
+    constexpr int MR = G::kRows, KS = D / 16, PIECES = D / 8, RPI = 32 / PIECES, ITERS = kDecKeys / RPI;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
     DecSeg* const segs = reinterpret_cast<DecSeg*>(smem + G::kSegs);
@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, MT>::kCtas)
             }
             const int64_t at = base + before.x, item_units = v.y ? v.x / p.Hkv : 1;
             const int32_t seq = seqs + before.y;
-            if (v.y && u >= at && u < at + v.x) flag[1] = uint32_t(seq * int32_t(p.Hkv) + int32_t((u - at) / item_units));
+            if (v.y && u >= at && u < at + v.x)
+                flag[1] = uint32_t(seq * int32_t(p.Hkv) + int32_t((u - at) / item_units));
             __syncthreads();
             const int64_t from = max(u, at), to = min(u_end, at + v.x);
             if (from < to) {
@@ -298,7 +299,7 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, MT>::kCtas)
             }
             cp_arrive(bar);
         };
-        uint32_t qf[MT == 1 ? KS : 1][4];
+        uint32_t qf[KS][4];
         auto queries = [&](const DecSeg& x) {  // as A fragments; zero past the rows
             const uint16_t* q[2];
             bool on[2];
@@ -315,171 +316,135 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, MT>::kCtas)
                 for (int i = 0; i < 4; ++i)
                     qf[kk][i] = on[i & 1] ? *reinterpret_cast<const uint32_t*>(q[i & 1] + kk * 16 + (i >> 1) * 8) : 0u;
         };
-        if constexpr (MT == 1) queries(segs[0]);  // ahead of the cache's stream
+        queries(segs[0]);  // ahead of the cache's stream
 #pragma unroll 1
         for (int i = 0; i < G::kStages; ++i) load();
 
         for (uint32_t c = 0; c < count; ++c) {
             const DecSeg& x = segs[c];
             const int32_t R = x.rows, steps = x.steps, h = x.h;
-            if constexpr (MT > 1) {
-                for (uint32_t i = tid; i < uint32_t(MR * PIECES); i += kDecThreads) {
-                    const uint32_t row = i / PIECES, piece = i % PIECES;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (int32_t(row) < R)
-                        v = *reinterpret_cast<const uint4*>(p.q + int64_t(x.q0 + int32_t(row) / g) * p.q_ts +
-                                                            int64_t(h * g + int32_t(row) % g) * p.q_hs + piece * 8);
-                    *reinterpret_cast<uint4*>(smem + G::kJoin + swz<MR>(row, piece)) = v;
-                }
-                __syncthreads();
+            int32_t pos[2];  // slot of the token of this lane's rows (-1: no row)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int32_t row = int32_t(lane >> 2) + 8 * i;
+                pos[i] = row < R ? max(x.f + row / g, -1) : -1;
             }
-            int32_t pos[MT][2];  // slot of the token of this lane's rows (-1: no row)
+            float o[2 * KS][4], m[2], l[2];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int n = 0; n < 2 * KS; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int32_t row = mt * 16 + int32_t(lane >> 2) + 8 * i;
-                    pos[mt][i] = row < R ? max(x.f + row / g, -1) : -1;
-                }
-            float o[MT][2 * KS][4], m[MT][2], l[MT][2];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                for (int n = 0; n < 2 * KS; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
-                m[mt][0] = m[mt][1] = -INFINITY;
-                l[mt][0] = l[mt][1] = 0.f;
-            }
+                for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+            m[0] = m[1] = -INFINITY;
+            l[0] = l[1] = 0.f;
 
             for (int32_t block = 0; block < steps; block += 32) {
-              const int32_t c_k = lay_out(c, block + int32_t(lane));
-              for (uint32_t todo = __ballot_sync(0xffffffffu, c_k & kSeen); todo; todo &= todo - 1) {
-                const int32_t kf = __shfl_sync(0xffffffffu, c_k, __ffs(int(todo)) - 1), k0 = kf & ~15;
-                const uint32_t st = used % G::kStages, ks = ring + st * G::kStage, vs = ks + G::kHalf;
-                if (!warp_wait(bar0 + 8 * st, (used / G::kStages) & 1u, deadline)) ok = false;
-                ++used;
-                // S = Q K^T
-                float sc[MT][2][4] = {};
+                const int32_t c_k = lay_out(c, block + int32_t(lane));
+                for (uint32_t todo = __ballot_sync(0xffffffffu, c_k & kSeen); todo; todo &= todo - 1) {
+                    const int32_t kf = __shfl_sync(0xffffffffu, c_k, __ffs(int(todo)) - 1), k0 = kf & ~15;
+                    const uint32_t st = used % G::kStages, ks = ring + st * G::kStage, vs = ks + G::kHalf;
+                    if (!warp_wait(bar0 + 8 * st, (used / G::kStages) & 1u, deadline)) ok = false;
+                    ++used;
+                    // S = Q K^T
+                    float sc[2][4] = {};
 #pragma unroll
-                for (int kk = 0; kk < KS; ++kk) {
-                    uint32_t bf[4];
-                    ldsm4(bf, ks + swz<kDecKeys>((lane & 7u) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1u)));
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        if constexpr (MT == 1) {
-                            T::mma(sc[mt][0], qf[kk], bf[0], bf[1]);
-                            T::mma(sc[mt][1], qf[kk], bf[2], bf[3]);
-                        } else {
-                            uint32_t af[4];
-                            ldsm4(af, sbase + G::kJoin + swz<MR>(mt * 16 + (lane & 15u), kk * 2 + (lane >> 4)));
-                            T::mma(sc[mt][0], af, bf[0], bf[1]);
-                            T::mma(sc[mt][1], af, bf[2], bf[3]);
-                        }
+                    for (int kk = 0; kk < KS; ++kk) {
+                        uint32_t bf[4];
+                        ldsm4(bf, ks + swz<kDecKeys>((lane & 7u) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1u)));
+                        T::mma(sc[0], qf[kk], bf[0], bf[1]);
+                        T::mma(sc[1], qf[kk], bf[2], bf[3]);
                     }
-                }
-                if (kf & kMasked) {
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                    if (kf & kMasked) {
 #pragma unroll
                         for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                if (!sees(p, pos[mt][e >> 1], k0 + nt * 8 + int32_t(lane & 3u) * 2 + (e & 1)))
-                                    sc[mt][nt][e] = -INFINITY;
-                }
-                if (p.logits) {
-                    float* lg = p.logits + ((int64_t(x.b) * p.Hkv + h) * p.wlen) * p.rows;
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                                if (!sees(p, pos[e >> 1], k0 + nt * 8 + int32_t(lane & 3u) * 2 + (e & 1)))
+                                    sc[nt][e] = -INFINITY;
+                    }
+                    if (p.logits) {
+                        float* lg = p.logits + ((int64_t(x.b) * p.Hkv + h) * p.wlen) * p.rows;
 #pragma unroll
                         for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const int32_t row = mt * 16 + int32_t(lane >> 2) + 8 * (e >> 1);
+                                const int32_t row = int32_t(lane >> 2) + 8 * (e >> 1);
                                 const int32_t key = k0 + nt * 8 + int32_t(lane & 3u) * 2 + (e & 1);
-                                if (row < R && key < x.hi) lg[int64_t(key) * p.rows + row] = sc[mt][nt][e] * p.c;
+                                if (row < R && key < x.hi) lg[int64_t(key) * p.rows + row] = sc[nt][e] * p.c;
                             }
-                }
-                // running maximum, probabilities and sums
-                uint32_t ph[MT][4], pl[MT][4];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
+                    }
+                    // running maximum, probabilities and sums
+                    uint32_t ph[4], pl[4];
                     float nm[2], bs[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float y = fmaxf(fmaxf(sc[mt][0][2 * i], sc[mt][0][2 * i + 1]),
-                                        fmaxf(sc[mt][1][2 * i], sc[mt][1][2 * i + 1]));
+                        float y = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]),
+                                        fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
                         y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
                         y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-                        nm[i] = fmaxf(m[mt][i], y);
+                        nm[i] = fmaxf(m[i], y);
                         bs[i] = nm[i] == -INFINITY ? 0.f : nm[i] * p.c;
                     }
-                    if (__any_sync(0xffffffffu, nm[0] > m[mt][0] || nm[1] > m[mt][1])) {
-                        const float al[2] = {ex2(m[mt][0] * p.c - bs[0]), ex2(m[mt][1] * p.c - bs[1])};
+                    if (__any_sync(0xffffffffu, nm[0] > m[0] || nm[1] > m[1])) {
+                        const float al[2] = {ex2(m[0] * p.c - bs[0]), ex2(m[1] * p.c - bs[1])};
 #pragma unroll
                         for (int n = 0; n < 2 * KS; ++n)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[mt][n][e] *= al[e >> 1];
+                            for (int e = 0; e < 4; ++e) o[n][e] *= al[e >> 1];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) l[mt][i] *= al[i], m[mt][i] = nm[i];
+                        for (int i = 0; i < 2; ++i) l[i] *= al[i], m[i] = nm[i];
                     }
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const float a = ex2(fmaf(sc[mt][nt][2 * i], p.c, -bs[i]));
-                            const float d = ex2(fmaf(sc[mt][nt][2 * i + 1], p.c, -bs[i]));
-                            l[mt][i] += a + d;
+                            const float a = ex2(fmaf(sc[nt][2 * i], p.c, -bs[i]));
+                            const float d = ex2(fmaf(sc[nt][2 * i + 1], p.c, -bs[i]));
+                            l[i] += a + d;
                             // A fragment: registers (row, row + 8) x (keys 0-7, 8-15)
-                            ph[mt][nt * 2 + i] = T::pack(a, d);
+                            ph[nt * 2 + i] = T::pack(a, d);
                             float ha, hd;
-                            T::unpack(ph[mt][nt * 2 + i], ha, hd);
-                            pl[mt][nt * 2 + i] = T::pack(a - ha, d - hd);
+                            T::unpack(ph[nt * 2 + i], ha, hd);
+                            pl[nt * 2 + i] = T::pack(a - ha, d - hd);
                         }
-                }
-                // O += P V. P enters as its 16-bit rounding plus the 16-bit
-                // rounding of what that leaves: the tensor cores are far from
-                // busy here, and the sum keeps about twice the bits.
+                    // O += P V. P enters as its 16-bit rounding plus the 16-bit
+                    // rounding of what that leaves: the tensor cores are far from
+                    // busy here, and the sum keeps about twice the bits.
 #pragma unroll
-                for (int n = 0; n < KS; ++n) {
-                    uint32_t vf[4];
-                    ldsm4t(vf, vs + swz<kDecKeys>((lane & 7u) + (((lane >> 3) & 1u) << 3), n * 2 + (lane >> 4)));
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        T::mma(o[mt][2 * n], ph[mt], vf[0], vf[1]);
-                        T::mma(o[mt][2 * n + 1], ph[mt], vf[2], vf[3]);
-                        T::mma(o[mt][2 * n], pl[mt], vf[0], vf[1]);
-                        T::mma(o[mt][2 * n + 1], pl[mt], vf[2], vf[3]);
+                    for (int n = 0; n < KS; ++n) {
+                        uint32_t vf[4];
+                        ldsm4t(vf, vs + swz<kDecKeys>((lane & 7u) + (((lane >> 3) & 1u) << 3), n * 2 + (lane >> 4)));
+                        T::mma(o[2 * n], ph, vf[0], vf[1]);
+                        T::mma(o[2 * n + 1], ph, vf[2], vf[3]);
+                        T::mma(o[2 * n], pl, vf[0], vf[1]);
+                        T::mma(o[2 * n + 1], pl, vf[2], vf[3]);
                     }
-                }
-                // the new tokens' keys and values go to their slots
-                if (p.fused && (kf & kEdge) && k0 + kDecKeys > x.f) {
-                    const int32_t id = p.table[int64_t(x.b) * p.table_s + (k0 >> p.pshift)];
-                    const uint32_t piece = lane % PIECES;
-                    if (uint32_t(id) < p.pages) {
+                    // the new tokens' keys and values go to their slots
+                    if (p.fused && (kf & kEdge) && k0 + kDecKeys > x.f) {
+                        const int32_t id = p.table[int64_t(x.b) * p.table_s + (k0 >> p.pshift)];
+                        const uint32_t piece = lane % PIECES;
+                        if (uint32_t(id) < p.pages) {
 #pragma unroll 2
-                        for (int i = 0; i < ITERS; ++i) {
-                            const int32_t row = i * RPI + int32_t(lane / PIECES), key = k0 + row;
-                            if (key >= x.f && key < x.hi) {
-                                const int64_t at = key & int32_t(p.P - 1);
-                                const uint8_t* kk = smem + (ks - sbase) + swz<kDecKeys>(row, piece);
-                                *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + at * p.kp_ss +
-                                                          int64_t(h) * p.kp_hs + piece * 8) =
-                                    *reinterpret_cast<const uint4*>(kk);
-                                *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + at * p.vp_ss +
-                                                          int64_t(h) * p.vp_hs + piece * 8) =
-                                    *reinterpret_cast<const uint4*>(kk + G::kHalf);
+                            for (int i = 0; i < ITERS; ++i) {
+                                const int32_t row = i * RPI + int32_t(lane / PIECES), key = k0 + row;
+                                if (key >= x.f && key < x.hi) {
+                                    const int64_t at = key & int32_t(p.P - 1);
+                                    const uint8_t* kk = smem + (ks - sbase) + swz<kDecKeys>(row, piece);
+                                    *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + at * p.kp_ss +
+                                                              int64_t(h) * p.kp_hs + piece * 8) =
+                                        *reinterpret_cast<const uint4*>(kk);
+                                    *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + at * p.vp_ss +
+                                                              int64_t(h) * p.vp_hs + piece * 8) =
+                                        *reinterpret_cast<const uint4*>(kk + G::kHalf);
+                                }
                             }
                         }
                     }
+                    // the stage's next contents come through the TMA's proxy: what the
+                    // copies wrote is ordered before
+                    if (kf & kEdge) proxy_fence();
+                    __syncwarp();
+                    load();
                 }
-                // the stage's next contents come through the TMA's proxy: what the
-                // copies wrote is ordered before
-                if (kf & kEdge) proxy_fence();
-                __syncwarp();
-                load();
-              }
             }
 
             // The warps' sums meet: maxima first, then the rows, those of several
@@ -487,46 +452,41 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, MT>::kCtas)
             float* const sm = reinterpret_cast<float*>(smem + G::kStat) + 32;  // [4][MR]
             float* const sl = sm + kDecWarps * MR;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float y = l[mt][i];
-                    y += __shfl_xor_sync(0xffffffffu, y, 1);
-                    y += __shfl_xor_sync(0xffffffffu, y, 2);
-                    if ((lane & 3u) == 0) {
-                        const uint32_t row = mt * 16 + (lane >> 2) + 8 * i;
-                        sm[warp * MR + row] = m[mt][i] * p.c;
-                        sl[warp * MR + row] = y;
-                    }
+            for (int i = 0; i < 2; ++i) {
+                float y = l[i];
+                y += __shfl_xor_sync(0xffffffffu, y, 1);
+                y += __shfl_xor_sync(0xffffffffu, y, 2);
+                if ((lane & 3u) == 0) {
+                    const uint32_t row = (lane >> 2) + 8 * i;
+                    sm[warp * MR + row] = m[i] * p.c;
+                    sl[warp * MR + row] = y;
                 }
-            __syncthreads();  // (and the queries of MT 2 have been read)
+            }
+            __syncthreads();
             const uint32_t side = R * 4 <= MR ? 4 : R * 2 <= MR ? 2 : 1;
             for (uint32_t turn = 0; turn < kDecWarps / side; ++turn) {
                 if (warp / side == turn) {
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t row = (lane >> 2) + 8 * i, at = warp % side * uint32_t(R) + row;
+                        if (int32_t(row) >= R) continue;
+                        float mx = sm[row];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t row = mt * 16 + (lane >> 2) + 8 * i, at = warp % side * uint32_t(R) + row;
-                            if (int32_t(row) >= R) continue;
-                            float mx = sm[row];
+                        for (int w = 1; w < kDecWarps; ++w) mx = fmaxf(mx, sm[w * MR + row]);
+                        const float f = mx == -INFINITY ? 0.f : ex2(m[i] * p.c - mx);
+                        float* to = join + at * D + (lane & 3u) * 2;
 #pragma unroll
-                            for (int w = 1; w < kDecWarps; ++w) mx = fmaxf(mx, sm[w * MR + row]);
-                            const float f = mx == -INFINITY ? 0.f : ex2(m[mt][i] * p.c - mx);
-                            float* to = join + at * D + (lane & 3u) * 2;
-#pragma unroll
-                            for (int n = 0; n < 2 * KS; ++n) {
-                                float2* cell = reinterpret_cast<float2*>(to + ((n * 8) ^ (at & 7u) * 8));
-                                float2 v = make_float2(o[mt][n][2 * i] * f, o[mt][n][2 * i + 1] * f);
-                                if (turn) v.x += cell->x, v.y += cell->y;
-                                *cell = v;
-                            }
+                        for (int n = 0; n < 2 * KS; ++n) {
+                            float2* cell = reinterpret_cast<float2*>(to + ((n * 8) ^ (at & 7u) * 8));
+                            float2 v = make_float2(o[n][2 * i] * f, o[n][2 * i + 1] * f);
+                            if (turn) v.x += cell->x, v.y += cell->y;
+                            *cell = v;
                         }
+                    }
                 }
                 __syncthreads();
             }
-            if constexpr (MT == 1)
-                if (c + 1 < count) queries(segs[c + 1]);
+            if (c + 1 < count) queries(segs[c + 1]);
             // rows by warps, D / 32 elements of a row per lane
             constexpr int E = D / 32;
             const bool whole = x.j0 == 0 && steps == x.tiles;
@@ -595,10 +555,8 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, MT>::kCtas)
 #pragma unroll
                                 for (int k = 0; k < 8; ++k) {
                                     const float* from = piece(min(i0 + k0 + k, pieces - 1)) + row * D + lane * E;
-                                    if constexpr (E == 4)
-                                        *reinterpret_cast<float4*>(y[k]) = __ldcg(reinterpret_cast<const float4*>(from));
-                                    else
-                                        *reinterpret_cast<float2*>(y[k]) = __ldcg(reinterpret_cast<const float2*>(from));
+                                    using Vec = typename std::conditional<E == 4, float4, float2>::type;
+                                    *reinterpret_cast<Vec*>(y[k]) = __ldcg(reinterpret_cast<const Vec*>(from));
                                 }
                                 if (!k0) {  // the maximum may grow with each 32 pieces
                                     float nm = pm;
@@ -685,14 +643,11 @@ uint32_t sm_count() {
     }
     return uint32_t(sms);
 }
-// 16-row MMA tiles that hold the rows of an item of the decode kernel
-uint32_t dec_mt(const ls_b200_attention_args& a) {
-    return uint64_t(a.max_q) * (a.q_heads / a.kv_heads) <= 16 ? 1 : 2;
-}
-
 // Rows of a sequence and kv head beyond which the call goes to the 128-row
-// tensor-core tiles of ls_attention_chunk.cu.
-constexpr uint64_t kChunkRows = 32;
+// tensor-core tiles of ls_attention_chunk.cu: what one 16-row MMA tile holds.
+// (Two such tiles in the decode kernel: 90 us for 7 new tokens of 16 sequences
+// of up to 6000 slots, 28 rows, against 69 us there.)
+constexpr uint64_t kChunkRows = 16;
 bool is_chunk(const ls_b200_attention_args& a) {
     const uint32_t g = a.q_heads / a.kv_heads;
     return uint64_t(a.max_q) * g > kChunkRows;
@@ -718,7 +673,7 @@ ScratchPlan scratch_plan(const ls_b200_attention_args& a) {
         s.total = s.lse + (w ? up256(uint64_t(a.tokens) * a.q_heads * sizeof(float)) : 0);
         return s;
     }
-    s.lse = s.part + up256(2ull * kMaxCtas * 16 * dec_mt(a) * (a.head_dim + 2) * sizeof(float));
+    s.lse = s.part + up256(2ull * kMaxCtas * 16 * (a.head_dim + 2) * sizeof(float));
     s.logits = s.lse + (w ? up256(uint64_t(a.tokens) * a.q_heads * sizeof(float)) : 0);
     s.total = s.logits + (w ? up256(uint64_t(a.batch) * a.q_heads * a.weights_length * a.max_q * sizeof(float)) : 0);
     return s;
@@ -728,21 +683,21 @@ bool stride8(int64_t v) { return v % 8 == 0 && v >= 0; }
 
 // The call's shape: everything that does not depend on pointers.
 int check_shape(const ls_b200_attention_args& a) {
-    if (a.dtype > LS_B200_BF16 || !a.kv_heads || !a.q_heads || a.q_heads % a.kv_heads || a.q_heads / a.kv_heads > 128 || a.q_heads > 65536 ||
-        (a.head_dim != 64 && a.head_dim != 128))
+    if (a.dtype > LS_B200_BF16 || !a.kv_heads || !a.q_heads || a.q_heads % a.kv_heads || a.q_heads / a.kv_heads > 128 ||
+        a.q_heads > 65536 || (a.head_dim != 64 && a.head_dim != 128))
         return EINVAL;
     if (a.page_size < 16 || a.page_size > 256 || (a.page_size & (a.page_size - 1))) return EINVAL;
-    if (uint64_t(a.table_pages) * a.page_size > 0x7fffff00ull || a.pages > 0x7fffffffu || a.batch > (1u << 22) ||
+    if (uint64_t(a.table_pages) * a.page_size > kMaxSlots || a.pages > 0x7fffffffu || a.batch > (1u << 22) ||
         a.tokens > 0x7fffff00u || uint64_t(a.max_q) * (a.q_heads / a.kv_heads) > 0x3fffffffull ||
-        a.weights_length > 0x7fffff00u || a.window > 0x7fffffffu || a.sinks > 0x7fffffffu)
+        a.weights_length > kMaxSlots || a.window > 0x7fffffffu || a.sinks > 0x7fffffffu)
         return EINVAL;
     if (!(a.scale > 0.f) || std::isinf(a.scale) || a.timeout_ns > kMaxTimeoutNs) return EINVAL;
     return 0;
 }
 
-template <class T, int D, int MT>
+template <class T, int D>
 int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
-    using G = GeoD<D, MT>;
+    using G = GeoD<D>;
     CUtensorMap km, vm;
     const uint64_t dims[5] = {64, p.P, D / 64, p.Hkv, p.pages};
     const int64_t ks[4] = {p.kp_ss, 64, p.kp_hs, p.kp_ps}, vs[4] = {p.vp_ss, 64, p.vp_hs, p.vp_ps};
@@ -755,24 +710,18 @@ int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
     if (e != cudaSuccess) return int(e);
     const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
     if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(attn_decode_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        e = cudaFuncSetAttribute(attn_decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  int(G::kSmem));
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attn_decode_kernel<T, D, MT>, cudaFuncAttributePreferredSharedMemoryCarveout,
+            e = cudaFuncSetAttribute(attn_decode_kernel<T, D>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                      int(cudaSharedmemCarveoutMaxShared));
         if (e != cudaSuccess) return int(e);
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
     const uint32_t grid = sm_count() * uint32_t(G::kCtas);
-    attn_decode_kernel<T, D, MT><<<grid < kMaxCtas ? grid : kMaxCtas, kDecThreads, G::kSmem, s>>>(p, km, vm);
+    attn_decode_kernel<T, D><<<grid < kMaxCtas ? grid : kMaxCtas, kDecThreads, G::kSmem, s>>>(p, km, vm);
     return int(cudaGetLastError());
 }
-template <class T>
-int launch_decode(const AttnParams& p, bool bf16, uint32_t mt, cudaStream_t s) {
-    if (p.D == 64) return mt == 1 ? launch_decode<T, 64, 1>(p, bf16, s) : launch_decode<T, 64, 2>(p, bf16, s);
-    return mt == 1 ? launch_decode<T, 128, 1>(p, bf16, s) : launch_decode<T, 128, 2>(p, bf16, s);
-}
-
 }  // namespace
 }  // namespace lsb
 
@@ -845,10 +794,10 @@ int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
                              reinterpret_cast<float*>(scratch + plan.w_part)};
         return launch_chunk(p, a->dtype, c, sm_count(), s);
     }
-    const uint32_t mt = dec_mt(*a);
     p.fused = p.k_new != nullptr;
-    const int rc =
-        a->dtype == LS_B200_FP16 ? launch_decode<F16>(p, false, mt, s) : launch_decode<BF16>(p, true, mt, s);
+    const bool bf16 = a->dtype == LS_B200_BF16;
+    const int rc = p.D == 64 ? (bf16 ? launch_decode<BF16, 64>(p, true, s) : launch_decode<F16, 64>(p, false, s))
+                             : (bf16 ? launch_decode<BF16, 128>(p, true, s) : launch_decode<F16, 128>(p, false, s));
     if (rc || !p.weights) return rc;
     return int(launch_after(attn_weights_kernel, p.B * p.Hkv * ((p.wlen + 255) / 256), 256, 0, s, p));
 }

@@ -11,6 +11,8 @@ namespace lsb {
 constexpr uint32_t kErrLength = 1u << 1;  // a sequence's lengths do not fit the call
 constexpr uint32_t kErrPage = 1u << 2;    // a visible slot's page index is outside the pool
 
+constexpr uint32_t kMaxSlots = 0x7fff0000u;  // of a sequence: a tile past the last slot still counts in 32 bits
+
 // ls_b200_attention_args in the kernels' units. Strides are in elements.
 struct AttnParams {
     const uint16_t* q;

@@ -10,12 +10,13 @@
 //     O_i += P_i V             A from tensor memory, V read as it lies (N-major)
 // Each row tile has two S buffers of a half, so that the next S is there when
 // its warps end with one: they go from exponentials to exponentials, and the
-// tensor cores run beside them. (With one buffer of 128 slots per row tile the
-// warps waited for P V and the next S in turn: 882 us for a 4096-token chunk
-// over 16384 slots.) Roles of the warps: 0-3 and 4-7 the rows of Q0 and
-// Q1, 8 and 11 issue their MMAs, 9 the TMA loads (Q by item; K and V tiles through
-// one ring of 128-slot stages, one box per page and 64 elements), 10 lays out
-// the CTA's pieces of items for the others.
+// tensor cores run beside them. (With one buffer of 128 slots per row tile, its
+// P handed over in halves: 910 us for a 4096-token chunk over 16384 slots of
+// 128-element heads, against 860; 64-element heads 474 against 392 us.) Roles
+// of the warps: 0-3 and 4-7 the rows of Q0 and Q1, 8 and 11 issue their MMAs, 9
+// the TMA loads (Q by item; K and V tiles through one ring of 128-slot stages,
+// one box per page and 64 elements), 10 lays out the CTA's pieces of items for
+// the others.
 //
 // The running maximum is only raised when a row's maximum grows by more than
 // 2^8 (probabilities then stay below 2^8, exact in either 16-bit type's
@@ -52,7 +53,7 @@ struct Geo {
     static constexpr uint32_t kPanels = D / 64, kTile = kPanels * kPanel;
     static constexpr uint32_t kStages = D == 128 ? 5 : 8;
     static constexpr uint32_t kRing = 2 * kTile, kBars = kRing + kStages * kTile;
-    static constexpr uint32_t kSegs = kBars + 336;
+    static constexpr uint32_t kSegs = kBars + 320;
     static constexpr uint32_t kSmem = kSegs + 320 + 1024;  // + alignment of the swizzled tiles
 };
 static_assert(Geo<128>::kSmem <= 227 * 1024 && Geo<64>::kSmem <= 227 * 1024, "shared memory of a CTA");
@@ -442,35 +443,42 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int32_t all_lo =
                 p.window ? int32_t(max(int64_t(0), int64_t(w.pos0) + min(w.left, t_tile + per_tile) - p.window)) : 0;
             float m = -INFINITY, l = 0.f;  // reference maximum and sum of the row
-            at.begin(na, w.ha, hb);
-            for (; at.t < count; ++n) {
+            // waits for S of the next half and clears the values that no row sees:
+            // they may be anything, and 0 * NaN is not 0 (the other row tile's warps
+            // write the same zeros)
+            auto arrived = [&](bool there) {
+                if (!there && !warp_wait(bar.s_full(i, n & 1u), (n >> 1) & 1u, deadline)) return false;
                 const int32_t k0 = at.h * kHalf;
-                const uint32_t b = n & 1u, tb = ts + b * kHalf;
-                const bool last = at.t + 1 == count;
-                ok = warp_wait(bar.s_full(i, b), (n >> 1) & 1u, deadline);
-                if (last && at.t) ok = warp_wait(bar.o_done(i), no++ & 1u, deadline) && ok;  // the P V before
-                if (!ok) break;
-                if (!(k0 >= seen_lo && k0 + kHalf <= seen_hi) && k0 + kHalf > sink) {
-                    // slots that no row sees: their values may be anything, and 0 * NaN is
-                    // not 0 (the other row tile's warps write the same zeros)
-                    if (!(ok = warp_wait(bar.full(at.stage), at.odd & 1u, deadline))) break;
-                    const int32_t k = k0 + int32_t(r & 63u);
-                    if ((r >> 6) < G::kPanels && !((k >= seen_lo && k < seen_hi) || k < sink)) {
-                        uint8_t* v = base + G::kRing + at.stage * G::kTile + (r >> 6) * kPanel +
-                                     (uint32_t(at.h & 1) * kHalf + (r & 63u)) * 128;
+                if (at.t && at.t + 1 == count && !warp_wait(bar.o_done(i), no++ & 1u, deadline)) return false;
+                if ((k0 >= seen_lo && k0 + kHalf <= seen_hi) || k0 + kHalf <= sink) return true;
+                if (!warp_wait(bar.full(at.stage), at.odd & 1u, deadline)) return false;
+                const int32_t k = k0 + int32_t(r & 63u);
+                if ((r >> 6) < G::kPanels && !((k >= seen_lo && k < seen_hi) || k < sink)) {
+                    uint8_t* v = base + G::kRing + at.stage * G::kTile + (r >> 6) * kPanel +
+                                 (uint32_t(at.h & 1) * kHalf + (r & 63u)) * 128;
 #pragma unroll
-                        for (uint32_t e = 0; e < 8; ++e)
-                            *reinterpret_cast<uint4*>(v + e * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    proxy_fence();
-                    __syncwarp();
+                    for (uint32_t e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(v + e * 16) = make_uint4(0, 0, 0, 0);
                 }
-                if (busy) {
-                    fence_after();
-                    float x[kHalf];
-                    ld32(tb, x);
-                    ld32(tb + 32, x + 32);
-                    wait_ld();
+                proxy_fence();
+                __syncwarp();
+                return true;
+            };
+            auto advance = [&]() {  // P is there; on to the next half
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar.p_ready(i, n & 1u));
+                if (at.next(count, na, hb)) at.next_stage<G::kStages>();
+                ++n;
+            };
+            at.begin(na, w.ha, hb);
+            if (!busy) {
+                while (at.t < count && (ok = arrived(false))) advance();
+            } else if (count) {
+                // The halves overlap: while the exponentials of one are computed, the
+                // scores of the next come from tensor memory, and their maximum is
+                // taken as soon as P is handed over.
+                float x[kHalf], mx;
+                auto mask_and_max = [&]() {
+                    const int32_t k0 = at.h * kHalf;
                     if (k0 + kHalf > all_hi || k0 < all_lo) {
                         // columns [lo, hi) and those below s
                         const int32_t hi = pos + 1 - k0, s = p.window ? int32_t(p.sinks) - k0 : 0;
@@ -485,16 +493,29 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) top[e] = max3(top[e], x[c + e], x[c + 4 + e]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], x[kHalf - 4 + e]);
-                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                    const bool raise = m == -INFINITY ? mx > -INFINITY : (mx - m) * p.c > kRaise;
+                    for (int e = 0; e < 4; ++e) top[e] = max3(top[e], top[e], x[kHalf - 4 + e]);
+                    mx = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+                };
+                if ((ok = arrived(false))) {
+                    fence_after();
+                    ld32(ts + (n & 1u) * kHalf, x);
+                    ld32(ts + (n & 1u) * kHalf + 32, x + 32);
+                    wait_ld();
+                    mask_and_max();
+                }
+                while (ok) {
+                    const uint32_t tb = ts + (n & 1u) * kHalf, tn = ts + (~n & 1u) * kHalf;
+                    const bool last = at.t + 1 == count;
+                    // (written so that NaN raises too: the row is NaN from there on, as
+                    // it is for an infinite logit)
+                    const bool raise = m == -INFINITY ? mx != -INFINITY : !((mx - m) * p.c <= kRaise);
                     if (__any_sync(0xffffffffu, raise)) {
-                        const float nm = raise ? mx : m;
+                        const float nm = !raise ? m : mx == INFINITY ? NAN : mx;
                         const float f2 = nm == -INFINITY ? 1.f : ex2((m - nm) * p.c);
                         l *= f2;
                         m = nm;
                         if (at.t) {  // the P V before has to be in O: it is when the next S is there
-                            if (!last && !warp_wait(bar.s_full(i, b ^ 1u), ((n + 1) >> 1) & 1u, deadline)) ok = false;
+                            if (!last && !warp_wait(bar.s_full(i, ~n & 1u), ((n + 1) >> 1) & 1u, deadline)) ok = false;
                             fence_after();
 #pragma unroll
                             for (int c = 0; c < D; c += 16) {
@@ -510,26 +531,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float ref = m == -INFINITY ? 0.f : -m * p.c;
                     const uint64_t c2 = pack2(p.c, p.c), ref2 = pack2(ref, ref);
                     uint64_t sum[2] = {0, 0};
-                    uint32_t pk[kHalf / 2];
+                    auto probabilities = [&](const float* y, uint32_t to_p) {  // of 32 columns
+                        uint32_t pk[16];
 #pragma unroll
-                    for (int e = 0; e < kHalf / 2; ++e) {
-                        float a, d;
-                        unpack2(fma2(pack2(x[2 * e], x[2 * e + 1]), c2, ref2), a, d);
-                        a = ex2(a);
-                        d = ex2(d);
-                        sum[e & 1] = add2(sum[e & 1], pack2(a, d));
-                        pk[e] = T::pack(a, d);
+                        for (int e = 0; e < 16; ++e) {
+                            float a, d;
+                            unpack2(fma2(pack2(y[2 * e], y[2 * e + 1]), c2, ref2), a, d);
+                            a = ex2(a), d = ex2(d);
+                            sum[e & 1] = add2(sum[e & 1], pack2(a, d));
+                            pk[e] = T::pack(a, d);
+                        }
+                        st16(to_p, pk);
+                    };
+                    probabilities(x, tb);
+                    // (128-element heads are bound by the tensor cores, and by the power
+                    // that they draw: there the early read costs 860 -> 942 us for a
+                    // 4096-token chunk over 16384 slots; 64-element heads, bound by the
+                    // exponentials, gain 436 -> 392 us for two chunks of 3000 tokens)
+                    const bool early = D == 64 && !last &&
+                                       __all_sync(0xffffffffu, bar_try(bar.s_full(i, ~n & 1u), ((n + 1) >> 1) & 1u));
+                    if (early) {
+                        fence_after();
+                        ld32(tn, x);
                     }
-                    st32(tb, pk);
+                    probabilities(x + 32, tb + 16);
                     float s0, s1;
                     unpack2(add2(sum[0], sum[1]), s0, s1);
                     l += s0 + s1;
                     wait_st();
                     fence_before();
+                    advance();
+                    if (last || !(ok = arrived(early))) break;
+                    fence_after();
+                    if (!early) ld32(tn, x);
+                    ld32(tn + 32, x + 32);
+                    wait_ld();
+                    mask_and_max();
                 }
-                __syncwarp();
-                if (lane == 0) bar_arrive(bar.p_ready(i, b));
-                if (at.next(count, na, hb)) at.next_stage<G::kStages>();
             }
             const bool any = count != 0;  // (otherwise O is not written)
             if (any && ok) ok = warp_wait(bar.o_done(i), no++ & 1u, deadline);
@@ -623,12 +661,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 c.next_stage<G::kStages>();
             };
             auto step_s = [&](uint32_t b) {  // S of the next half, into buffer b
-                const uint32_t k = k_lo + cs.stage * (G::kTile / 16) + (cs.h & 1) * (kHalf * 128 / 16);
+                const uint32_t k = uniform(k_lo + cs.stage * (G::kTile / 16) + (cs.h & 1) * (kHalf * 128 / 16));
+                const uint32_t d = uniform(t_s + b * kHalf), q = uniform(q_lo);
                 if (lead) {
 #pragma unroll
                     for (uint32_t x = 0; x < D / 16; ++x) {
                         const uint32_t off = ((x / 4) * kPanel + (x % 4) * 32) / 16;
-                        mma_ss(t_s + b * kHalf, desc_of<1024>(q_lo + off), desc_of<1024>(k + off), kIs, x > 0);
+                        mma_ss(d, desc_of<1024>(q + off), desc_of<1024>(k + off), kIs, x > 0);
                     }
                     commit(bar.s_full(i, b));
                 }
@@ -646,11 +685,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                            warp_wait(bar.p_ready(i, b), (n >> 1) & 1u, deadline)))
                     break;
                 fence_after();
-                const uint32_t v = v_lo + cp.stage * (G::kTile / 16) + (cp.h & 1) * (kHalf * 128 / 16);
+                const uint32_t v = uniform(v_lo + cp.stage * (G::kTile / 16) + (cp.h & 1) * (kHalf * 128 / 16));
+                const uint32_t pt = uniform(t_s + b * kHalf), ot = uniform(t_o);
                 if (lead) {
 #pragma unroll
                     for (uint32_t x = 0; x < kHalf / 16; ++x)
-                        mma_ts(t_o, t_s + b * kHalf + x * 8, desc_of<1024>(v + x * 128), kIo, x > 0 || cp.t > 0);
+                        mma_ts(ot, pt + x * 8, desc_of<1024>(v + x * 128), kIo, x > 0 || cp.t > 0);
                     if (!more) commit(bar.o_done(i));
                 }
                 if (more) step_s(b);
