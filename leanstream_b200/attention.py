@@ -40,9 +40,14 @@ def _element(dtype) -> torch.dtype:
     return got
 
 
-def _handle(stream) -> int:
+# torch's current stream as an integer, without the stream object around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _handle(stream, device: int) -> int:
     if stream is None:
-        stream = torch.cuda.current_stream()
+        return _raw_stream(device)
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
@@ -75,6 +80,8 @@ class PagedAttention:
         self.max_sequences, self.max_tokens = max_sequences, max_tokens
         self.max_queries, self.max_weights_length = max_queries, max_weights_length
         self._code, self._scale = _CODES[self.dtype], head_dim ** -0.5 if head_dim > 0 else 1.0
+        self._row, self._page, self._new = (q_heads, head_dim), (page_size, kv_heads, head_dim), (kv_heads, head_dim)
+        self._call = self.lib.ls_b200_paged_attention
         shape = N.AttentionArgs(dtype=self._code, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim,
                                 page_size=page_size, batch=max_sequences, tokens=max_tokens, max_q=max_queries,
                                 weights_length=max_weights_length, scale=1.0)
@@ -131,55 +138,55 @@ class PagedAttention:
         max_q: the most new tokens of one sequence. scale: 1 / sqrt(head_dim)
         unless given. lse [tokens][q_heads] and weights [sequences][kv_heads]
         [slots] float32, optional."""
-        e, hq, hk, dim = self.dtype, self.q_heads, self.kv_heads, self.head_dim
-        tokens, batch, pages = len(q) if q.dim() else 0, len(kv_len) if kv_len.dim() else 0, len(k_pages)
-        pool, table_shape = (pages, self.page_size, hk, dim), page_table.shape
-        kn = vn = ls = ws = length = 0
-        kn0 = kn1 = vn0 = vn1 = ws0 = ws1 = 0
-        good = (q.dtype is e and output.dtype is e and k_pages.dtype is e and v_pages.dtype is e and
-                q.shape == (tokens, hq, dim) and output.shape == q.shape and k_pages.shape == pool and
-                v_pages.shape == pool and kv_len.dtype is _INT and page_table.dtype is _INT and
-                q_start.dtype is _INT and kv_len.dim() == 1 and len(table_shape) == 2 and
-                table_shape[0] == batch and q_start.shape == (batch + 1,) and q.is_cuda and output.is_cuda and
-                k_pages.is_cuda and v_pages.is_cuda and page_table.is_cuda and q_start.is_cuda and kv_len.is_cuda and
-                tokens <= self.max_tokens and batch <= self.max_sequences and max_q <= self.max_queries and
-                max_q >= 0 and window >= 0 and sinks >= 0 and (k_new is None) == (v_new is None))
-        if good and k_new is not None:
-            kn, vn = k_new.data_ptr(), v_new.data_ptr()
-            kn0, kn1, last = k_new.stride()
-            vn0, vn1, last2 = v_new.stride()
-            good = (k_new.dtype is e and v_new.dtype is e and k_new.shape == (tokens, hk, dim) and
-                    v_new.shape == (tokens, hk, dim) and k_new.is_cuda and v_new.is_cuda and
-                    (last == last2 == 1 or not tokens))
-        if good and lse is not None:
-            ls = lse.data_ptr()
-            good = lse.dtype is _FLOAT and lse.shape == (tokens, hq) and lse.is_contiguous() and lse.is_cuda
-        if good and weights is not None:
-            ws, shape = weights.data_ptr(), weights.shape
-            good = weights.dtype is _FLOAT and len(shape) == 3 and shape[0] == batch and shape[1] == hk and \
-                shape[2] <= self.max_weights_length and weights.is_cuda
-            if good:
-                length = shape[2]
-                ws0, ws1, last = weights.stride()
-                good = last == 1 or not weights.numel()
+        # one pass over the tensors: each attribute of a tensor costs about 0.1 us
+        e, rows, pool = self.dtype, q.shape, k_pages.shape
+        table, lengths = page_table.shape, kv_len.shape
+        kn = vn = ls = ws = slots = kn0 = kn1 = vn0 = vn1 = ws0 = ws1 = q0 = q1 = o0 = o1 = t0 = 0
+        k0 = k1 = k2 = v0 = v1 = v2 = batch = tokens = 0
+        good = (len(rows) == 3 and rows[1:] == self._row and len(pool) == 4 and pool[1:] == self._page and
+                len(table) == 2 and len(lengths) == 1 and output.shape == rows and v_pages.shape == pool and
+                q.dtype is e and output.dtype is e and k_pages.dtype is e and v_pages.dtype is e and
+                page_table.dtype is _INT and kv_len.dtype is _INT and q_start.dtype is _INT and q.is_cuda and
+                output.is_cuda and k_pages.is_cuda and v_pages.is_cuda and page_table.is_cuda and kv_len.is_cuda and
+                q_start.is_cuda and window >= 0 and sinks >= 0 and 0 <= max_q <= self.max_queries)
         if good:
+            tokens, batch = rows[0], lengths[0]
             q0, q1, a = q.stride()
             o0, o1, b = output.stride()
             k0, k1, k2, c = k_pages.stride()
             v0, v1, v2, d = v_pages.stride()
             t0, f = page_table.stride()
-            good = (a == b == 1 or not tokens) and (c == d == 1 or not pages) and \
-                (f == 1 or not page_table.numel()) and kv_len.is_contiguous() and q_start.is_contiguous()
+            good = (table[0] == batch <= self.max_sequences and tokens <= self.max_tokens and
+                    (a == b == 1 or not tokens) and (c == d == 1 or not pool[0]) and (f == 1 or not table[1]) and
+                    q_start.shape == (batch + 1,) and kv_len.is_contiguous() and q_start.is_contiguous() and
+                    (k_new is None) == (v_new is None))
+        if good and k_new is not None:
+            kn, vn = k_new.data_ptr(), v_new.data_ptr()
+            kn0, kn1, a = k_new.stride()
+            vn0, vn1, b = v_new.stride()
+            good = (k_new.shape == v_new.shape == (tokens, *self._new) and k_new.dtype is e and v_new.dtype is e and
+                    k_new.is_cuda and v_new.is_cuda and (a == b == 1 or not tokens))
+        if good and lse is not None:
+            ls = lse.data_ptr()
+            good = lse.shape == rows[:2] and lse.dtype is _FLOAT and lse.is_contiguous() and lse.is_cuda
+        if good and weights is not None:
+            ws, wide = weights.data_ptr(), weights.shape
+            good = weights.dtype is _FLOAT and wide[:2] == (batch, self.kv_heads) and len(wide) == 3 and \
+                wide[2] <= self.max_weights_length and weights.is_cuda
+            if good:
+                slots = wide[2]
+                ws0, ws1, a = weights.stride()
+                good = a == 1 or not weights.numel()
         if not good:
             self._refuse(q, output, k_pages, v_pages, page_table, q_start, kv_len, max_q, k_new, v_new, lse, weights,
                          window, sinks)
-        a = _ATTENTION.pack(
-            self._code, hq, hk, dim, self.page_size, pages, batch, tokens, max_q, table_shape[1], window, sinks,
-            self._scale if scale is None else scale, length, q.data_ptr(), kn, vn, k_pages.data_ptr(),
-            v_pages.data_ptr(), page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), output.data_ptr(), ls, ws,
-            q0, q1, kn0, kn1, vn0, vn1, k0, k1, k2, v0, v1, v2, o0, o1, t0, ws0, ws1, self.scratch_ptr,
-            self.scratch_bytes, self.error_ptr, timeout_ns)
-        rc = self.lib.ls_b200_paged_attention(a, _handle(stream))
+        args = _ATTENTION.pack(
+            self._code, self.q_heads, self.kv_heads, self.head_dim, self.page_size, pool[0], batch, tokens, max_q,
+            table[1], window, sinks, self._scale if scale is None else scale, slots, q.data_ptr(), kn, vn,
+            k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
+            output.data_ptr(), ls, ws, q0, q1, kn0, kn1, vn0, vn1, k0, k1, k2, v0, v1, v2, o0, o1, t0, ws0, ws1,
+            self.scratch_ptr, self.scratch_bytes, self.error_ptr, timeout_ns)
+        rc = self._call(args, _raw_stream(q.get_device()) if stream is None else _handle(stream, 0))
         if rc:
             _check(rc, "ls_b200_paged_attention")
 
@@ -228,9 +235,10 @@ def evict_cache(*, k_pages, v_pages, page_table, kv_len, weights, budget: int, n
     optional int32 device tensor, N.ATTN_* bits are ORed in. `stream` as in
     PagedAttention.run."""
     pool, table, new, wide = k_pages.shape, page_table.shape, new_table.shape, weights.shape
-    batch = len(kv_len) if kv_len.dim() else 0
+    lengths = kv_len.shape
+    batch = lengths[0] if lengths else 0
     good = (len(pool) == 4 and len(table) == len(new) == 2 and len(wide) == 3 and k_pages.dtype in _CODES and
-            v_pages.dtype is k_pages.dtype and v_pages.shape == pool and kv_len.dim() == 1 and
+            v_pages.dtype is k_pages.dtype and v_pages.shape == pool and len(lengths) == 1 and
             kv_len.dtype is _INT and page_table.dtype is _INT and new_table.dtype is _INT and
             weights.dtype is _FLOAT and new_len.dtype is _INT and kept.dtype is _INT and table[0] == batch and
             new[0] == batch and wide[0] == batch and wide[1] == pool[2] and new_len.shape == (batch,) and
@@ -261,6 +269,6 @@ def evict_cache(*, k_pages, v_pages, page_table, kv_len, weights, budget: int, n
                        k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), new_table.data_ptr(),
                        kv_len.data_ptr(), weights.data_ptr(), new_len.data_ptr(), kept.data_ptr(), nw, k0, k1, k2, v0,
                        v1, v2, t0, n0, w0, w1, er)
-    rc = N.load().ls_b200_evict_cache(args, _handle(stream))
+    rc = N.load().ls_b200_evict_cache(args, _handle(stream, kv_len.get_device()))
     if rc:
         _check(rc, "ls_b200_evict_cache")

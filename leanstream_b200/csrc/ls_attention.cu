@@ -635,12 +635,19 @@ constexpr uint64_t kMaxTimeoutNs = 60000000000ull;
 constexpr uint64_t kTimeoutNs = 2000000000ull;
 
 uint32_t sm_count() {
+    static std::atomic<uint32_t> known[16];
     int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
+    if (cudaGetDevice(&dev) != cudaSuccess) {
         cudaGetLastError();
         return 148;
     }
+    const bool slot = dev >= 0 && dev < 16;
+    if (const uint32_t n = slot ? known[dev].load(std::memory_order_relaxed) : 0) return n;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
+        cudaGetLastError();
+        return 148;
+    }
+    if (slot) known[dev].store(uint32_t(sms), std::memory_order_relaxed);
     return uint32_t(sms);
 }
 // Rows of a sequence and kv head beyond which the call goes to the 128-row
