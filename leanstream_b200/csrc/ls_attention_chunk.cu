@@ -82,6 +82,8 @@ template <bool WEIGHTS>
 __device__ void lay_out(const AttnParams& p, ChunkPlan* plan, ChunkItem* list, int32_t cap, uint32_t grid) {
     __shared__ int32_t first[257];  // items before each sequence of the batch piece
     __shared__ int64_t wsum[8];
+    constexpr uint32_t kShared = 1024;
+    __shared__ int64_t before_item[kShared];  // units before the first items, for the search below
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t per_tile = int32_t(chunk_tokens(p.g));
     int32_t items = 0;
@@ -140,7 +142,10 @@ __device__ void lay_out(const AttnParams& p, ChunkPlan* plan, ChunkItem* list, i
             }
             const int64_t sum = scan(int64_t(it.tiles) * p.Hkv, before);
             it.units = units + before;
-            if (i < total) list[items + i] = it;
+            if (i < total) {
+                list[items + i] = it;
+                if (items + i < int32_t(kShared)) before_item[items + i] = it.units;
+            }
             units += sum;
         }
         items += total;
@@ -156,11 +161,15 @@ __device__ void lay_out(const AttnParams& p, ChunkPlan* plan, ChunkItem* list, i
     }
     for (uint32_t c = tid; c < kMaxCtas; c += 256) plan->open[c] = make_int2(-1, 0);
     __syncthreads();
-    for (int32_t i = int32_t(tid); i < items; i += 256) {  // what this block wrote
-        const int64_t u = list[i].units, end = u + int64_t(list[i].tiles) * p.Hkv;
-        if (u < end)
-            for (int64_t c = (u * G + units - 1) / units; c < G && cut_begin(units, G, c) < end; ++c)
-                plan->start[c] = i;
+    for (int64_t c = tid; c < G && items; c += 256) {  // the item that holds the CTA's first unit
+        const int64_t u = cut_begin(units, G, c);
+        int32_t at = 0, end = items;
+        while (end - at > 1) {
+            const int32_t mid = (at + end) / 2;
+            if ((mid < int32_t(kShared) ? before_item[mid] : list[mid].units) <= u) at = mid;
+            else end = mid;
+        }
+        plan->start[c] = at;
     }
 }
 
@@ -603,8 +612,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     } else if (real) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<float4*>(part + row * D + c + e) =
+                        for (int e = 0; e < 32; e += 4)  // (rows side by side)
+                            *reinterpret_cast<float4*>(part + ((c + e) * 256 + row * 4)) =
                                 make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                     }
                     __syncwarp();
@@ -711,100 +720,73 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Joins the parts of one item cut over several CTAs: CTA (c, block of 32 rows),
-// for the item that begins in c and goes on; a warp takes four rows, a lane
-// D / 32 elements of each (lane k the statistics of part k).
+// Joins the parts of one item cut over several CTAs: block (c, 16 columns), for
+// the item that begins in CTA c and goes on; one thread per row. A part holds its
+// sums as [D / 4][256 rows][4], then the rows' maxima and sums.
 template <class T, int D>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const AttnParams p, const ChunkScratch sc) {
-    constexpr int E = D / 32, kRowsPerWarp = 4;
+    constexpr int64_t kPart = 256 * (D + 2);
+    constexpr int kBatch = 4;  // parts under way at a time
     after_start();
     after_wait();
     const int2 open = sc.plan->open[blockIdx.x];
     if (open.x < 0) return;
     const int64_t U = sc.plan->units, G = sc.plan->ctas;
     const ChunkItem it = sc.items[open.x];
-    const uint32_t lane = threadIdx.x & 31, row0 = blockIdx.y * 32 + (threadIdx.x >> 5) * kRowsPerWarp;
+    const uint32_t row = threadIdx.x, r = row & 127u;
     const int32_t per_tile = int32_t(chunk_tokens(p.g));
+    const int32_t lt = int32_t(r / p.g), t = it.t0 + int32_t(row >> 7) * per_tile + lt;
+    if (lt >= per_tile || t >= it.nq) return;
     const int64_t item = it.units + int64_t(open.y) * it.tiles;
     const int64_t c0 = blockIdx.x, c1 = cut_owner(U, G, item + it.tiles - 1);
     const int32_t parts = int32_t(c1 - c0) + 1;
-    constexpr int64_t kPart = 256 * (D + 2);
     const float* const p0 = sc.part + (2 * c0 + (cut_begin(U, G, c0) != item)) * kPart;
-    auto part = [&](int32_t i) { return i ? sc.part + 2 * (c0 + i) * kPart : p0; };
-    float mx[kRowsPerWarp], sum[kRowsPerWarp], v[kRowsPerWarp][E];
-    bool real[kRowsPerWarp], any = false;
-    int32_t token[kRowsPerWarp], head[kRowsPerWarp];
+    float mx = -INFINITY, sum = 0.f;
+    float4 v[4] = {};
+    for (int32_t i0 = 0; i0 < parts; i0 += kBatch) {
+        float pm[kBatch], ps[kBatch];
+        float4 y[kBatch][4];
 #pragma unroll
-    for (int x = 0; x < kRowsPerWarp; ++x) {
-        const uint32_t row = row0 + x, r = row & 127u;
-        const int32_t lt = int32_t(r / p.g), t = it.t0 + int32_t(row >> 7) * per_tile + lt;
-        real[x] = lt < per_tile && t < it.nq;
-        any = any || real[x];
-        token[x] = it.q0 + t;
-        head[x] = open.y * int32_t(p.g) + int32_t(r % p.g);
-        mx[x] = -INFINITY;
-        sum[x] = 0.f;
+        for (int k = 0; k < kBatch; ++k) {
+            const int32_t i = min(i0 + k, parts - 1);
+            const float* from = i ? sc.part + 2 * (c0 + i) * kPart : p0;
+            pm[k] = i0 + k < parts ? from[256 * D + row] : -INFINITY;
+            ps[k] = from[256 * D + 256 + row];
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[x][e] = 0.f;
-    }
-    if (!any) return;
-    for (int32_t i0 = 0; i0 < parts; i0 += 32) {
-        const int32_t i = i0 + int32_t(lane), n = min(32, parts - i0);
-        float f[kRowsPerWarp];
-#pragma unroll
-        for (int x = 0; x < kRowsPerWarp; ++x) {
-            const bool on = i < parts && real[x];
-            const float pm = on ? part(i)[256 * D + row0 + x] : -INFINITY;
-            const float ps = on ? part(i)[256 * D + 256 + row0 + x] : 0.f;
-            float nm = pm;
-#pragma unroll
-            for (int d = 16; d; d >>= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, d));
-            nm = fmaxf(nm, mx[x]);
-            const float ref = nm == -INFINITY ? 0.f : nm, old = ex2(mx[x] - ref);
-            f[x] = ex2(pm - ref);
-            sum[x] = fmaf(f[x], ps, sum[x] * old);
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[x][e] *= old;
-            mx[x] = nm;
+            for (int e = 0; e < 4; ++e)
+                y[k][e] = *reinterpret_cast<const float4*>(from + ((blockIdx.y * 4 + e) * 256 + row) * 4);
         }
-#pragma unroll 2
-        for (int32_t k = 0; k < n; ++k) {
-            const float* from = part(i0 + k) + row0 * D + lane * E;
-            float y[kRowsPerWarp][E];
+        float nm = mx;
 #pragma unroll
-            for (int x = 0; x < kRowsPerWarp; ++x) {
+        for (int k = 0; k < kBatch; ++k) nm = fmaxf(nm, pm[k]);
+        const float ref = nm == -INFINITY ? 0.f : nm, old = ex2(mx - ref);
+        mx = nm;
+        sum *= old;
 #pragma unroll
-                for (int e = 0; e < E; ++e) y[x][e] = 0.f;
-                if (!real[x]) continue;
-                if constexpr (E == 4)
-                    *reinterpret_cast<float4*>(y[x]) = *reinterpret_cast<const float4*>(from + x * D);
-                else
-                    *reinterpret_cast<float2*>(y[x]) = *reinterpret_cast<const float2*>(from + x * D);
-            }
+        for (int e = 0; e < 4; ++e) v[e].x *= old, v[e].y *= old, v[e].z *= old, v[e].w *= old;
 #pragma unroll
-            for (int x = 0; x < kRowsPerWarp; ++x) {
-                const float fk = __shfl_sync(0xffffffffu, f[x], k);
+        for (int k = 0; k < kBatch; ++k) {
+            const float f = ex2(pm[k] - ref);
+            sum = fmaf(f, ps[k], sum);
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[x][e] = fmaf(fk, y[x][e], v[x][e]);
+            for (int e = 0; e < 4; ++e) {
+                v[e].x = fmaf(f, y[k][e].x, v[e].x), v[e].y = fmaf(f, y[k][e].y, v[e].y);
+                v[e].z = fmaf(f, y[k][e].z, v[e].z), v[e].w = fmaf(f, y[k][e].w, v[e].w);
             }
         }
     }
-#pragma unroll
-    for (int x = 0; x < kRowsPerWarp; ++x) {
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], d);
-        if (!real[x]) continue;
-        const float inv = sum[x] > 0.f ? 1.f / sum[x] : sum[x] == 0.f ? 0.f : NAN;
-        uint16_t* out = p.out + int64_t(token[x]) * p.o_ts + int64_t(head[x]) * p.o_hs + lane * E;
-        if constexpr (E == 4)
-            *reinterpret_cast<uint2*>(out) =
-                make_uint2(T::pack(v[x][0] * inv, v[x][1] * inv), T::pack(v[x][2] * inv, v[x][3] * inv));
-        else
-            *reinterpret_cast<uint32_t*>(out) = T::pack(v[x][0] * inv, v[x][1] * inv);
-        if (lane == 0 && p.lse)
-            p.lse[int64_t(token[x]) * p.Hq + head[x]] =
-                sum[x] == 0.f ? -INFINITY : (mx[x] + lg2(sum[x])) * kLn2;
-    }
+    const int64_t token = it.q0 + t;
+    const int32_t head = open.y * int32_t(p.g) + int32_t(r % p.g);
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+    uint4 w[2];
+    w[0] = make_uint4(T::pack(v[0].x * inv, v[0].y * inv), T::pack(v[0].z * inv, v[0].w * inv),
+                      T::pack(v[1].x * inv, v[1].y * inv), T::pack(v[1].z * inv, v[1].w * inv));
+    w[1] = make_uint4(T::pack(v[2].x * inv, v[2].y * inv), T::pack(v[2].z * inv, v[2].w * inv),
+                      T::pack(v[3].x * inv, v[3].y * inv), T::pack(v[3].z * inv, v[3].w * inv));
+    uint16_t* out = p.out + token * p.o_ts + int64_t(head) * p.o_hs + blockIdx.y * 16;
+    *reinterpret_cast<uint4*>(out) = w[0];
+    *reinterpret_cast<uint4*>(out + 8) = w[1];
+    if (!blockIdx.y && p.lse) p.lse[token * p.Hq + head] = sum == 0.f ? -INFINITY : (mx + lg2(sum)) * kLn2;
 }
 
 // weights[b, h, slot] of a call, once the rows' lse are known: per tile of 128
@@ -1142,7 +1124,7 @@ int launch(const AttnParams& p, bool bf16, const ChunkScratch& s, uint32_t grid,
     e = cudaGetLastError();
     if (e == cudaSuccess)
         e = launch_after(chunk_attn_kernel<T, D>, grid, kThreads, Geo<D>::kSmem, stream, p, s, qm, km, vm);
-    if (e == cudaSuccess) e = launch_after(chunk_join_kernel<T, D>, dim3(grid, 8), 256, 0, stream, p, s);
+    if (e == cudaSuccess) e = launch_after(chunk_join_kernel<T, D>, dim3(grid, D / 16), 256, 0, stream, p, s);
     if (e != cudaSuccess || !p.weights) return int(e);
     return launch_chunk_weights<T, D>(p, s, grid, qm, km, stream);
 }
