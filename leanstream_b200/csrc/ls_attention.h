@@ -198,10 +198,14 @@ __device__ __forceinline__ int64_t cut_begin(int64_t U, int64_t G, int64_t c) { 
 __device__ __forceinline__ int64_t cut_owner(int64_t U, int64_t G, int64_t u) { return ((u + 1) * G - 1) / U; }
 
 // The pieces of items that a CTA works on, in order.
+// Each (item, kv head) counts as kItemCost tiles more than it has: its start,
+// its end and its masked tiles. With 0, 1, 2 and 4 the attention of 2 x 1024 new
+// tokens took 141, 139, 135, 135 us, and its weights with 0, 2, 4 85, 71, 69.
+constexpr int kItemCost = 2;
 struct Walk {
     int64_t U, G, u, u_begin, u_end;
     int64_t item;  // first unit of (item, kv head)
-    int32_t i, h, j0, steps;
+    int32_t i, h, j0, steps, taken;
     ChunkItem it;
     __device__ bool begin(const ChunkPlan* plan) {
         U = plan->units;
@@ -210,20 +214,23 @@ struct Walk {
         u = u_begin = cut_begin(U, G, blockIdx.x);
         u_end = cut_begin(U, G, blockIdx.x + 1);
         i = plan->start[blockIdx.x] - 1;
-        it.units = it.tiles = steps = 0;
+        it.units = it.tiles = taken = 0;
         return true;
     }
     __device__ bool next(const AttnParams& p, const ChunkPlan* plan, const ChunkItem* items) {
-        u += steps;
-        if (u >= u_end) return false;
-        while (u >= it.units + int64_t(it.tiles) * p.Hkv || !it.tiles) {
-            if (++i >= plan->items) return false;
-            it = items[i];
-        }
-        h = int32_t((u - it.units) / it.tiles);
-        item = it.units + int64_t(h) * it.tiles;
-        j0 = int32_t(u - item);
-        steps = int32_t(min(u_end, item + it.tiles) - u);
+        do {
+            u += taken;
+            if (u >= u_end) return false;
+            while (u >= it.units + int64_t(it.tiles + kItemCost) * p.Hkv || !it.tiles) {
+                if (++i >= plan->items) return false;
+                it = items[i];
+            }
+            h = int32_t((u - it.units) / (it.tiles + kItemCost));
+            item = it.units + int64_t(h) * (it.tiles + kItemCost);
+            j0 = int32_t(u - item);
+            taken = int32_t(min(u_end, item + it.tiles + kItemCost) - u);
+            steps = min(taken, it.tiles - j0);
+        } while (steps <= 0);
         return true;
     }
 };

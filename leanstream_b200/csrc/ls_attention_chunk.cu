@@ -33,6 +33,7 @@
 
 #include <atomic>
 #include <cerrno>
+#include <type_traits>
 
 #include "ls_attention.h"
 #include "ls_tc.h"
@@ -140,7 +141,7 @@ __device__ void lay_out(const AttnParams& p, ChunkPlan* plan, ChunkItem* list, i
                     it.tiles = key_range<kKeys>(p, q, it.t0, min(q.nq, it.t0 + 2 * per_tile)).tiles;
                 }
             }
-            const int64_t sum = scan(int64_t(it.tiles) * p.Hkv, before);
+            const int64_t sum = scan(it.tiles ? int64_t(it.tiles + kItemCost) * p.Hkv : 0, before);
             it.units = units + before;
             if (i < total) {
                 list[items + i] = it;
@@ -737,7 +738,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const AttnParams p, con
     const int32_t per_tile = int32_t(chunk_tokens(p.g));
     const int32_t lt = int32_t(r / p.g), t = it.t0 + int32_t(row >> 7) * per_tile + lt;
     if (lt >= per_tile || t >= it.nq) return;
-    const int64_t item = it.units + int64_t(open.y) * it.tiles;
+    const int64_t item = it.units + int64_t(open.y) * (it.tiles + kItemCost);
     const int64_t c0 = blockIdx.x, c1 = cut_owner(U, G, item + it.tiles - 1);
     const int32_t parts = int32_t(c1 - c0) + 1;
     const float* const p0 = sc.part + (2 * c0 + (cut_begin(U, G, c0) != item)) * kPart;
@@ -792,16 +793,24 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const AttnParams p, con
 // weights[b, h, slot] of a call, once the rows' lse are known: per tile of 128
 // slots and row tile S^T = K Q^T (M the slots, N the rows), then each thread
 // sums exp2(S c - lse) over the rows of its slot, with no exchange between
-// threads and in a fixed order. Warps 0-3 and 4-7 take the row tiles in turn; two score buffers each in
-// tensor memory let the MMAs run ahead. A slot tile cut over several CTAs is
-// summed, in order, by the one that arrives last. The exponentials bound it:
-// 128 x 128 of them per 2 * 128^2 * head_dim operations.
+// threads and in a fixed order. Four groups of four warps take the row tiles in
+// turn, a score buffer in tensor memory each, so that the MMAs of one run under
+// the sums of the others. A slot tile cut over several CTAs is summed, in order,
+// by the one that arrives last. The exponentials bound it: 128 x 128 of them per
+// 2 * 128^2 * head_dim operations. Two sequences of
+// up to 4096 slots, 1024 tokens each, 32 heads of 128 over 8: 71 us, 47 us of
+// them the exponentials at 16 a clock and SM. (With two groups 103 us; 85 us
+// before short items were charged for their start.)
+constexpr uint32_t kGroups = 4, kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1, kLseWarp = kMmaWarp + 1;
+constexpr uint32_t kThreadsW = 32 * (kLseWarp + 1), kLses = 8;
+
 template <int D>
 struct GeoW {
     static constexpr uint32_t kPanels = D / 64, kTile = kPanels * kPanel, kStages = 4;
     static constexpr uint32_t kRing = 2 * kTile, kBars = kRing + kStages * kTile;  // two K tiles, then Q tiles
-    static constexpr uint32_t kLse = kBars + 512;                                  // [2 groups][2][128] floats
-    static constexpr uint32_t kSmem = kLse + 2048 + 1024;
+    static constexpr uint32_t kLse = kBars + 512;           // [kLses][128] floats
+    static constexpr uint32_t kSums = kLse + kLses * 512;  // [2][groups][128]
+    static constexpr uint32_t kSmem = kSums + 2 * kGroups * 512 + 1024;
 };
 struct BarsW {
     uint32_t base;
@@ -811,9 +820,12 @@ struct BarsW {
     __device__ uint32_t q_empty(uint32_t i) const { return base + 8 * (8 + i); }
     __device__ uint32_t s_full(uint32_t i) const { return base + 8 * (12 + i); }
     __device__ uint32_t s_empty(uint32_t i) const { return base + 8 * (16 + i); }
-    __device__ uint32_t sums() const { return base + 8 * 20; }
-    __device__ uint32_t summed() const { return base + 8 * 21; }
-    __device__ uint32_t drain() const { return base + 8 * 22; }
+    __device__ uint32_t sums(uint32_t i) const { return base + 8 * (20 + i); }
+    __device__ uint32_t summed(uint32_t i) const { return base + 8 * (22 + i); }
+    __device__ uint32_t drain() const { return base + 8 * 24; }
+    __device__ uint32_t l_full(uint32_t i) const { return base + 8 * (25 + i); }
+    __device__ uint32_t l_empty(uint32_t i) const { return base + 8 * (25 + kLses + i); }
+    static constexpr uint32_t kEnd = 8 * (25 + 2 * kLses);
 };
 
 __device__ __forceinline__ void group_sync(uint32_t group) {
@@ -821,7 +833,7 @@ __device__ __forceinline__ void group_sync(uint32_t group) {
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreadsW, 1)
     chunk_weights_kernel(const AttnParams p, const ChunkScratch sc, const __grid_constant__ CUtensorMap qmap,
                          const __grid_constant__ CUtensorMap kmap) {
     using G = GeoW<D>;
@@ -829,7 +841,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t* const base = raw + (smem - smem_u32(raw));
     const BarsW bar{smem + G::kBars};
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(base + G::kBars + 8 * 23);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(base + G::kBars + BarsW::kEnd);
+    uint32_t* const last_s = tmem_slot + 1;  // by group
     float* const lse_s = reinterpret_cast<float*>(base + G::kLse);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t per_tile = int32_t(chunk_tokens(p.g));
@@ -838,20 +851,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t i = 0; i < 2; ++i) {
             bar_init(bar.k_full(i), 1);
             bar_init(bar.k_empty(i), 1);
+            bar_init(bar.sums(i), 128 * (kGroups - 1));
+            bar_init(bar.summed(i), 128);
         }
-        for (uint32_t i = 0; i < 4; ++i) {
+        for (uint32_t i = 0; i < G::kStages; ++i) {
             bar_init(bar.q_full(i), 1);
             bar_init(bar.q_empty(i), 1);
+        }
+        for (uint32_t i = 0; i < kGroups; ++i) {
             bar_init(bar.s_full(i), 1);
             bar_init(bar.s_empty(i), 4);
         }
-        bar_init(bar.sums(), 128);
-        bar_init(bar.summed(), 128);
+        for (uint32_t i = 0; i < kLses; ++i) {
+            bar_init(bar.l_full(i), 32);
+            bar_init(bar.l_empty(i), 4);
+        }
         bar_init(bar.drain(), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) alloc<512>(smem_u32(tmem_slot));
-    if (warp == 9 && lane == 0) {
+    if (warp == kMmaWarp) alloc<512>(smem_u32(tmem_slot));
+    if (warp == kLoadWarp && lane == 0) {
         prefetch_map(&qmap);
         prefetch_map(&kmap);
     }
@@ -865,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Walk w;
     if (w.begin(sc.w_plan)) {
         uint32_t seg = 0, n = 0;  // pieces begun, row tiles passed
-        if (warp == 9) {
+        if (warp == kLoadWarp) {
             const uint32_t box = min(p.P, 128u), boxes = 128 / box;
             for (; ok && w.next(p, sc.w_plan, sc.w_items); ++seg) {
                 const SeqRange s{w.it.q0, w.it.nq, w.it.n, w.it.n - w.it.nq};
@@ -918,7 +937,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 warp_wait(bar.k_full(x & 1u), (x / 2) & 1u, grace);
                 if (ok) warp_wait(bar.k_empty(x & 1u), (x / 2) & 1u, grace);
             }
-        } else if (warp == 8) {
+        } else if (warp == kMmaWarp) {
             constexpr uint32_t kIs = instr(T::kUmmaFormat, 128, 128, false);
             const uint32_t k_lo = desc_lo(smem, 16), q_lo = desc_lo(smem + G::kRing, 16);
             const bool lead = elect();
@@ -927,9 +946,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t kb = seg & 1u;
                 ok = warp_wait(bar.k_full(kb), (seg / 2) & 1u, deadline);
                 for (int32_t j = 0; j < steps && ok; ++j, ++n) {
-                    const uint32_t st = n % G::kStages, sb = n & 3u;
+                    const uint32_t st = n % G::kStages, sb = n % kGroups;
                     if (!warp_wait(bar.q_full(st), (n / G::kStages) & 1u, deadline) ||
-                        (n >= 4 && !warp_wait(bar.s_empty(sb), (n / 4 - 1) & 1u, deadline))) {
+                        (n >= kGroups && !warp_wait(bar.s_empty(sb), (n / kGroups - 1) & 1u, deadline))) {
                         ok = false;
                         break;
                     }
@@ -951,121 +970,168 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lead) commit(bar.drain());
             warp_wait(bar.drain(), 0, now() + kGraceNs);
             __syncwarp();
-        } else if (warp < 8) {
+        } else if (warp == kLseWarp) {
+            // -lse (base 2) of each row tile, one tile under way while the one before is stored
+            float held[4];
+            auto store = [&](uint32_t at) {
+                const uint32_t sl = at % kLses;
+                if (at >= kLses && !warp_wait(bar.l_empty(sl), (at / kLses - 1) & 1u, deadline)) return false;
+#pragma unroll
+                for (uint32_t x = 0; x < 4; ++x) lse_s[sl * 128 + x * 32 + lane] = -held[x] * kLog2e;
+                bar_arrive(bar.l_full(sl));
+                return true;
+            };
+            int32_t ct[4], ch[4];
+#pragma unroll
+            for (int32_t x = 0; x < 4; ++x) {
+                const int32_t r = x * 32 + int32_t(lane);
+                ct[x] = r / int32_t(p.g), ch[x] = r % int32_t(p.g);
+            }
+            while (ok && w.next(p, sc.w_plan, sc.w_items)) {
+                const SeqRange s{w.it.q0, w.it.nq, w.it.n, w.it.n - w.it.nq};
+                const int32_t tile0 = row_tiles(p, s, w.it.t0).begin + w.j0;
+                for (int32_t j = 0; j < w.steps && ok; ++j, ++n) {
+                    float y[4];
+#pragma unroll
+                    for (int32_t x = 0; x < 4; ++x) {
+                        const int32_t t = (tile0 + j) * per_tile + ct[x];
+                        y[x] = ct[x] < per_tile && t < s.nq
+                                   ? p.lse[int64_t(s.q0 + t) * p.Hq + w.h * int32_t(p.g) + ch[x]] : 0.f;
+                    }
+                    if (n) ok = store(n - 1);
+#pragma unroll
+                    for (int32_t x = 0; x < 4; ++x) held[x] = y[x];
+                }
+            }
+            if (ok && n) ok = store(n - 1);
+        } else {
             const uint32_t grp = warp >> 2, r = tid & 127u;
-            const uint32_t ts = tmem + ((warp & 3u) << 21);
-            const int32_t ct = int32_t(r / p.g), ch = int32_t(r % p.g);  // this thread's row when it fetches lse
-            float* const mine = lse_s + grp * 256;
-            uint32_t buf = 0;
-            // (after a wait that gave up the pieces still go by, without further
-            // waits, so that every thread meets its group's barriers)
+            const uint32_t ts = tmem + ((warp & 3u) << 21) + grp * 128;
+            float* const sums_s = reinterpret_cast<float*>(base + G::kSums);
+            // (after a wait that gave up the pieces still go by, so that every
+            // thread meets its group's barriers)
             for (; w.next(p, sc.w_plan, sc.w_items); ++seg) {
                 const SeqRange s{w.it.q0, w.it.nq, w.it.n, w.it.n - w.it.nq};
                 const int32_t tile0 = row_tiles(p, s, w.it.t0).begin + w.j0;
                 const int32_t k0 = w.it.t0, k = k0 + int32_t(r);
-                // -lse (base 2) of row r of a row tile
-                auto fetch = [&](int32_t j) -> float {
-                    const int32_t t = (tile0 + j) * per_tile + ct;
-                    if (j >= w.steps || ct >= per_tile || t >= s.nq) return 0.f;
-                    return -p.lse[int64_t(s.q0 + t) * p.Hq + w.h * p.g + ch] * kLog2e;
-                };
-                float acc = 0.f;
-                const int32_t odd = int32_t((grp ^ n) & 1u);  // this group's first row tile of the piece
-                float nxt = fetch(odd);
-                for (int32_t j = odd; j < w.steps; j += 2) {
-                    const uint32_t at = n + uint32_t(j), sb = at & 3u;
-                    mine[buf * 128 + r] = nxt;
-                    group_sync(grp);
-                    nxt = fetch(j + 2);
-                    if (!warp_wait(bar.s_full(sb), (at / 4) & 1u, deadline)) ok = false;
+                const uint32_t closer = (n + uint32_t(w.steps) - 1) % kGroups;  // group of the last row tile
+                float* const wt = p.weights + int64_t(w.it.b) * p.w_ss + int64_t(w.h) * p.w_hs + k;
+                const bool kept = k < s.n && (!p.window || int64_t(k) > int64_t(s.f) - int64_t(p.window) ||
+                                              uint32_t(k) < p.sinks);
+                float old = 0.f, acc = 0.f;
+                if (grp == closer && kept && k < s.f) old = *wt;
+                for (int32_t j = int32_t((grp - n) % kGroups); j < w.steps; j += int32_t(kGroups)) {
+                    const uint32_t at = n + uint32_t(j), sl = at % kLses;
+                    if (!warp_wait(bar.l_full(sl), (at / kLses) & 1u, deadline) ||
+                        !warp_wait(bar.s_full(grp), (at / kGroups) & 1u, deadline))
+                        ok = false;
                     const int32_t t0 = (tile0 + j) * per_tile, cols = min(per_tile, s.nq - t0) * int32_t(p.g);
                     const int32_t p0 = s.f + t0, p1 = p0 + min(per_tile, s.nq - t0) - 1;
-                    const float4* ls = reinterpret_cast<const float4*>(mine + buf * 128);
-                    const bool full = cols == 128 && k0 + kKeys - 1 <= p0 &&
-                                      (!p.window || int64_t(p1) < int64_t(k0) + p.window);
-                    // columns [lo, hi): rows whose token sees slot k
-                    const int64_t last = p.window && uint32_t(k) >= p.sinks ? int64_t(k) + p.window - p0 : per_tile;
-                    const int32_t lo = max(k - p0, 0), hi = int32_t(max(int64_t(0), min(last, int64_t(per_tile))));
-                    const int32_t c_lo = min(lo, per_tile) * int32_t(p.g), c_hi = min(hi * int32_t(p.g), cols);
+                    const float4* ls = reinterpret_cast<const float4*>(lse_s + sl * 128);
+                    const uint64_t c2 = pack2(p.c, p.c);
+                    uint64_t sum[2] = {0, 0};
+                    auto four = [&](const float* x, const float4 v, float (&y)[4]) {
+                        unpack2(fma2(pack2(x[0], x[1]), c2, pack2(v.x, v.y)), y[0], y[1]);
+                        unpack2(fma2(pack2(x[2], x[3]), c2, pack2(v.z, v.w)), y[2], y[3]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] = ex2(y[i]);
+                    };
                     fence_after();
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    float x[2][32];
-                    ld32(ts + sb * 128, x[0]);
-                    wait_ld();
+                    if (cols == 128 && k0 + kKeys - 1 <= p0 && (!p.window || int64_t(p1) < int64_t(k0) + p.window)) {
+                        float x[2][32];
+                        ld32(ts, x[0]);
+                        wait_ld();
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (c < 3) ld32(ts + sb * 128 + (c + 1) * 32, x[(c + 1) & 1]);
+                        for (int c = 0; c < 4; ++c) {
+                            if (c < 3) ld32(ts + (c + 1) * 32, x[(c + 1) & 1]);
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 v = ls[c * 8 + e / 4];
-                            float y[4] = {ex2(fmaf(x[c & 1][e], p.c, v.x)), ex2(fmaf(x[c & 1][e + 1], p.c, v.y)),
-                                          ex2(fmaf(x[c & 1][e + 2], p.c, v.z)), ex2(fmaf(x[c & 1][e + 3], p.c, v.w))};
-                            if (!full) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const int32_t col = c * 32 + e + i;
-                                    if (col < c_lo || col >= c_hi) y[i] = 0.f;
-                                }
+                            for (int e = 0; e < 32; e += 4) {
+                                float y[4];
+                                four(x[c & 1] + e, ls[c * 8 + e / 4], y);
+                                sum[0] = add2(sum[0], pack2(y[0], y[1]));
+                                sum[1] = add2(sum[1], pack2(y[2], y[3]));
                             }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) sum[i] += y[i];
+                            if (c < 3) wait_ld();
                         }
-                        if (c < 3) wait_ld();
+                    } else {
+                        // columns [lo, hi): rows whose token sees slot k. A loop of its own: with
+                        // the selects in it the loop above took 1.75 times as long
+                        const int64_t last = p.window && uint32_t(k) >= p.sinks ? int64_t(k) + p.window - p0 : per_tile;
+                        const int32_t lo = min(max(k - p0, 0), per_tile) * int32_t(p.g);
+                        const int32_t hi =
+                            min(int32_t(max(int64_t(0), min(last, int64_t(per_tile)))) * int32_t(p.g), cols);
+#pragma unroll 1
+                        for (int c = 0; c < 128; c += 16) {
+                            if (!__any_sync(0xffffffffu, max(lo, c) < min(hi, c + 16))) continue;
+                            float x[16];
+                            ld16(ts + c, x);
+                            wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; e += 4) {
+                                float y[4];
+                                four(x + e, ls[(c + e) / 4], y);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (c + e + i < lo || c + e + i >= hi) y[i] = 0.f;
+                                sum[0] = add2(sum[0], pack2(y[0], y[1]));
+                                sum[1] = add2(sum[1], pack2(y[2], y[3]));
+                            }
+                        }
                     }
-                    acc += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    float s0, s1, s2, s3;
+                    unpack2(sum[0], s0, s1);
+                    unpack2(sum[1], s2, s3);
+                    acc += (s0 + s1) + (s2 + s3);
                     fence_before();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(bar.s_empty(sb));
-                    buf ^= 1u;
+                    if (lane == 0) {
+                        bar_arrive(bar.s_empty(grp));
+                        bar_arrive(bar.l_empty(sl));
+                    }
                 }
                 n += uint32_t(w.steps);
-                // the groups' sums meet in the second group's second lse buffer
-                float* const other = lse_s + 384;
-                if (grp == 1) {
-                    group_sync(1);
-                    other[r] = acc;
-                    buf = 0;  // the other buffer goes on
-                    bar_arrive(bar.sums());
-                    if (!bar_wait(bar.summed(), seg & 1u, deadline)) ok = false;
-                } else {
-                    if (!bar_wait(bar.sums(), seg & 1u, deadline)) ok = false;
-                    acc += other[r];
-                    bar_arrive(bar.summed());
-                    const bool whole = w.j0 == 0 && w.steps == w.it.tiles;
-                    bool write = whole;
-                    if (!whole) {
-                        const int64_t c0 = cut_owner(w.U, w.G, w.item);
-                        const int64_t c1 = cut_owner(w.U, w.G, w.item + w.it.tiles - 1);
-                        auto piece = [&](int64_t c) {
-                            return sc.w_part + (2 * c + (c == c0 && cut_begin(w.U, w.G, c0) != w.item ? 1 : 0)) * 128;
-                        };
-                        sc.w_part[(2 * int64_t(blockIdx.x) + (w.u == w.u_begin ? 0 : 1)) * 128 + r] = acc;
-                        __threadfence();
-                        group_sync(0);
-                        uint32_t* last_s = reinterpret_cast<uint32_t*>(base + G::kBars + 8 * 24);
-                        if (r == 0) {
-                            const bool last = atomicAdd(p.count + c0, 1u) == uint32_t(c1 - c0);
-                            if (last) p.count[c0] = 0;
-                            *last_s = last;
-                        }
-                        group_sync(0);
-                        write = *last_s != 0;
-                        if (write) {
-                            __threadfence();
-                            acc = 0.f;
-                            for (int64_t c = c0; c <= c1; ++c) acc += __ldcg(piece(c) + r);
-                        }
-                        group_sync(0);  // last_s is free again
-                    }
-                    if (write && k < s.n) {
-                        const bool seen = (!p.window || int64_t(k) > int64_t(s.f) - int64_t(p.window)) ||
-                                          uint32_t(k) < p.sinks;
-                        if (seen) {
-                            float* wt = p.weights + int64_t(w.it.b) * p.w_ss + int64_t(w.h) * p.w_hs + k;
-                            *wt = (k >= s.f ? 0.f : *wt) + acc;
-                        }
-                    }
+                // the group that had the last row tile adds the groups' sums, in their order
+                const uint32_t pb = seg & 1u;
+                float* const sums = sums_s + pb * kGroups * 128;
+                // (every group meets every phase of `summed`: a closer that ran ahead would
+                // take the phase of `sums` two pieces back for its own)
+                if (seg >= 2 && !bar_wait(bar.summed(pb), (seg / 2 - 1) & 1u, deadline)) ok = false;
+                if (grp != closer) {
+                    sums[grp * 128 + r] = acc;
+                    bar_arrive(bar.sums(pb));
+                    continue;
                 }
+                if (!bar_wait(bar.sums(pb), (seg / 2) & 1u, deadline)) ok = false;
+                const float own = acc;
+                acc = 0.f;
+#pragma unroll
+                for (uint32_t x = 0; x < kGroups; ++x) acc += x == grp ? own : sums[x * 128 + r];
+                bar_arrive(bar.summed(pb));
+                bool write = true;
+                if (w.steps != w.it.tiles) {
+                    const int64_t c0 = cut_owner(w.U, w.G, w.item);
+                    const int64_t c1 = cut_owner(w.U, w.G, w.item + w.it.tiles - 1);
+                    auto piece = [&](int64_t c) {
+                        return sc.w_part + (2 * c + (c == c0 && cut_begin(w.U, w.G, c0) != w.item ? 1 : 0)) * 128;
+                    };
+                    sc.w_part[(2 * int64_t(blockIdx.x) + (w.u == w.u_begin ? 0 : 1)) * 128 + r] = acc;
+                    __threadfence();
+                    group_sync(grp);
+                    if (r == 0) {
+                        const bool last = atomicAdd(p.count + c0, 1u) == uint32_t(c1 - c0);
+                        if (last) p.count[c0] = 0;
+                        last_s[grp] = last;
+                    }
+                    group_sync(grp);
+                    write = last_s[grp] != 0;
+                    if (write) {
+                        __threadfence();
+                        acc = 0.f;
+                        for (int64_t c = c0; c <= c1; ++c) acc += __ldcg(piece(c) + r);
+                    }
+                    group_sync(grp);  // last_s is free again
+                }
+                if (write && kept) *wt = old + acc;
             }
             ok = __all_sync(0xffffffffu, ok);
         }
@@ -1073,7 +1139,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
         fence_after();
         dealloc<512>(tmem);
     }
@@ -1093,7 +1159,7 @@ int launch_chunk_weights(const AttnParams& p, const ChunkScratch& s, uint32_t gr
         if (e != cudaSuccess) return int(e);
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
-    return int(launch_after(chunk_weights_kernel<T, D>, grid, kThreads, GeoW<D>::kSmem, stream, p, s, qm, km));
+    return int(launch_after(chunk_weights_kernel<T, D>, grid, kThreadsW, GeoW<D>::kSmem, stream, p, s, qm, km));
 }
 
 template <class T, int D>
