@@ -36,7 +36,7 @@ _predictor = None
 def build(reference: bool = True) -> None:
     """Compiles the oracle; the reference objects too when the reference is mounted."""
     subprocess.run(["make", "-s", "-C", str(HERE)], check=True)
-    if reference and REFERENCE_ROOT.exists():
+    if reference and (REFERENCE_ROOT / "predictor").exists():  # (an empty mount point has no sources)
         subprocess.run(["make", "-s", "-C", str(HERE), "ref", "ref-cuda", f"REF={REFERENCE_ROOT}"], check=True)
 
 
@@ -160,7 +160,7 @@ def predictor() -> C.CDLL:
     global _predictor
     if _predictor is None:
         if not PREDICTOR_LIB.exists():
-            if not REFERENCE_ROOT.exists():
+            if not (REFERENCE_ROOT / "predictor").exists():
                 raise RuntimeError(f"{PREDICTOR_LIB} missing and the reference is not mounted to build it")
             build(reference=True)
         L = C.CDLL(str(PREDICTOR_LIB))
