@@ -42,8 +42,8 @@ class BoundedLayer:
         long, short = -(-longest // page), -(-(budget + slack) // page)
         pool = sequences * (long + 2 * short)
         self.k_pages, self.v_pages = (torch.zeros(pool, page, kv_heads, head_dim, **half) for _ in range(2))
-        order = torch.randperm(pool, generator=gen, device=device).int().split([sequences * n for n in (long, short, short)])
-        self.tables = [o.reshape(sequences, -1) for o in order]
+        order = torch.randperm(pool, generator=gen, device=device).int()
+        self.tables = [o.reshape(sequences, -1) for o in order.split([sequences * n for n in (long, short, short)])]
         self.table, self.turn = self.tables[0], 0
         self.kv_len = torch.zeros(sequences, **int32)
         self.lengths = [0] * sequences  # the same on the host: they follow from the calls

@@ -439,7 +439,9 @@ enum {
  * k > p - window or k < sinks. Slots are counted in the cache, so after an
  * eviction the window is over the slots that are left. A row that sees nothing
  * gives output 0 and lse -inf. Slots that no row of the call sees are not
- * read, whatever their memory or their page index holds. Strides are in
+ * read, whatever their memory or their page index holds. (A value that is not
+ * finite, in a slot that some rows of a sequence's call see, may reach its other
+ * rows too: their probability 0 meets it in a matrix product.) Strides are in
  * elements, non-negative multiples of 8 for 16-bit tensors, whose last
  * dimension is contiguous and which start on 16 bytes. */
 typedef struct ls_b200_attention_args {

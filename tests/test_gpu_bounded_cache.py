@@ -73,7 +73,8 @@ def watch_evict(module, seen):
                     assert torch.equal(kept, torch.arange(n, device="cuda"))
                 else:
                     middle = w[b, h, sinks:n - recent].sort(descending=True, stable=True).indices + sinks
-                    want = torch.cat([torch.arange(sinks, device="cuda"), middle[:budget - sinks - recent].sort().values,
+                    middle = middle[:budget - sinks - recent].sort().values
+                    want = torch.cat([torch.arange(sinks, device="cuda"), middle,
                                       torch.arange(n - recent, n, device="cuda")])
                     assert torch.equal(kept, want)
                 assert torch.equal(a["new_weights"][b, h, :m], w[b, h, kept])
