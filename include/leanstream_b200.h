@@ -427,7 +427,8 @@ enum { LS_B200_FP16 = 0, LS_B200_BF16 = 1 };
 /* Bits that the kernels of this section set in a call's `error` word. What a
  * flagged sequence or page would have touched is skipped. */
 enum {
-    LS_B200_ATTN_TIMEOUT = 1u << 0, /* a bounded wait gave up: the call's outputs are invalid */
+    LS_B200_ATTN_TIMEOUT = 1u << 0, /* a bounded wait gave up: output, lse and weights of the call are invalid; a
+                                     * new token's slot holds its key and value, or what it held before */
     LS_B200_ATTN_LENGTH = 1u << 1,  /* q_start / kv_len of a sequence do not fit the call: skipped */
     LS_B200_ATTN_PAGE = 1u << 2     /* a page index of a visible slot is outside the pool */
 };

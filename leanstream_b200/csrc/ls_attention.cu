@@ -171,9 +171,11 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
     const int64_t NC = max(int64_t(1), min(int64_t(gridDim.x), (U + kDecMinUnits - 1) / kDecMinUnits));
     if (int64_t(blockIdx.x) >= NC) return;
     const int64_t cta = blockIdx.x, u_begin = cut_begin(U, NC, cta), u_end = cut_begin(U, NC, cta + 1);
-    const uint64_t deadline = now() + p.timeout_ns;
+    const Bound bound = bound_of(p.timeout_ns);
+    // after a wait that gave up the warp loads, computes and appends no more, and
+    // only meets the CTA's barriers
     bool ok = true;
-    uint32_t used = 0, filled = 0;  // steps of this warp: computed, loaded
+    uint32_t used = 0, filled = 0;  // steps of this warp: landed, loaded
 
     for (int64_t u = u_begin; u < u_end;) {
         // the next pieces, listed by the threads of their sequences: items (y
@@ -322,7 +324,7 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
         };
         queries(segs[0]);  // ahead of the cache's stream
 #pragma unroll 1
-        for (int i = 0; i < G::kStages; ++i) load();
+        for (int i = 0; ok && i < G::kStages; ++i) load();
 
         for (uint32_t c = 0; c < count; ++c) {
             const DecSeg& x = segs[c];
@@ -341,12 +343,12 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
             m[0] = m[1] = -INFINITY;
             l[0] = l[1] = 0.f;
 
-            for (int32_t block = 0; block < steps; block += 32) {
+            for (int32_t block = 0; ok && block < steps; block += 32) {
                 const int32_t c_k = lay_out(c, block + int32_t(lane));
                 for (uint32_t todo = __ballot_sync(0xffffffffu, c_k & kSeen); todo; todo &= todo - 1) {
                     const int32_t kf = __shfl_sync(0xffffffffu, c_k, __ffs(int(todo)) - 1), k0 = kf & ~15;
                     const uint32_t st = used % G::kStages, ks = ring + st * G::kStage, vs = ks + G::kHalf;
-                    if (!warp_wait(bar0 + 8 * st, (used / G::kStages) & 1u, deadline)) ok = false;
+                    if (!(ok = warp_wait(bar0 + 8 * st, (used / G::kStages) & 1u, bound))) break;
                     ++used;
                     // S = Q K^T
                     float sc[2][4] = {};
@@ -593,9 +595,14 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
         }
         u = segs[count - 1].item + segs[count - 1].j0 + segs[count - 1].steps;
     }
-    // every load has landed before the CTA ends (they all have, unless a wait gave up)
-    for (uint32_t i = filled - min(filled, uint32_t(G::kStages)); i < filled; ++i)
-        warp_wait(bar0 + 8 * (i % G::kStages), (i / G::kStages) & 1u, deadline + kGraceNs);
+    // every load has landed before the CTA ends (they all have, unless a wait gave
+    // up: a stage is filled again only after its last load was waited for, so each
+    // of the rest is the one fill under way in its stage)
+    if (used != filled) {
+        const Bound grace = bound_of(kGraceNs);
+        for (uint32_t i = used; i != filled; ++i)
+            warp_wait(bar0 + 8 * (i % G::kStages), (i / G::kStages) & 1u, grace);
+    }
     if (!ok && lane == 0 && p.err) atomicOr(p.err, uint32_t(LS_B200_ATTN_TIMEOUT));
 }
 
