@@ -479,7 +479,7 @@ typedef struct ls_b200_attention_args {
                                      * overlap. After an error it is to be zeroed again */
     uint64_t scratch_bytes;
     uint32_t* error;                /* optional device word, LS_B200_ATTN_* bits are ORed in */
-    uint64_t timeout_ns;            /* bound of every wait (0 = 2 s, at most 60 s) */
+    uint64_t timeout_ns;            /* bound of every wait, each on its own (0 = 2 s, at most 60 s) */
 } ls_b200_attention_args;
 /* Scratch of a call of this shape (dtype, heads, sizes, batch, tokens, max_q,
  * weights_length; pointers are not read); 0 when the shape is refused. */

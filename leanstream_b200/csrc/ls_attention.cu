@@ -36,6 +36,7 @@ constexpr uint32_t kDecSegs = 12;               // pieces of items listed at a t
 constexpr int64_t kDecItemCost = 2;             // units that beginning and joining an item counts as
 constexpr int64_t kDecMinUnits = 2 + kDecItemCost;  // units that a CTA takes at least
 constexpr uint64_t kGraceNs = 1000000000ull;
+constexpr uint64_t kShortNs = 100000;  // bounds that a barrier's try may sleep over: a load takes less
 
 // Three CTAs per SM by registers; the ring takes the shared memory that leaves.
 template <int D>
@@ -171,7 +172,6 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
     const int64_t NC = max(int64_t(1), min(int64_t(gridDim.x), (U + kDecMinUnits - 1) / kDecMinUnits));
     if (int64_t(blockIdx.x) >= NC) return;
     const int64_t cta = blockIdx.x, u_begin = cut_begin(U, NC, cta), u_end = cut_begin(U, NC, cta + 1);
-    const Bound bound = bound_of(p.timeout_ns);
     // after a wait that gave up the warp loads, computes and appends no more, and
     // only meets the CTA's barriers
     bool ok = true;
@@ -348,7 +348,10 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
                 for (uint32_t todo = __ballot_sync(0xffffffffu, c_k & kSeen); todo; todo &= todo - 1) {
                     const int32_t kf = __shfl_sync(0xffffffffu, c_k, __ffs(int(todo)) - 1), k0 = kf & ~15;
                     const uint32_t st = used % G::kStages, ks = ring + st * G::kStage, vs = ks + G::kHalf;
-                    if (!(ok = warp_wait(bar0 + 8 * st, (used / G::kStages) & 1u, bound))) break;
+                    const uint32_t landed = bar0 + 8 * st, phase = (used / G::kStages) & 1u;
+                    ok = p.timeout_ns < kShortNs ? warp_wait_short(landed, phase, uint32_t(p.timeout_ns))
+                                                 : warp_wait(landed, phase, p.timeout_ns);
+                    if (!ok) break;
                     ++used;
                     // S = Q K^T
                     float sc[2][4] = {};
@@ -598,12 +601,9 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
     // every load has landed before the CTA ends (they all have, unless a wait gave
     // up: a stage is filled again only after its last load was waited for, so each
     // of the rest is the one fill under way in its stage)
-    if (used != filled) {
-        const Bound grace = bound_of(kGraceNs);
-        for (uint32_t i = used; i != filled; ++i)
-            warp_wait(bar0 + 8 * (i % G::kStages), (i / G::kStages) & 1u, grace);
-    }
-    if (!ok && lane == 0 && p.err) atomicOr(p.err, uint32_t(LS_B200_ATTN_TIMEOUT));
+    for (uint32_t i = used; i != filled; ++i)
+        warp_wait(bar0 + 8 * (i % G::kStages), (i / G::kStages) & 1u, kGraceNs);
+    if (!ok) gave_up(p);
 }
 
 // weights[b, h, slot] from the stored logits, once the rows' lse are known.

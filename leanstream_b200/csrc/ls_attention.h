@@ -137,6 +137,11 @@ __device__ __forceinline__ RowTiles row_tiles(const AttnParams& p, const SeqRang
     return {begin, t_lo < t_hi ? (t_hi + T - 1) / T : begin};
 }
 
+// A wait of this warp gave up.
+__device__ __forceinline__ void gave_up(const AttnParams& p) {
+    if ((threadIdx.x & 31u) == 0 && p.err) atomicOr(p.err, uint32_t(LS_B200_ATTN_TIMEOUT));
+}
+
 // Whether position pos sees slot k (pos < 0: nothing).
 __device__ __forceinline__ bool sees(const AttnParams& p, int32_t pos, int32_t k) {
     return k <= pos && (!p.window || int64_t(k) > int64_t(pos) - int64_t(p.window) || uint32_t(k) < p.sinks);

@@ -326,7 +326,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *tmem_slot;
     after_start();
     after_wait();
-    const Bound bound = bound_of(p.timeout_ns);
     constexpr uint32_t kS = 0, kO = 256;  // columns: S_0, S_1 (128 each), O_0, O_1 (D each)
     bool ok = true;
     const Seg* const segs = reinterpret_cast<const Seg*>(base + G::kSegs);
@@ -334,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the next piece; false when there is none (or when a wait gave up)
     uint32_t sg = 0;
     auto next = [&]() -> bool {
-        if (!warp_wait(bar.seg_full(sg % kSegs), (sg / kSegs) & 1u, bound)) return ok = false;
+        if (!warp_wait(bar.seg_full(sg % kSegs), (sg / kSegs) & 1u, p.timeout_ns)) return ok = false;
         return uniform(segs[sg % kSegs].steps) != 0;
     };
     auto release = [&]() {
@@ -350,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             KeyRange kr{};
             bool more = w.begin(sc.plan);
             for (; ok; ++sg) {
-                if (sg >= kSegs && !bar_wait(bar.seg_empty(sg % kSegs), (sg / kSegs - 1) & 1u, bound)) {
+                if (sg >= kSegs && !bar_wait(bar.seg_empty(sg % kSegs), (sg / kSegs - 1) & 1u, p.timeout_ns)) {
                     ok = false;
                     break;
                 }
@@ -380,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (ok && next()) {
             const Seg w = segs[sg % kSegs];
             const int32_t two = w.left > per_tile ? 2 : 1;
-            if (sg && !warp_wait(bar.q_empty(), (sg - 1) & 1u, bound)) {
+            if (sg && !warp_wait(bar.q_empty(), (sg - 1) & 1u, p.timeout_ns)) {
                 ok = false;
                 break;
             }
@@ -408,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int32_t in = (w.slot0(j) + int32_t(lane * box)) & int32_t(p.P - 1);
                 for (int kv = 0; kv < 2; ++kv, ++slot) {
                     const uint32_t s = slot % G::kStages, n = slot / G::kStages;
-                    if (n && !warp_wait(bar.empty(s), (n - 1) & 1u, bound)) {
+                    if (n && !warp_wait(bar.empty(s), (n - 1) & 1u, p.timeout_ns)) {
                         ok = false;
                         break;
                     }
@@ -424,12 +423,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             release();
         }
         // every load has landed and every stage been released before the CTA ends
-        const Bound grace = bound_of((ok ? p.timeout_ns : 0) + kGraceNs);
+        const uint64_t grace = (ok ? p.timeout_ns : 0) + kGraceNs;
         const uint32_t last = min(slot, G::kStages);
+        bool rest = ok;
         for (uint32_t x = slot - last; x < slot; ++x) {
             const uint32_t s = x % G::kStages, n = x / G::kStages;
             warp_wait(bar.full(s), n & 1u, grace);
-            if (ok) warp_wait(bar.empty(s), n & 1u, grace);
+            rest = rest && warp_wait(bar.empty(s), n & 1u, grace);
         }
         if (sg) warp_wait(bar.q_full(), (sg - 1) & 1u, grace);
     } else if (warp < 8) {
@@ -460,11 +460,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             // they may be anything, and 0 * NaN is not 0 (the other row tile's warps
             // write the same zeros)
             auto arrived = [&](bool there) {
-                if (!there && !warp_wait(bar.s_full(i, n & 1u), (n >> 1) & 1u, bound)) return false;
+                if (!there && !warp_wait(bar.s_full(i, n & 1u), (n >> 1) & 1u, p.timeout_ns)) return false;
                 const int32_t k0 = at.h * kHalf;
-                if (at.t && at.t + 1 == count && !warp_wait(bar.o_done(i), no++ & 1u, bound)) return false;
+                if (at.t && at.t + 1 == count && !warp_wait(bar.o_done(i), no++ & 1u, p.timeout_ns)) return false;
                 if ((k0 >= seen_lo && k0 + kHalf <= seen_hi) || k0 + kHalf <= sink) return true;
-                if (!warp_wait(bar.full(at.stage), at.odd & 1u, bound)) return false;
+                if (!warp_wait(bar.full(at.stage), at.odd & 1u, p.timeout_ns)) return false;
                 const int32_t k = k0 + int32_t(r & 63u);
                 if ((r >> 6) < G::kPanels && !((k >= seen_lo && k < seen_hi) || k < sink)) {
                     uint8_t* v = base + G::kRing + at.stage * G::kTile + (r >> 6) * kPanel +
@@ -528,8 +528,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         l *= f2;
                         m = nm;
                         if (at.t) {  // the P V before has to be in O: it is when the next S is there
-                            if (!last && !(ok = warp_wait(bar.s_full(i, ~n & 1u), ((n + 1) >> 1) & 1u, bound)))
-                                break;
+                            if (!last && !warp_wait(bar.s_full(i, ~n & 1u), ((n + 1) >> 1) & 1u, p.timeout_ns))
+                                gave_up(p);
                             fence_after();
 #pragma unroll
                             for (int c = 0; c < D; c += 16) {
@@ -575,10 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     wait_st();
                     fence_before();
                     advance();
-                    if (last || !(ok = arrived(early))) {
-                        if (early) wait_ld();
-                        break;
-                    }
+                    if (last || !(ok = arrived(early))) break;
                     fence_after();
                     if (!early) ld32(tn, x);
                     ld32(tn + 32, x + 32);
@@ -586,8 +583,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mask_and_max();
                 }
             }
+            if (!ok) wait_ld();  // (an early read may be under way)
             const bool any = count != 0;  // (otherwise O is not written)
-            if (any && ok) ok = warp_wait(bar.o_done(i), no++ & 1u, bound);
+            if (any && ok) ok = warp_wait(bar.o_done(i), no++ & 1u, p.timeout_ns);
             if (!ok) break;
             if (!any)
                 for (int32_t j = w.steps; j; --j) at.next_stage<G::kStages>();
@@ -654,11 +652,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (ok && next()) {
             const Seg& w = segs[sg % kSegs];
             const int32_t count = uniform(w.halves), na = uniform(w.na), ha = uniform(w.ha), hb = uniform(w.hb);
-            ok = warp_wait(bar.q_full(), sg & 1u, bound);
+            ok = warp_wait(bar.q_full(), sg & 1u, p.timeout_ns);
             if (int32_t(i) * per_tile >= uniform(w.left) || !count) {  // no such row tile, or nothing seen
                 for (int32_t j = uniform(w.steps); j && ok; --j)
                     for (Halves* c : {&cs, &cp}) {
-                        if (!(ok = ok && warp_wait(bar.full(c->stage), c->odd & 1u, bound))) break;
+                        if (!(ok = ok && warp_wait(bar.full(c->stage), c->odd & 1u, p.timeout_ns))) break;
                         if (lead) commit(bar.empty(c->stage));
                         c->next_stage<G::kStages>();
                     }
@@ -669,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             cs.begin(na, ha, hb);
             cp.begin(na, ha, hb);
             auto landed = [&](const Halves& c) {
-                return !c.fresh || warp_wait(bar.full(c.stage), c.odd & 1u, bound);
+                return !c.fresh || warp_wait(bar.full(c.stage), c.odd & 1u, p.timeout_ns);
             };
             auto advance = [&](Halves& c) {  // a tile's last half releases its stage
                 const uint32_t stage = c.stage;
@@ -699,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t b = n & 1u;
                 const bool more = cs.t < count;
                 if (!(ok = landed(cp) && (!more || landed(cs)) &&
-                           warp_wait(bar.p_ready(i, b), (n >> 1) & 1u, bound)))
+                           warp_wait(bar.p_ready(i, b), (n >> 1) & 1u, p.timeout_ns)))
                     break;
                 fence_after();
                 const uint32_t v = uniform(v_lo + cp.stage * (G::kTile / 16) + (cp.h & 1) * (kHalf * 128 / 16));
@@ -717,9 +715,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // MMAs in flight end (bounded) before the tensor memory goes
         if (lead) commit(bar.drain(i));
-        warp_wait(bar.drain(i), 0, bound_of(kGraceNs));
+        warp_wait(bar.drain(i), 0, kGraceNs);
     }
-    if (!ok && lane == 0 && p.err) atomicOr(p.err, uint32_t(LS_B200_ATTN_TIMEOUT));
+    if (!ok) gave_up(p);
     fence_before();
     __syncthreads();
     if (warp == 8) {
@@ -886,7 +884,6 @@ __global__ void __launch_bounds__(kThreadsW, 1)
     fence_after();
     const uint32_t tmem = *tmem_slot;
     after_wait();
-    const Bound bound = bound_of(p.timeout_ns);
     bool ok = true;
     Walk w;
     if (w.begin(sc.w_plan)) {
@@ -897,7 +894,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
                 const SeqRange s{w.it.q0, w.it.nq, w.it.n, w.it.n - w.it.nq};
                 const int32_t tile0 = row_tiles(p, s, w.it.t0).begin + w.j0;
                 const uint32_t kb = seg & 1u;
-                if (seg >= 2 && !warp_wait(bar.k_empty(kb), (seg / 2 - 1) & 1u, bound)) {
+                if (seg >= 2 && !warp_wait(bar.k_empty(kb), (seg / 2 - 1) & 1u, p.timeout_ns)) {
                     ok = false;
                     break;
                 }
@@ -918,7 +915,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
                              int32_t(c * 64), k0 & int32_t(p.P - 1), w.h, id);
                 for (int32_t j = 0; j < w.steps; ++j, ++n) {
                     const uint32_t st = n % G::kStages;
-                    if (n >= G::kStages && !warp_wait(bar.q_empty(st), (n / G::kStages - 1) & 1u, bound)) {
+                    if (n >= G::kStages && !warp_wait(bar.q_empty(st), (n / G::kStages - 1) & 1u, p.timeout_ns)) {
                         ok = false;
                         break;
                     }
@@ -935,14 +932,15 @@ __global__ void __launch_bounds__(kThreadsW, 1)
                     break;
                 }
             }
-            const Bound grace = bound_of((ok ? p.timeout_ns : 0) + kGraceNs);
+            const uint64_t grace = (ok ? p.timeout_ns : 0) + kGraceNs;
+            bool rest = ok;
             for (uint32_t x = n - min(n, G::kStages); x < n; ++x) {
                 warp_wait(bar.q_full(x % G::kStages), (x / G::kStages) & 1u, grace);
-                if (ok) warp_wait(bar.q_empty(x % G::kStages), (x / G::kStages) & 1u, grace);
+                rest = rest && warp_wait(bar.q_empty(x % G::kStages), (x / G::kStages) & 1u, grace);
             }
             for (uint32_t x = seg - min(seg, 2u); x < seg; ++x) {
                 warp_wait(bar.k_full(x & 1u), (x / 2) & 1u, grace);
-                if (ok) warp_wait(bar.k_empty(x & 1u), (x / 2) & 1u, grace);
+                rest = rest && warp_wait(bar.k_empty(x & 1u), (x / 2) & 1u, grace);
             }
         } else if (warp == kMmaWarp) {
             constexpr uint32_t kIs = instr(T::kUmmaFormat, 128, 128, false);
@@ -951,11 +949,11 @@ __global__ void __launch_bounds__(kThreadsW, 1)
             while (ok && w.next(p, sc.w_plan, sc.w_items)) {
                 const int32_t steps = uniform(w.steps);
                 const uint32_t kb = seg & 1u;
-                ok = warp_wait(bar.k_full(kb), (seg / 2) & 1u, bound);
+                ok = warp_wait(bar.k_full(kb), (seg / 2) & 1u, p.timeout_ns);
                 for (int32_t j = 0; j < steps && ok; ++j, ++n) {
                     const uint32_t st = n % G::kStages, sb = n % kGroups;
-                    if (!warp_wait(bar.q_full(st), (n / G::kStages) & 1u, bound) ||
-                        (n >= kGroups && !warp_wait(bar.s_empty(sb), (n / kGroups - 1) & 1u, bound))) {
+                    if (!warp_wait(bar.q_full(st), (n / G::kStages) & 1u, p.timeout_ns) ||
+                        (n >= kGroups && !warp_wait(bar.s_empty(sb), (n / kGroups - 1) & 1u, p.timeout_ns))) {
                         ok = false;
                         break;
                     }
@@ -975,14 +973,14 @@ __global__ void __launch_bounds__(kThreadsW, 1)
                 ++seg;
             }
             if (lead) commit(bar.drain());
-            warp_wait(bar.drain(), 0, bound_of(kGraceNs));
+            warp_wait(bar.drain(), 0, kGraceNs);
             __syncwarp();
         } else if (warp == kLseWarp) {
             // -lse (base 2) of each row tile, one tile under way while the one before is stored
             float held[4];
             auto store = [&](uint32_t at) {
                 const uint32_t sl = at % kLses;
-                if (at >= kLses && !warp_wait(bar.l_empty(sl), (at / kLses - 1) & 1u, bound)) return false;
+                if (at >= kLses && !warp_wait(bar.l_empty(sl), (at / kLses - 1) & 1u, p.timeout_ns)) return false;
 #pragma unroll
                 for (uint32_t x = 0; x < 4; ++x) lse_s[sl * 128 + x * 32 + lane] = -held[x] * kLog2e;
                 bar_arrive(bar.l_full(sl));
@@ -1030,8 +1028,8 @@ __global__ void __launch_bounds__(kThreadsW, 1)
                 if (grp == closer && kept && k < s.f) old = *wt;
                 for (int32_t j = int32_t((grp - n) % kGroups); j < w.steps; j += int32_t(kGroups)) {
                     const uint32_t at = n + uint32_t(j), sl = at % kLses;
-                    if (!(ok = ok && warp_wait(bar.l_full(sl), (at / kLses) & 1u, bound) &&
-                               warp_wait(bar.s_full(grp), (at / kGroups) & 1u, bound)))
+                    if (!(ok = ok && warp_wait(bar.l_full(sl), (at / kLses) & 1u, p.timeout_ns) &&
+                               warp_wait(bar.s_full(grp), (at / kGroups) & 1u, p.timeout_ns)))
                         break;
                     const int32_t t0 = (tile0 + j) * per_tile, cols = min(per_tile, s.nq - t0) * int32_t(p.g);
                     const int32_t p0 = s.f + t0, p1 = p0 + min(per_tile, s.nq - t0) - 1;
@@ -1103,7 +1101,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
                 float* const sums = sums_s + pb * kGroups * 128;
                 // (every group meets every phase of `summed`: a closer that ran ahead would
                 // take the phase of `sums` two pieces back for its own)
-                if (seg >= 2) ok = ok && warp_wait(bar.summed(pb), (seg / 2 - 1) & 1u, bound);
+                if (seg >= 2) ok = ok && warp_wait(bar.summed(pb), (seg / 2 - 1) & 1u, p.timeout_ns);
                 if (grp != closer) {
                     if (ok) {
                         sums[grp * 128 + r] = acc;
@@ -1111,7 +1109,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
                     }
                     continue;
                 }
-                ok = ok && warp_wait(bar.sums(pb), (seg / 2) & 1u, bound);
+                ok = ok && warp_wait(bar.sums(pb), (seg / 2) & 1u, p.timeout_ns);
                 const float own = acc;
                 acc = 0.f;
 #pragma unroll
@@ -1144,7 +1142,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
                 if (write && kept && ok) *wt = old + acc;
             }
         }
-        if (!ok && lane == 0 && p.err) atomicOr(p.err, uint32_t(LS_B200_ATTN_TIMEOUT));
+        if (!ok) gave_up(p);
     }
     fence_before();
     __syncthreads();

@@ -45,45 +45,38 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ bool bar_poll(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// What bounds the waits. One bar_try may sleep for longer than a short bound (a
-// hint of its length is not kept), and %globaltimer ticks too coarsely for one:
-// waits with a bound below kSleepNs poll, and count SM cycles, two per ns.
-struct Bound {
-    uint64_t deadline;
-    bool poll;
-};
-constexpr uint64_t kSleepNs = 100000;
-__device__ __forceinline__ uint64_t ticks(bool poll) { return poll ? uint64_t(clock64()) : now(); }
-__device__ __forceinline__ Bound bound_of(uint64_t ns) {
-    const bool poll = ns < kSleepNs;
-    return {ticks(poll) + (poll ? 2 * ns : ns), poll};
-}
-static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, uint64_t deadline, bool poll) {
+// Waits are bounded one by one, in units of 1024 ns (%globaltimer ticks about as
+// coarsely, and a try may sleep for some us): a wait that goes on begins its time
+// here. 32-bit arguments and no call from here: with 64-bit ones, or a second way
+// for short bounds, chunks took 1 to 2 % longer.
+static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, uint32_t limit) {
+    const uint32_t begin = uint32_t(now() >> 10);
     for (;;) {
-        if (poll) {
-            if (bar_poll(bar, parity)) return true;
-        } else {
-            for (int i = 0; i < 16; ++i)
-                if (bar_try(bar, parity)) return true;
-        }
-        if (ticks(poll) > deadline) return false;
+        for (int i = 0; i < 16; ++i)
+            if (bar_try(bar, parity)) return true;
+        if (uint32_t(now() >> 10) - begin > limit) return false;
     }
 }
-// Waits until phase `parity` has completed; false where the bound runs out.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const Bound& b) {
-    return (!b.poll && bar_try(bar, parity)) || bar_wait_slow(bar, parity, b.deadline, b.poll);
+// Waits until phase `parity` has completed; false after ns (below 2^42).
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint64_t ns) {
+    return bar_try(bar, parity) || bar_wait_slow(bar, parity, uint32_t(ns >> 10));
 }
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const Bound& b) {
-    return __all_sync(0xffffffffu, bar_wait(bar, parity, b)) != 0;
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint64_t ns) {
+    return __all_sync(0xffffffffu, bar_wait(bar, parity, ns)) != 0;
+}
+// The same for a bound below a try's sleep: polls, and counts SM cycles, two per ns.
+static __device__ __noinline__ bool warp_wait_short(uint32_t bar, uint32_t parity, uint32_t ns) {
+    const uint64_t begin = uint64_t(clock64());
+    uint32_t ok;
+    do {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    } while (!ok && uint64_t(clock64()) - begin <= 2ull * ns);
+    return __all_sync(0xffffffffu, ok) != 0;
 }
 // One lane of a converged warp, as a predicate that keeps the code around it
 // uniform: tcgen05.mma takes its operands from uniform registers, and issued

@@ -1,9 +1,8 @@
 """Waits of the paged attention that give up: the kernels end, say so, leave no
-row in the cache that is not a new token's, and work again once cleared. A
-bound of 1 ns is shorter than a load takes. (The decode kernel issues its first
-loads so early that they may have landed by its first wait; over a cache that
-streams from memory its waits do run out.) Bounds of the results as in
-test_gpu_attention.py."""
+row in the cache that is not a new token's, and work again once cleared. Whether
+the waits of a small call run out under a bound of 1 ns depends on how long one
+try of a barrier sleeps; over a cache that streams from memory they do. Bounds of
+the results as in test_gpu_attention.py."""
 import pytest
 import torch
 
@@ -54,7 +53,7 @@ def test_expired_waits(cuda_device, native_lib, name, dim, weights, window):
     for _ in range(3):
         engine.run(**call.kwargs(), timeout_ns=1)
     torch.cuda.synchronize()
-    assert engine.error() in ((N.ATTN_TIMEOUT,) if "chunk" in name else (0, N.ATTN_TIMEOUT))
+    assert engine.error() in (0, N.ATTN_TIMEOUT)
     check_cache(call, old)
     engine.clear_error()
     if weights:
@@ -67,9 +66,9 @@ def test_expired_waits(cuda_device, native_lib, name, dim, weights, window):
 
 @pytest.mark.parametrize("weights", [False, True])
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("q", [1, 4])
+@pytest.mark.parametrize("q", [1, 4, 200])
 def test_expired_waits_over_a_long_cache(cuda_device, native_lib, q, dim, weights):
-    """Decode over more than the L2 cache holds: against the same call with the default bound."""
+    """More than the L2 cache holds: against the same call with the default bound."""
     from leanstream_b200 import _native as N
 
     call = Call([(q, 16 + q)] * 16, dim=dim, weights=weights, page=64)
@@ -88,7 +87,8 @@ def test_expired_waits_over_a_long_cache(cuda_device, native_lib, q, dim, weight
     engine = call.engine()
     if weights:
         call.weights = before.clone()
-    engine.run(**call.kwargs(), timeout_ns=1)
+    for _ in range(5):
+        engine.run(**call.kwargs(), timeout_ns=1)
     torch.cuda.synchronize()
     assert engine.error() == N.ATTN_TIMEOUT
     check_cache(call, old)
