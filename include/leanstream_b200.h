@@ -481,8 +481,10 @@ typedef struct ls_b200_attention_args {
     uint32_t* error;                /* optional device word, LS_B200_ATTN_* bits are ORed in */
     uint64_t timeout_ns;            /* bound of every wait, each on its own (0 = 2 s, at most 60 s) */
 } ls_b200_attention_args;
-/* Scratch of a call of this shape (dtype, heads, sizes, batch, tokens, max_q,
- * weights_length; pointers are not read); 0 when the shape is refused. */
+/* Scratch that holds every call with these heads and head_dim and with at most
+ * this batch, tokens, max_q and weights_length (pointers are not read); 0 when the
+ * shape is refused. With weights, calls of up to 16 / group new tokens a sequence
+ * take batch * q_heads * weights_length * 4 B for each of those tokens. */
 uint64_t ls_b200_attention_scratch_bytes(const ls_b200_attention_args* args);
 /* weights[b][h][k] += sum over the new tokens and the query heads of kv head h
  * of the slot's softmax weight; the new tokens' own slots start at this call's

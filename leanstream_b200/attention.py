@@ -66,10 +66,12 @@ class PagedAttention:
     """Attention of new tokens over a paged cache at fixed head sizes. Scratch
     is allocated here, for calls of at most `max_sequences` sequences and
     `max_tokens` new tokens in all, `max_queries` of one sequence, and with
-    weights of at most `max_weights_length` slots; calls on one PagedAttention
-    must not overlap. `scratch` = (pointer, bytes) supplies caller-owned, zeroed
-    device memory instead; `error` is then the device address of a
-    caller-owned, zeroed 32-bit error word (or None)."""
+    weights of at most `max_weights_length` slots (those cost scratch:
+    max_sequences * q_heads * max_weights_length * 4 B for each of up to 16 /
+    group new tokens of a sequence); calls on one PagedAttention must not
+    overlap. `scratch` = (pointer, bytes) supplies caller-owned, zeroed device
+    memory instead; `error` is then the device address of a caller-owned, zeroed
+    32-bit error word (or None)."""
 
     def __init__(self, q_heads: int, kv_heads: int, head_dim: int, *, page_size: int, dtype="float16",
                  max_sequences: int, max_tokens: int, max_queries: int = 1, max_weights_length: int = 0, device=None,

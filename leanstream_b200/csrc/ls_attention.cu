@@ -699,6 +699,20 @@ ScratchPlan scratch_plan(const ls_b200_attention_args& a) {
     return s;
 }
 
+// Scratch of every call of at most this batch, tokens, max_q and
+// weights_length. Either layout grows with them, but a call of few rows among the
+// smaller ones goes to the other one (stored logits).
+uint64_t scratch_bytes(ls_b200_attention_args a) {
+    uint64_t total = scratch_plan(a).total;
+    const uint32_t g = a.q_heads / a.kv_heads;
+    if (is_chunk(a) && g <= kChunkRows) {
+        a.max_q = uint32_t(kChunkRows) / g;
+        const uint64_t few = scratch_plan(a).total;
+        total = few > total ? few : total;
+    }
+    return total;
+}
+
 bool stride8(int64_t v) { return v % 8 == 0 && v >= 0; }
 
 // The call's shape: everything that does not depend on pointers.
@@ -749,7 +763,7 @@ extern "C" {
 
 uint64_t ls_b200_attention_scratch_bytes(const ls_b200_attention_args* a) {
     if (!a || lsb::check_shape(*a)) return 0;
-    return lsb::scratch_plan(*a).total;
+    return lsb::scratch_bytes(*a);
 }
 
 int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
