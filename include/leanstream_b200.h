@@ -442,9 +442,10 @@ enum {
  * gives output 0 and lse -inf. Slots that no row of the call sees are not
  * read, whatever their memory or their page index holds. (A value that is not
  * finite, in a slot that some rows of a sequence's call see, may reach its other
- * rows too: their probability 0 meets it in a matrix product.) Strides are in
- * elements, non-negative multiples of 8 for 16-bit tensors, whose last
- * dimension is contiguous and which start on 16 bytes. */
+ * rows too: their probability 0 meets it in a matrix product.) With float16 a
+ * probability below 2^-32 of its row's largest may count as 0 in the output (not
+ * in lse and weights). Strides are in elements, non-negative multiples of 8 for
+ * 16-bit tensors, whose last dimension is contiguous and which start on 16 bytes. */
 typedef struct ls_b200_attention_args {
     uint32_t dtype;                 /* LS_B200_FP16 / LS_B200_BF16: q, keys, values and output */
     uint32_t q_heads, kv_heads;     /* head i reads kv head i / group; group = q_heads / kv_heads, whole, <= 128 */

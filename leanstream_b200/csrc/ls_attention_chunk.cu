@@ -19,10 +19,10 @@
 // the others.
 //
 // The running maximum is only raised when a row's maximum grows by more than
-// 2^8 (probabilities then stay below 2^8, exact in either 16-bit type's
-// range); raising it rescales O_i in tensor memory, which is rare after the
-// first tiles. P is rounded once to the 16-bit type (the MMA's operand); sums
-// and maxima stay in 32 bits, the row sum over the unrounded P.
+// 2^kRaise; raising it rescales O_i in tensor memory, which is rare after the
+// first tiles. P is rounded once to the 16-bit type (the MMA's operand), where
+// float16 takes it times 2^kChunkShift (ls_attention.h); sums and maxima stay in
+// 32 bits, the row sum over the unrounded P.
 //
 // The tiles of all items, in order, are cut evenly over one CTA per SM, so a
 // few long sequences fill the GPU as many short ones do. An item cut over
@@ -50,7 +50,6 @@ constexpr int kKeys = kChunkKeys, kHalf = kKeys / 2;
 constexpr int kThreads = 384;  // twelve warps, 168 registers per thread
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows of 64 elements
 constexpr uint64_t kGraceNs = 1000000000ull;
-constexpr float kRaise = 8.f;  // base-2 growth of a row's maximum that raises the reference
 
 template <int D>
 struct Geo {
@@ -521,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool last = at.t + 1 == count;
                     // (written so that NaN raises too: the row is NaN from there on, as
                     // it is for an infinite logit)
-                    const bool raise = m == -INFINITY ? mx != -INFINITY : !((mx - m) * p.c <= kRaise);
+                    const bool raise = m == -INFINITY ? mx != -INFINITY : !((mx - m) * p.c <= T::kRaise);
                     if (__any_sync(0xffffffffu, raise)) {
                         const float nm = !raise ? m : mx == INFINITY ? NAN : mx;
                         const float f2 = nm == -INFINITY ? 1.f : ex2((m - nm) * p.c);
@@ -542,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                     }
-                    const float ref = m == -INFINITY ? 0.f : -m * p.c;
+                    const float ref = m == -INFINITY ? 0.f : fmaf(-m, p.c, T::kChunkShift);
                     const uint64_t c2 = pack2(p.c, p.c), ref2 = pack2(ref, ref);
                     uint64_t sum[2] = {0, 0};
                     auto probabilities = [&](const float* y, uint32_t to_p) {  // of 32 columns
@@ -625,10 +624,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                 }
                 if (real) {
+                    const float ref = fmaf(m, p.c, -T::kChunkShift);
                     if (whole) {
-                        if (p.lse) p.lse[token * p.Hq + head] = l == 0.f ? -INFINITY : (m * p.c + lg2(l)) * kLn2;
+                        if (p.lse) p.lse[token * p.Hq + head] = l == 0.f ? -INFINITY : (ref + lg2(l)) * kLn2;
                     } else {
-                        part[256 * D + row] = m * p.c;
+                        part[256 * D + row] = ref;
                         part[256 * D + 256 + row] = l;
                     }
                 }
