@@ -177,7 +177,9 @@ __device__ void lay_out(const AttnParams& p, ChunkPlan* plan, ChunkItem* list, i
 }
 
 // Lays out the attention's items (block 0) and the weights' (block 1), and
-// appends the new keys and values (blocks 2 .., a warp per token).
+// appends the new keys and values (blocks 2 .., the same number for each
+// sequence, a warp per token at a time).
+constexpr uint64_t kAppendBlocks = 16384;  // about: max_q may be far above what the sequences bring
 __global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, const ChunkScratch sc, uint32_t grid) {
     after_start();
     if (blockIdx.x == 0) {
@@ -187,33 +189,37 @@ __global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, 
     } else {
         const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         const uint32_t pieces = p.D / 8, per_token = p.Hkv * pieces;
-        const uint32_t per_seq = (p.max_q + 7) / 8, at = blockIdx.x - 2, b = at / per_seq;
+        const uint32_t per_seq = (gridDim.x - 2) / p.B, at = blockIdx.x - 2, b = at / per_seq;
         const SeqRange s = load_seq(p, b);
-        const int32_t t = int32_t(at % per_seq * 8 + warp), slot = s.f + t;
-        if (t >= s.nq || slot < 0) return;
-        const int32_t id = p.table[int64_t(b) * p.table_s + (slot >> p.pshift)];
-        if (uint32_t(id) >= p.pages) {
-            if (p.err) atomicOr(p.err, kErrPage);
-            return;
-        }
-        const int64_t in = slot & int32_t(p.P - 1), tok = s.q0 + t;
-        for (uint32_t i0 = lane; i0 < per_token; i0 += 128) {  // four pieces of each under way at a time
-            uint4 k[4], v[4];
-#pragma unroll
-            for (uint32_t x = 0; x < 4; ++x) {
-                const uint32_t i = i0 + 32 * x;
-                if (i >= per_token) break;
-                const int64_t h = i / pieces, e = (i % pieces) * 8;
-                k[x] = *reinterpret_cast<const uint4*>(p.k_new + tok * p.kn_ts + h * p.kn_hs + e);
-                v[x] = *reinterpret_cast<const uint4*>(p.v_new + tok * p.vn_ts + h * p.vn_hs + e);
+        for (int64_t t = at % per_seq * 8 + warp; t < s.nq; t += per_seq * 8) {
+            const int32_t slot = s.f + int32_t(t);
+            if (slot < 0) continue;
+            const int32_t id = p.table[int64_t(b) * p.table_s + (slot >> p.pshift)];
+            if (uint32_t(id) >= p.pages) {
+                if (p.err) atomicOr(p.err, kErrPage);
+                continue;
             }
+            const int64_t in = slot & int32_t(p.P - 1), tok = s.q0 + t;
+            for (uint32_t i0 = lane; i0 < per_token; i0 += 128) {  // four pieces of each under way at a time
+                uint4 k[4], v[4];
 #pragma unroll
-            for (uint32_t x = 0; x < 4; ++x) {
-                const uint32_t i = i0 + 32 * x;
-                if (i >= per_token) break;
-                const int64_t h = i / pieces, e = (i % pieces) * 8;
-                *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + in * p.kp_ss + h * p.kp_hs + e) = k[x];
-                *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + in * p.vp_ss + h * p.vp_hs + e) = v[x];
+                for (uint32_t x = 0; x < 4; ++x) {
+                    const uint32_t i = i0 + 32 * x;
+                    if (i >= per_token) break;
+                    const int64_t h = i / pieces, e = (i % pieces) * 8;
+                    k[x] = *reinterpret_cast<const uint4*>(p.k_new + tok * p.kn_ts + h * p.kn_hs + e);
+                    v[x] = *reinterpret_cast<const uint4*>(p.v_new + tok * p.vn_ts + h * p.vn_hs + e);
+                }
+#pragma unroll
+                for (uint32_t x = 0; x < 4; ++x) {
+                    const uint32_t i = i0 + 32 * x;
+                    if (i >= per_token) break;
+                    const int64_t h = i / pieces, e = (i % pieces) * 8;
+                    *reinterpret_cast<uint4*>(p.k_pages + int64_t(id) * p.kp_ps + in * p.kp_ss + h * p.kp_hs + e) =
+                        k[x];
+                    *reinterpret_cast<uint4*>(p.v_pages + int64_t(id) * p.vp_ps + in * p.vp_ss + h * p.vp_hs + e) =
+                        v[x];
+                }
             }
         }
     }
@@ -1192,7 +1198,8 @@ int launch(const AttnParams& p, bool bf16, const ChunkScratch& s, uint32_t grid,
         if (e != cudaSuccess) return int(e);
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
-    const uint32_t append = p.k_new ? p.B * ((p.max_q + 7) / 8) : 0;
+    const uint64_t most = (uint64_t(p.max_q < p.tokens ? p.max_q : p.tokens) + 7) / 8, fair = kAppendBlocks / p.B + 1;
+    const uint32_t append = p.k_new ? p.B * uint32_t(most < fair ? most : fair) : 0;
     chunk_prepare_kernel<<<2 + append, 256, 0, stream>>>(p, s, grid);
     e = cudaGetLastError();
     if (e == cudaSuccess)
