@@ -8,12 +8,13 @@ from ._native import load as load_library, LIBRARY  # noqa: F401
 from .backend import B200Backend, DeviceQueue, ExecutionQueue, quantize_io_load  # noqa: F401
 from .batch import BatchMLP, union_plan  # noqa: F401
 
-__all__ = ["B200Backend", "BatchMLP", "DeviceQueue", "ExecutionQueue", "PagedAttention", "evict_cache", "quantize_io_load",
-           "union_plan", "load_library", "LIBRARY"]
+__all__ = ["B200Backend", "BatchMLP", "DeviceQueue", "ExecutionQueue", "quantize_io_load", "union_plan",
+           "load_library", "LIBRARY"]
 
 
 def __getattr__(name):
-    # the paged cache operators check torch tensors: torch is imported with their first use
+    # the paged cache operators check torch tensors: torch is imported with their
+    # first use (and they are not among __all__, which needs none)
     if name in ("PagedAttention", "evict_cache"):
         from . import attention
 
