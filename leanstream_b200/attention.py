@@ -216,12 +216,15 @@ class PagedAttention:
         if not good:
             self._refuse(q, output, k_pages, v_pages, page_table, q_start, kv_len, max_q, k_new, v_new, lse, weights,
                          window, sinks)
-        args = _ATTENTION.pack(
-            self._code, self.q_heads, self.kv_heads, self.head_dim, self.page_size, pool[0], batch, tokens, max_q,
-            table[1], window, sinks, self._scale if scale is None else scale, slots, q.data_ptr(), kn, vn,
-            k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
-            output.data_ptr(), ls, ws, q0, q1, kn0, kn1, vn0, vn1, k0, k1, k2, v0, v1, v2, o0, o1, t0, ws0, ws1,
-            self.scratch_ptr, self.scratch_bytes, self.error_ptr, timeout_ns)
+        try:
+            args = _ATTENTION.pack(
+                self._code, self.q_heads, self.kv_heads, self.head_dim, self.page_size, pool[0], batch, tokens, max_q,
+                table[1], window, sinks, self._scale if scale is None else scale, slots, q.data_ptr(), kn, vn,
+                k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
+                output.data_ptr(), ls, ws, q0, q1, kn0, kn1, vn0, vn1, k0, k1, k2, v0, v1, v2, o0, o1, t0, ws0, ws1,
+                self.scratch_ptr, self.scratch_bytes, self.error_ptr, timeout_ns)
+        except (struct.error, OverflowError) as e:
+            raise ValueError(f"window {window}, sinks {sinks}, scale {scale}, timeout_ns {timeout_ns}: {e}") from None
         if stream is None and dev == _current_device():
             rc = self._call(args, _raw_stream(dev))
         else:

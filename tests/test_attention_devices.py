@@ -111,3 +111,11 @@ def test_two_devices_are_refused(calls):
     with pytest.raises(ValueError):
         evict_cache(stream=stream, **cut(0))
     assert not calls
+
+
+@pytest.mark.parametrize("change", [dict(window=1 << 32), dict(sinks=1 << 40), dict(timeout_ns=-1),
+                                    dict(timeout_ns=1 << 64), dict(scale=1e39)], ids=str)
+def test_numbers_that_do_not_fit_are_refused(calls, change):
+    with pytest.raises(ValueError):
+        engine().run(**attend(0, **change))
+    assert not calls
