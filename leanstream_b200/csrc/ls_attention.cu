@@ -45,7 +45,7 @@ struct GeoD {
     static constexpr uint32_t kHalf = kDecKeys * D * 2, kStage = 2 * kHalf;  // a step's keys, and its values
     static constexpr int kStages = 2 * (128 / D);
     static constexpr uint32_t kRing = kDecWarps * kStages * kStage;
-    static constexpr uint32_t kJoin = kRing, kJoinBytes = kRows * D * 4;  // sums of the warps; queries before
+    static constexpr uint32_t kJoin = kRing, kJoinBytes = kRows * D * 4;  // sums of the warps
     static constexpr uint32_t kSegs = kJoin + kJoinBytes, kBars = kSegs + kDecSegs * 64;
     static constexpr uint32_t kStat = kBars + 8 * kDecWarps * kStages;  // scan words, flags; row maxima and sums
     static constexpr uint32_t kSmem = kStat + 128 + 2 * kDecWarps * kRows * 4;
@@ -127,7 +127,7 @@ __device__ __forceinline__ Pair block_scan(Pair v, Pair* sh, Pair& before) {
 // probabilities meet the values as the sum of two 16-bit numbers, about twice the
 // bits of one (down to float16's smallest step, 2^-40 of the row's largest): the
 // multiplier is idle beside the loads. Two sequences
-// of up to 131072 slots, 64 heads of 128 over 8: 180 us, 5.6 TB/s of the cache;
+// of up to 131072 slots, 64 heads of 128 over 8: 180 us, 5.7 TB/s of the cache;
 // 32 of up to 4096 slots, 32 heads: 60 us, 4.6 TB/s; one of 97 slots: 8.5 us.
 template <class T, int D>
 __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
@@ -668,7 +668,7 @@ uint32_t sm_count() {
 // Rows of a sequence and kv head beyond which the call goes to the 128-row
 // tensor-core tiles of ls_attention_chunk.cu: what one 16-row MMA tile holds.
 // (Two such tiles in the decode kernel: 90 us for 7 new tokens of 16 sequences
-// of up to 6000 slots, 28 rows, against 69 us there.)
+// of up to 6000 slots, 28 rows, against 63 us there.)
 constexpr uint64_t kChunkRows = 16;
 bool is_chunk(const ls_b200_attention_args& a) {
     const uint32_t g = a.q_heads / a.kv_heads;

@@ -28,9 +28,11 @@
 // few long sequences fill the GPU as many short ones do. An item cut over
 // several CTAs leaves its parts in scratch, and a short kernel joins them in
 // order. A 4096-token chunk over 16384 slots, 32 heads of 128 over 8, takes 860
-// to 960 us, 1.0 to 1.1 PFLOP/s: there the board's power limit holds the clock
-// near 1.6 GHz. Smaller calls are bound by the rows' chain of maximum and
-// exponentials, which the two row tiles run at the same time.
+// to 990 us, 0.97 to 1.1 PFLOP/s; there the board's power limit holds the clock
+// near 1.6 GHz. What bounds it and the smaller calls is the rows' chain of maximum
+// and exponentials, which the two row tiles run at the same time, so that the
+// exponential unit and the tensor cores (49 and 46 % of a mixed call's 227 us)
+// take turns more than they overlap.
 #include <cuda.h>
 #include <stdint.h>
 
@@ -811,7 +813,8 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const AttnParams p, con
 // 2 * 128^2 * head_dim operations. Two sequences of
 // up to 4096 slots, 1024 tokens each, 32 heads of 128 over 8: 71 us, 47 us of
 // them the exponentials at 16 a clock and SM. (With two groups 103 us; 85 us
-// before short items were charged for their start.)
+// before short items were charged for their start.) Groups that do not divide 128
+// leave columns of a row tile empty: all their tiles take the loop with selects.
 constexpr uint32_t kGroups = 4, kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1, kLseWarp = kMmaWarp + 1;
 constexpr uint32_t kThreadsW = 32 * (kLseWarp + 1), kLses = 8;
 
