@@ -419,18 +419,19 @@ uint64_t ls_b200_batch_scratch_bytes(uint32_t hidden, uint32_t group_size, uint3
 int ls_b200_batch_mlp(const ls_b200_batch_args* args, void* stream);
 
 /* ------------------------------------------------------------------ */
-/* Paged key/value cache: attention of new tokens, eviction            */
+/* Paged key/value cache: appending, attention of new tokens, eviction */
 /* (new; the reference leaves attention to its applications).          */
 /* ------------------------------------------------------------------ */
 
-enum { LS_B200_FP16 = 0, LS_B200_BF16 = 1 };
+enum { LS_B200_FP16 = 0, LS_B200_BF16 = 1, LS_B200_INT8 = 2 };
 /* Bits that the kernels of this section set in a call's `error` word. What a
  * flagged sequence or page would have touched is skipped. */
 enum {
     LS_B200_ATTN_TIMEOUT = 1u << 0, /* a bounded wait gave up: output, lse and weights of the call are invalid; a
                                      * new token's slot holds its key and value, or what it held before */
     LS_B200_ATTN_LENGTH = 1u << 1,  /* q_start / kv_len of a sequence do not fit the call: skipped */
-    LS_B200_ATTN_PAGE = 1u << 2     /* a page index of a visible slot is outside the pool */
+    LS_B200_ATTN_PAGE = 1u << 2,    /* a page index of a visible slot is outside the pool */
+    LS_B200_ATTN_POSITION = 1u << 3 /* a token's position has no angles: skipped */
 };
 
 /* Attention of the new tokens of `batch` sequences over their cache. Token t of
@@ -491,6 +492,68 @@ uint64_t ls_b200_attention_scratch_bytes(const ls_b200_attention_args* args);
  * of the slot's softmax weight; the new tokens' own slots start at this call's
  * sum. Returns 0, EINVAL, ENOSPC or a CUDA error code. */
 int ls_b200_paged_attention(const ls_b200_attention_args* args, void* stream);
+
+/* A cache in 8 bits: k_pages and v_pages hold whole numbers of [-127, 127], and a
+ * value is code * 2^exponent with one exponent for the LS_B200_CACHE_BLOCK slots
+ * of a block, kv head, and keys or values: exponents [pages][kv_heads]
+ * [page_size / LS_B200_CACHE_BLOCK][2], the key's before the value's. -128 marks a
+ * block that took a value that is not finite; all its values read as NaN, until
+ * the block is begun anew. */
+enum { LS_B200_CACHE_BLOCK = 16 };
+
+/* Writes the new tokens' keys and values to their cache slots (lengths, pages
+ * and slots as in ls_b200_paged_attention, which then gets no k_new and v_new),
+ * with the position rotation on the way, and rotates their queries. With
+ * cos_sin [angles][rotary_dim] (the cosines of the rotary_dim / 2 pairs, then
+ * their sines) the first rotary_dim elements of each key and query turn by their
+ * position's angles: pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where
+ * interleaved. A token's position is positions[its row of q], or its cache slot
+ * where positions is NULL. Values, and all without cos_sin, are not rotated.
+ *
+ * Into a cache in 8 bits (cache_dtype LS_B200_INT8, any dtype of the new tokens)
+ * a block's exponent is the smallest with max |x| <= 127 * 2^exponent over its
+ * rows; where older rows of the sequence lie in the block, it only grows, and
+ * they are rounded to the new step then (an old row is off by less than one step
+ * in all). float16 takes exponents -24 to 9, bfloat16 -126 to 120: what lies
+ * beyond saturates. A block whose first slot is among the new ones begins anew.
+ *
+ * A token whose position has no angles is skipped: its slot, and its row of
+ * q_out, are left as they were; so is everything behind the last sequence, and
+ * the slots behind the last token. Pages that the call writes must be listed
+ * once. Strides are in elements, non-negative multiples of 8 (pages in 8 bits:
+ * 16; exponents: 2; cos_sin: 4); q_out may be q. */
+typedef struct ls_b200_append_args {
+    uint32_t dtype;                 /* LS_B200_FP16 / LS_B200_BF16: q, k_new, v_new, q_out */
+    uint32_t cache_dtype;           /* dtype, or LS_B200_INT8 */
+    uint32_t q_heads;               /* 0 without q */
+    uint32_t kv_heads, head_dim;    /* head_dim 64 or 128 */
+    uint32_t page_size, pages, batch;
+    uint32_t tokens;                /* rows of q, k_new, v_new; at most 2^27 */
+    uint32_t table_pages;
+    uint32_t rotary_dim;            /* a multiple of 16, at most head_dim; 0 without cos_sin */
+    uint32_t angles;                /* rows of cos_sin */
+    uint32_t interleaved;           /* 0 or 1 */
+    uint32_t reserved;              /* 0 */
+    const void* q;                  /* optional [tokens][q_heads][head_dim] */
+    void* q_out;                    /* [tokens][q_heads][head_dim], with q */
+    const void* k_new;              /* [tokens][kv_heads][head_dim] */
+    const void* v_new;
+    void* k_pages;                  /* [pages][page_size][kv_heads][head_dim] */
+    void* v_pages;
+    int8_t* exponents;              /* of a cache in 8 bits */
+    const int32_t* page_table;      /* device [batch][table_pages] */
+    const int32_t* q_start;         /* device [batch + 1], ascending */
+    const int32_t* kv_len;          /* device [batch], new tokens included */
+    const int32_t* positions;       /* optional device [tokens] */
+    const float* cos_sin;           /* optional device [angles][rotary_dim] */
+    int64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+    int64_t k_new_token_stride, k_new_head_stride, v_new_token_stride, v_new_head_stride;
+    int64_t k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;
+    int64_t exponents_page_stride, exponents_head_stride, table_stride, cos_sin_stride;
+    uint32_t* error;                /* optional device word, LS_B200_ATTN_* bits are ORed in */
+} ls_b200_append_args;
+/* Returns 0, EINVAL or a CUDA error code. */
+int ls_b200_append_cache(const ls_b200_append_args* args, void* stream);
 
 /* Keeps `budget` slots of each sequence and kv head: the first `sinks`, the
  * last `recent`, and between them those of the largest weight (equal weights:

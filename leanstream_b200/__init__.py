@@ -15,7 +15,7 @@ __all__ = ["B200Backend", "BatchMLP", "DeviceQueue", "ExecutionQueue", "quantize
 def __getattr__(name):
     # the paged cache operators check torch tensors: torch is imported with their
     # first use (and they are not among __all__, which needs none)
-    if name in ("PagedAttention", "evict_cache"):
+    if name in ("PagedAttention", "append_cache", "evict_cache"):
         from . import attention
 
         globals()[name] = getattr(attention, name)

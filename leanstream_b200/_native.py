@@ -132,8 +132,9 @@ class BatchArgs(C.Structure):
                 ("rms_eps", C.c_float), ("norm_weight", C.c_void_p), ("error", C.c_void_p),
                 ("timeout_ns", C.c_uint64)]
 
-FP16, BF16 = 0, 1
-ATTN_TIMEOUT, ATTN_LENGTH, ATTN_PAGE = 1, 2, 4
+FP16, BF16, INT8 = 0, 1, 2
+ATTN_TIMEOUT, ATTN_LENGTH, ATTN_PAGE, ATTN_POSITION = 1, 2, 4, 8
+CACHE_BLOCK = 16  # slots of a cache in 8 bits that share an exponent
 
 
 class AttentionArgs(C.Structure):
@@ -153,6 +154,22 @@ class AttentionArgs(C.Structure):
                 ("timeout_ns", C.c_uint64)]
 
 
+class AppendArgs(C.Structure):
+    """ls_b200_append_args: new keys and values into a paged cache, with the position rotation."""
+    _fields_ = [(n, C.c_uint32) for n in ("dtype", "cache_dtype", "q_heads", "kv_heads", "head_dim", "page_size",
+                                          "pages", "batch", "tokens", "table_pages", "rotary_dim", "angles",
+                                          "interleaved", "reserved")] + \
+               [(n, C.c_void_p) for n in ("q", "q_out", "k_new", "v_new", "k_pages", "v_pages", "exponents",
+                                          "page_table", "q_start", "kv_len", "positions", "cos_sin")] + \
+               [(n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "q_out_token_stride",
+                                         "q_out_head_stride", "k_new_token_stride", "k_new_head_stride",
+                                         "v_new_token_stride", "v_new_head_stride", "k_page_stride",
+                                         "k_slot_stride", "k_head_stride", "v_page_stride", "v_slot_stride",
+                                         "v_head_stride", "exponents_page_stride", "exponents_head_stride",
+                                         "table_stride", "cos_sin_stride")] + \
+               [("error", C.c_void_p)]
+
+
 class EvictArgs(C.Structure):
     """ls_b200_evict_args: eviction from a paged cache by accumulated weight."""
     _fields_ = [(n, C.c_uint32) for n in ("kv_heads", "head_dim", "page_size", "pages", "batch", "table_pages",
@@ -166,6 +183,7 @@ class EvictArgs(C.Structure):
                [("error", C.c_void_p)]
 
 
+assert C.sizeof(AppendArgs) == 56 + 12 * 8 + 18 * 8 + 8
 assert C.sizeof(AttentionArgs) == 56 + 11 * 8 + 17 * 8 + 32 and C.sizeof(EvictArgs) == 48 + 9 * 8 + 10 * 8 + 8
 assert C.sizeof(IOCompletion) == 24 and C.sizeof(IOBackend) == 64 and C.sizeof(StreamConfig) == 104
 assert C.sizeof(ExecDesc) == 20 and C.sizeof(QueueControl) == 128 and C.sizeof(DeviceExecQueue) == 32
@@ -213,6 +231,7 @@ SIGNATURES = {
     "ls_b200_batch_mlp": (C.c_int, [C.POINTER(BatchArgs), C.c_void_p]),
     "ls_b200_attention_scratch_bytes": (C.c_uint64, [C.POINTER(AttentionArgs)]),
     "ls_b200_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "ls_b200_append_cache": (C.c_int, [C.c_void_p, C.c_void_p]),
     "ls_b200_evict_cache": (C.c_int, [C.c_void_p, C.c_void_p]),
     "ls_b200_stream_create": (C.c_void_p, [C.POINTER(StreamConfig)]),
     "ls_b200_stream_view": (C.c_int, [C.c_void_p, C.POINTER(IOBackend)]),

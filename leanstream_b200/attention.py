@@ -1,5 +1,6 @@
-"""Attention over a paged key/value cache, and eviction from it, over the C ABI
-(ls_b200_paged_attention, ls_b200_evict_cache).
+"""Appending to a paged key/value cache, attention over it, and eviction from it,
+over the C ABI (ls_b200_append_cache, ls_b200_paged_attention,
+ls_b200_evict_cache).
 
 The cache is a pool of pages, `k_pages` and `v_pages` [pages][page_size]
 [kv_heads][head_dim]; row b of `page_table` lists the pages of sequence b in
@@ -9,6 +10,10 @@ ones, or a chunk of a prompt, mixed as they come. With a `window` the last
 `window` slots and the first `sinks` are visible. With `weights` the softmax
 weight that each slot received is summed per kv head, and `evict_cache` keeps
 the slots of a budget by those sums.
+
+`append_cache` writes new keys and values by itself, with the position rotation
+of keys and queries on the way, into 16-bit pages or into a cache of 8-bit
+integers with an exponent for each block of 16 slots and kv head.
 
 The caller owns every buffer until the stream has run; nothing synchronises.
 """
@@ -27,9 +32,11 @@ from .backend import _check
 # few microseconds that filling ctypes fields one by one would take.
 _ATTENTION = struct.Struct("=12IfI11Q17qQQQQ")
 _EVICT = struct.Struct("=12I9Q10qQ")
+_APPEND = struct.Struct("=14I12Q18qQ")
+assert _APPEND.size == C.sizeof(N.AppendArgs)
 assert _ATTENTION.size == C.sizeof(N.AttentionArgs) and _EVICT.size == C.sizeof(N.EvictArgs)
 
-_INT, _FLOAT = torch.int32, torch.float32
+_INT, _FLOAT, _BYTE = torch.int32, torch.float32, torch.int8
 _CODES = {torch.float16: N.FP16, torch.bfloat16: N.BF16}
 
 
@@ -245,6 +252,129 @@ class PagedAttention:
             raise RuntimeError("the error word is caller-owned (PagedAttention(error=...)): clear it there")
         self._error.zero_()
         self._scratch.zero_()
+
+
+def _refuse_append(k_new, v_new, k_pages, v_pages, page_table, q_start, kv_len, q, q_out, cos_sin, positions,
+                   exponents, error):
+    e, on = _element(k_new.dtype), kv_len.get_device()
+    _want("kv_len", kv_len, _INT, (-1,), on, contiguous=True)
+    _want("k_new", k_new, e, (-1, -1, -1), on)
+    _want("v_new", v_new, e, tuple(k_new.shape), on)
+    tokens, hk, dim = k_new.shape
+    cached = e if exponents is None else _BYTE
+    _want("k_pages", k_pages, cached, (-1, -1, hk, dim), on)
+    _want("v_pages", v_pages, cached, tuple(k_pages.shape), on)
+    _want("page_table", page_table, _INT, (kv_len.shape[0], -1), on)
+    _want("q_start", q_start, _INT, (kv_len.shape[0] + 1,), on, contiguous=True)
+    if exponents is not None:
+        _want("exponents", exponents, _BYTE, (k_pages.shape[0], hk, k_pages.shape[1] // N.CACHE_BLOCK, 2), on)
+        if exponents.stride(2) != 2:
+            raise ValueError("exponents: contiguous last dimensions expected")
+    if (q is None) != (q_out is None):
+        raise ValueError("q and q_out come together")
+    if cos_sin is None and (q is not None or positions is not None):
+        raise ValueError("q and positions come with cos_sin")
+    if q is not None:
+        _want("q", q, e, (tokens, -1, dim), on)
+        _want("q_out", q_out, e, tuple(q.shape), on)
+    if cos_sin is not None:
+        _want("cos_sin", cos_sin, _FLOAT, (-1, -1), on)
+    if positions is not None:
+        _want("positions", positions, _INT, (tokens,), on, contiguous=True)
+    if error is not None:
+        _want("error", error, _INT, (1,), on)
+    raise ValueError("the arguments do not fit together")
+
+
+def append_cache(*, k_new, v_new, k_pages, v_pages, page_table, q_start, kv_len, q=None, q_out=None, cos_sin=None,
+                 positions=None, interleaved: bool = False, exponents=None, error=None, stream=None) -> None:
+    """Writes the new tokens' k_new and v_new [tokens][kv_heads][head_dim] to their
+    cache slots (page_table, q_start and kv_len as in PagedAttention.run, which is
+    then called without k_new and v_new).
+
+    With cos_sin [positions][rotary] float32, the cosines of the rotary / 2 pairs
+    and then their sines, the first `rotary` elements of each key, and of q
+    [tokens][q_heads][head_dim] into q_out (which may be q), are rotated by the
+    angles of the token's position: positions [tokens] int32, or its cache slot.
+    Pairs are (i, i + rotary / 2), or neighbours where `interleaved`.
+
+    A cache in 8 bits has int8 pages and `exponents` [pages][kv_heads]
+    [page_size / 16][2] int8 (keys', values'): the values are code * 2^exponent.
+    A block's exponent is the smallest that reaches its largest value; it grows
+    with later tokens, and the block's older codes are rounded to the new step
+    then. A block with a value that is not finite reads as NaN (exponent -128).
+
+    error: an optional int32 device tensor, N.ATTN_* bits are ORed in (lengths,
+    pages and positions that do not fit: what they would have touched is left as
+    it was). `stream` as in PagedAttention.run."""
+    new, pool, table, lengths = k_new.shape, k_pages.shape, page_table.shape, kv_len.shape
+    e, cached, dev = k_new.dtype, k_pages.dtype, kv_len.get_device()
+    qp = op = hq = q0 = q1 = o0 = o1 = ps = cs = rotary = angles = cs0 = ex = ex0 = ex1 = er = 0
+    good = (len(new) == 3 and len(pool) == 4 and len(table) == 2 and len(lengths) == 1 and e in _CODES and
+            v_new.shape == new and v_new.dtype is e and v_pages.shape == pool and v_pages.dtype is cached and
+            pool[2:] == new[1:] and page_table.dtype is _INT and kv_len.dtype is _INT and q_start.dtype is _INT and
+            table[0] == lengths[0] and q_start.shape == (lengths[0] + 1,) and kv_len.is_contiguous() and
+            q_start.is_contiguous() and dev >= 0 and k_new.get_device() == v_new.get_device() == dev and
+            k_pages.get_device() == v_pages.get_device() == dev and
+            page_table.get_device() == q_start.get_device() == dev)
+    if good and exponents is None:
+        good = cached is e
+    elif good:
+        good = cached is _BYTE and exponents.dtype is _BYTE and exponents.get_device() == dev and \
+            exponents.shape == (pool[0], pool[2], pool[1] // 16, 2)
+        if good:
+            ex = exponents.data_ptr()
+            ex0, ex1, a, b = exponents.stride()
+            good = (a == 2 and b == 1) or not exponents.numel()
+    if good and q is not None:
+        wide = q.shape
+        good = q_out is not None and len(wide) == 3 and q_out.shape == wide and wide[0] == new[0] and \
+            wide[2] == new[2] and q.dtype is e and q_out.dtype is e and q.get_device() == q_out.get_device() == dev \
+            and cos_sin is not None
+        if good:
+            qp, op, hq = q.data_ptr(), q_out.data_ptr(), wide[1]
+            q0, q1, a = q.stride()
+            o0, o1, b = q_out.stride()
+            good = a == b == 1 or not q.numel()
+    elif good:
+        good = q_out is None
+    if good and cos_sin is not None:
+        good = cos_sin.dtype is _FLOAT and len(cos_sin.shape) == 2 and cos_sin.get_device() == dev
+        if good:
+            angles, rotary = cos_sin.shape
+            cs = cos_sin.data_ptr()
+            cs0, a = cos_sin.stride()
+            good = a == 1 or not cos_sin.numel()
+    if good and positions is not None:
+        ps = positions.data_ptr()
+        good = cos_sin is not None and positions.dtype is _INT and positions.shape == new[:1] and \
+            positions.is_contiguous() and positions.get_device() == dev
+    if good and error is not None:
+        er = error.data_ptr()
+        good = error.dtype is _INT and error.shape == (1,) and error.get_device() == dev
+    if good:
+        kn0, kn1, a = k_new.stride()
+        vn0, vn1, b = v_new.stride()
+        k0, k1, k2, c = k_pages.stride()
+        v0, v1, v2, d = v_pages.stride()
+        t0, f = page_table.stride()
+        good = (a == b == 1 or not new[0]) and (c == d == 1 or not pool[0]) and (f == 1 or not table[1])
+    if not good:
+        _refuse_append(k_new, v_new, k_pages, v_pages, page_table, q_start, kv_len, q, q_out, cos_sin, positions,
+                       exponents, error)
+    code = _CODES[e]
+    args = _APPEND.pack(code, code if exponents is None else N.INT8, hq, new[1], new[2], pool[1], pool[0], lengths[0],
+                        new[0], table[1], rotary, angles, bool(interleaved), 0, qp, op, k_new.data_ptr(),
+                        v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ex, page_table.data_ptr(),
+                        q_start.data_ptr(), kv_len.data_ptr(), ps, cs, q0, q1, o0, o1, kn0, kn1, vn0, vn1, k0, k1, k2,
+                        v0, v1, v2, ex0, ex1, t0, cs0, er)
+    call = N.load().ls_b200_append_cache
+    if stream is None and dev == _current_device():
+        rc = call(args, _raw_stream(dev))
+    else:
+        rc = _run_on(dev, call, args, _handle(stream, dev))
+    if rc:
+        _check(rc, "ls_b200_append_cache")
 
 
 def _refuse_evict(k_pages, v_pages, page_table, kv_len, weights, budget, new_table, new_len, kept, sinks, recent,

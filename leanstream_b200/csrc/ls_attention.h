@@ -1,5 +1,5 @@
-// Internal types of the paged-cache attention (ls_attention.cu) and of the
-// cache eviction (ls_evict.cu). Not part of the public ABI.
+// Internal types of the paged-cache attention (ls_attention.cu), of the append
+// (ls_append.cu) and of the cache eviction (ls_evict.cu). Not part of the public ABI.
 #pragma once
 #include <cuda.h>
 #include <stdint.h>
@@ -12,6 +12,12 @@ constexpr uint32_t kErrLength = 1u << 1;  // a sequence's lengths do not fit the
 constexpr uint32_t kErrPage = 1u << 2;    // a visible slot's page index is outside the pool
 
 constexpr uint32_t kMaxSlots = 0x7fff0000u;  // of a sequence: a tile past the last slot still counts in 32 bits
+
+// The cache in 8 bits: slots that share an exponent, and the exponent of a block
+// with a value that is not finite (it reads as NaN).
+constexpr int kBlockShift = 4, kBlock = 1 << kBlockShift;
+constexpr int32_t kNoExponent = -128;
+static_assert(kBlock == LS_B200_CACHE_BLOCK, "public block size");
 
 // ls_b200_attention_args in the kernels' units. Strides are in elements.
 struct AttnParams {
@@ -75,6 +81,7 @@ inline uint64_t chunk_part_floats(uint32_t D) { return 256ull * (D + 2); }  // o
 // from the second dimension on. False when the driver refuses it.
 bool encode_map(CUtensorMap* map, bool bf16, const void* base, uint32_t rank, const uint64_t* dims,
                 const int64_t* strides, const uint32_t* box);
+uint32_t sm_count();  // of the current device
 int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream);
 
 // A sequence of the call: its new tokens are rows q0 .. q0 + nq - 1 of q and
