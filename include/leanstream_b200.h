@@ -501,6 +501,17 @@ int ls_b200_paged_attention(const ls_b200_attention_args* args, void* stream);
  * the block is begun anew. */
 enum { LS_B200_CACHE_BLOCK = 16 };
 
+/* Attention over a cache in 8 bits that holds the new tokens already: k_pages and
+ * v_pages are int8 (strides in bytes, multiples of 16), dtype is that of q and
+ * output; no k_new, v_new, weights. Everything else, the scratch too, is as for
+ * ls_b200_paged_attention. */
+typedef struct ls_b200_cache_exponents {
+    const int8_t* exponents;        /* [pages][kv_heads][page_size / LS_B200_CACHE_BLOCK][2] */
+    int64_t page_stride, head_stride; /* even */
+} ls_b200_cache_exponents;
+int ls_b200_paged_attention_int8(const ls_b200_attention_args* args, const ls_b200_cache_exponents* exponents,
+                                 void* stream);
+
 /* Writes the new tokens' keys and values to their cache slots (lengths, pages
  * and slots as in ls_b200_paged_attention, which then gets no k_new and v_new),
  * with the position rotation on the way, and rotates their queries. With

@@ -154,6 +154,11 @@ class AttentionArgs(C.Structure):
                 ("timeout_ns", C.c_uint64)]
 
 
+class CacheExponents(C.Structure):
+    """ls_b200_cache_exponents: of the blocks of a cache in 8 bits."""
+    _fields_ = [("exponents", C.c_void_p), ("page_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
 class AppendArgs(C.Structure):
     """ls_b200_append_args: new keys and values into a paged cache, with the position rotation."""
     _fields_ = [(n, C.c_uint32) for n in ("dtype", "cache_dtype", "q_heads", "kv_heads", "head_dim", "page_size",
@@ -231,6 +236,7 @@ SIGNATURES = {
     "ls_b200_batch_mlp": (C.c_int, [C.POINTER(BatchArgs), C.c_void_p]),
     "ls_b200_attention_scratch_bytes": (C.c_uint64, [C.POINTER(AttentionArgs)]),
     "ls_b200_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "ls_b200_paged_attention_int8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "ls_b200_append_cache": (C.c_int, [C.c_void_p, C.c_void_p]),
     "ls_b200_evict_cache": (C.c_int, [C.c_void_p, C.c_void_p]),
     "ls_b200_stream_create": (C.c_void_p, [C.POINTER(StreamConfig)]),

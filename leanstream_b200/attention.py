@@ -33,6 +33,7 @@ from .backend import _check
 _ATTENTION = struct.Struct("=12IfI11Q17qQQQQ")
 _EVICT = struct.Struct("=12I9Q10qQ")
 _APPEND = struct.Struct("=14I12Q18qQ")
+_EXPONENTS = struct.Struct("=Q2q")
 assert _APPEND.size == C.sizeof(N.AppendArgs)
 assert _ATTENTION.size == C.sizeof(N.AttentionArgs) and _EVICT.size == C.sizeof(N.EvictArgs)
 
@@ -96,19 +97,26 @@ class PagedAttention:
     group new tokens of a sequence); calls on one PagedAttention must not
     overlap. `scratch` = (pointer, bytes) supplies caller-owned, zeroed device
     memory instead; `error` is then the device address of a caller-owned, zeroed
-    32-bit error word (or None)."""
+    32-bit error word (or None). cache_dtype "int8": the cache is in 8 bits, as
+    append_cache fills it (no weights; the call does not append)."""
 
     def __init__(self, q_heads: int, kv_heads: int, head_dim: int, *, page_size: int, dtype="float16",
                  max_sequences: int, max_tokens: int, max_queries: int = 1, max_weights_length: int = 0, device=None,
-                 scratch: Optional[tuple] = None, error: Optional[int] = None):
+                 scratch: Optional[tuple] = None, error: Optional[int] = None, cache_dtype=None):
         self.lib = N.load()
         self.q_heads, self.kv_heads, self.head_dim, self.page_size = q_heads, kv_heads, head_dim, page_size
         self.dtype = _element(dtype)
+        self._int8 = cache_dtype in (_BYTE, "int8")
+        self.cache_dtype = _BYTE if self._int8 else self.dtype
+        if cache_dtype is not None and not self._int8 and _element(cache_dtype) is not self.dtype:
+            raise ValueError(f"cache_dtype: {self.dtype} or int8, got {cache_dtype}")
+        if self._int8 and max_weights_length:
+            raise ValueError("weights are of 16-bit caches")
         self.max_sequences, self.max_tokens = max_sequences, max_tokens
         self.max_queries, self.max_weights_length = max_queries, max_weights_length
         self._code, self._scale = _CODES[self.dtype], head_dim ** -0.5 if head_dim > 0 else 1.0
         self._row, self._page, self._new = (q_heads, head_dim), (page_size, kv_heads, head_dim), (kv_heads, head_dim)
-        self._call = self.lib.ls_b200_paged_attention
+        self._call = self.lib.ls_b200_paged_attention_int8 if self._int8 else self.lib.ls_b200_paged_attention
         shape = N.AttentionArgs(dtype=self._code, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim,
                                 page_size=page_size, batch=max_sequences, tokens=max_tokens, max_q=max_queries,
                                 weights_length=max_weights_length, scale=1.0)
@@ -140,14 +148,22 @@ class PagedAttention:
             self.error_ptr = self._error.data_ptr()
 
     def _refuse(self, q, output, k_pages, v_pages, page_table, q_start, kv_len, max_q, k_new, v_new, lse, weights,
-                window, sinks):
+                window, sinks, exponents):
         """Names what is wrong with the arguments of a call."""
         hq, hk, dim, size, e = self.q_heads, self.kv_heads, self.head_dim, self.page_size, self.dtype
         on = q.get_device() if self._device is None else self._device
         _want("q", q, e, (-1, hq, dim), on)
         _want("output", output, e, (q.shape[0], hq, dim), on)
-        _want("k_pages", k_pages, e, (-1, size, hk, dim), on)
-        _want("v_pages", v_pages, e, (k_pages.shape[0], size, hk, dim), on)
+        _want("k_pages", k_pages, self.cache_dtype, (-1, size, hk, dim), on)
+        _want("v_pages", v_pages, self.cache_dtype, (k_pages.shape[0], size, hk, dim), on)
+        if (exponents is not None) != self._int8:
+            raise ValueError("exponents come with a cache in 8 bits")
+        if self._int8:
+            if k_new is not None or weights is not None:
+                raise ValueError("a cache in 8 bits is filled by append_cache, and keeps no weights")
+            _want("exponents", exponents, _BYTE, (k_pages.shape[0], hk, size // N.CACHE_BLOCK, 2), on)
+            if exponents.stride(2) != 2:
+                raise ValueError("exponents: contiguous last dimensions expected")
         _want("kv_len", kv_len, _INT, (-1,), on)
         _want("page_table", page_table, _INT, (kv_len.shape[0], -1), on)
         _want("q_start", q_start, _INT, (kv_len.shape[0] + 1,), on)
@@ -167,7 +183,7 @@ class PagedAttention:
 
     def run(self, stream=None, *, q, output, k_pages, v_pages, page_table, q_start, kv_len, max_q: int, k_new=None,
             v_new=None, scale: Optional[float] = None, window: int = 0, sinks: int = 0, lse=None, weights=None,
-            timeout_ns: int = 0) -> None:
+            timeout_ns: int = 0, exponents=None) -> None:
         """Enqueues one call on `stream` (a torch stream, a raw cudaStream_t as
         int, or None for torch's current stream) of the tensors' device, which
         is the engine's and need not be the current one. q, output [tokens][q_heads]
@@ -177,7 +193,8 @@ class PagedAttention:
         kv_len [sequences] int32 on the device, kv_len with the new tokens;
         max_q: the most new tokens of one sequence. scale: 1 / sqrt(head_dim)
         unless given. lse [tokens][q_heads] and weights [sequences][kv_heads]
-        [slots] float32, optional."""
+        [slots] float32, optional. exponents [pages][kv_heads][page_size / 16][2]
+        int8: of a cache in 8 bits."""
         # one pass over the tensors: each attribute of a tensor costs about 0.1 us
         e, rows, pool = self.dtype, q.shape, k_pages.shape
         table, lengths, dev = page_table.shape, kv_len.shape, q.get_device()
@@ -185,7 +202,7 @@ class PagedAttention:
         k0 = k1 = k2 = v0 = v1 = v2 = batch = tokens = 0
         good = (len(rows) == 3 and rows[1:] == self._row and len(pool) == 4 and pool[1:] == self._page and
                 len(table) == 2 and len(lengths) == 1 and output.shape == rows and v_pages.shape == pool and
-                q.dtype is e and output.dtype is e and k_pages.dtype is e and v_pages.dtype is e and
+                q.dtype is e and output.dtype is e and k_pages.dtype is v_pages.dtype is self.cache_dtype and
                 page_table.dtype is _INT and kv_len.dtype is _INT and q_start.dtype is _INT and
                 dev >= 0 and (self._device is None or self._device == dev) and dev == output.get_device() and
                 dev == k_pages.get_device() and dev == v_pages.get_device() and dev == page_table.get_device() and
@@ -208,6 +225,15 @@ class PagedAttention:
             vn0, vn1, b = v_new.stride()
             good = (k_new.shape == v_new.shape == (tokens, *self._new) and k_new.dtype is e and v_new.dtype is e and
                     k_new.get_device() == v_new.get_device() == dev and (a == b == 1 or not tokens))
+        if good and exponents is not None:
+            good = self._int8 and k_new is None and weights is None and exponents.dtype is _BYTE and \
+                exponents.shape == (pool[0], self.kv_heads, self.page_size // 16, 2) and \
+                exponents.get_device() == dev
+            if good:
+                ex0, ex1, a, b = exponents.stride()
+                good = a == 2 and b == 1 or not pool[0]
+        elif good:
+            good = not self._int8
         if good and lse is not None:
             ls = lse.data_ptr()
             good = lse.shape == rows[:2] and lse.dtype is _FLOAT and lse.is_contiguous() and \
@@ -222,7 +248,7 @@ class PagedAttention:
                 good = a == 1 or not weights.numel()
         if not good:
             self._refuse(q, output, k_pages, v_pages, page_table, q_start, kv_len, max_q, k_new, v_new, lse, weights,
-                         window, sinks)
+                         window, sinks, exponents)
         try:
             args = _ATTENTION.pack(
                 self._code, self.q_heads, self.kv_heads, self.head_dim, self.page_size, pool[0], batch, tokens, max_q,
@@ -232,10 +258,11 @@ class PagedAttention:
                 self.scratch_ptr, self.scratch_bytes, self.error_ptr, timeout_ns)
         except (struct.error, OverflowError) as e:
             raise ValueError(f"window {window}, sinks {sinks}, scale {scale}, timeout_ns {timeout_ns}: {e}") from None
+        more = (_EXPONENTS.pack(exponents.data_ptr(), ex0, ex1),) if self._int8 else ()
         if stream is None and dev == _current_device():
-            rc = self._call(args, _raw_stream(dev))
+            rc = self._call(args, *more, _raw_stream(dev))
         else:
-            rc = _run_on(dev, self._call, args, _handle(stream, dev))
+            rc = _run_on(dev, self._call, args, *more, _handle(stream, dev))
         if rc:
             _check(rc, "ls_b200_paged_attention")
 

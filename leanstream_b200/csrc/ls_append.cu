@@ -150,7 +150,6 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
     }
     return r;
 }
-__device__ __forceinline__ float two_to(int32_t e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 // Keys (VALUES false) or values of one kv head.
 template <class T, int D, bool Q8, bool VALUES>

@@ -57,11 +57,11 @@ constexpr uint64_t kGraceNs = 1000000000ull;
 constexpr uint64_t kShortNs = 100000;  // bounds that a barrier's try may sleep over: a load takes less
 
 // Three CTAs per SM by registers; the ring takes the shared memory that leaves.
-template <int D>
+template <int D, bool Q8>
 struct GeoD {
     static constexpr int kCtas = 3, kRows = 16;
-    static constexpr uint32_t kHalf = kDecKeys * D * 2, kStage = 2 * kHalf;  // a step's keys, and its values
-    static constexpr int kStages = 2 * (128 / D);
+    static constexpr uint32_t kHalf = kDecKeys * D * (Q8 ? 1 : 2), kStage = 2 * kHalf;  // a step's keys, its values
+    static constexpr int kStages = (Q8 ? 4 : 2) * (128 / D);
     static constexpr uint32_t kRing = kDecWarps * kStages * kStage;
     static constexpr uint32_t kJoin = kRing, kJoinBytes = kRows * D * 4;  // sums of the warps
     static constexpr uint32_t kSegs = kJoin + kJoinBytes, kBars = kSegs + kDecSegs * 64;
@@ -105,6 +105,21 @@ template <int ROWS>
 __device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t piece) {
     return (piece >> 3) * (ROWS * 128) + row * 128 + (((piece ^ row) & 7u) << 4);
 }
+// The same in a tile of codes, rows of D bytes: for 64 the pieces of two rows
+// share 128 bytes (the 64-byte swizzle).
+template <int D>
+__device__ __forceinline__ uint32_t swz8(uint32_t row, uint32_t piece) {
+    return D == 128 ? row * 128 + (((piece ^ row) & 7u) << 4) : row * 64 + (((piece ^ (row >> 1)) & 3u) << 4);
+}
+// Codes to float16 pairs, exactly: a code + 128 in the low byte of 1024 reads 1024
+// + 128 + code. Pairs of the four codes of v by their places.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t v, uint32_t select) {
+    uint32_t r;
+    asm("{.reg .b32 t;\n\tprmt.b32 t, %1, %2, %3;\n\tsub.rn.f16x2 %0, t, %4;}"
+        : "=r"(r) : "r"(v), "r"(0x64646464u), "r"(select), "r"(0x64806480u));
+    return r;
+}
+constexpr uint32_t kCodes01 = 0x4140, kCodes23 = 0x4342, kCodes02 = 0x4240, kCodes13 = 0x4341;
 
 // Sums of (x, y) over the block, and over the threads before this one.
 struct Pair {
@@ -147,11 +162,21 @@ __device__ __forceinline__ Pair block_scan(Pair v, Pair* sh, Pair& before) {
 // multiplier is idle beside the loads. Two sequences
 // of up to 131072 slots, 64 heads of 128 over 8: 180 us, 5.7 TB/s of the cache;
 // 32 of up to 4096 slots, 32 heads: 60 us, 4.6 TB/s; one of 97 slots: 8.5 us.
-template <class T, int D>
-__global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
+//
+// Q8, a cache in 8 bits (value = code * 2^e, one e for the 16 slots of a step): the
+// codes go to the matrix instructions as whole numbers in float16, whatever the
+// type of the queries, which enter it by a power of two of their own per row
+// (bfloat16: what lies 2^-29 below a row's largest loses bits). The exponents meet
+// the logits in 32 bits, and the probabilities as 2^(e - E), E the largest
+// exponent of the values so far; when that grows the sums are scaled down. Every
+// slot of a step that a row sees is a number, so no slot is cleared.
+template <class T, int D, bool Q8>
+__global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
     attn_decode_kernel(const AttnParams p, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
-    using G = GeoD<D>;
+    using G = GeoD<D, Q8>;
+    using M = std::conditional_t<Q8, F16, T>;  // of the matrix instructions
+    constexpr float kShift = Q8 ? 0.f : T::kShift;
     constexpr int MR = G::kRows, KS = D / 16, PIECES = D / 8, RPI = 32 / PIECES, ITERS = kDecKeys / RPI;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -166,9 +191,10 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
 
     after_start();
     if (lane == 0) {
-        for (int i = 0; i < G::kStages; ++i) bar_init(bar0 + 8 * i, 32);
+        for (int i = 0; i < G::kStages; ++i) bar_init(bar0 + 8 * i, Q8 ? 1 : 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if constexpr (Q8) after_wait();
     // units of this thread's sequence (of the first 128), and of the call; y: 1
     // where the sequence has rows
     auto units_of = [&](uint32_t b, SeqRange& s) -> Pair {
@@ -270,6 +296,9 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
             if (p.err) atomicOr(p.err, kErrPage);
             return int32_t(p.pages);
         };
+        // Q8: where the exponents of a stage's step lie (lane: stage), and these
+        const uint8_t* ex_at = nullptr;
+        uint32_t ex = 0;
         int32_t l_k = lay_out(0, int32_t(lane)), l_id = page_of(0, l_k), n_k, n_id;
         after(n_seg, n_base);
         n_k = lay_out(n_seg, n_base + int32_t(lane));
@@ -291,6 +320,18 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
             const int32_t k0 = kf & ~15, in = k0 & int32_t(p.P - 1);
             const uint32_t st = filled % G::kStages, dst = ring + st * G::kStage, bar = bar0 + 8 * st;
             ++filled;
+            if constexpr (Q8) {
+                const int32_t h = segs[l_seg].h;
+                if (lane == 0) {
+                    bar_arrive_tx(bar, G::kStage);
+                    tma4(dst, &kmap, bar, 0, in, h, id);
+                    tma4(dst + G::kHalf, &vmap, bar, 0, in, h, id);
+                }
+                if (lane == st)
+                    ex_at = uint32_t(id) < p.pages ? p.ex + int64_t(id) * p.ex_ps + int64_t(h) * p.ex_hs + (in >> 3)
+                                                   : nullptr;
+                return;
+            }
             if (!(kf & kEdge)) {
                 if (lane == 0) {
                     const int32_t h = segs[l_seg].h;
@@ -324,7 +365,13 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
             }
             cp_arrive(bar);
         };
+        // the exponents of the step in `stage` (all stages where it is kStages)
+        auto fetch = [&](uint32_t stage) {
+            if (stage == G::kStages ? lane < filled && lane < G::kStages : lane == stage)
+                ex = ex_at ? *reinterpret_cast<const uint16_t*>(ex_at) : 0u;
+        };
         uint32_t qf[KS][4];
+        int32_t qe[2] = {0, 0};  // Q8: the rows' own exponents
         auto queries = [&](const DecSeg& x) {  // as A fragments; zero past the rows
             const uint16_t* q[2];
             bool on[2];
@@ -333,7 +380,39 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
                 const int32_t r = int32_t(lane >> 2) + 8 * i;
                 on[i] = r < x.rows;
                 q[i] = p.q + int64_t(x.q0 + (on[i] ? r / g : 0)) * p.q_ts +
-                       int64_t(x.h * g + (on[i] ? r % g : 0)) * p.q_hs + (lane & 3u) * 2;
+                       int64_t(x.h * g + (on[i] ? r % g : 0)) * p.q_hs + (lane & 3u) * (Q8 ? 4 : 2);
+            }
+            if constexpr (Q8) {  // elements 4 t .. 4 t + 3 of each 16, as the codes come
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint2 v[KS];
+#pragma unroll
+                    for (int kk = 0; kk < KS; ++kk)
+                        v[kk] = on[i] ? *reinterpret_cast<const uint2*>(q[i] + kk * 16) : make_uint2(0u, 0u);
+                    if constexpr (std::is_same_v<T, BF16>) {
+                        uint32_t top = 0;  // bits of the largest |q| of the row
+#pragma unroll
+                        for (int kk = 0; kk < KS; ++kk)
+                            top = max(max(top, max(v[kk].x & 0x7fffu, (v[kk].x >> 16) & 0x7fffu)),
+                                      max(v[kk].y & 0x7fffu, (v[kk].y >> 16) & 0x7fffu));
+                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        // to [2^14, 2^15); infinities and NaN stay what they are
+                        qe[i] = top >= 0x7f80u ? 0 : max(int32_t(top >> 7) - 127 - 14, -112);
+                        const float f = two_to(-qe[i]);
+#pragma unroll
+                        for (int kk = 0; kk < KS; ++kk) {
+                            float a, b;
+                            BF16::unpack(v[kk].x, a, b);
+                            v[kk].x = F16::pack(a * f, b * f);
+                            BF16::unpack(v[kk].y, a, b);
+                            v[kk].y = F16::pack(a * f, b * f);
+                        }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < KS; ++kk) qf[kk][i] = v[kk].x, qf[kk][2 + i] = v[kk].y;
+                }
+                return;
             }
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk)
@@ -344,6 +423,7 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
         queries(segs[0]);  // ahead of the cache's stream
 #pragma unroll 1
         for (int i = 0; ok && i < G::kStages; ++i) load();
+        if constexpr (Q8) fetch(G::kStages);
 
         for (uint32_t c = 0; c < count; ++c) {
             const DecSeg& x = segs[c];
@@ -361,6 +441,7 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
                 for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
             m[0] = m[1] = -INFINITY;
             l[0] = l[1] = 0.f;
+            int32_t most = -126;  // Q8: the largest exponent of the values, the sums' own
 
             for (int32_t block = 0; ok && block < steps; block += 32) {
                 const int32_t c_k = lay_out(c, block + int32_t(lane));
@@ -374,12 +455,43 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
                     ++used;
                     // S = Q K^T
                     float sc[2][4] = {};
+                    float c = p.c, pw = 1.f;  // Q8: the logits come in the base-2 exponent's units
+                    if constexpr (Q8) {
 #pragma unroll
-                    for (int kk = 0; kk < KS; ++kk) {
-                        uint32_t bf[4];
-                        ldsm4(bf, ks + swz<kDecKeys>((lane & 7u) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1u)));
-                        T::mma(sc[0], qf[kk], bf[0], bf[1]);
-                        T::mma(sc[1], qf[kk], bf[2], bf[3]);
+                        for (int kk = 0; kk < KS; kk += 2) {
+                            uint32_t bf[4];
+                            ldsm4(bf, ks + swz8<D>((lane & 7u) + ((lane >> 4) << 3), kk + ((lane >> 3) & 1u)));
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) {
+                                const uint32_t v = bf[y] ^ 0x80808080u;
+                                M::mma(sc[y >> 1], qf[kk + (y & 1)], codes_f16(v, kCodes01), codes_f16(v, kCodes23));
+                            }
+                        }
+                        const uint32_t both = __shfl_sync(0xffffffffu, ex, int(st));
+                        const int32_t ek = int8_t(both), ev = int8_t(both >> 8);
+                        c = 1.f;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float f = ek == kNoExponent ? NAN : p.c * two_to(min(max(ek + qe[i], -126), 127));
+                            sc[0][2 * i] *= f, sc[0][2 * i + 1] *= f, sc[1][2 * i] *= f, sc[1][2 * i + 1] *= f;
+                        }
+                        if (ev > most) {
+                            const float f = two_to(max(most - ev, -126));
+#pragma unroll
+                            for (int n = 0; n < 2 * KS; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[n][e] *= f;
+                            most = ev;
+                        }
+                        pw = ev == kNoExponent ? NAN : two_to(max(ev - most + int(F16::kShift), -126));
+                    } else {
+#pragma unroll
+                        for (int kk = 0; kk < KS; ++kk) {
+                            uint32_t bf[4];
+                            ldsm4(bf, ks + swz<kDecKeys>((lane & 7u) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1u)));
+                            M::mma(sc[0], qf[kk], bf[0], bf[1]);
+                            M::mma(sc[1], qf[kk], bf[2], bf[3]);
+                        }
                     }
                     if (kf & kMasked) {
 #pragma unroll
@@ -410,11 +522,11 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
                         y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
                         y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
                         nm[i] = fmaxf(m[i], y);
-                        bs[i] = nm[i] == -INFINITY ? 0.f : fmaf(nm[i], p.c, -T::kShift);
+                        bs[i] = nm[i] == -INFINITY ? 0.f : fmaf(nm[i], c, -kShift);
                     }
                     if (__any_sync(0xffffffffu, nm[0] > m[0] || nm[1] > m[1])) {
-                        const float al[2] = {ex2(fmaf(m[0], p.c, -T::kShift) - bs[0]),
-                                             ex2(fmaf(m[1], p.c, -T::kShift) - bs[1])};
+                        const float al[2] = {ex2(fmaf(m[0], c, -kShift) - bs[0]),
+                                             ex2(fmaf(m[1], c, -kShift) - bs[1])};
 #pragma unroll
                         for (int n = 0; n < 2 * KS; ++n)
 #pragma unroll
@@ -426,29 +538,49 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
                     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const float a = ex2(fmaf(sc[nt][2 * i], p.c, -bs[i]));
-                            const float d = ex2(fmaf(sc[nt][2 * i + 1], p.c, -bs[i]));
+                            float a = ex2(fmaf(sc[nt][2 * i], c, -bs[i]));
+                            float d = ex2(fmaf(sc[nt][2 * i + 1], c, -bs[i]));
                             l[i] += a + d;
+                            if constexpr (Q8) a *= pw, d *= pw;
                             // A fragment: registers (row, row + 8) x (keys 0-7, 8-15)
-                            ph[nt * 2 + i] = T::pack(a, d);
+                            ph[nt * 2 + i] = M::pack(a, d);
                             float ha, hd;
-                            T::unpack(ph[nt * 2 + i], ha, hd);
-                            pl[nt * 2 + i] = T::pack(a - ha, d - hd);
+                            M::unpack(ph[nt * 2 + i], ha, hd);
+                            pl[nt * 2 + i] = M::pack(a - ha, d - hd);
                         }
                     // O += P V. P enters as its 16-bit rounding plus the 16-bit
                     // rounding of what that leaves: the tensor cores are far from
                     // busy here, and the sum keeps about twice the bits.
+                    if constexpr (Q8) {
+                        // (two codes of a slot lie side by side: the even ones of each 16
+                        // elements in one product, the odd ones in the other)
 #pragma unroll
-                    for (int n = 0; n < KS; ++n) {
-                        uint32_t vf[4];
-                        ldsm4t(vf, vs + swz<kDecKeys>((lane & 7u) + (((lane >> 3) & 1u) << 3), n * 2 + (lane >> 4)));
-                        T::mma(o[2 * n], ph, vf[0], vf[1]);
-                        T::mma(o[2 * n + 1], ph, vf[2], vf[3]);
-                        T::mma(o[2 * n], pl, vf[0], vf[1]);
-                        T::mma(o[2 * n + 1], pl, vf[2], vf[3]);
+                        for (int n = 0; n < KS; n += 2) {
+                            uint32_t vf[4];
+                            ldsm4t(vf, vs + swz8<D>((lane & 7u) + (((lane >> 3) & 1u) << 3), n + (lane >> 4)));
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) vf[y] ^= 0x80808080u;
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) {
+                                const uint32_t select = y & 1 ? kCodes13 : kCodes02;
+                                const uint32_t v0 = codes_f16(vf[y & 2], select), v1 = codes_f16(vf[(y & 2) + 1], select);
+                                M::mma(o[2 * n + y], ph, v0, v1);
+                                M::mma(o[2 * n + y], pl, v0, v1);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < KS; ++n) {
+                            uint32_t vf[4];
+                            ldsm4t(vf, vs + swz<kDecKeys>((lane & 7u) + (((lane >> 3) & 1u) << 3), n * 2 + (lane >> 4)));
+                            M::mma(o[2 * n], ph, vf[0], vf[1]);
+                            M::mma(o[2 * n + 1], ph, vf[2], vf[3]);
+                            M::mma(o[2 * n], pl, vf[0], vf[1]);
+                            M::mma(o[2 * n + 1], pl, vf[2], vf[3]);
+                        }
                     }
                     // the new tokens' keys and values go to their slots
-                    if (p.fused && (kf & kEdge) && k0 + kDecKeys > x.f) {
+                    if (!Q8 && p.fused && (kf & kEdge) && k0 + kDecKeys > x.f) {
                         const int32_t id = p.table[int64_t(x.b) * p.table_s + (k0 >> p.pshift)];
                         const uint32_t piece = lane % PIECES;
                         if (uint32_t(id) < p.pages) {
@@ -470,9 +602,15 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
                     }
                     // the stage's next contents come through the TMA's proxy: what the
                     // copies wrote is ordered before
-                    if (kf & kEdge) proxy_fence();
+                    if (!Q8 && (kf & kEdge)) proxy_fence();
                     __syncwarp();
-                    load();
+                    if constexpr (Q8) {
+                        const uint32_t before = filled;
+                        load();
+                        if (filled != before) fetch(before % G::kStages);
+                    } else {
+                        load();
+                    }
                 }
             }
 
@@ -487,7 +625,7 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
                 y += __shfl_xor_sync(0xffffffffu, y, 2);
                 if ((lane & 3u) == 0) {
                     const uint32_t row = (lane >> 2) + 8 * i;
-                    sm[warp * MR + row] = fmaf(m[i], p.c, -T::kShift);  // (the reference)
+                    sm[warp * MR + row] = Q8 ? m[i] : fmaf(m[i], p.c, -kShift);  // (the reference)
                     sl[warp * MR + row] = y;
                 }
             }
@@ -502,7 +640,21 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
                         float mx = sm[row];
 #pragma unroll
                         for (int w = 1; w < kDecWarps; ++w) mx = fmaxf(mx, sm[w * MR + row]);
-                        const float f = mx == -INFINITY ? 0.f : ex2(fmaf(m[i], p.c, -T::kShift) - mx);
+                        float f = mx == -INFINITY ? 0.f : ex2((Q8 ? m[i] : fmaf(m[i], p.c, -kShift)) - mx);
+                        if constexpr (Q8) {
+                            f *= two_to(max(most - int(F16::kShift), -126));
+                            float* to = join + at * D;
+#pragma unroll
+                            for (int n = 0; n < KS; ++n) {
+                                float4* cell = reinterpret_cast<float4*>(
+                                    to + ((n * 16 + (lane & 3u) * 4) ^ (at & 7u) * 8));
+                                float4 v = make_float4(o[2 * n][2 * i] * f, o[2 * n + 1][2 * i] * f,
+                                                       o[2 * n][2 * i + 1] * f, o[2 * n + 1][2 * i + 1] * f);
+                                if (turn) v.x += cell->x, v.y += cell->y, v.z += cell->z, v.w += cell->w;
+                                *cell = v;
+                            }
+                            continue;
+                        }
                         float* to = join + at * D + (lane & 3u) * 2;
 #pragma unroll
                         for (int n = 0; n < 2 * KS; ++n) {
@@ -733,47 +885,52 @@ int check_shape(const ls_b200_attention_args& a) {
     return 0;
 }
 
-template <class T, int D>
+template <class T, int D, bool Q8>
 int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
-    using G = GeoD<D>;
+    using G = GeoD<D, Q8>;
     CUtensorMap km, vm;
-    const uint64_t dims[5] = {64, p.P, D / 64, p.Hkv, p.pages};
-    const int64_t ks[4] = {p.kp_ss, 64, p.kp_hs, p.kp_ps}, vs[4] = {p.vp_ss, 64, p.vp_hs, p.vp_ps};
-    const uint32_t box[5] = {64, uint32_t(kDecKeys), D / 64, 1, 1};
-    if (!encode_map(&km, bf16, p.k_pages, 5, dims, ks, box) || !encode_map(&vm, bf16, p.v_pages, 5, dims, vs, box))
-        return EINVAL;
+    if constexpr (Q8) {
+        if (!encode_codes(&km, p.k_pages, p, p.kp_ss, p.kp_hs, p.kp_ps, kDecKeys) ||
+            !encode_codes(&vm, p.v_pages, p, p.vp_ss, p.vp_hs, p.vp_ps, kDecKeys))
+            return EINVAL;
+    } else {
+        const uint64_t dims[5] = {64, p.P, D / 64, p.Hkv, p.pages};
+        const int64_t ks[4] = {p.kp_ss, 64, p.kp_hs, p.kp_ps}, vs[4] = {p.vp_ss, 64, p.vp_hs, p.vp_ps};
+        const uint32_t box[5] = {64, uint32_t(kDecKeys), D / 64, 1, 1};
+        if (!encode_map(&km, bf16, p.k_pages, 5, dims, ks, box) || !encode_map(&vm, bf16, p.v_pages, 5, dims, vs, box))
+            return EINVAL;
+    }
+    const auto kernel = attn_decode_kernel<T, D, Q8>;
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return int(e);
     const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
     if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(attn_decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 int(G::kSmem));
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(G::kSmem));
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attn_decode_kernel<T, D>, cudaFuncAttributePreferredSharedMemoryCarveout,
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                                      int(cudaSharedmemCarveoutMaxShared));
         if (e != cudaSuccess) return int(e);
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
-    const uint32_t grid = sm_count() * uint32_t(G::kCtas);
-    attn_decode_kernel<T, D><<<grid < kMaxCtas ? grid : kMaxCtas, kDecThreads, G::kSmem, s>>>(p, km, vm);
+    const uint32_t sms = sm_count() * uint32_t(G::kCtas), grid = sms < kMaxCtas ? sms : kMaxCtas;
+    // (the append before a call over 8 bits lets it begin early)
+    if constexpr (Q8) return int(launch_after(kernel, grid, kDecThreads, G::kSmem, s, p, km, vm));
+    kernel<<<grid, kDecThreads, G::kSmem, s>>>(p, km, vm);
     return int(cudaGetLastError());
 }
-}  // namespace
-}  // namespace lsb
-
-extern "C" {
-
-uint64_t ls_b200_attention_scratch_bytes(const ls_b200_attention_args* a) {
-    if (!a || lsb::check_shape(*a)) return 0;
-    return lsb::scratch_bytes(*a);
+template <bool Q8>
+int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
+    return p.D == 64 ? (bf16 ? launch_decode<BF16, 64, Q8>(p, true, s) : launch_decode<F16, 64, Q8>(p, false, s))
+                     : (bf16 ? launch_decode<BF16, 128, Q8>(p, true, s) : launch_decode<F16, 128, Q8>(p, false, s));
 }
 
-int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
-    using namespace lsb;
+// A call over a cache of 16 bits (x NULL) or 8 bits.
+int attend(const ls_b200_attention_args* a, const ls_b200_cache_exponents* x, void* stream) {
     if (!a) return EINVAL;
     if (const int e = check_shape(*a)) return e;
+    if (x && (a->k_new || a->v_new || a->weights || a->weights_length)) return EINVAL;
     if (!a->batch || !a->tokens || !a->max_q) return 0;  // no new token: nothing to write
     if (!a->q || !a->output || !a->k_pages || !a->v_pages || !a->page_table || !a->q_start || !a->kv_len ||
         !a->scratch || !a->pages || !a->table_pages || (!a->k_new) != (!a->v_new) ||
@@ -787,6 +944,14 @@ int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
                             a->k_page_stride, a->k_slot_stride, a->k_head_stride, a->v_page_stride, a->v_slot_stride,
                             a->v_head_stride})
         if (!stride8(v)) return EINVAL;
+    if (x) {
+        for (const int64_t v : {a->k_page_stride, a->k_slot_stride, a->k_head_stride, a->v_page_stride,
+                                a->v_slot_stride, a->v_head_stride})
+            if (v % 16) return EINVAL;
+        if (!x->exponents || (reinterpret_cast<uintptr_t>(x->exponents) & 1u) || x->page_stride % 2 ||
+            x->head_stride % 2 || x->page_stride < 0 || x->head_stride < 0)
+            return EINVAL;
+    }
     const ScratchPlan plan = scratch_plan(*a);
     if (a->scratch_bytes < plan.total) return ENOSPC;
     uint8_t* scratch = static_cast<uint8_t*>(a->scratch);
@@ -822,7 +987,12 @@ int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
     p.sinks = a->sinks, p.wlen = a->weights_length;
     p.rows = p.max_q * p.g;
     p.timeout_ns = a->timeout_ns ? a->timeout_ns : kTimeoutNs;
+    if (x) {
+        p.ex = reinterpret_cast<const uint8_t*>(x->exponents);
+        p.ex_ps = x->page_stride, p.ex_hs = x->head_stride;
+    }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (x && is_chunk(*a)) return EINVAL;
     if (is_chunk(*a)) {
         const ChunkScratch c{reinterpret_cast<ChunkPlan*>(scratch + plan.plan),
                              reinterpret_cast<ChunkItem*>(scratch + plan.items),
@@ -834,10 +1004,27 @@ int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
     }
     p.fused = p.k_new != nullptr;
     const bool bf16 = a->dtype == LS_B200_BF16;
-    const int rc = p.D == 64 ? (bf16 ? launch_decode<BF16, 64>(p, true, s) : launch_decode<F16, 64>(p, false, s))
-                             : (bf16 ? launch_decode<BF16, 128>(p, true, s) : launch_decode<F16, 128>(p, false, s));
+    const int rc = x ? launch_decode<true>(p, bf16, s) : launch_decode<false>(p, bf16, s);
     if (rc || !p.weights) return rc;
     return int(launch_after(attn_weights_kernel, p.B * p.Hkv * ((p.wlen + 255) / 256), 256, 0, s, p));
+}
+}  // namespace
+}  // namespace lsb
+
+extern "C" {
+
+uint64_t ls_b200_attention_scratch_bytes(const ls_b200_attention_args* a) {
+    if (!a || lsb::check_shape(*a)) return 0;
+    return lsb::scratch_bytes(*a);
+}
+
+int ls_b200_paged_attention(const ls_b200_attention_args* a, void* stream) {
+    return lsb::attend(a, nullptr, stream);
+}
+
+int ls_b200_paged_attention_int8(const ls_b200_attention_args* a, const ls_b200_cache_exponents* exponents,
+                                 void* stream) {
+    return exponents ? lsb::attend(a, exponents, stream) : EINVAL;
 }
 
 }  // extern "C"

@@ -39,6 +39,8 @@ struct AttnParams {
     int64_t q_ts, q_hs, kn_ts, kn_hs, vn_ts, vn_hs, o_ts, o_hs;
     int64_t kp_ps, kp_ss, kp_hs, vp_ps, vp_ss, vp_hs;
     int64_t table_s, w_ss, w_hs;
+    const uint8_t* ex;  // a cache in 8 bits: its exponents (keys, values of a block side by side)
+    int64_t ex_ps, ex_hs;
     float c;  // scale * log2(e)
     uint32_t B, Hq, Hkv, g, D, P, pshift, pages, tpages, tokens, max_q, window, sinks, wlen;
     uint32_t rows;   // max_q * g: row capacity of `logits`
@@ -81,6 +83,9 @@ inline uint64_t chunk_part_floats(uint32_t D) { return 256ull * (D + 2); }  // o
 // from the second dimension on. False when the driver refuses it.
 bool encode_map(CUtensorMap* map, bool bf16, const void* base, uint32_t rank, const uint64_t* dims,
                 const int64_t* strides, const uint32_t* box);
+// One of codes: boxes of `slots` rows of a head, rows of D bytes in its swizzle.
+bool encode_codes(CUtensorMap* map, const void* base, const AttnParams& p, int64_t ss, int64_t hs, int64_t ps,
+                  uint32_t slots);
 uint32_t sm_count();  // of the current device
 int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream);
 
@@ -164,6 +169,7 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float two_to(int32_t e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLog2e = 1.44269504088896341f;
 

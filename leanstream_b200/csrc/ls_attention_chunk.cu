@@ -1246,6 +1246,18 @@ bool encode_map(CUtensorMap* map, bool bf16, const void* base, uint32_t rank, co
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_codes(CUtensorMap* map, const void* base, const AttnParams& p, int64_t ss, int64_t hs, int64_t ps,
+                  uint32_t slots) {
+    const cuuint64_t size[4] = {p.D, p.P, p.Hkv, p.pages};
+    const cuuint64_t bytes[3] = {cuuint64_t(ss), p.Hkv > 1 ? cuuint64_t(hs) : p.D, p.pages > 1 ? cuuint64_t(ps) : p.D};
+    const cuuint32_t part[4] = {p.D, slots, 1, 1}, ones[4] = {1, 1, 1, 1};
+    return encoder() &&
+           encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), size, bytes, part, ones,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     p.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream) {
     const uint32_t grid = sms < kMaxCtas ? sms : kMaxCtas;
     if (p.D == 64)
