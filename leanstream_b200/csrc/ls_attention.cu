@@ -992,7 +992,6 @@ int attend(const ls_b200_attention_args* a, const ls_b200_cache_exponents* x, vo
         p.ex_ps = x->page_stride, p.ex_hs = x->head_stride;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (x && is_chunk(*a)) return EINVAL;
     if (is_chunk(*a)) {
         const ChunkScratch c{reinterpret_cast<ChunkPlan*>(scratch + plan.plan),
                              reinterpret_cast<ChunkItem*>(scratch + plan.items),

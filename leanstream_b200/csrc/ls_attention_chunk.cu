@@ -50,22 +50,65 @@ using namespace tc;
 
 constexpr int kKeys = kChunkKeys, kHalf = kKeys / 2;
 constexpr int kThreads = 384;  // twelve warps, 168 registers per thread
+// Over 8 bits sixteen, 128 registers per thread at the launch; the rows' two
+// warpgroups take 176, the other two leave 48 of theirs.
+constexpr int kThreads8 = 512, kRegs8 = 128, kRowRegs8 = 176, kOtherRegs8 = 80;
+static_assert(2 * (kRowRegs8 + kOtherRegs8) <= 4 * kRegs8, "registers of the launch");
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows of 64 elements
 constexpr uint64_t kGraceNs = 1000000000ull;
 
-template <int D>
+template <int D, bool Q8>
 struct Geo {
     static constexpr uint32_t kPanels = D / 64, kTile = kPanels * kPanel;
-    static constexpr uint32_t kStages = D == 128 ? 5 : 8;
-    static constexpr uint32_t kRing = 2 * kTile, kBars = kRing + kStages * kTile;
-    static constexpr uint32_t kSegs = kBars + 320;
+    static constexpr uint32_t kStages = D == 128 ? (Q8 ? 4 : 5) : 8;
+    static constexpr uint32_t kCodes = 128 * D, kCodeStages = 256 / D;  // over 8 bits: tiles as they lie in the cache
+    static constexpr uint32_t kRing = 2 * kTile, kCodeRing = kRing + kStages * kTile;
+    static constexpr uint32_t kBars = kCodeRing + (Q8 ? kCodeStages * kCodes : 0);
+    static constexpr uint32_t kSegs = kBars + 384;
     static constexpr uint32_t kSmem = kSegs + 320 + 1024;  // + alignment of the swizzled tiles
 };
-static_assert(Geo<128>::kSmem <= 227 * 1024 && Geo<64>::kSmem <= 227 * 1024, "shared memory of a CTA");
+static_assert(Geo<128, false>::kSmem <= 227 * 1024 && Geo<64, false>::kSmem <= 227 * 1024 &&
+                  Geo<128, true>::kSmem <= 227 * 1024 && Geo<64, true>::kSmem <= 227 * 1024,
+              "shared memory of a CTA");
+
+// Codes (the four of v) and their block's 2^e as a pair of the 16-bit type, exactly.
+__device__ __forceinline__ uint32_t permute(uint32_t v, uint32_t with, uint32_t select) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(with), "r"(select));
+    return r;
+}
+template <class T>
+__device__ __forceinline__ uint32_t step_of(int32_t e) {  // a pair of 2^e; NaN for a marked block
+    uint32_t one;
+    if constexpr (std::is_same_v<T, F16>)
+        one = e == kNoExponent ? 0x7e00u : e >= -14 ? uint32_t(min(e, 15) + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
+    else
+        one = e == kNoExponent ? 0x7fc0u : uint32_t(max(e, -126) + 127) << 7;
+    return one * 0x10001u;
+}
+template <class T>
+__device__ __forceinline__ uint2 values4(uint32_t v, uint32_t step) {
+    uint2 r;
+    if constexpr (std::is_same_v<T, F16>) {  // code + 128 in the low byte of 1024
+        v ^= 0x80808080u;
+        const uint32_t a = permute(v, 0x64646464u, 0x4140u), b = permute(v, 0x64646464u, 0x4342u);
+        asm("{.reg .b32 t;\n\tsub.rn.f16x2 t, %1, %3;\n\tmul.rn.f16x2 %0, t, %2;}"
+            : "=r"(r.x) : "r"(a), "r"(step), "r"(0x64806480u));
+        asm("{.reg .b32 t;\n\tsub.rn.f16x2 t, %1, %3;\n\tmul.rn.f16x2 %0, t, %2;}"
+            : "=r"(r.y) : "r"(b), "r"(step), "r"(0x64806480u));
+    } else {  // its low seven bits in 128, less 128, or 256 where the code is below 0
+        const uint32_t a = permute(v, 0x43434343u, 0x4140u), b = permute(v, 0x43434343u, 0x4342u);
+        asm("{.reg .b32 t;\n\tsub.rn.bf16x2 t, %1, %2;\n\tmul.rn.bf16x2 %0, t, %3;}"
+            : "=r"(r.x) : "r"(a & 0x437f437fu), "r"(a & 0x43804380u), "r"(step));
+        asm("{.reg .b32 t;\n\tsub.rn.bf16x2 t, %1, %2;\n\tmul.rn.bf16x2 %0, t, %3;}"
+            : "=r"(r.y) : "r"(b & 0x437f437fu), "r"(b & 0x43804380u), "r"(step));
+    }
+    return r;
+}
 
 // Barriers: ring full / empty, Q full / empty; S full and P ready by row tile
 // and buffer, the last two P V of a piece by row tile; the last MMAs of the
-// CTA, pieces full / empty.
+// CTA, pieces full / empty; over 8 bits the ring of codes full / empty.
 struct Bars {
     uint32_t base;
     __device__ uint32_t full(uint32_t s) const { return base + 8 * s; }
@@ -78,6 +121,8 @@ struct Bars {
     __device__ uint32_t drain(uint32_t i) const { return base + 8 * (28 + i); }
     __device__ uint32_t seg_full(uint32_t s) const { return base + 8 * (30 + s); }
     __device__ uint32_t seg_empty(uint32_t s) const { return base + 8 * (34 + s); }
+    __device__ uint32_t codes_full(uint32_t s) const { return base + 8 * (40 + s); }
+    __device__ uint32_t codes_empty(uint32_t s) const { return base + 8 * (44 + s); }
 };
 
 // Lays out the items of a call in `plan` and `items`: for the attention
@@ -184,6 +229,7 @@ __device__ void lay_out(const AttnParams& p, ChunkPlan* plan, ChunkItem* list, i
 constexpr uint64_t kAppendBlocks = 16384;  // about: max_q may be far above what the sequences bring
 __global__ void __launch_bounds__(256) chunk_prepare_kernel(const AttnParams p, const ChunkScratch sc, uint32_t grid) {
     after_start();
+    after_wait();
     if (blockIdx.x == 0) {
         lay_out<false>(p, sc.plan, sc.items, int32_t(chunk_items(p.tokens, p.B, p.g)), grid);
     } else if (blockIdx.x == 1) {
@@ -259,7 +305,7 @@ struct Seg {
     }
 };
 static_assert(sizeof(Seg) == 80, "four pieces fit");
-constexpr uint32_t kSegs = 4, kSegReaders = 11;
+constexpr uint32_t kSegs = 4;
 
 // Goes through the halves of a piece, and through the ring stages of their keys
 // (values) from piece to piece.
@@ -287,11 +333,12 @@ struct Halves {
     }
 };
 
-template <class T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+template <class T, int D, bool Q8>
+__global__ void __launch_bounds__(Q8 ? kThreads8 : kThreads, 1)
     chunk_attn_kernel(const AttnParams p, const ChunkScratch sc, const __grid_constant__ CUtensorMap qmap,
                       const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    using G = Geo<D>;
+    using G = Geo<D, Q8>;
+    constexpr uint32_t kSegReaders = (Q8 ? kThreads8 : kThreads) / 32 - 1;  // all warps but warp 10
     extern __shared__ uint8_t raw[];
     const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t* const base = raw + (smem - smem_u32(raw));
@@ -302,9 +349,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (tid == 0) {
         for (uint32_t s = 0; s < G::kStages; ++s) {
-            bar_init(bar.full(s), 1);
-            bar_init(bar.empty(s), 2);  // the two MMA warps
+            bar_init(bar.full(s), Q8 ? 4 : 1);  // (the four warps that write a stage's values)
+            bar_init(bar.empty(s), 2);          // the two MMA warps
         }
+        if constexpr (Q8)
+            for (uint32_t s = 0; s < G::kCodeStages; ++s) {
+                bar_init(bar.codes_full(s), 1);
+                bar_init(bar.codes_empty(s), 4);
+            }
         bar_init(bar.q_full(), 1);
         bar_init(bar.q_empty(), 2);
         for (uint32_t i = 0; i < 2; ++i) {
@@ -340,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the next piece; false when there is none (or when a wait gave up)
     uint32_t sg = 0;
     auto next = [&]() -> bool {
-        if (!warp_wait(bar.seg_full(sg % kSegs), (sg / kSegs) & 1u, p.timeout_ns)) return ok = false;
+        if (!warp_wait<!Q8>(bar.seg_full(sg % kSegs), (sg / kSegs) & 1u, p.timeout_ns)) return ok = false;
         return uniform(segs[sg % kSegs].steps) != 0;
     };
     auto release = [&]() {
@@ -349,98 +401,89 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++sg;
     };
 
-    if (warp == 10) {
-        // ---- pieces
-        if (lane == 0) {
-            Walk w;
-            KeyRange kr{};
-            bool more = w.begin(sc.plan);
-            for (; ok; ++sg) {
-                if (sg >= kSegs && !bar_wait(bar.seg_empty(sg % kSegs), (sg / kSegs - 1) & 1u, p.timeout_ns)) {
-                    ok = false;
-                    break;
-                }
-                more = more && w.next(p, sc.plan, sc.items);
-                Seg x{};
-                if (more) {
-                    const SeqRange q{w.it.q0, w.it.nq, w.it.n, w.it.n - w.it.nq};
-                    kr = key_range<kKeys>(p, q, w.it.t0, min(w.it.nq, w.it.t0 + 2 * per_tile));
-                    x.steps = w.steps, x.row0 = w.it.q0 + w.it.t0, x.left = w.it.nq - w.it.t0;
-                    x.pos0 = w.it.n - w.it.nq + w.it.t0, x.h = w.h, x.b = w.it.b, x.j0 = w.j0;
-                    x.ns = kr.ns, x.first = kr.first, x.lo = kr.lo, x.hi = kr.hi, x.sink = kr.sink;
-                    x.set_halves();
-                    x.whole = w.j0 == 0 && w.steps == w.it.tiles;
-                    x.part = w.u != w.u_begin;
-                    if (!x.whole && !w.j0) sc.plan->open[blockIdx.x] = make_int2(w.i, w.h);
-                }
-                *reinterpret_cast<Seg*>(base + G::kSegs + (sg % kSegs) * sizeof(Seg)) = x;
-                bar_arrive(bar.seg_full(sg % kSegs));
-                if (!more) break;
-            }
-        }
-        __syncwarp();
-    } else if (warp == 9) {
-        // ---- loads
+    auto convert = [&](auto) {  // (a template: only instantiated over 8 bits)
+        // ---- codes to values: each of four warps 32 slots of every tile
+        const uint32_t mine = (warp - 12) * 32;
         uint32_t slot = 0;  // ring slots filled
-        const uint32_t box = min(p.P, 128u), boxes = 128 / box;
         while (ok && next()) {
             const Seg w = segs[sg % kSegs];
-            const int32_t two = w.left > per_tile ? 2 : 1;
-            if (sg && !warp_wait(bar.q_empty(), (sg - 1) & 1u, p.timeout_ns)) {
-                ok = false;
-                break;
-            }
-            if (lane == 0) {
-                bar_arrive_tx(bar.q_full(), uint32_t(two) * G::kPanels * uint32_t(per_tile) * p.g * 128);
-                for (int32_t i = 0; i < two; ++i)
-                    for (uint32_t c = 0; c < G::kPanels; ++c)
-                        tma3(smem + uint32_t(i) * G::kTile + c * kPanel, &qmap, bar.q_full(), int32_t(c * 64),
-                             w.h * int32_t(p.g), w.row0 + i * per_tile);
-            }
             const int32_t* trow = p.table + int64_t(w.b) * p.table_s;
-            auto page_of = [&](int32_t step) -> int32_t {  // this lane's page of a step (outside the pool: zeros)
-                if (step >= w.steps || lane >= boxes) return int32_t(p.pages);
-                const int32_t k0 = w.slot0(step) + int32_t(lane * box), k1 = k0 + int32_t(box);
-                if (!((k0 < w.hi && k1 > w.lo) || k0 < w.sink)) return int32_t(p.pages);
-                const int32_t id = trow[k0 >> p.pshift];
-                if (uint32_t(id) < p.pages) return id;
-                if (p.err) atomicOr(p.err, kErrPage);
-                return int32_t(p.pages);
+            const uint8_t* eh = p.ex + int64_t(w.h) * p.ex_hs;
+            // lanes 0 and 1: where the exponents of their block of a step lie; blocks that no
+            // row sees are zeros (-127)
+            auto page_of = [&](int32_t step) -> int32_t {
+                if (step >= w.steps || lane >= 2) return -1;
+                const int32_t k0 = w.slot0(step) + int32_t(mine + lane * 16), k1 = k0 + 16;
+                return (k0 < w.hi && k1 > w.lo) || k0 < w.sink ? trow[k0 >> p.pshift] : -1;
             };
-            int32_t next_id = page_of(0);
+            auto exponents_of = [&](int32_t step, int32_t id) -> uint32_t {
+                if (uint32_t(id) >= p.pages) return 0x8181u;
+                const int32_t in = (w.slot0(step) + int32_t(mine + lane * 16)) & int32_t(p.P - 1);
+                return *reinterpret_cast<const uint16_t*>(eh + int64_t(id) * p.ex_ps + (in >> 3));
+            };
+            uint32_t ex = exponents_of(0, page_of(0)), next_ex = 0x8181u;
             for (int32_t j = 0; j < w.steps; ++j) {
-                const int32_t id = next_id;
-                next_id = page_of(j + 1);
-                const int32_t in = (w.slot0(j) + int32_t(lane * box)) & int32_t(p.P - 1);
+                const int32_t next_id = page_of(j + 1);
                 for (int kv = 0; kv < 2; ++kv, ++slot) {
                     const uint32_t s = slot % G::kStages, n = slot / G::kStages;
-                    if (n && !warp_wait(bar.empty(s), (n - 1) & 1u, p.timeout_ns)) {
-                        ok = false;
-                        break;
+                    const uint32_t cs = slot % G::kCodeStages, cn = slot / G::kCodeStages;
+                    uint32_t step[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int32_t e = int8_t(__shfl_sync(0xffffffffu, ex, i) >> (8 * kv));
+                        step[i] = e == -127 ? 0u : step_of<T>(e);
                     }
-                    if (lane == 0) bar_arrive_tx(bar.full(s), G::kTile);
+                    if (kv) next_ex = exponents_of(j + 1, next_id);
+                    if (!(ok = warp_wait<!Q8>(bar.codes_full(cs), cn & 1u, p.timeout_ns))) break;
+                    // eight lanes take four pieces of two neighbouring rows at a time: reads and
+                    // writes meet no bank twice
+                    constexpr int kPasses = D / 64;
+                    const uint32_t half = (lane >> 2) & 1u, row0 = mine + (lane >> 3) * 2 + half;
+                    const uint8_t* from = base + G::kCodeRing + cs * G::kCodes;
+                    uint4 v[4][kPasses];
+#pragma unroll
+                    for (uint32_t it = 0; it < 4; ++it)
+#pragma unroll
+                        for (uint32_t x = 0; x < kPasses; ++x) {
+                            const uint32_t row = row0 + it * 8, piece = ((half ^ x) & (kPasses - 1)) * 4 + (lane & 3u);
+                            v[it][x] = *reinterpret_cast<const uint4*>(
+                                from + row * D + ((piece ^ (D == 128 ? row & 7u : (row >> 1) & 3u)) << 4));
+                        }
                     __syncwarp();
-                    if (lane < boxes)
-                        for (uint32_t c = 0; c < G::kPanels; ++c)
-                            tma4(smem + G::kRing + s * G::kTile + c * kPanel + lane * box * 128, kv ? &vmap : &kmap,
-                                 bar.full(s), int32_t(c * 64), in, w.h, id);
+                    if (lane == 0) bar_arrive(bar.codes_empty(cs));
+                    if (n && !(ok = warp_wait<!Q8>(bar.empty(s), (n - 1) & 1u, p.timeout_ns))) break;
+                    uint8_t* to = base + G::kRing + s * G::kTile;
+#pragma unroll
+                    for (uint32_t it = 0; it < 4; ++it)
+#pragma unroll
+                        for (uint32_t x = 0; x < kPasses; ++x) {
+                            const uint32_t row = row0 + it * 8, panel = (half ^ x) & (kPasses - 1);
+                            uint8_t* at = to + panel * kPanel + row * 128;
+                            const uint32_t chunk = ((lane & 3u) * 2) ^ (row & 7u), f = step[it >> 1];
+                            const uint2 a = values4<T>(v[it][x].x, f), b = values4<T>(v[it][x].y, f);
+                            const uint2 c = values4<T>(v[it][x].z, f), d = values4<T>(v[it][x].w, f);
+                            *reinterpret_cast<uint4*>(at + (chunk << 4)) = make_uint4(a.x, a.y, b.x, b.y);
+                            *reinterpret_cast<uint4*>(at + ((chunk ^ 1u) << 4)) = make_uint4(c.x, c.y, d.x, d.y);
+                        }
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(bar.full(s));
                 }
                 if (!ok) break;
+                ex = next_ex;
             }
             release();
         }
-        // every load has landed and every stage been released before the CTA ends
+        // every stage has been released before the CTA ends
         const uint64_t grace = (ok ? p.timeout_ns : 0) + kGraceNs;
         const uint32_t last = min(slot, G::kStages);
-        bool rest = ok;
-        for (uint32_t x = slot - last; x < slot; ++x) {
-            const uint32_t s = x % G::kStages, n = x / G::kStages;
-            warp_wait(bar.full(s), n & 1u, grace);
-            rest = rest && warp_wait(bar.empty(s), n & 1u, grace);
-        }
-        if (sg) warp_wait(bar.q_full(), (sg - 1) & 1u, grace);
-    } else if (warp < 8) {
+        for (uint32_t x = slot - last; x < slot && ok; ++x)
+            ok = warp_wait<!Q8>(bar.empty(x % G::kStages), (x / G::kStages) & 1u, grace);
+    };
+
+    if (warp < 8) {
         // ---- rows: thread r of row tile i
+        if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs8));
         const uint32_t i = warp >> 2;
         const uint32_t r = tid & 127u, quarter = (warp & 3u) << 21;  // lane 32 * (warp % 4) of tensor memory
         const uint32_t ts = tmem + quarter + kS + i * 128, to = tmem + quarter + kO + i * D;
@@ -467,11 +510,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             // they may be anything, and 0 * NaN is not 0 (the other row tile's warps
             // write the same zeros)
             auto arrived = [&](bool there) {
-                if (!there && !warp_wait(bar.s_full(i, n & 1u), (n >> 1) & 1u, p.timeout_ns)) return false;
+                if (!there && !warp_wait<!Q8>(bar.s_full(i, n & 1u), (n >> 1) & 1u, p.timeout_ns)) return false;
                 const int32_t k0 = at.h * kHalf;
-                if (at.t && at.t + 1 == count && !warp_wait(bar.o_done(i), no++ & 1u, p.timeout_ns)) return false;
+                if (at.t && at.t + 1 == count && !warp_wait<!Q8>(bar.o_done(i), no++ & 1u, p.timeout_ns)) return false;
+                if constexpr (Q8) return true;  // (every value there is a number, or of a block that reads as NaN)
                 if ((k0 >= seen_lo && k0 + kHalf <= seen_hi) || k0 + kHalf <= sink) return true;
-                if (!warp_wait(bar.full(at.stage), at.odd & 1u, p.timeout_ns)) return false;
+                if (!warp_wait<!Q8>(bar.full(at.stage), at.odd & 1u, p.timeout_ns)) return false;
                 const int32_t k = k0 + int32_t(r & 63u);
                 if ((r >> 6) < G::kPanels && !((k >= seen_lo && k < seen_hi) || k < sink)) {
                     uint8_t* v = base + G::kRing + at.stage * G::kTile + (r >> 6) * kPanel +
@@ -535,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         l *= f2;
                         m = nm;
                         if (at.t) {  // the P V before has to be in O: it is when the next S is there
-                            if (!last && !warp_wait(bar.s_full(i, ~n & 1u), ((n + 1) >> 1) & 1u, p.timeout_ns))
+                            if (!last && !warp_wait<!Q8>(bar.s_full(i, ~n & 1u), ((n + 1) >> 1) & 1u, p.timeout_ns))
                                 gave_up(p);
                             fence_after();
 #pragma unroll
@@ -592,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (!ok) wait_ld();  // (an early read may be under way)
             const bool any = count != 0;  // (otherwise O is not written)
-            if (any && ok) ok = warp_wait(bar.o_done(i), no++ & 1u, p.timeout_ns);
+            if (any && ok) ok = warp_wait<!Q8>(bar.o_done(i), no++ & 1u, p.timeout_ns);
             if (!ok) break;
             if (!any)
                 for (int32_t j = w.steps; j; --j) at.next_stage<G::kStages>();
@@ -645,85 +689,197 @@ __global__ void __launch_bounds__(kThreads, 1)
             release();
         }
     } else {
-        // ---- MMAs of row tile i: the warp goes through the pieces together, one
-        // lane issues. A warp per row tile, so that one's waits and counting
-        // pass beside the other's MMAs.
-        const uint32_t i = warp == 8 ? 0 : 1;
-        constexpr uint32_t kIs = instr(T::kUmmaFormat, 128, kHalf, false);
-        constexpr uint32_t kIo = instr(T::kUmmaFormat, 128, D, true);
-        const uint32_t q_lo = desc_lo(smem + i * G::kTile, 16), k_lo = desc_lo(smem + G::kRing, 16);
-        const uint32_t v_lo = desc_lo(smem + G::kRing, kPanel);
-        const uint32_t t_s = tmem + kS + i * 128, t_o = tmem + kO + i * D;
-        const bool lead = elect();
-        uint32_t n = 0;  // halves passed
-        Halves cs{0, 0, 0, 0, false}, cp{1, 0, 0, 0, false};  // for S, and two halves behind for P V
-        while (ok && next()) {
-            const Seg& w = segs[sg % kSegs];
-            const int32_t count = uniform(w.halves), na = uniform(w.na), ha = uniform(w.ha), hb = uniform(w.hb);
-            ok = warp_wait(bar.q_full(), sg & 1u, p.timeout_ns);
-            if (int32_t(i) * per_tile >= uniform(w.left) || !count) {  // no such row tile, or nothing seen
-                for (int32_t j = uniform(w.steps); j && ok; --j)
-                    for (Halves* c : {&cs, &cp}) {
-                        if (!(ok = ok && warp_wait(bar.full(c->stage), c->odd & 1u, p.timeout_ns))) break;
-                        if (lead) commit(bar.empty(c->stage));
-                        c->next_stage<G::kStages>();
+        // (one instruction for a whole warpgroup, in a branch that ends the kernel)
+        if constexpr (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs8));
+        if (warp >= 12) {
+            if constexpr (Q8) convert(0);
+        } else if (warp == 10) {
+            // ---- pieces
+            if (lane == 0) {
+                Walk w;
+                KeyRange kr{};
+                bool more = w.begin(sc.plan);
+                for (; ok; ++sg) {
+                    if (sg >= kSegs && !bar_wait<!Q8>(bar.seg_empty(sg % kSegs), (sg / kSegs - 1) & 1u, p.timeout_ns)) {
+                        ok = false;
+                        break;
                     }
-                if (ok && lead) commit(bar.q_empty());
-                release();
-                continue;
-            }
-            cs.begin(na, ha, hb);
-            cp.begin(na, ha, hb);
-            auto landed = [&](const Halves& c) {
-                return !c.fresh || warp_wait(bar.full(c.stage), c.odd & 1u, p.timeout_ns);
-            };
-            auto advance = [&](Halves& c) {  // a tile's last half releases its stage
-                const uint32_t stage = c.stage;
-                if (!c.next(count, na, hb)) return;
-                if (lead) commit(bar.empty(stage));
-                c.next_stage<G::kStages>();
-            };
-            auto step_s = [&](uint32_t b) {  // S of the next half, into buffer b
-                const uint32_t k = uniform(k_lo + cs.stage * (G::kTile / 16) + (cs.h & 1) * (kHalf * 128 / 16));
-                const uint32_t d = uniform(t_s + b * kHalf), q = uniform(q_lo);
-                if (lead) {
-#pragma unroll
-                    for (uint32_t x = 0; x < D / 16; ++x) {
-                        const uint32_t off = ((x / 4) * kPanel + (x % 4) * 32) / 16;
-                        mma_ss(d, desc_of<1024>(q + off), desc_of<1024>(k + off), kIs, x > 0);
+                    more = more && w.next(p, sc.plan, sc.items);
+                    Seg x{};
+                    if (more) {
+                        const SeqRange q{w.it.q0, w.it.nq, w.it.n, w.it.n - w.it.nq};
+                        kr = key_range<kKeys>(p, q, w.it.t0, min(w.it.nq, w.it.t0 + 2 * per_tile));
+                        x.steps = w.steps, x.row0 = w.it.q0 + w.it.t0, x.left = w.it.nq - w.it.t0;
+                        x.pos0 = w.it.n - w.it.nq + w.it.t0, x.h = w.h, x.b = w.it.b, x.j0 = w.j0;
+                        x.ns = kr.ns, x.first = kr.first, x.lo = kr.lo, x.hi = kr.hi, x.sink = kr.sink;
+                        x.set_halves();
+                        x.whole = w.j0 == 0 && w.steps == w.it.tiles;
+                        x.part = w.u != w.u_begin;
+                        if (!x.whole && !w.j0) sc.plan->open[blockIdx.x] = make_int2(w.i, w.h);
                     }
-                    commit(bar.s_full(i, b));
+                    *reinterpret_cast<Seg*>(base + G::kSegs + (sg % kSegs) * sizeof(Seg)) = x;
+                    bar_arrive(bar.seg_full(sg % kSegs));
+                    if (!more) break;
                 }
-                advance(cs);
-                if (cs.t == count && lead) commit(bar.q_empty());
-            };
-            for (uint32_t t = 0; t < 2 && ok && cs.t < count; ++t) {
-                if (!(ok = landed(cs))) break;
-                step_s((n + t) & 1u);
             }
-            for (; ok && cp.t < count; ++n) {
-                const uint32_t b = n & 1u;
-                const bool more = cs.t < count;
-                if (!(ok = landed(cp) && (!more || landed(cs)) &&
-                           warp_wait(bar.p_ready(i, b), (n >> 1) & 1u, p.timeout_ns)))
+            __syncwarp();
+        } else if (warp == 9) {
+            // ---- loads
+            uint32_t slot = 0;  // ring slots filled
+            const uint32_t box = min(p.P, 128u), boxes = 128 / box;
+            while (ok && next()) {
+                const Seg w = segs[sg % kSegs];
+                const int32_t two = w.left > per_tile ? 2 : 1;
+                if (sg && !warp_wait<!Q8>(bar.q_empty(), (sg - 1) & 1u, p.timeout_ns)) {
+                    ok = false;
                     break;
-                fence_after();
-                const uint32_t v = uniform(v_lo + cp.stage * (G::kTile / 16) + (cp.h & 1) * (kHalf * 128 / 16));
-                const uint32_t pt = uniform(t_s + b * kHalf), ot = uniform(t_o);
-                if (lead) {
-#pragma unroll
-                    for (uint32_t x = 0; x < kHalf / 16; ++x)
-                        mma_ts(ot, pt + x * 8, desc_of<1024>(v + x * 128), kIo, x > 0 || cp.t > 0);
-                    if (!more) commit(bar.o_done(i));
                 }
-                if (more) step_s(b);
-                advance(cp);
+                if (lane == 0) {
+                    bar_arrive_tx(bar.q_full(), uint32_t(two) * G::kPanels * uint32_t(per_tile) * p.g * 128);
+                    for (int32_t i = 0; i < two; ++i)
+                        for (uint32_t c = 0; c < G::kPanels; ++c)
+                            tma3(smem + uint32_t(i) * G::kTile + c * kPanel, &qmap, bar.q_full(), int32_t(c * 64),
+                                 w.h * int32_t(p.g), w.row0 + i * per_tile);
+                }
+                const int32_t* trow = p.table + int64_t(w.b) * p.table_s;
+                auto page_of = [&](int32_t step) -> int32_t {  // this lane's page of a step (outside the pool: zeros)
+                    if (step >= w.steps || lane >= boxes) return int32_t(p.pages);
+                    const int32_t k0 = w.slot0(step) + int32_t(lane * box), k1 = k0 + int32_t(box);
+                    if (!((k0 < w.hi && k1 > w.lo) || k0 < w.sink)) return int32_t(p.pages);
+                    const int32_t id = trow[k0 >> p.pshift];
+                    if (uint32_t(id) < p.pages) return id;
+                    if (p.err) atomicOr(p.err, kErrPage);
+                    return int32_t(p.pages);
+                };
+                int32_t next_id = page_of(0);
+                for (int32_t j = 0; j < w.steps; ++j) {
+                    const int32_t id = next_id;
+                    next_id = page_of(j + 1);
+                    const int32_t in = (w.slot0(j) + int32_t(lane * box)) & int32_t(p.P - 1);
+                    for (int kv = 0; kv < 2; ++kv, ++slot) {
+                        if constexpr (Q8) {
+                            const uint32_t s = slot % G::kCodeStages, n = slot / G::kCodeStages;
+                            if (n && !(ok = warp_wait<!Q8>(bar.codes_empty(s), (n - 1) & 1u, p.timeout_ns))) break;
+                            if (lane == 0) bar_arrive_tx(bar.codes_full(s), G::kCodes);
+                            __syncwarp();
+                            if (lane < boxes)
+                                tma4(smem + G::kCodeRing + s * G::kCodes + lane * box * D, kv ? &vmap : &kmap,
+                                     bar.codes_full(s), 0, in, w.h, id);
+                            continue;
+                        }
+                        const uint32_t s = slot % G::kStages, n = slot / G::kStages;
+                        if (n && !warp_wait<!Q8>(bar.empty(s), (n - 1) & 1u, p.timeout_ns)) {
+                            ok = false;
+                            break;
+                        }
+                        if (lane == 0) bar_arrive_tx(bar.full(s), G::kTile);
+                        __syncwarp();
+                        if (lane < boxes)
+                            for (uint32_t c = 0; c < G::kPanels; ++c)
+                                tma4(smem + G::kRing + s * G::kTile + c * kPanel + lane * box * 128, kv ? &vmap : &kmap,
+                                     bar.full(s), int32_t(c * 64), in, w.h, id);
+                    }
+                    if (!ok) break;
+                }
+                release();
             }
-            release();
+            // every load has landed and every stage been released before the CTA ends
+            const uint64_t grace = (ok ? p.timeout_ns : 0) + kGraceNs;
+            if constexpr (Q8) {
+                const uint32_t last = min(slot, G::kCodeStages);
+                for (uint32_t x = slot - last; x < slot; ++x)
+                    warp_wait<!Q8>(bar.codes_full(x % G::kCodeStages), (x / G::kCodeStages) & 1u, grace);
+                slot = 0;
+            }
+            const uint32_t last = min(slot, G::kStages);
+            bool rest = ok;
+            for (uint32_t x = slot - last; x < slot; ++x) {
+                const uint32_t s = x % G::kStages, n = x / G::kStages;
+                warp_wait<!Q8>(bar.full(s), n & 1u, grace);
+                rest = rest && warp_wait<!Q8>(bar.empty(s), n & 1u, grace);
+            }
+            if (sg) warp_wait<!Q8>(bar.q_full(), (sg - 1) & 1u, grace);
+        } else {
+            // ---- MMAs of row tile i: the warp goes through the pieces together, one
+            // lane issues. A warp per row tile, so that one's waits and counting
+            // pass beside the other's MMAs.
+            const uint32_t i = warp == 8 ? 0 : 1;
+            constexpr uint32_t kIs = instr(T::kUmmaFormat, 128, kHalf, false);
+            constexpr uint32_t kIo = instr(T::kUmmaFormat, 128, D, true);
+            const uint32_t q_lo = desc_lo(smem + i * G::kTile, 16), k_lo = desc_lo(smem + G::kRing, 16);
+            const uint32_t v_lo = desc_lo(smem + G::kRing, kPanel);
+            const uint32_t t_s = tmem + kS + i * 128, t_o = tmem + kO + i * D;
+            const bool lead = elect();
+            uint32_t n = 0;  // halves passed
+            Halves cs{0, 0, 0, 0, false}, cp{1, 0, 0, 0, false};  // for S, and two halves behind for P V
+            while (ok && next()) {
+                const Seg& w = segs[sg % kSegs];
+                const int32_t count = uniform(w.halves), na = uniform(w.na), ha = uniform(w.ha), hb = uniform(w.hb);
+                ok = warp_wait<!Q8>(bar.q_full(), sg & 1u, p.timeout_ns);
+                if (int32_t(i) * per_tile >= uniform(w.left) || !count) {  // no such row tile, or nothing seen
+                    for (int32_t j = uniform(w.steps); j && ok; --j)
+                        for (Halves* c : {&cs, &cp}) {
+                            if (!(ok = ok && warp_wait<!Q8>(bar.full(c->stage), c->odd & 1u, p.timeout_ns))) break;
+                            if (lead) commit(bar.empty(c->stage));
+                            c->next_stage<G::kStages>();
+                        }
+                    if (ok && lead) commit(bar.q_empty());
+                    release();
+                    continue;
+                }
+                cs.begin(na, ha, hb);
+                cp.begin(na, ha, hb);
+                auto landed = [&](const Halves& c) {
+                    return !c.fresh || warp_wait<!Q8>(bar.full(c.stage), c.odd & 1u, p.timeout_ns);
+                };
+                auto advance = [&](Halves& c) {  // a tile's last half releases its stage
+                    const uint32_t stage = c.stage;
+                    if (!c.next(count, na, hb)) return;
+                    if (lead) commit(bar.empty(stage));
+                    c.next_stage<G::kStages>();
+                };
+                auto step_s = [&](uint32_t b) {  // S of the next half, into buffer b
+                    const uint32_t k = uniform(k_lo + cs.stage * (G::kTile / 16) + (cs.h & 1) * (kHalf * 128 / 16));
+                    const uint32_t d = uniform(t_s + b * kHalf), q = uniform(q_lo);
+                    if (lead) {
+#pragma unroll
+                        for (uint32_t x = 0; x < D / 16; ++x) {
+                            const uint32_t off = ((x / 4) * kPanel + (x % 4) * 32) / 16;
+                            mma_ss(d, desc_of<1024>(q + off), desc_of<1024>(k + off), kIs, x > 0);
+                        }
+                        commit(bar.s_full(i, b));
+                    }
+                    advance(cs);
+                    if (cs.t == count && lead) commit(bar.q_empty());
+                };
+                for (uint32_t t = 0; t < 2 && ok && cs.t < count; ++t) {
+                    if (!(ok = landed(cs))) break;
+                    step_s((n + t) & 1u);
+                }
+                for (; ok && cp.t < count; ++n) {
+                    const uint32_t b = n & 1u;
+                    const bool more = cs.t < count;
+                    if (!(ok = landed(cp) && (!more || landed(cs)) &&
+                               warp_wait<!Q8>(bar.p_ready(i, b), (n >> 1) & 1u, p.timeout_ns)))
+                        break;
+                    fence_after();
+                    const uint32_t v = uniform(v_lo + cp.stage * (G::kTile / 16) + (cp.h & 1) * (kHalf * 128 / 16));
+                    const uint32_t pt = uniform(t_s + b * kHalf), ot = uniform(t_o);
+                    if (lead) {
+#pragma unroll
+                        for (uint32_t x = 0; x < kHalf / 16; ++x)
+                            mma_ts(ot, pt + x * 8, desc_of<1024>(v + x * 128), kIo, x > 0 || cp.t > 0);
+                        if (!more) commit(bar.o_done(i));
+                    }
+                    if (more) step_s(b);
+                    advance(cp);
+                }
+                release();
+            }
+            // MMAs in flight end (bounded) before the tensor memory goes
+            if (lead) commit(bar.drain(i));
+            warp_wait<!Q8>(bar.drain(i), 0, kGraceNs);
         }
-        // MMAs in flight end (bounded) before the tensor memory goes
-        if (lead) commit(bar.drain(i));
-        warp_wait(bar.drain(i), 0, kGraceNs);
     }
     if (!ok) gave_up(p);
     fence_before();
@@ -1178,7 +1334,7 @@ int launch_chunk_weights(const AttnParams& p, const ChunkScratch& s, uint32_t gr
     return int(launch_after(chunk_weights_kernel<T, D>, grid, kThreadsW, GeoW<D>::kSmem, stream, p, s, qm, km));
 }
 
-template <class T, int D>
+template <class T, int D, bool Q8>
 int launch(const AttnParams& p, bool bf16, const ChunkScratch& s, uint32_t grid, cudaStream_t stream) {
     CUtensorMap qm, km, vm;
     const uint64_t qd[3] = {D, p.Hq, p.tokens};
@@ -1187,29 +1343,48 @@ int launch(const AttnParams& p, bool bf16, const ChunkScratch& s, uint32_t grid,
     const uint64_t kd[4] = {D, p.P, p.Hkv, p.pages};
     const int64_t ks[3] = {p.kp_ss, p.kp_hs, p.kp_ps}, vs[3] = {p.vp_ss, p.vp_hs, p.vp_ps};
     const uint32_t kb[4] = {64, p.P < 128 ? p.P : 128, 1, 1};
-    if (!encode_map(&qm, bf16, p.q, 3, qd, qs, qb) || !encode_map(&km, bf16, p.k_pages, 4, kd, ks, kb) ||
-        !encode_map(&vm, bf16, p.v_pages, 4, kd, vs, kb))
+    if (!encode_map(&qm, bf16, p.q, 3, qd, qs, qb)) return EINVAL;
+    if constexpr (Q8) {
+        if (!encode_codes(&km, p.k_pages, p, p.kp_ss, p.kp_hs, p.kp_ps, kb[1]) ||
+            !encode_codes(&vm, p.v_pages, p, p.vp_ss, p.vp_hs, p.vp_ps, kb[1]))
+            return EINVAL;
+    } else if (!encode_map(&km, bf16, p.k_pages, 4, kd, ks, kb) || !encode_map(&vm, bf16, p.v_pages, 4, kd, vs, kb)) {
         return EINVAL;
+    }
+    const auto kernel = chunk_attn_kernel<T, D, Q8>;
+    constexpr uint32_t kSmem = Geo<D, Q8>::kSmem, kBlock = Q8 ? kThreads8 : kThreads;
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return int(e);
     const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
     if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(chunk_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 int(Geo<D>::kSmem));
+        if constexpr (Q8) {  // the split of the registers counts on those of the launch
+            cudaFuncAttributes has;
+            e = cudaFuncGetAttributes(&has, kernel);
+            if (e != cudaSuccess) return int(e);
+            if (has.numRegs != kRegs8) return ENOTSUP;
+        }
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem));
         if (e != cudaSuccess) return int(e);
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
     const uint64_t most = (uint64_t(p.max_q < p.tokens ? p.max_q : p.tokens) + 7) / 8, fair = kAppendBlocks / p.B + 1;
     const uint32_t append = p.k_new ? p.B * uint32_t(most < fair ? most : fair) : 0;
-    chunk_prepare_kernel<<<2 + append, 256, 0, stream>>>(p, s, grid);
-    e = cudaGetLastError();
-    if (e == cudaSuccess)
-        e = launch_after(chunk_attn_kernel<T, D>, grid, kThreads, Geo<D>::kSmem, stream, p, s, qm, km, vm);
+    if (Q8) {  // (the append before it lets it begin early)
+        e = launch_after(chunk_prepare_kernel, 2, 256, 0, stream, p, s, grid);
+    } else {
+        chunk_prepare_kernel<<<2 + append, 256, 0, stream>>>(p, s, grid);
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess) e = launch_after(kernel, grid, kBlock, kSmem, stream, p, s, qm, km, vm);
     if (e == cudaSuccess) e = launch_after(chunk_join_kernel<T, D>, dim3(grid, D / 16), 256, 0, stream, p, s);
-    if (e != cudaSuccess || !p.weights) return int(e);
+    if (Q8 || e != cudaSuccess || !p.weights) return int(e);
     return launch_chunk_weights<T, D>(p, s, grid, qm, km, stream);
+}
+template <class T, int D>
+int launch(const AttnParams& p, bool bf16, const ChunkScratch& s, uint32_t grid, cudaStream_t stream) {
+    return p.ex ? launch<T, D, true>(p, bf16, s, grid, stream) : launch<T, D, false>(p, bf16, s, grid, stream);
 }
 
 using Encode = decltype(&cuTensorMapEncodeTiled);

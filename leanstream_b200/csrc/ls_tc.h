@@ -49,7 +49,7 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
 // coarsely, and a try may sleep for some us): a wait that goes on begins its time
 // here. 32-bit arguments and no call from here: with 64-bit ones, or a second way
 // for short bounds, chunks took 1 to 2 % longer.
-static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, uint32_t limit) {
+__device__ __forceinline__ bool bar_wait_on(uint32_t bar, uint32_t parity, uint32_t limit) {
     const uint32_t begin = uint32_t(now() >> 10);
     for (;;) {
         for (int i = 0; i < 16; ++i)
@@ -57,12 +57,20 @@ static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity,
         if (uint32_t(now() >> 10) - begin > limit) return false;
     }
 }
-// Waits until phase `parity` has completed; false after ns (below 2^42).
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint64_t ns) {
-    return bar_try(bar, parity) || bar_wait_slow(bar, parity, uint32_t(ns >> 10));
+static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, uint32_t limit) {
+    return bar_wait_on(bar, parity, limit);
 }
+// Waits until phase `parity` has completed; false after ns (below 2^42). kCall: a
+// wait that goes on is a call, which a kernel that splits its registers by
+// setmaxnreg cannot have.
+template <bool kCall = true>
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint64_t ns) {
+    const uint32_t limit = uint32_t(ns >> 10);
+    return bar_try(bar, parity) || (kCall ? bar_wait_slow(bar, parity, limit) : bar_wait_on(bar, parity, limit));
+}
+template <bool kCall = true>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint64_t ns) {
-    return __all_sync(0xffffffffu, bar_wait(bar, parity, ns)) != 0;
+    return __all_sync(0xffffffffu, bar_wait<kCall>(bar, parity, ns)) != 0;
 }
 // The same for a bound below a try's sleep: polls, and counts SM cycles, two per ns.
 static __device__ __noinline__ bool warp_wait_short(uint32_t bar, uint32_t parity, uint32_t ns) {
