@@ -56,12 +56,14 @@ constexpr int64_t kDecMinUnits = 2 + kDecItemCost;  // units that a CTA takes at
 constexpr uint64_t kGraceNs = 1000000000ull;
 constexpr uint64_t kShortNs = 100000;  // bounds that a barrier's try may sleep over: a load takes less
 
-// Three CTAs per SM by registers; the ring takes the shared memory that leaves.
-template <int D, bool Q8>
+// NT: 0 over 16 bits, else tiles of eight rows over 8 bits. CTAs per SM by
+// registers; the ring takes the shared memory that leaves.
+template <int D, int NT>
 struct GeoD {
-    static constexpr int kCtas = 3, kRows = 16;
-    static constexpr uint32_t kHalf = kDecKeys * D * (Q8 ? 1 : 2), kStage = 2 * kHalf;  // a step's keys, its values
-    static constexpr int kStages = (Q8 ? 4 : 2) * (128 / D);
+    static constexpr bool kQ8 = NT != 0;
+    static constexpr int kCtas = NT == 1 ? 4 : 3, kRows = kQ8 ? 8 * NT : 16;
+    static constexpr uint32_t kHalf = kDecKeys * D * (kQ8 ? 1 : 2), kStage = 2 * kHalf;  // a step's keys, its values
+    static constexpr int kStages = (NT == 0 ? 2 : NT == 1 ? 3 : 4) * (128 / D);
     static constexpr uint32_t kRing = kDecWarps * kStages * kStage;
     static constexpr uint32_t kJoin = kRing, kJoinBytes = kRows * D * 4;  // sums of the warps
     static constexpr uint32_t kSegs = kJoin + kJoinBytes, kBars = kSegs + kDecSegs * 64;
@@ -147,6 +149,205 @@ __device__ __forceinline__ Pair block_scan(Pair v, Pair* sh, Pair& before) {
     return total;
 }
 
+// The rows of a warp over a cache in 8 bits (value = code * 2^e, one e for the 16
+// slots of a step), NT tiles of eight. Slots and elements are the M dimension of
+// the products and rows their N, so that few rows leave no tile half empty:
+//     S^T = K Q^T     16 slots x 8 rows,     O^T += V^T P^T     16 elements x 8 rows.
+// Codes enter as whole numbers in float16, whatever the type of the queries; those
+// enter it by a power of two of their own per row (bfloat16: what lies 2^-29 below
+// a row's largest loses bits). The exponents meet the logits in 32 bits, and the
+// probabilities as 2^(e - E), E the largest exponent of the values so far; when that
+// grows the sums are scaled down. A row's reference is only raised when a logit
+// passes it by 2^kRaise. P is rounded once, to float16, times 2^kChunkShift.
+// Every slot of a step is a number, so those that no row sees are not cleared.
+//
+// Lane (g, t) = (lane / 4, lane % 4) holds the rows 2 t and 2 t + 1 of each tile
+// for the slots g and g + 8, and for the elements 16 n + 2 g and + 1 of all n.
+template <class T, int D, int NT>
+struct Rows8 {
+    static constexpr int KS = D / 16;
+    uint2 q[NT][KS];     // row g: elements 4 t .. 4 t + 3 of each 16, as the codes come
+    float cq[NT][2];     // scale * log2 e and the rows' own powers of two
+    float o[NT][KS][4];  // in units of 2^(most - kChunkShift)
+    float m[NT][2], l[NT][2];  // l: of this lane's slots
+    int32_t pos[NT][2];  // slot of the rows' tokens (-1: no row)
+    int32_t most;
+
+    __device__ __forceinline__ void queries(const AttnParams& p, const DecSeg& x, uint32_t lane) {
+        const int32_t g = int32_t(p.g);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int32_t r = int32_t(lane >> 2) + 8 * i;
+            const bool on = r < x.rows;
+            const uint16_t* at = p.q + int64_t(x.q0 + (on ? r / g : 0)) * p.q_ts +
+                                 int64_t(x.h * g + (on ? r % g : 0)) * p.q_hs + (lane & 3u) * 4;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+                q[i][k] = on ? *reinterpret_cast<const uint2*>(at + k * 16) : make_uint2(0u, 0u);
+        }
+    }
+    __device__ __forceinline__ void begin(const AttnParams& p, const DecSeg& x, uint32_t lane) {
+        const int32_t g = int32_t(p.g), t = int32_t(lane & 3u);
+        most = -126;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            float c = p.c;
+            if constexpr (std::is_same_v<T, BF16>) {
+                uint32_t top = 0;  // bits of the largest |q| of the row
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+                    top = max(max(top, max(q[i][k].x & 0x7fffu, (q[i][k].x >> 16) & 0x7fffu)),
+                              max(q[i][k].y & 0x7fffu, (q[i][k].y >> 16) & 0x7fffu));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // to [2^14, 2^15); infinities and NaN stay what they are
+                const int32_t e = top >= 0x7f80u ? 0 : max(int32_t(top >> 7) - 127 - 14, -112);
+                const float f = two_to(-e);
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    float a, b;
+                    BF16::unpack(q[i][k].x, a, b);
+                    q[i][k].x = F16::pack(a * f, b * f);
+                    BF16::unpack(q[i][k].y, a, b);
+                    q[i][k].y = F16::pack(a * f, b * f);
+                }
+                c *= two_to(e);
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int32_t row = 8 * i + 2 * t + y;
+                cq[i][y] = __shfl_sync(0xffffffffu, c, (2 * t + y) * 4);
+                pos[i][y] = row < x.rows ? max(x.f + row / g, -1) : -1;
+                m[i][y] = -INFINITY, l[i][y] = 0.f;
+            }
+#pragma unroll
+            for (int n = 0; n < KS; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+        }
+    }
+    // 16 slots from k0, codes of their keys and values at ks and vs, both exponents in `ex`
+    __device__ __forceinline__ void step(const AttnParams& p, uint32_t ks, uint32_t vs, uint32_t ex, int32_t k0,
+                                         bool masked, uint32_t lane) {
+        float s[NT][4] = {};
+#pragma unroll
+        for (int k = 0; k < KS; k += 2) {
+            uint32_t v[4];  // slots 0-7 and 8-15 (v[2], v[3]) of two 16-byte pieces
+            ldsm4(v, ks + swz8<D>((lane & 7u) + ((lane >> 4) << 3), k + ((lane >> 3) & 1u)));
+#pragma unroll
+            for (int y = 0; y < 4; ++y) v[y] ^= 0x80808080u;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const uint32_t a[4] = {codes_f16(v[y], kCodes01), codes_f16(v[2 + y], kCodes01),
+                                       codes_f16(v[y], kCodes23), codes_f16(v[2 + y], kCodes23)};
+#pragma unroll
+                for (int i = 0; i < NT; ++i) F16::mma(s[i], a, q[i][k + y].x, q[i][k + y].y);
+            }
+        }
+        const int32_t ek = int8_t(ex), ev = int8_t(ex >> 8);
+        const float fk = ek == kNoExponent ? NAN : two_to(max(ek, -126));
+        bool raise = false;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[i][e] *= cq[i][e & 1] * fk;
+                if (masked && !sees(p, pos[i][e & 1], k0 + int32_t(lane >> 2) + 8 * (e >> 1))) s[i][e] = -INFINITY;
+                raise = raise || s[i][e] > m[i][e & 1] + F16::kRaise;
+            }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    float top = fmaxf(m[i][y], fmaxf(s[i][y], s[i][2 + y]));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    const float f = top == -INFINITY ? 1.f : ex2(m[i][y] - top);
+                    m[i][y] = top;
+                    l[i][y] *= f;
+#pragma unroll
+                    for (int n = 0; n < KS; ++n) o[i][n][y] *= f, o[i][n][2 + y] *= f;
+                }
+        }
+        if (ev > most) {
+            const float f = two_to(max(most - ev, -126));
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int n = 0; n < KS; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][n][e] *= f;
+            most = ev;
+        }
+        const float pw = ev == kNoExponent ? NAN : two_to(max(ev - most + int(F16::kChunkShift), -126));
+        uint32_t b[NT][2];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            float a[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                a[e] = ex2(s[i][e] - (m[i][e & 1] == -INFINITY ? 0.f : m[i][e & 1]));
+                l[i][e & 1] += a[e];
+                a[e] *= pw;
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y)  // slots by rows, to rows by slots
+                asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;"
+                             : "=r"(b[i][y]) : "r"(F16::pack(a[2 * y], a[2 * y + 1])));
+        }
+#pragma unroll
+        for (int n = 0; n < KS; n += 2) {
+            uint32_t v[4];  // of two 16-byte pieces, slots 0-7 and 8-15 each; a register holds elements 2 g, 2 g + 1
+            ldsm4t(v, vs + swz8<D>((lane & 7u) + (((lane >> 3) & 1u) << 3), n + (lane >> 4)));
+#pragma unroll
+            for (int y = 0; y < 4; ++y) v[y] ^= 0x80808080u;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const uint32_t a[4] = {codes_f16(v[2 * y], kCodes02), codes_f16(v[2 * y], kCodes13),
+                                       codes_f16(v[2 * y + 1], kCodes02), codes_f16(v[2 * y + 1], kCodes13)};
+#pragma unroll
+                for (int i = 0; i < NT; ++i) F16::mma(o[i][n + y], a, b[i][0], b[i][1]);
+            }
+        }
+    }
+    // Maxima and sums of the rows to sm, sl [8 NT].
+    __device__ __forceinline__ void stats(float* sm, float* sl, uint32_t lane) const {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                float sum = l[i][y];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const uint32_t row = 8 * i + 2 * lane + y;
+                if (lane < 4) sm[row] = m[i][y], sl[row] = sum;
+            }
+    }
+    // The sums times 2^(own maximum - top[row]) to row `at0 + row` of `join`, or added there.
+    template <class F>
+    __device__ __forceinline__ void sums(float* join, uint32_t at0, int32_t R, bool add, F top, uint32_t lane) const {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const uint32_t row = 8 * i + 2 * (lane & 3u) + y, at = at0 + row;
+                if (int32_t(row) >= R) continue;
+                const float mx = top(row);
+                const float unit = two_to(max(most - int(F16::kChunkShift), -126));
+                const float f = mx == -INFINITY ? 0.f : ex2(m[i][y] - mx) * unit;
+                float* to = join + at * D;
+#pragma unroll
+                for (int n = 0; n < KS; ++n) {
+                    float2* cell = reinterpret_cast<float2*>(to + ((n * 16 + (lane >> 2) * 2) ^ (at & 7u) * 8));
+                    float2 v = make_float2(o[i][n][y] * f, o[i][n][2 + y] * f);
+                    if (add) v.x += cell->x, v.y += cell->y;
+                    *cell = v;
+                }
+            }
+    }
+};
+
 // The kernel for few rows per sequence and kv head (decoding, drafts): bound
 // by the read of the cache. An item is a sequence and kv head; its rows are
 // (token, head of the group), so all heads that share a key read it once. The
@@ -162,21 +363,14 @@ __device__ __forceinline__ Pair block_scan(Pair v, Pair* sh, Pair& before) {
 // multiplier is idle beside the loads. Two sequences
 // of up to 131072 slots, 64 heads of 128 over 8: 180 us, 5.7 TB/s of the cache;
 // 32 of up to 4096 slots, 32 heads: 60 us, 4.6 TB/s; one of 97 slots: 8.5 us.
-//
-// Q8, a cache in 8 bits (value = code * 2^e, one e for the 16 slots of a step): the
-// codes go to the matrix instructions as whole numbers in float16, whatever the
-// type of the queries, which enter it by a power of two of their own per row
-// (bfloat16: what lies 2^-29 below a row's largest loses bits). The exponents meet
-// the logits in 32 bits, and the probabilities as 2^(e - E), E the largest
-// exponent of the values so far; when that grows the sums are scaled down. Every
-// slot of a step that a row sees is a number, so no slot is cleared.
-template <class T, int D, bool Q8>
-__global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
+// Over 8 bits (NT > 0) the rows' part is Rows8's, a step is a block of the cache,
+// and nothing is appended or cleared.
+template <class T, int D, int NT>
+__global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
     attn_decode_kernel(const AttnParams p, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
-    using G = GeoD<D, Q8>;
-    using M = std::conditional_t<Q8, F16, T>;  // of the matrix instructions
-    constexpr float kShift = Q8 ? 0.f : T::kShift;
+    using G = GeoD<D, NT>;
+    constexpr bool Q8 = G::kQ8;
     constexpr int MR = G::kRows, KS = D / 16, PIECES = D / 8, RPI = 32 / PIECES, ITERS = kDecKeys / RPI;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -296,7 +490,7 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
             if (p.err) atomicOr(p.err, kErrPage);
             return int32_t(p.pages);
         };
-        // Q8: where the exponents of a stage's step lie (lane: stage), and these
+        // over 8 bits: where the exponents of a stage's step lie (lane: stage), and these
         const uint8_t* ex_at = nullptr;
         uint32_t ex = 0;
         int32_t l_k = lay_out(0, int32_t(lane)), l_id = page_of(0, l_k), n_k, n_id;
@@ -370,9 +564,13 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
             if (stage == G::kStages ? lane < filled && lane < G::kStages : lane == stage)
                 ex = ex_at ? *reinterpret_cast<const uint16_t*>(ex_at) : 0u;
         };
+        Rows8<T, D, Q8 ? NT : 1> rows8;
         uint32_t qf[KS][4];
-        int32_t qe[2] = {0, 0};  // Q8: the rows' own exponents
         auto queries = [&](const DecSeg& x) {  // as A fragments; zero past the rows
+            if constexpr (Q8) {
+                rows8.queries(p, x, lane);
+                return;
+            }
             const uint16_t* q[2];
             bool on[2];
 #pragma unroll
@@ -380,39 +578,7 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
                 const int32_t r = int32_t(lane >> 2) + 8 * i;
                 on[i] = r < x.rows;
                 q[i] = p.q + int64_t(x.q0 + (on[i] ? r / g : 0)) * p.q_ts +
-                       int64_t(x.h * g + (on[i] ? r % g : 0)) * p.q_hs + (lane & 3u) * (Q8 ? 4 : 2);
-            }
-            if constexpr (Q8) {  // elements 4 t .. 4 t + 3 of each 16, as the codes come
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint2 v[KS];
-#pragma unroll
-                    for (int kk = 0; kk < KS; ++kk)
-                        v[kk] = on[i] ? *reinterpret_cast<const uint2*>(q[i] + kk * 16) : make_uint2(0u, 0u);
-                    if constexpr (std::is_same_v<T, BF16>) {
-                        uint32_t top = 0;  // bits of the largest |q| of the row
-#pragma unroll
-                        for (int kk = 0; kk < KS; ++kk)
-                            top = max(max(top, max(v[kk].x & 0x7fffu, (v[kk].x >> 16) & 0x7fffu)),
-                                      max(v[kk].y & 0x7fffu, (v[kk].y >> 16) & 0x7fffu));
-                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                        // to [2^14, 2^15); infinities and NaN stay what they are
-                        qe[i] = top >= 0x7f80u ? 0 : max(int32_t(top >> 7) - 127 - 14, -112);
-                        const float f = two_to(-qe[i]);
-#pragma unroll
-                        for (int kk = 0; kk < KS; ++kk) {
-                            float a, b;
-                            BF16::unpack(v[kk].x, a, b);
-                            v[kk].x = F16::pack(a * f, b * f);
-                            BF16::unpack(v[kk].y, a, b);
-                            v[kk].y = F16::pack(a * f, b * f);
-                        }
-                    }
-#pragma unroll
-                    for (int kk = 0; kk < KS; ++kk) qf[kk][i] = v[kk].x, qf[kk][2 + i] = v[kk].y;
-                }
-                return;
+                       int64_t(x.h * g + (on[i] ? r % g : 0)) * p.q_hs + (lane & 3u) * 2;
             }
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk)
@@ -441,7 +607,7 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
                 for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
             m[0] = m[1] = -INFINITY;
             l[0] = l[1] = 0.f;
-            int32_t most = -126;  // Q8: the largest exponent of the values, the sums' own
+            if constexpr (Q8) rows8.begin(p, x, lane);
 
             for (int32_t block = 0; ok && block < steps; block += 32) {
                 const int32_t c_k = lay_out(c, block + int32_t(lane));
@@ -453,45 +619,22 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
                                                  : warp_wait(landed, phase, p.timeout_ns);
                     if (!ok) break;
                     ++used;
+                    if constexpr (Q8) {
+                        rows8.step(p, ks, vs, __shfl_sync(0xffffffffu, ex, int(st)), k0, kf & kMasked, lane);
+                        __syncwarp();
+                        const uint32_t before = filled;
+                        load();
+                        if (filled != before) fetch(before % G::kStages);
+                        continue;
+                    }
                     // S = Q K^T
                     float sc[2][4] = {};
-                    float c = p.c, pw = 1.f;  // Q8: the logits come in the base-2 exponent's units
-                    if constexpr (Q8) {
 #pragma unroll
-                        for (int kk = 0; kk < KS; kk += 2) {
-                            uint32_t bf[4];
-                            ldsm4(bf, ks + swz8<D>((lane & 7u) + ((lane >> 4) << 3), kk + ((lane >> 3) & 1u)));
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) {
-                                const uint32_t v = bf[y] ^ 0x80808080u;
-                                M::mma(sc[y >> 1], qf[kk + (y & 1)], codes_f16(v, kCodes01), codes_f16(v, kCodes23));
-                            }
-                        }
-                        const uint32_t both = __shfl_sync(0xffffffffu, ex, int(st));
-                        const int32_t ek = int8_t(both), ev = int8_t(both >> 8);
-                        c = 1.f;
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float f = ek == kNoExponent ? NAN : p.c * two_to(min(max(ek + qe[i], -126), 127));
-                            sc[0][2 * i] *= f, sc[0][2 * i + 1] *= f, sc[1][2 * i] *= f, sc[1][2 * i + 1] *= f;
-                        }
-                        if (ev > most) {
-                            const float f = two_to(max(most - ev, -126));
-#pragma unroll
-                            for (int n = 0; n < 2 * KS; ++n)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) o[n][e] *= f;
-                            most = ev;
-                        }
-                        pw = ev == kNoExponent ? NAN : two_to(max(ev - most + int(F16::kShift), -126));
-                    } else {
-#pragma unroll
-                        for (int kk = 0; kk < KS; ++kk) {
-                            uint32_t bf[4];
-                            ldsm4(bf, ks + swz<kDecKeys>((lane & 7u) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1u)));
-                            M::mma(sc[0], qf[kk], bf[0], bf[1]);
-                            M::mma(sc[1], qf[kk], bf[2], bf[3]);
-                        }
+                    for (int kk = 0; kk < KS; ++kk) {
+                        uint32_t bf[4];
+                        ldsm4(bf, ks + swz<kDecKeys>((lane & 7u) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1u)));
+                        T::mma(sc[0], qf[kk], bf[0], bf[1]);
+                        T::mma(sc[1], qf[kk], bf[2], bf[3]);
                     }
                     if (kf & kMasked) {
 #pragma unroll
@@ -522,11 +665,11 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
                         y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
                         y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
                         nm[i] = fmaxf(m[i], y);
-                        bs[i] = nm[i] == -INFINITY ? 0.f : fmaf(nm[i], c, -kShift);
+                        bs[i] = nm[i] == -INFINITY ? 0.f : fmaf(nm[i], p.c, -T::kShift);
                     }
                     if (__any_sync(0xffffffffu, nm[0] > m[0] || nm[1] > m[1])) {
-                        const float al[2] = {ex2(fmaf(m[0], c, -kShift) - bs[0]),
-                                             ex2(fmaf(m[1], c, -kShift) - bs[1])};
+                        const float al[2] = {ex2(fmaf(m[0], p.c, -T::kShift) - bs[0]),
+                                             ex2(fmaf(m[1], p.c, -T::kShift) - bs[1])};
 #pragma unroll
                         for (int n = 0; n < 2 * KS; ++n)
 #pragma unroll
@@ -538,49 +681,29 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
                     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float a = ex2(fmaf(sc[nt][2 * i], c, -bs[i]));
-                            float d = ex2(fmaf(sc[nt][2 * i + 1], c, -bs[i]));
+                            const float a = ex2(fmaf(sc[nt][2 * i], p.c, -bs[i]));
+                            const float d = ex2(fmaf(sc[nt][2 * i + 1], p.c, -bs[i]));
                             l[i] += a + d;
-                            if constexpr (Q8) a *= pw, d *= pw;
                             // A fragment: registers (row, row + 8) x (keys 0-7, 8-15)
-                            ph[nt * 2 + i] = M::pack(a, d);
+                            ph[nt * 2 + i] = T::pack(a, d);
                             float ha, hd;
-                            M::unpack(ph[nt * 2 + i], ha, hd);
-                            pl[nt * 2 + i] = M::pack(a - ha, d - hd);
+                            T::unpack(ph[nt * 2 + i], ha, hd);
+                            pl[nt * 2 + i] = T::pack(a - ha, d - hd);
                         }
                     // O += P V. P enters as its 16-bit rounding plus the 16-bit
                     // rounding of what that leaves: the tensor cores are far from
                     // busy here, and the sum keeps about twice the bits.
-                    if constexpr (Q8) {
-                        // (two codes of a slot lie side by side: the even ones of each 16
-                        // elements in one product, the odd ones in the other)
 #pragma unroll
-                        for (int n = 0; n < KS; n += 2) {
-                            uint32_t vf[4];
-                            ldsm4t(vf, vs + swz8<D>((lane & 7u) + (((lane >> 3) & 1u) << 3), n + (lane >> 4)));
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) vf[y] ^= 0x80808080u;
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) {
-                                const uint32_t select = y & 1 ? kCodes13 : kCodes02;
-                                const uint32_t v0 = codes_f16(vf[y & 2], select), v1 = codes_f16(vf[(y & 2) + 1], select);
-                                M::mma(o[2 * n + y], ph, v0, v1);
-                                M::mma(o[2 * n + y], pl, v0, v1);
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < KS; ++n) {
-                            uint32_t vf[4];
-                            ldsm4t(vf, vs + swz<kDecKeys>((lane & 7u) + (((lane >> 3) & 1u) << 3), n * 2 + (lane >> 4)));
-                            M::mma(o[2 * n], ph, vf[0], vf[1]);
-                            M::mma(o[2 * n + 1], ph, vf[2], vf[3]);
-                            M::mma(o[2 * n], pl, vf[0], vf[1]);
-                            M::mma(o[2 * n + 1], pl, vf[2], vf[3]);
-                        }
+                    for (int n = 0; n < KS; ++n) {
+                        uint32_t vf[4];
+                        ldsm4t(vf, vs + swz<kDecKeys>((lane & 7u) + (((lane >> 3) & 1u) << 3), n * 2 + (lane >> 4)));
+                        T::mma(o[2 * n], ph, vf[0], vf[1]);
+                        T::mma(o[2 * n + 1], ph, vf[2], vf[3]);
+                        T::mma(o[2 * n], pl, vf[0], vf[1]);
+                        T::mma(o[2 * n + 1], pl, vf[2], vf[3]);
                     }
                     // the new tokens' keys and values go to their slots
-                    if (!Q8 && p.fused && (kf & kEdge) && k0 + kDecKeys > x.f) {
+                    if (p.fused && (kf & kEdge) && k0 + kDecKeys > x.f) {
                         const int32_t id = p.table[int64_t(x.b) * p.table_s + (k0 >> p.pshift)];
                         const uint32_t piece = lane % PIECES;
                         if (uint32_t(id) < p.pages) {
@@ -602,15 +725,9 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
                     }
                     // the stage's next contents come through the TMA's proxy: what the
                     // copies wrote is ordered before
-                    if (!Q8 && (kf & kEdge)) proxy_fence();
+                    if (kf & kEdge) proxy_fence();
                     __syncwarp();
-                    if constexpr (Q8) {
-                        const uint32_t before = filled;
-                        load();
-                        if (filled != before) fetch(before % G::kStages);
-                    } else {
-                        load();
-                    }
+                    load();
                 }
             }
 
@@ -618,14 +735,15 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
             // warps at a time where they fit beside one another.
             float* const sm = reinterpret_cast<float*>(smem + G::kStat) + 32;  // [4][MR]
             float* const sl = sm + kDecWarps * MR;
+            if constexpr (Q8) rows8.stats(sm + warp * MR, sl + warp * MR, lane);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; !Q8 && i < 2; ++i) {
                 float y = l[i];
                 y += __shfl_xor_sync(0xffffffffu, y, 1);
                 y += __shfl_xor_sync(0xffffffffu, y, 2);
                 if ((lane & 3u) == 0) {
                     const uint32_t row = (lane >> 2) + 8 * i;
-                    sm[warp * MR + row] = Q8 ? m[i] : fmaf(m[i], p.c, -kShift);  // (the reference)
+                    sm[warp * MR + row] = fmaf(m[i], p.c, -T::kShift);  // (the reference)
                     sl[warp * MR + row] = y;
                 }
             }
@@ -633,28 +751,19 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, Q8>::kCtas)
             const uint32_t side = R * 4 <= MR ? 4 : R * 2 <= MR ? 2 : 1;
             for (uint32_t turn = 0; turn < kDecWarps / side; ++turn) {
                 if (warp / side == turn) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t row = (lane >> 2) + 8 * i, at = warp % side * uint32_t(R) + row;
-                        if (int32_t(row) >= R) continue;
+                    auto top = [&](uint32_t row) {
                         float mx = sm[row];
 #pragma unroll
                         for (int w = 1; w < kDecWarps; ++w) mx = fmaxf(mx, sm[w * MR + row]);
-                        float f = mx == -INFINITY ? 0.f : ex2((Q8 ? m[i] : fmaf(m[i], p.c, -kShift)) - mx);
-                        if constexpr (Q8) {
-                            f *= two_to(max(most - int(F16::kShift), -126));
-                            float* to = join + at * D;
+                        return mx;
+                    };
+                    if constexpr (Q8) rows8.sums(join, warp % side * uint32_t(R), R, turn != 0, top, lane);
 #pragma unroll
-                            for (int n = 0; n < KS; ++n) {
-                                float4* cell = reinterpret_cast<float4*>(
-                                    to + ((n * 16 + (lane & 3u) * 4) ^ (at & 7u) * 8));
-                                float4 v = make_float4(o[2 * n][2 * i] * f, o[2 * n + 1][2 * i] * f,
-                                                       o[2 * n][2 * i + 1] * f, o[2 * n + 1][2 * i + 1] * f);
-                                if (turn) v.x += cell->x, v.y += cell->y, v.z += cell->z, v.w += cell->w;
-                                *cell = v;
-                            }
-                            continue;
-                        }
+                    for (int i = 0; !Q8 && i < 2; ++i) {
+                        const uint32_t row = (lane >> 2) + 8 * i, at = warp % side * uint32_t(R) + row;
+                        if (int32_t(row) >= R) continue;
+                        const float mx = top(row);
+                        const float f = mx == -INFINITY ? 0.f : ex2(fmaf(m[i], p.c, -T::kShift) - mx);
                         float* to = join + at * D + (lane & 3u) * 2;
 #pragma unroll
                         for (int n = 0; n < 2 * KS; ++n) {
@@ -836,7 +945,7 @@ ScratchPlan scratch_plan(const ls_b200_attention_args& a) {
     ScratchPlan s{};
     const bool w = a.weights_length != 0;
     s.count = 0;
-    s.part = up256(kMaxCtas * sizeof(uint32_t));
+    s.part = up256(kMaxCounts * sizeof(uint32_t));
     if (is_chunk(a)) {
         const uint32_t g = a.q_heads / a.kv_heads;
         s.plan = s.part;
@@ -885,9 +994,10 @@ int check_shape(const ls_b200_attention_args& a) {
     return 0;
 }
 
-template <class T, int D, bool Q8>
+template <class T, int D, int NT>
 int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
-    using G = GeoD<D, Q8>;
+    using G = GeoD<D, NT>;
+    constexpr bool Q8 = G::kQ8;
     CUtensorMap km, vm;
     if constexpr (Q8) {
         if (!encode_codes(&km, p.k_pages, p, p.kp_ss, p.kp_hs, p.kp_ps, kDecKeys) ||
@@ -900,7 +1010,7 @@ int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
         if (!encode_map(&km, bf16, p.k_pages, 5, dims, ks, box) || !encode_map(&vm, bf16, p.v_pages, 5, dims, vs, box))
             return EINVAL;
     }
-    const auto kernel = attn_decode_kernel<T, D, Q8>;
+    const auto kernel = attn_decode_kernel<T, D, NT>;
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -914,16 +1024,17 @@ int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
         if (e != cudaSuccess) return int(e);
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
-    const uint32_t sms = sm_count() * uint32_t(G::kCtas), grid = sms < kMaxCtas ? sms : kMaxCtas;
+    const uint32_t ctas = sm_count() * uint32_t(G::kCtas), most = kMaxCtas * 16 / G::kRows;  // (by the scratch)
+    const uint32_t grid = ctas < most ? ctas : most;
     // (the append before a call over 8 bits lets it begin early)
     if constexpr (Q8) return int(launch_after(kernel, grid, kDecThreads, G::kSmem, s, p, km, vm));
     kernel<<<grid, kDecThreads, G::kSmem, s>>>(p, km, vm);
     return int(cudaGetLastError());
 }
-template <bool Q8>
+template <int NT>
 int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
-    return p.D == 64 ? (bf16 ? launch_decode<BF16, 64, Q8>(p, true, s) : launch_decode<F16, 64, Q8>(p, false, s))
-                     : (bf16 ? launch_decode<BF16, 128, Q8>(p, true, s) : launch_decode<F16, 128, Q8>(p, false, s));
+    return p.D == 64 ? (bf16 ? launch_decode<BF16, 64, NT>(p, true, s) : launch_decode<F16, 64, NT>(p, false, s))
+                     : (bf16 ? launch_decode<BF16, 128, NT>(p, true, s) : launch_decode<F16, 128, NT>(p, false, s));
 }
 
 // A call over a cache of 16 bits (x NULL) or 8 bits.
@@ -1003,7 +1114,9 @@ int attend(const ls_b200_attention_args* a, const ls_b200_cache_exponents* x, vo
     }
     p.fused = p.k_new != nullptr;
     const bool bf16 = a->dtype == LS_B200_BF16;
-    const int rc = x ? launch_decode<true>(p, bf16, s) : launch_decode<false>(p, bf16, s);
+    const int rc = !x              ? launch_decode<0>(p, bf16, s)
+                   : p.rows <= 8u ? launch_decode<1>(p, bf16, s)
+                                  : launch_decode<2>(p, bf16, s);
     if (rc || !p.weights) return rc;
     return int(launch_after(attn_weights_kernel, p.B * p.Hkv * ((p.wlen + 255) / 256), 256, 0, s, p));
 }

@@ -50,7 +50,8 @@ struct AttnParams {
 
 // The tensor-core path of chunks (ls_attention_chunk.cu): one item is two
 // 128-row tiles of one kv head, a row being a (token, head of the group).
-constexpr uint32_t kMaxCtas = 512;  // CTAs of a launch, and counters in the scratch header
+constexpr uint32_t kMaxCtas = 512;  // CTAs of a launch (of the decode kernel with eight rows: twice as many)
+constexpr uint32_t kMaxCounts = 2 * kMaxCtas;  // counters in the scratch header
 constexpr int kChunkKeys = 128;     // slots of a tile
 struct ChunkItem {                  // written by the plan kernel
     int32_t b, q0, nq, n;           // the sequence, as SeqRange
