@@ -18,7 +18,8 @@ ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 LIBRARY = PACKAGE / "libleanstream_b200.so"
 SOURCES = ("ls_kernel.cu", "ls_kernel_traced.cu", "ls_backend.cu", "ls_aux.cu", "ls_stream.cu", "ls_batch.cu",
-           "ls_attention.cu", "ls_attention_chunk.cu", "ls_append.cu", "ls_evict.cu")
+           "ls_attention.cu", "ls_attention8.cu", "ls_attention_chunk.cu",
+           "ls_append.cu", "ls_evict.cu")
 HEADERS = ("ls_internal.h", "ls_attention.h", "ls_tc.h")
 ARCH = ("-gencode", "arch=compute_100a,code=sm_100a")
 

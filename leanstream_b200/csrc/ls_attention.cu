@@ -56,14 +56,12 @@ constexpr int64_t kDecMinUnits = 2 + kDecItemCost;  // units that a CTA takes at
 constexpr uint64_t kGraceNs = 1000000000ull;
 constexpr uint64_t kShortNs = 100000;  // bounds that a barrier's try may sleep over: a load takes less
 
-// NT: 0 over 16 bits, else tiles of eight rows over 8 bits. CTAs per SM by
-// registers; the ring takes the shared memory that leaves.
-template <int D, int NT>
+// Three CTAs per SM by registers; the ring takes the shared memory that leaves.
+template <int D>
 struct GeoD {
-    static constexpr bool kQ8 = NT != 0;
-    static constexpr int kCtas = NT == 1 ? 4 : 3, kRows = kQ8 ? 8 * NT : 16;
-    static constexpr uint32_t kHalf = kDecKeys * D * (kQ8 ? 1 : 2), kStage = 2 * kHalf;  // a step's keys, its values
-    static constexpr int kStages = (NT == 0 ? 2 : NT == 1 ? 3 : 4) * (128 / D);
+    static constexpr int kCtas = 3, kRows = 16;
+    static constexpr uint32_t kHalf = kDecKeys * D * 2, kStage = 2 * kHalf;  // a step's keys, and its values
+    static constexpr int kStages = 2 * (128 / D);
     static constexpr uint32_t kRing = kDecWarps * kStages * kStage;
     static constexpr uint32_t kJoin = kRing, kJoinBytes = kRows * D * 4;  // sums of the warps
     static constexpr uint32_t kSegs = kJoin + kJoinBytes, kBars = kSegs + kDecSegs * 64;
@@ -92,14 +90,6 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {  
 __device__ __forceinline__ void cp_arrive(uint32_t bar) {  // one arrival, when this thread's copies have landed
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
 // 16-byte piece of a row in a tile of ROWS rows: panels of 64 elements, each
 // row's pieces XORed with its low bits (the 128-byte swizzle of the TMA), so
 // that the eight rows of an ldmatrix lie in different banks.
@@ -107,21 +97,6 @@ template <int ROWS>
 __device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t piece) {
     return (piece >> 3) * (ROWS * 128) + row * 128 + (((piece ^ row) & 7u) << 4);
 }
-// The same in a tile of codes, rows of D bytes: for 64 the pieces of two rows
-// share 128 bytes (the 64-byte swizzle).
-template <int D>
-__device__ __forceinline__ uint32_t swz8(uint32_t row, uint32_t piece) {
-    return D == 128 ? row * 128 + (((piece ^ row) & 7u) << 4) : row * 64 + (((piece ^ (row >> 1)) & 3u) << 4);
-}
-// Codes to float16 pairs, exactly: a code + 128 in the low byte of 1024 reads 1024
-// + 128 + code. Pairs of the four codes of v by their places.
-__device__ __forceinline__ uint32_t codes_f16(uint32_t v, uint32_t select) {
-    uint32_t r;
-    asm("{.reg .b32 t;\n\tprmt.b32 t, %1, %2, %3;\n\tsub.rn.f16x2 %0, t, %4;}"
-        : "=r"(r) : "r"(v), "r"(0x64646464u), "r"(select), "r"(0x64806480u));
-    return r;
-}
-constexpr uint32_t kCodes01 = 0x4140, kCodes23 = 0x4342, kCodes02 = 0x4240, kCodes13 = 0x4341;
 
 // Sums of (x, y) over the block, and over the threads before this one.
 struct Pair {
@@ -149,205 +124,6 @@ __device__ __forceinline__ Pair block_scan(Pair v, Pair* sh, Pair& before) {
     return total;
 }
 
-// The rows of a warp over a cache in 8 bits (value = code * 2^e, one e for the 16
-// slots of a step), NT tiles of eight. Slots and elements are the M dimension of
-// the products and rows their N, so that few rows leave no tile half empty:
-//     S^T = K Q^T     16 slots x 8 rows,     O^T += V^T P^T     16 elements x 8 rows.
-// Codes enter as whole numbers in float16, whatever the type of the queries; those
-// enter it by a power of two of their own per row (bfloat16: what lies 2^-29 below
-// a row's largest loses bits). The exponents meet the logits in 32 bits, and the
-// probabilities as 2^(e - E), E the largest exponent of the values so far; when that
-// grows the sums are scaled down. A row's reference is only raised when a logit
-// passes it by 2^kRaise. P is rounded once, to float16, times 2^kChunkShift.
-// Every slot of a step is a number, so those that no row sees are not cleared.
-//
-// Lane (g, t) = (lane / 4, lane % 4) holds the rows 2 t and 2 t + 1 of each tile
-// for the slots g and g + 8, and for the elements 16 n + 2 g and + 1 of all n.
-template <class T, int D, int NT>
-struct Rows8 {
-    static constexpr int KS = D / 16;
-    uint2 q[NT][KS];     // row g: elements 4 t .. 4 t + 3 of each 16, as the codes come
-    float cq[NT][2];     // scale * log2 e and the rows' own powers of two
-    float o[NT][KS][4];  // in units of 2^(most - kChunkShift)
-    float m[NT][2], l[NT][2];  // l: of this lane's slots
-    int32_t pos[NT][2];  // slot of the rows' tokens (-1: no row)
-    int32_t most;
-
-    __device__ __forceinline__ void queries(const AttnParams& p, const DecSeg& x, uint32_t lane) {
-        const int32_t g = int32_t(p.g);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int32_t r = int32_t(lane >> 2) + 8 * i;
-            const bool on = r < x.rows;
-            const uint16_t* at = p.q + int64_t(x.q0 + (on ? r / g : 0)) * p.q_ts +
-                                 int64_t(x.h * g + (on ? r % g : 0)) * p.q_hs + (lane & 3u) * 4;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-                q[i][k] = on ? *reinterpret_cast<const uint2*>(at + k * 16) : make_uint2(0u, 0u);
-        }
-    }
-    __device__ __forceinline__ void begin(const AttnParams& p, const DecSeg& x, uint32_t lane) {
-        const int32_t g = int32_t(p.g), t = int32_t(lane & 3u);
-        most = -126;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            float c = p.c;
-            if constexpr (std::is_same_v<T, BF16>) {
-                uint32_t top = 0;  // bits of the largest |q| of the row
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-                    top = max(max(top, max(q[i][k].x & 0x7fffu, (q[i][k].x >> 16) & 0x7fffu)),
-                              max(q[i][k].y & 0x7fffu, (q[i][k].y >> 16) & 0x7fffu));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // to [2^14, 2^15); infinities and NaN stay what they are
-                const int32_t e = top >= 0x7f80u ? 0 : max(int32_t(top >> 7) - 127 - 14, -112);
-                const float f = two_to(-e);
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    float a, b;
-                    BF16::unpack(q[i][k].x, a, b);
-                    q[i][k].x = F16::pack(a * f, b * f);
-                    BF16::unpack(q[i][k].y, a, b);
-                    q[i][k].y = F16::pack(a * f, b * f);
-                }
-                c *= two_to(e);
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const int32_t row = 8 * i + 2 * t + y;
-                cq[i][y] = __shfl_sync(0xffffffffu, c, (2 * t + y) * 4);
-                pos[i][y] = row < x.rows ? max(x.f + row / g, -1) : -1;
-                m[i][y] = -INFINITY, l[i][y] = 0.f;
-            }
-#pragma unroll
-            for (int n = 0; n < KS; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
-        }
-    }
-    // 16 slots from k0, codes of their keys and values at ks and vs, both exponents in `ex`
-    __device__ __forceinline__ void step(const AttnParams& p, uint32_t ks, uint32_t vs, uint32_t ex, int32_t k0,
-                                         bool masked, uint32_t lane) {
-        float s[NT][4] = {};
-#pragma unroll
-        for (int k = 0; k < KS; k += 2) {
-            uint32_t v[4];  // slots 0-7 and 8-15 (v[2], v[3]) of two 16-byte pieces
-            ldsm4(v, ks + swz8<D>((lane & 7u) + ((lane >> 4) << 3), k + ((lane >> 3) & 1u)));
-#pragma unroll
-            for (int y = 0; y < 4; ++y) v[y] ^= 0x80808080u;
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const uint32_t a[4] = {codes_f16(v[y], kCodes01), codes_f16(v[2 + y], kCodes01),
-                                       codes_f16(v[y], kCodes23), codes_f16(v[2 + y], kCodes23)};
-#pragma unroll
-                for (int i = 0; i < NT; ++i) F16::mma(s[i], a, q[i][k + y].x, q[i][k + y].y);
-            }
-        }
-        const int32_t ek = int8_t(ex), ev = int8_t(ex >> 8);
-        const float fk = ek == kNoExponent ? NAN : two_to(max(ek, -126));
-        bool raise = false;
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[i][e] *= cq[i][e & 1] * fk;
-                if (masked && !sees(p, pos[i][e & 1], k0 + int32_t(lane >> 2) + 8 * (e >> 1))) s[i][e] = -INFINITY;
-                raise = raise || s[i][e] > m[i][e & 1] + F16::kRaise;
-            }
-        if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    float top = fmaxf(m[i][y], fmaxf(s[i][y], s[i][2 + y]));
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    const float f = top == -INFINITY ? 1.f : ex2(m[i][y] - top);
-                    m[i][y] = top;
-                    l[i][y] *= f;
-#pragma unroll
-                    for (int n = 0; n < KS; ++n) o[i][n][y] *= f, o[i][n][2 + y] *= f;
-                }
-        }
-        if (ev > most) {
-            const float f = two_to(max(most - ev, -126));
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int n = 0; n < KS; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[i][n][e] *= f;
-            most = ev;
-        }
-        const float pw = ev == kNoExponent ? NAN : two_to(max(ev - most + int(F16::kChunkShift), -126));
-        uint32_t b[NT][2];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            float a[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                a[e] = ex2(s[i][e] - (m[i][e & 1] == -INFINITY ? 0.f : m[i][e & 1]));
-                l[i][e & 1] += a[e];
-                a[e] *= pw;
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y)  // slots by rows, to rows by slots
-                asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;"
-                             : "=r"(b[i][y]) : "r"(F16::pack(a[2 * y], a[2 * y + 1])));
-        }
-#pragma unroll
-        for (int n = 0; n < KS; n += 2) {
-            uint32_t v[4];  // of two 16-byte pieces, slots 0-7 and 8-15 each; a register holds elements 2 g, 2 g + 1
-            ldsm4t(v, vs + swz8<D>((lane & 7u) + (((lane >> 3) & 1u) << 3), n + (lane >> 4)));
-#pragma unroll
-            for (int y = 0; y < 4; ++y) v[y] ^= 0x80808080u;
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const uint32_t a[4] = {codes_f16(v[2 * y], kCodes02), codes_f16(v[2 * y], kCodes13),
-                                       codes_f16(v[2 * y + 1], kCodes02), codes_f16(v[2 * y + 1], kCodes13)};
-#pragma unroll
-                for (int i = 0; i < NT; ++i) F16::mma(o[i][n + y], a, b[i][0], b[i][1]);
-            }
-        }
-    }
-    // Maxima and sums of the rows to sm, sl [8 NT].
-    __device__ __forceinline__ void stats(float* sm, float* sl, uint32_t lane) const {
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                float sum = l[i][y];
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                const uint32_t row = 8 * i + 2 * lane + y;
-                if (lane < 4) sm[row] = m[i][y], sl[row] = sum;
-            }
-    }
-    // The sums times 2^(own maximum - top[row]) to row `at0 + row` of `join`, or added there.
-    template <class F>
-    __device__ __forceinline__ void sums(float* join, uint32_t at0, int32_t R, bool add, F top, uint32_t lane) const {
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const uint32_t row = 8 * i + 2 * (lane & 3u) + y, at = at0 + row;
-                if (int32_t(row) >= R) continue;
-                const float mx = top(row);
-                const float unit = two_to(max(most - int(F16::kChunkShift), -126));
-                const float f = mx == -INFINITY ? 0.f : ex2(m[i][y] - mx) * unit;
-                float* to = join + at * D;
-#pragma unroll
-                for (int n = 0; n < KS; ++n) {
-                    float2* cell = reinterpret_cast<float2*>(to + ((n * 16 + (lane >> 2) * 2) ^ (at & 7u) * 8));
-                    float2 v = make_float2(o[i][n][y] * f, o[i][n][2 + y] * f);
-                    if (add) v.x += cell->x, v.y += cell->y;
-                    *cell = v;
-                }
-            }
-    }
-};
-
 // The kernel for few rows per sequence and kv head (decoding, drafts): bound
 // by the read of the cache. An item is a sequence and kv head; its rows are
 // (token, head of the group), so all heads that share a key read it once. The
@@ -363,14 +139,11 @@ struct Rows8 {
 // multiplier is idle beside the loads. Two sequences
 // of up to 131072 slots, 64 heads of 128 over 8: 180 us, 5.7 TB/s of the cache;
 // 32 of up to 4096 slots, 32 heads: 60 us, 4.6 TB/s; one of 97 slots: 8.5 us.
-// Over 8 bits (NT > 0) the rows' part is Rows8's, a step is a block of the cache,
-// and nothing is appended or cleared.
-template <class T, int D, int NT>
-__global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
+template <class T, int D>
+__global__ void __launch_bounds__(kDecThreads, GeoD<D>::kCtas)
     attn_decode_kernel(const AttnParams p, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
-    using G = GeoD<D, NT>;
-    constexpr bool Q8 = G::kQ8;
+    using G = GeoD<D>;
     constexpr int MR = G::kRows, KS = D / 16, PIECES = D / 8, RPI = 32 / PIECES, ITERS = kDecKeys / RPI;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -385,10 +158,9 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
 
     after_start();
     if (lane == 0) {
-        for (int i = 0; i < G::kStages; ++i) bar_init(bar0 + 8 * i, Q8 ? 1 : 32);
+        for (int i = 0; i < G::kStages; ++i) bar_init(bar0 + 8 * i, 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if constexpr (Q8) after_wait();
     // units of this thread's sequence (of the first 128), and of the call; y: 1
     // where the sequence has rows
     auto units_of = [&](uint32_t b, SeqRange& s) -> Pair {
@@ -490,9 +262,6 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
             if (p.err) atomicOr(p.err, kErrPage);
             return int32_t(p.pages);
         };
-        // over 8 bits: where the exponents of a stage's step lie (lane: stage), and these
-        const uint8_t* ex_at = nullptr;
-        uint32_t ex = 0;
         int32_t l_k = lay_out(0, int32_t(lane)), l_id = page_of(0, l_k), n_k, n_id;
         after(n_seg, n_base);
         n_k = lay_out(n_seg, n_base + int32_t(lane));
@@ -514,18 +283,6 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
             const int32_t k0 = kf & ~15, in = k0 & int32_t(p.P - 1);
             const uint32_t st = filled % G::kStages, dst = ring + st * G::kStage, bar = bar0 + 8 * st;
             ++filled;
-            if constexpr (Q8) {
-                const int32_t h = segs[l_seg].h;
-                if (lane == 0) {
-                    bar_arrive_tx(bar, G::kStage);
-                    tma4(dst, &kmap, bar, 0, in, h, id);
-                    tma4(dst + G::kHalf, &vmap, bar, 0, in, h, id);
-                }
-                if (lane == st)
-                    ex_at = uint32_t(id) < p.pages ? p.ex + int64_t(id) * p.ex_ps + int64_t(h) * p.ex_hs + (in >> 3)
-                                                   : nullptr;
-                return;
-            }
             if (!(kf & kEdge)) {
                 if (lane == 0) {
                     const int32_t h = segs[l_seg].h;
@@ -559,18 +316,8 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
             }
             cp_arrive(bar);
         };
-        // the exponents of the step in `stage` (all stages where it is kStages)
-        auto fetch = [&](uint32_t stage) {
-            if (stage == G::kStages ? lane < filled && lane < G::kStages : lane == stage)
-                ex = ex_at ? *reinterpret_cast<const uint16_t*>(ex_at) : 0u;
-        };
-        Rows8<T, D, Q8 ? NT : 1> rows8;
         uint32_t qf[KS][4];
         auto queries = [&](const DecSeg& x) {  // as A fragments; zero past the rows
-            if constexpr (Q8) {
-                rows8.queries(p, x, lane);
-                return;
-            }
             const uint16_t* q[2];
             bool on[2];
 #pragma unroll
@@ -589,7 +336,6 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
         queries(segs[0]);  // ahead of the cache's stream
 #pragma unroll 1
         for (int i = 0; ok && i < G::kStages; ++i) load();
-        if constexpr (Q8) fetch(G::kStages);
 
         for (uint32_t c = 0; c < count; ++c) {
             const DecSeg& x = segs[c];
@@ -607,7 +353,6 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
                 for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
             m[0] = m[1] = -INFINITY;
             l[0] = l[1] = 0.f;
-            if constexpr (Q8) rows8.begin(p, x, lane);
 
             for (int32_t block = 0; ok && block < steps; block += 32) {
                 const int32_t c_k = lay_out(c, block + int32_t(lane));
@@ -619,14 +364,6 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
                                                  : warp_wait(landed, phase, p.timeout_ns);
                     if (!ok) break;
                     ++used;
-                    if constexpr (Q8) {
-                        rows8.step(p, ks, vs, __shfl_sync(0xffffffffu, ex, int(st)), k0, kf & kMasked, lane);
-                        __syncwarp();
-                        const uint32_t before = filled;
-                        load();
-                        if (filled != before) fetch(before % G::kStages);
-                        continue;
-                    }
                     // S = Q K^T
                     float sc[2][4] = {};
 #pragma unroll
@@ -735,9 +472,8 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
             // warps at a time where they fit beside one another.
             float* const sm = reinterpret_cast<float*>(smem + G::kStat) + 32;  // [4][MR]
             float* const sl = sm + kDecWarps * MR;
-            if constexpr (Q8) rows8.stats(sm + warp * MR, sl + warp * MR, lane);
 #pragma unroll
-            for (int i = 0; !Q8 && i < 2; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 float y = l[i];
                 y += __shfl_xor_sync(0xffffffffu, y, 1);
                 y += __shfl_xor_sync(0xffffffffu, y, 2);
@@ -751,18 +487,13 @@ __global__ void __launch_bounds__(kDecThreads, GeoD<D, NT>::kCtas)
             const uint32_t side = R * 4 <= MR ? 4 : R * 2 <= MR ? 2 : 1;
             for (uint32_t turn = 0; turn < kDecWarps / side; ++turn) {
                 if (warp / side == turn) {
-                    auto top = [&](uint32_t row) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t row = (lane >> 2) + 8 * i, at = warp % side * uint32_t(R) + row;
+                        if (int32_t(row) >= R) continue;
                         float mx = sm[row];
 #pragma unroll
                         for (int w = 1; w < kDecWarps; ++w) mx = fmaxf(mx, sm[w * MR + row]);
-                        return mx;
-                    };
-                    if constexpr (Q8) rows8.sums(join, warp % side * uint32_t(R), R, turn != 0, top, lane);
-#pragma unroll
-                    for (int i = 0; !Q8 && i < 2; ++i) {
-                        const uint32_t row = (lane >> 2) + 8 * i, at = warp % side * uint32_t(R) + row;
-                        if (int32_t(row) >= R) continue;
-                        const float mx = top(row);
                         const float f = mx == -INFINITY ? 0.f : ex2(fmaf(m[i], p.c, -T::kShift) - mx);
                         float* to = join + at * D + (lane & 3u) * 2;
 #pragma unroll
@@ -945,7 +676,7 @@ ScratchPlan scratch_plan(const ls_b200_attention_args& a) {
     ScratchPlan s{};
     const bool w = a.weights_length != 0;
     s.count = 0;
-    s.part = up256(kMaxCounts * sizeof(uint32_t));
+    s.part = up256(kMaxCtas * sizeof(uint32_t));
     if (is_chunk(a)) {
         const uint32_t g = a.q_heads / a.kv_heads;
         s.plan = s.part;
@@ -994,49 +725,33 @@ int check_shape(const ls_b200_attention_args& a) {
     return 0;
 }
 
-template <class T, int D, int NT>
+template <class T, int D>
 int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
-    using G = GeoD<D, NT>;
-    constexpr bool Q8 = G::kQ8;
+    using G = GeoD<D>;
     CUtensorMap km, vm;
-    if constexpr (Q8) {
-        if (!encode_codes(&km, p.k_pages, p, p.kp_ss, p.kp_hs, p.kp_ps, kDecKeys) ||
-            !encode_codes(&vm, p.v_pages, p, p.vp_ss, p.vp_hs, p.vp_ps, kDecKeys))
-            return EINVAL;
-    } else {
-        const uint64_t dims[5] = {64, p.P, D / 64, p.Hkv, p.pages};
-        const int64_t ks[4] = {p.kp_ss, 64, p.kp_hs, p.kp_ps}, vs[4] = {p.vp_ss, 64, p.vp_hs, p.vp_ps};
-        const uint32_t box[5] = {64, uint32_t(kDecKeys), D / 64, 1, 1};
-        if (!encode_map(&km, bf16, p.k_pages, 5, dims, ks, box) || !encode_map(&vm, bf16, p.v_pages, 5, dims, vs, box))
-            return EINVAL;
-    }
-    const auto kernel = attn_decode_kernel<T, D, NT>;
+    const uint64_t dims[5] = {64, p.P, D / 64, p.Hkv, p.pages};
+    const int64_t ks[4] = {p.kp_ss, 64, p.kp_hs, p.kp_ps}, vs[4] = {p.vp_ss, 64, p.vp_hs, p.vp_ps};
+    const uint32_t box[5] = {64, uint32_t(kDecKeys), D / 64, 1, 1};
+    if (!encode_map(&km, bf16, p.k_pages, 5, dims, ks, box) || !encode_map(&vm, bf16, p.v_pages, 5, dims, vs, box))
+        return EINVAL;
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return int(e);
     const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
     if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(G::kSmem));
+        e = cudaFuncSetAttribute(attn_decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 int(G::kSmem));
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+            e = cudaFuncSetAttribute(attn_decode_kernel<T, D>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                      int(cudaSharedmemCarveoutMaxShared));
         if (e != cudaSuccess) return int(e);
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
-    const uint32_t ctas = sm_count() * uint32_t(G::kCtas), most = kMaxCtas * 16 / G::kRows;  // (by the scratch)
-    const uint32_t grid = ctas < most ? ctas : most;
-    // (the append before a call over 8 bits lets it begin early)
-    if constexpr (Q8) return int(launch_after(kernel, grid, kDecThreads, G::kSmem, s, p, km, vm));
-    kernel<<<grid, kDecThreads, G::kSmem, s>>>(p, km, vm);
+    const uint32_t grid = sm_count() * uint32_t(G::kCtas);
+    attn_decode_kernel<T, D><<<grid < kMaxCtas ? grid : kMaxCtas, kDecThreads, G::kSmem, s>>>(p, km, vm);
     return int(cudaGetLastError());
 }
-template <int NT>
-int launch_decode(const AttnParams& p, bool bf16, cudaStream_t s) {
-    return p.D == 64 ? (bf16 ? launch_decode<BF16, 64, NT>(p, true, s) : launch_decode<F16, 64, NT>(p, false, s))
-                     : (bf16 ? launch_decode<BF16, 128, NT>(p, true, s) : launch_decode<F16, 128, NT>(p, false, s));
-}
-
 // A call over a cache of 16 bits (x NULL) or 8 bits.
 int attend(const ls_b200_attention_args* a, const ls_b200_cache_exponents* x, void* stream) {
     if (!a) return EINVAL;
@@ -1103,6 +818,10 @@ int attend(const ls_b200_attention_args* a, const ls_b200_cache_exponents* x, vo
         p.ex_ps = x->page_stride, p.ex_hs = x->head_stride;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (x && p.rows <= kMaxRows8) {
+        if (is_chunk(*a)) p.part = reinterpret_cast<float*>(scratch + plan.chunk_part);  // (the larger one)
+        return launch_decode8(p, a->dtype, s);
+    }
     if (is_chunk(*a)) {
         const ChunkScratch c{reinterpret_cast<ChunkPlan*>(scratch + plan.plan),
                              reinterpret_cast<ChunkItem*>(scratch + plan.items),
@@ -1114,9 +833,8 @@ int attend(const ls_b200_attention_args* a, const ls_b200_cache_exponents* x, vo
     }
     p.fused = p.k_new != nullptr;
     const bool bf16 = a->dtype == LS_B200_BF16;
-    const int rc = !x              ? launch_decode<0>(p, bf16, s)
-                   : p.rows <= 8u ? launch_decode<1>(p, bf16, s)
-                                  : launch_decode<2>(p, bf16, s);
+    const int rc = p.D == 64 ? (bf16 ? launch_decode<BF16, 64>(p, true, s) : launch_decode<F16, 64>(p, false, s))
+                             : (bf16 ? launch_decode<BF16, 128>(p, true, s) : launch_decode<F16, 128>(p, false, s));
     if (rc || !p.weights) return rc;
     return int(launch_after(attn_weights_kernel, p.B * p.Hkv * ((p.wlen + 255) / 256), 256, 0, s, p));
 }

@@ -50,8 +50,7 @@ struct AttnParams {
 
 // The tensor-core path of chunks (ls_attention_chunk.cu): one item is two
 // 128-row tiles of one kv head, a row being a (token, head of the group).
-constexpr uint32_t kMaxCtas = 512;  // CTAs of a launch (of the decode kernel with eight rows: twice as many)
-constexpr uint32_t kMaxCounts = 2 * kMaxCtas;  // counters in the scratch header
+constexpr uint32_t kMaxCtas = 512;  // CTAs of a launch, and counters in the scratch header
 constexpr int kChunkKeys = 128;     // slots of a tile
 struct ChunkItem {                  // written by the plan kernel
     int32_t b, q0, nq, n;           // the sequence, as SeqRange
@@ -88,6 +87,9 @@ bool encode_map(CUtensorMap* map, bool bf16, const void* base, uint32_t rank, co
 bool encode_codes(CUtensorMap* map, const void* base, const AttnParams& p, int64_t ss, int64_t hs, int64_t ps,
                   uint32_t slots);
 uint32_t sm_count();  // of the current device
+// Few rows over a cache in 8 bits (ls_attention8.cu).
+constexpr uint32_t kMaxRows8 = 24;
+int launch_decode8(const AttnParams& p, uint32_t dtype, cudaStream_t stream);
 int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream);
 
 // A sequence of the call: its new tokens are rows q0 .. q0 + nq - 1 of q and

@@ -1,0 +1,736 @@
+// Attention of few new tokens per sequence (decoding, drafts) over a paged cache
+// in 8 bits. The formula is that of ls_attention.cu; a value of the cache is code *
+// 2^e, one e for the 16 slots of a block, kv head, and keys or values.
+//
+// An item is a sequence and kv head; its rows are (token, head of the group). Its
+// slots go by in steps of 32 (two blocks); the steps of all items, in order, are
+// cut evenly over one CTA per SM. One warp of a CTA loads: it lays out up to 32
+// steps at a time, a lane each, and fills one ring of stages with what each step
+// needs (first slot, exponents, codes of keys and values). The other warps
+// take the steps in turn, with maxima and sums of their own, and meet at the end of
+// an item's piece; the loads run on into the next piece meanwhile. An item cut over
+// several CTAs is joined, in the order of its pieces, by the CTA that arrives last.
+// Which warp takes which step follows from the step, so results do not depend on
+// timing.
+//
+// Slots and elements are the M dimension of the products and rows their N, so that
+// few rows leave no tile half empty, and a code is turned into a number once for
+// all of them:
+//     S^T = K Q^T     16 slots x 8 rows,     O^T += V^T P^T     16 elements x 8 rows.
+// Codes enter as whole numbers in float16, whatever the type of the queries; those
+// enter it by a power of two of their own per row (bfloat16: what lies 2^-29 below
+// a row's largest loses bits). The exponents meet the logits in 32 bits, and the
+// probabilities as 2^(e - E), E the largest exponent of the values so far; when that
+// grows the sums are scaled down. A row's reference is only raised when a logit
+// passes it by 2^kRaise. P is rounded once, to float16, times 2^kChunkShift.
+#include <stdint.h>
+
+#include <atomic>
+#include <cerrno>
+#include <type_traits>
+
+#include "ls_attention.h"
+#include "ls_tc.h"
+
+namespace lsb {
+namespace {
+
+using namespace tc;
+
+constexpr int kStep = 2 * kBlock;          // slots of a step
+constexpr int kSegCount = 48;              // pieces listed at a time
+constexpr int64_t kItemCost8 = 8;          // steps that beginning and joining an item counts as
+constexpr int64_t kMinUnits8 = 24;         // steps that a CTA takes at least
+constexpr int kLoadLanes = 8;              // steps that the loading warp waits for at a time
+constexpr uint64_t kGraceNs = 1000000000ull;
+constexpr uint64_t kShortNs = 100000;      // bounds that a barrier's try may sleep over: a load takes less
+
+// NT tiles of eight rows, kWarps that compute. One CTA per SM; the ring takes the
+// shared memory that the warps' sums, half of them at a time, leave.
+template <int D, int NT>
+struct Geo8 {
+    static constexpr int kWarps = NT == 1 ? 11 : NT == 2 ? 10 : 7, kThreads = 32 * (kWarps + 1), kSide = (kWarps + 1) / 2;
+    static constexpr int kRows = 8 * NT;
+    static constexpr uint32_t kHalf = kStep * D, kStage = 2 * kHalf;  // a step's keys, and its values
+    // A stage is always the same warp's: then its next round cannot be taken for the
+    // one before, whose load may still be under way.
+    static constexpr int kStages = kWarps * (NT == 3 ? 3 : 2) * (128 / D);
+    static constexpr uint32_t kJoin = kStages * kStage, kSegs = kJoin + kSide * kRows * D * 4;
+    static constexpr uint32_t kNotes = kSegs + kSegCount * 64, kBars = kNotes + 8 * kStages;
+    static constexpr uint32_t kStat = kBars + 16 * kStages, kScan = kStat + 8 * kWarps * kRows;
+    static constexpr uint32_t kSmem = kScan + 16 * (kWarps + 1) + 16 + 1024;  // + alignment of the swizzled tiles
+    static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
+};
+
+// A piece of an item: `steps` steps from step j0 of a sequence and kv head.
+struct Seg8 {
+    int32_t b, h, q0, rows;
+    int32_t f, hi, lo, sink;  // as SeqRange, KeyRange
+    int32_t ns, first, j0, steps;
+    int32_t tiles, own;       // steps of the item; own: it does not begin the CTA's range
+    int64_t item;             // first unit of the item
+    __device__ __forceinline__ int32_t slot0(int32_t step) const {
+        const int32_t j = j0 + step;
+        return (j < ns ? j : first + j - ns) * kStep;
+    }
+    __device__ __forceinline__ int32_t loads() const { return hi ? steps : 0; }  // (rows that see nothing have a step)
+};
+static_assert(sizeof(Seg8) == 64, "list entries");
+
+// What a stage's step needs beside its codes: its first slot, 1 where a row does
+// not see all of it; the exponents of both blocks (key's, value's).
+struct Note {
+    uint32_t k, ex;
+};
+
+// 16-byte piece of a row in a tile of codes, rows of D bytes, as the TMA's swizzle
+// lays them, so that the eight rows of an ldmatrix lie in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t swz8(uint32_t row, uint32_t piece) {
+    return D == 128 ? row * 128 + (((piece ^ row) & 7u) << 4) : row * 64 + (((piece ^ (row >> 1)) & 3u) << 4);
+}
+// Pairs of the four codes of v to float16, exactly: a code + 128 in the low byte of
+// 1024 reads 1024 + 128 + code. `v` with the codes' highest bits turned.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t v, uint32_t select) {
+    uint32_t r;
+    asm("{.reg .b32 t;\n\tprmt.b32 t, %1, %2, %3;\n\tsub.rn.f16x2 %0, t, %4;}"
+        : "=r"(r) : "r"(v), "r"(0x64646464u), "r"(select), "r"(0x64806480u));
+    return r;
+}
+constexpr uint32_t kCodes01 = 0x4140, kCodes23 = 0x4342, kCodes02 = 0x4240, kCodes13 = 0x4341;
+
+// The rows of a warp. Lane (g, t) = (lane / 4, lane % 4) holds the rows 2 t and
+// 2 t + 1 of each tile for the slots g and g + 8 of a block, and for the elements 16 n
+// + 2 g and + 1 of all n.
+template <class T, int D, int NT>
+struct Rows8 {
+    static constexpr int KS = D / 16;
+    uint2 q[NT][KS];     // row g: elements 4 t .. 4 t + 3 of each 16, as the codes come
+    float cq[NT][2];     // scale * log2 e and the rows' own powers of two
+    float o[NT][KS][4];  // in units of 2^(most - kChunkShift)
+    float m[NT][2], l[NT][2];  // l: of this lane's slots
+    int32_t pos[NT][2];  // slot of the rows' tokens (-1: no row)
+    int32_t most;
+
+    __device__ __forceinline__ void queries(const AttnParams& p, const Seg8& x, uint32_t lane) {
+        const int32_t g = int32_t(p.g);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int32_t r = int32_t(lane >> 2) + 8 * i;
+            const bool on = r < x.rows;
+            const uint16_t* at = p.q + int64_t(x.q0 + (on ? r / g : 0)) * p.q_ts +
+                                 int64_t(x.h * g + (on ? r % g : 0)) * p.q_hs + (lane & 3u) * 4;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+                q[i][k] = on ? *reinterpret_cast<const uint2*>(at + k * 16) : make_uint2(0u, 0u);
+        }
+    }
+    __device__ __forceinline__ void begin(const AttnParams& p, const Seg8& x, uint32_t lane) {
+        const int32_t g = int32_t(p.g), t = int32_t(lane & 3u);
+        most = -126;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            float c = p.c;
+            if constexpr (std::is_same_v<T, BF16>) {
+                uint32_t top = 0;  // bits of the largest |q| of the row
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+                    top = max(max(top, max(q[i][k].x & 0x7fffu, (q[i][k].x >> 16) & 0x7fffu)),
+                              max(q[i][k].y & 0x7fffu, (q[i][k].y >> 16) & 0x7fffu));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // to [2^14, 2^15); infinities and NaN stay what they are
+                const int32_t e = top >= 0x7f80u ? 0 : max(int32_t(top >> 7) - 127 - 14, -112);
+                const float f = two_to(-e);
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    float a, b;
+                    BF16::unpack(q[i][k].x, a, b);
+                    q[i][k].x = F16::pack(a * f, b * f);
+                    BF16::unpack(q[i][k].y, a, b);
+                    q[i][k].y = F16::pack(a * f, b * f);
+                }
+                c *= two_to(e);
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int32_t row = 8 * i + 2 * t + y;
+                cq[i][y] = __shfl_sync(0xffffffffu, c, (2 * t + y) * 4);
+                pos[i][y] = row < x.rows ? max(x.f + row / g, -1) : -1;
+                m[i][y] = -INFINITY, l[i][y] = 0.f;
+            }
+#pragma unroll
+            for (int n = 0; n < KS; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+        }
+    }
+    // 32 slots, codes of their keys and values at ks and vs
+    __device__ __forceinline__ void step(const AttnParams& p, uint32_t ks, uint32_t vs, Note note, uint32_t lane) {
+        const int32_t k0 = int32_t(note.k & ~1u);
+        float s[2][NT][4] = {};
+#pragma unroll
+        for (int k = 0; k < KS; k += 2)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                uint32_t v[4];  // slots 0-7 and 8-15 (v[2], v[3]) of two 16-byte pieces
+                ldsm4(v, ks + z * (kBlock * D) + swz8<D>((lane & 7u) + ((lane >> 4) << 3), k + ((lane >> 3) & 1u)));
+#pragma unroll
+                for (int y = 0; y < 4; ++y) v[y] ^= 0x80808080u;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const uint32_t a[4] = {codes_f16(v[y], kCodes01), codes_f16(v[2 + y], kCodes01),
+                                           codes_f16(v[y], kCodes23), codes_f16(v[2 + y], kCodes23)};
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) F16::mma(s[z][i], a, q[i][k + y].x, q[i][k + y].y);
+                }
+            }
+        int32_t ev[2];
+        float fk[2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const int32_t ek = int8_t(note.ex >> (16 * z));
+            ev[z] = int8_t(note.ex >> (16 * z + 8));
+            fk[z] = ek == kNoExponent ? NAN : two_to(max(ek, -126));
+        }
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[z][i][e] *= cq[i][e & 1] * fk[z];
+        if (note.k & 1u) {
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!sees(p, pos[i][e & 1], k0 + z * kBlock + int32_t(lane >> 2) + 8 * (e >> 1)))
+                            s[z][i][e] = -INFINITY;
+        }
+        bool raise = false;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const float top = fmaxf(fmaxf(s[0][i][y], s[0][i][2 + y]), fmaxf(s[1][i][y], s[1][i][2 + y]));
+                raise = raise | (top > m[i][y] + F16::kRaise);
+            }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    float top = fmaxf(fmaxf(s[0][i][y], s[0][i][2 + y]), fmaxf(s[1][i][y], s[1][i][2 + y]));
+                    top = fmaxf(m[i][y], top);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    const float f = top == -INFINITY ? 1.f : ex2(m[i][y] - top);
+                    m[i][y] = top;
+                    l[i][y] *= f;
+#pragma unroll
+                    for (int n = 0; n < KS; ++n) o[i][n][y] *= f, o[i][n][2 + y] *= f;
+                }
+        }
+        if (max(ev[0], ev[1]) > most) {
+            const int32_t top = max(ev[0], ev[1]);
+            const float f = two_to(max(most - top, -126));
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int n = 0; n < KS; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][n][e] *= f;
+            most = top;
+        }
+        uint32_t b[2][NT][2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const float pw = ev[z] == kNoExponent ? NAN : two_to(max(ev[z] - most + int(F16::kChunkShift), -126));
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                float a[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    a[e] = ex2(s[z][i][e] - (m[i][e & 1] == -INFINITY ? 0.f : m[i][e & 1]));
+                    l[i][e & 1] += a[e];
+                    a[e] *= pw;
+                }
+#pragma unroll
+                for (int y = 0; y < 2; ++y)  // slots by rows, to rows by slots
+                    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;"
+                                 : "=r"(b[z][i][y]) : "r"(F16::pack(a[2 * y], a[2 * y + 1])));
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < KS; n += 2)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                // of two 16-byte pieces, slots 0-7 and 8-15 each; a register holds elements 2 g, 2 g + 1
+                uint32_t v[4];
+                ldsm4t(v, vs + z * (kBlock * D) + swz8<D>((lane & 7u) + (((lane >> 3) & 1u) << 3), n + (lane >> 4)));
+#pragma unroll
+                for (int y = 0; y < 4; ++y) v[y] ^= 0x80808080u;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const uint32_t a[4] = {codes_f16(v[2 * y], kCodes02), codes_f16(v[2 * y], kCodes13),
+                                           codes_f16(v[2 * y + 1], kCodes02), codes_f16(v[2 * y + 1], kCodes13)};
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) F16::mma(o[i][n + y], a, b[z][i][0], b[z][i][1]);
+                }
+            }
+    }
+    // Maxima and sums of the rows to sm, sl [8 NT].
+    __device__ __forceinline__ void stats(float* sm, float* sl, uint32_t lane) const {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                float sum = l[i][y];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const uint32_t row = 8 * i + 2 * lane + y;
+                if (lane < 4) sm[row] = m[i][y], sl[row] = sum;
+            }
+    }
+    // The sums times 2^(own maximum - top(row)) to row at0 + row of `join`, or added there.
+    template <class F>
+    __device__ __forceinline__ void sums(float* join, uint32_t at0, int32_t R, bool add, F top, uint32_t lane) const {
+        const float unit = two_to(max(most - int(F16::kChunkShift), -126));
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const uint32_t row = 8 * i + 2 * (lane & 3u) + y, at = at0 + row;
+                if (int32_t(row) >= R) continue;
+                const float mx = top(row);
+                const float f = mx == -INFINITY ? 0.f : ex2(m[i][y] - mx) * unit;
+                float* to = join + at * D;
+#pragma unroll
+                for (int n = 0; n < KS; ++n) {
+                    float2* cell = reinterpret_cast<float2*>(to + ((n * 16 + (lane >> 2) * 2) ^ (at & 7u) * 8));
+                    float2 v = make_float2(o[i][n][y] * f, o[i][n][2 + y] * f);
+                    if (add) v.x += cell->x, v.y += cell->y;
+                    *cell = v;
+                }
+            }
+    }
+};
+
+// Sums of (x, y) over the block, and over the threads before this one.
+struct Pair8 {
+    int64_t x;
+    int32_t y;
+};
+template <int WARPS>
+__device__ __forceinline__ Pair8 block_scan8(Pair8 v, Pair8* sh, Pair8& before) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Pair8 inc = v;
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, inc.x, o);
+        const int32_t y = __shfl_up_sync(0xffffffffu, inc.y, o);
+        if (int(lane) >= o) inc.x += x, inc.y += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh[warp] = inc;
+    __syncthreads();
+    Pair8 total{0, 0};
+    before = Pair8{inc.x - v.x, inc.y - v.y};
+    for (uint32_t w = 0; w < WARPS; ++w) {
+        if (w < warp) before.x += sh[w].x, before.y += sh[w].y;
+        total.x += sh[w].x, total.y += sh[w].y;
+    }
+    return total;
+}
+
+template <class T, int D, int NT>
+__global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
+    attn_decode8_kernel(const AttnParams p, const __grid_constant__ CUtensorMap kmap,
+                        const __grid_constant__ CUtensorMap vmap) {
+    using G = Geo8<D, NT>;
+    constexpr int W = G::kWarps, MR = G::kRows;
+    extern __shared__ uint8_t raw[];
+    const uint32_t sbase = (smem_u32(raw) + 1023u) & ~1023u;
+    uint8_t* const smem = raw + (sbase - smem_u32(raw));
+    Seg8* const segs = reinterpret_cast<Seg8*>(smem + G::kSegs);
+    Note* const notes = reinterpret_cast<Note*>(smem + G::kNotes);
+    float* const join = reinterpret_cast<float*>(smem + G::kJoin);
+    Pair8* const scan = reinterpret_cast<Pair8*>(smem + G::kScan);
+    volatile uint32_t* const flag = reinterpret_cast<uint32_t*>(scan + W + 1);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int32_t g = int32_t(p.g);
+    auto full = [&](uint32_t s) { return sbase + G::kBars + 8 * s; };
+    auto empty = [&](uint32_t s) { return sbase + G::kBars + 8 * (G::kStages + s); };
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        return p.timeout_ns < kShortNs ? warp_wait_short(bar, parity, uint32_t(p.timeout_ns))
+                                       : warp_wait(bar, parity, p.timeout_ns);
+    };
+
+    if (warp == W) {
+        for (uint32_t i = lane; i < 2u * G::kStages; i += 32) bar_init(full(i), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (lane < 2) prefetch_map(lane ? &vmap : &kmap);
+    }
+    after_start();
+    after_wait();
+    // units of this thread's sequence (of the first kThreads), and of the call; y: 1
+    // where the sequence has rows
+    auto units_of = [&](uint32_t b, SeqRange& s) -> Pair8 {
+        s = SeqRange{0, 0, 0, 0};
+        if (b < p.B) s = load_seq(p, b);
+        if (!s.nq) return Pair8{0, 0};
+        return Pair8{(key_range<kStep>(p, s, 0, s.nq).tiles + kItemCost8) * p.Hkv, 1};
+    };
+    SeqRange seq0;
+    const Pair8 v0 = units_of(tid, seq0);
+    Pair8 before0;
+    const Pair8 total0 = block_scan8<W + 1>(v0, scan, before0);
+    int64_t U = total0.x;
+    for (uint32_t b0 = G::kThreads; b0 < p.B; b0 += G::kThreads) {
+        SeqRange s;
+        Pair8 before;
+        U += block_scan8<W + 1>(units_of(b0 + tid, s), scan, before).x;
+    }
+    if (!U) return;
+    const int64_t NC = max(int64_t(1), min(int64_t(gridDim.x), (U + kMinUnits8 - 1) / kMinUnits8));
+    if (int64_t(blockIdx.x) >= NC) return;
+    const int64_t cta = blockIdx.x, u_begin = cut_begin(U, NC, cta), u_end = cut_begin(U, NC, cta + 1);
+    // after a wait that gave up the warp loads and computes no more, and only meets
+    // the others
+    bool ok = true;
+    uint32_t done = 0;                      // steps of the pieces so far
+    uint32_t turn = warp, t_stage = warp, t_round = 0;  // this warp's next step, its stage and its round
+    uint32_t loaded = 0, loaded_to = 0;     // steps loaded
+    static_assert(G::kStages % W == 0, "a stage is always the same warp's");
+    Rows8<T, D, NT> rows;
+
+    for (int64_t u = u_begin; u < u_end;) {
+        // the next pieces, listed by the threads of their sequences: items (y
+        // counts sequences with rows) from the one that holds unit u
+        if (tid == 0) flag[0] = flag[1] = 0;
+        __syncthreads();
+        int64_t base = 0;
+        int32_t seqs = 0;
+        for (uint32_t b0 = 0; b0 < p.B && base < u_end; b0 += G::kThreads) {
+            SeqRange s = seq0;
+            Pair8 v = v0, before = before0, total = total0;
+            if (b0) {
+                v = units_of(b0 + tid, s);
+                total = block_scan8<W + 1>(v, scan, before);
+            }
+            const int64_t at = base + before.x, item_units = v.y ? v.x / p.Hkv : 1;
+            const int32_t seq = seqs + before.y;
+            if (v.y && u >= at && u < at + v.x)
+                flag[1] = uint32_t(seq * int32_t(p.Hkv) + int32_t((u - at) / item_units));
+            __syncthreads();
+            const int64_t from = max(u, at), to = min(u_end, at + v.x);
+            if (from < to) {
+                const KeyRange kr = key_range<kStep>(p, s, 0, s.nq);
+                int32_t h = int32_t((from - at) / item_units);
+                int32_t idx = seq * int32_t(p.Hkv) + h - int32_t(flag[1]);
+                for (; h < int32_t(p.Hkv) && idx < kSegCount; ++h, ++idx) {
+                    Seg8 x;
+                    x.item = at + h * item_units + kItemCost8;
+                    const int64_t a = max(x.item, u), e = min(x.item + kr.tiles, u_end);
+                    if (a >= e) break;  // only the item's cost lies in the range
+                    x.b = int32_t(b0 + tid), x.h = h, x.q0 = s.q0, x.rows = s.nq * g;
+                    x.f = s.f, x.hi = kr.hi, x.lo = kr.lo, x.sink = kr.sink, x.ns = kr.ns, x.first = kr.first;
+                    x.tiles = kr.tiles;
+                    x.j0 = int32_t(a - x.item), x.steps = int32_t(e - a);
+                    x.own = a != u_begin;
+                    segs[idx] = x;
+                    atomicMax(const_cast<uint32_t*>(flag), uint32_t(idx + 1));
+                }
+            }
+            base += total.x;
+            seqs += total.y;
+        }
+        __syncthreads();
+        const uint32_t count = flag[0];
+        if (!count) break;  // what is left of the range is the cost of an item
+
+        if (warp == W) {
+            // ---- loads: blocks of steps of a piece, a lane and a stage each; the pages of
+            // the block after it are under way
+            constexpr int32_t kBlockSteps = G::kStages < 32 ? G::kStages : 32;
+            const bool pairs = p.P >= uint32_t(kStep);  // a step lies in one page
+            auto seen = [&](const Seg8& x, int32_t k) { return (k < x.hi && k + kBlock > x.lo) || k < x.sink; };
+            // pages of both blocks of a step (-1: no row sees the block)
+            auto pages_of = [&](uint32_t c, int32_t step) -> int2 {
+                int2 id = make_int2(-1, -1);
+                if (c >= count) return id;
+                const Seg8& x = segs[c];
+                if (step >= x.loads()) return id;
+                const int32_t k = x.slot0(step);
+                const int32_t* row = p.table + int64_t(x.b) * p.table_s;
+                auto page = [&](int32_t slot) {
+                    const int32_t at = row[slot >> p.pshift];
+                    if (uint32_t(at) < p.pages) return at;
+                    if (p.err) atomicOr(p.err, kErrPage);
+                    return int32_t(p.pages);
+                };
+                if (seen(x, k)) id.x = page(k);
+                if (seen(x, k + kBlock)) id.y = pairs && id.x >= 0 ? id.x : page(k + kBlock);
+                return id;
+            };
+            auto exponents_of = [&](uint32_t c, int32_t step, int2 id) -> uint32_t {
+                uint32_t ex = 0;
+                if (c >= count) return ex;
+                const Seg8& x = segs[c];
+                const int32_t in = step < x.loads() ? x.slot0(step) & int32_t(p.P - 1) : 0;
+                const uint8_t* at = p.ex + int64_t(x.h) * p.ex_hs;
+                if (uint32_t(id.x) < p.pages)
+                    ex = *reinterpret_cast<const uint16_t*>(at + int64_t(id.x) * p.ex_ps + (in >> 3));
+                if (uint32_t(id.y) < p.pages)
+                    ex |= uint32_t(*reinterpret_cast<const uint16_t*>(at + int64_t(id.y) * p.ex_ps +
+                                                                      (((in + kBlock) & int32_t(p.P - 1)) >> 3)))
+                          << 16;
+                return ex;
+            };
+            uint32_t c = 0, n_c = 0;
+            int32_t at = 0, n_at = 0;
+            auto after = [&]() {
+                n_at += kBlockSteps;
+                if (n_c < count && n_at >= segs[n_c].loads()) ++n_c, n_at = 0;
+            };
+            int2 id = pages_of(0, int32_t(lane)), n_id;
+            uint32_t ex = exponents_of(0, int32_t(lane), id), n_ex = 0;
+            after();
+            n_id = pages_of(n_c, n_at + int32_t(lane));
+            while (ok && c < count) {
+                const Seg8& x = segs[c];
+                const int32_t n = min(kBlockSteps, x.loads() - at), h = x.h;
+                const bool mine = int32_t(lane) < n;
+                const int32_t k = mine ? x.slot0(at + int32_t(lane)) : 0, in = k & int32_t(p.P - 1);
+                const bool masked = k + kStep - 1 > x.f ||
+                                    (p.window && int64_t(k) <= int64_t(x.hi) - 1 - int64_t(p.window));
+                const uint32_t boxes = pairs ? 2u : 2u * uint32_t((id.x >= 0) + (id.y >= 0));
+                const uint32_t st = (loaded + lane) % G::kStages, round = (loaded + lane) / G::kStages;
+                const uint32_t dst = sbase + st * G::kStage, bar = full(st);
+                // Lanes load when their stage is free, some at a time (of the first block
+                // all, so that its loads are under way when the exponents are waited for).
+                for (int32_t i0 = 0, size = loaded ? kLoadLanes : 32; ok && i0 < n; i0 += size) {
+                    const bool turn_of = mine && uint32_t(int32_t(lane) - i0) < uint32_t(size);
+                    bool left = turn_of;
+                    const uint64_t begin = now();
+                    for (uint32_t spin = 1;; ++spin) {
+                        if (left && (!round || bar_test(empty(st), (round - 1) & 1u))) {
+                            if (pairs) {
+                                tma4(dst, &kmap, bar, 0, in, h, max(id.x, id.y));
+                                tma4(dst + G::kHalf, &vmap, bar, 0, in, h, max(id.x, id.y));
+                            } else {
+                                if (id.x >= 0) {
+                                    tma4(dst, &kmap, bar, 0, in, h, id.x);
+                                    tma4(dst + G::kHalf, &vmap, bar, 0, in, h, id.x);
+                                }
+                                if (id.y >= 0) {
+                                    tma4(dst + kBlock * D, &kmap, bar, 0, 0, h, id.y);
+                                    tma4(dst + G::kHalf + kBlock * D, &vmap, bar, 0, 0, h, id.y);
+                                }
+                            }
+                            notes[st] = Note{uint32_t(k) | uint32_t(masked), ex};
+                            bar_arrive_tx(bar, boxes * (pairs ? G::kHalf : G::kHalf / 2));
+                            left = false;
+                        }
+                        if (!__any_sync(0xffffffffu, left)) break;
+                        if (spin % 64 == 0 && __any_sync(0xffffffffu, now() - begin > p.timeout_ns)) {
+                            ok = false;  // (what this group has loaded lands before the CTA ends)
+                            if (turn_of && !left) bar_wait(bar, round & 1u, kGraceNs);
+                            break;
+                        }
+                    }
+                    __syncwarp();
+                    if (i0 == 0) n_ex = exponents_of(n_c, n_at + int32_t(lane), n_id);
+                    if (ok) loaded_to = loaded + uint32_t(min(n, i0 + size));
+                }
+                if (n <= 0) n_ex = exponents_of(n_c, n_at + int32_t(lane), n_id);
+                loaded = loaded_to;
+                c = n_c, at = n_at, id = n_id, ex = n_ex;
+                after();
+                n_id = pages_of(n_c, n_at + int32_t(lane));
+            }
+        } else {
+            // ---- rows
+            float* const sm = reinterpret_cast<float*>(smem + G::kStat);  // [W][MR]
+            float* const sl = sm + W * MR;
+            auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory"); };
+            auto top = [&](uint32_t row) {
+                float mx = sm[row];
+#pragma unroll
+                for (int w = 1; w < W; ++w) mx = fmaxf(mx, sm[w * MR + row]);
+                return mx;
+            };
+            rows.queries(p, segs[0], lane);
+            for (uint32_t c = 0; c < count; ++c) {
+                const Seg8& x = segs[c];
+                const int32_t R = x.rows, h = x.h;
+                const uint32_t n = uint32_t(x.loads());
+                rows.begin(p, x, lane);
+                while (ok && turn - done < n) {
+                    if (!(ok = wait(full(t_stage), t_round & 1u))) break;
+                    const uint32_t ks = sbase + t_stage * G::kStage;
+                    rows.step(p, ks, ks + G::kHalf, notes[t_stage], lane);
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(empty(t_stage));
+                    turn += W;
+                    t_stage += W;
+                    if (t_stage >= uint32_t(G::kStages)) t_stage -= G::kStages, ++t_round;
+                }
+                done += n;
+                // the warps' sums meet: maxima first, then the rows, half of the warps at a time
+                rows.stats(sm + warp * MR, sl + warp * MR, lane);
+                meet();
+                if (warp < G::kSide) rows.sums(join, warp * uint32_t(R), R, false, top, lane);
+                meet();
+                if (warp >= G::kSide) rows.sums(join, (warp - G::kSide) * uint32_t(R), R, true, top, lane);
+                if (c + 1 < count) rows.queries(p, segs[c + 1], lane);
+                meet();
+                // rows by warps, D / 32 elements of a row per lane
+                constexpr int E = D / 32;
+                const bool whole = x.j0 == 0 && x.steps == x.tiles;
+                constexpr int64_t kPart = MR * (D + 2);
+                float* const slot = p.part + (2 * cta + x.own) * kPart;
+                auto finish = [&](int32_t row, const float (&v)[E], float mx, float sum) {
+                    const int32_t token = x.q0 + row / g;
+                    const int64_t head = h * g + row % g;
+                    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+                    uint16_t* out = p.out + int64_t(token) * p.o_ts + head * p.o_hs + lane * E;
+                    if constexpr (E == 4)
+                        *reinterpret_cast<uint2*>(out) =
+                            make_uint2(T::pack(v[0] * inv, v[1] * inv), T::pack(v[2] * inv, v[3] * inv));
+                    else
+                        *reinterpret_cast<uint32_t*>(out) = T::pack(v[0] * inv, v[1] * inv);
+                    if (lane == 0 && p.lse)
+                        p.lse[int64_t(token) * p.Hq + head] = sum == 0.f ? -INFINITY : (mx + lg2(sum)) * kLn2;
+                };
+                for (int32_t row = int32_t(warp); row < R; row += W) {
+                    const float mx = top(uint32_t(row));
+                    float sum = 0.f, v[E];
+#pragma unroll
+                    for (int w = 0; w < W; ++w)
+                        sum = fmaf(mx == -INFINITY ? 0.f : ex2(sm[w * MR + row] - mx), sl[w * MR + row], sum);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll
+                    for (uint32_t w = 0; w < uint32_t(G::kSide); ++w) {
+                        const uint32_t at = w * uint32_t(R) + uint32_t(row);
+                        const float* from = join + at * D + ((lane * E) ^ (at & 7u) * 8);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[e] += from[e];
+                    }
+                    if (whole) {
+                        finish(row, v, mx, sum);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) slot[row * D + lane * E + e] = v[e];
+                        if (lane == 0) slot[MR * D + row] = mx, slot[MR * D + MR + row] = sum;
+                    }
+                }
+                if (!whole) {
+                    const int64_t c0 = cut_owner(U, NC, x.item), c1 = cut_owner(U, NC, x.item + x.tiles - 1);
+                    __threadfence();
+                    meet();
+                    if (tid == 0) {
+                        const bool last = atomicAdd(p.count + c0, 1u) == uint32_t(c1 - c0);
+                        if (last) p.count[c0] = 0;
+                        flag[2] = last;
+                    }
+                    meet();
+                    if (flag[2]) {
+                        __threadfence();
+                        const int32_t pieces = int32_t(c1 - c0) + 1;
+                        const float* const p0 = p.part + (2 * c0 + (cut_begin(U, NC, c0) != x.item)) * kPart;
+                        auto piece = [&](int32_t i) { return i ? p.part + 2 * (c0 + i) * kPart : p0; };
+                        for (int32_t row = int32_t(warp); row < R; row += W) {
+                            float mx = -INFINITY, sum = 0.f, v[E] = {};
+                            for (int32_t i0 = 0; i0 < pieces; i0 += 32) {
+                                const int32_t i = i0 + int32_t(lane), n = min(32, pieces - i0);
+                                const float pm = i < pieces ? __ldcg(piece(i) + MR * D + row) : -INFINITY;
+                                const float ps = i < pieces ? __ldcg(piece(i) + MR * D + MR + row) : 0.f;
+                                float f = 0.f;
+                                for (int32_t k0 = 0; k0 < n; k0 += 16) {
+                                    float y[16][E];
+#pragma unroll
+                                    for (int k = 0; k < 16; ++k) {
+                                        const float* from = piece(min(i0 + k0 + k, pieces - 1)) + row * D + lane * E;
+                                        using Vec = std::conditional_t<E == 4, float4, float2>;
+                                        *reinterpret_cast<Vec*>(y[k]) = __ldcg(reinterpret_cast<const Vec*>(from));
+                                    }
+                                    if (!k0) {  // the maximum may grow with each 32 pieces
+                                        float nm = pm;
+#pragma unroll
+                                        for (int d = 16; d; d >>= 1)
+                                            nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, d));
+                                        nm = fmaxf(nm, mx);
+                                        const float ref = nm == -INFINITY ? 0.f : nm, old = ex2(mx - ref);
+                                        f = ex2(pm - ref);
+                                        sum = fmaf(f, ps, sum * old);
+#pragma unroll
+                                        for (int e = 0; e < E; ++e) v[e] *= old;
+                                        mx = nm;
+                                    }
+#pragma unroll
+                                    for (int k = 0; k < 16; ++k) {
+                                        const float fk = __shfl_sync(0xffffffffu, f, (k0 + k) & 31);
+                                        if (k0 + k < n)
+#pragma unroll
+                                            for (int e = 0; e < E; ++e) v[e] = fmaf(fk, y[k][e], v[e]);
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                            finish(row, v, mx, sum);
+                        }
+                    }
+                }
+                meet();  // the joined sums and maxima have been read
+            }
+        }
+        __syncthreads();  // the list has been read
+        u = segs[count - 1].item + segs[count - 1].j0 + segs[count - 1].steps;
+    }
+    if (warp == W)  // every load has landed before the CTA ends
+        for (uint32_t i = loaded - min(loaded, uint32_t(G::kStages)); i != loaded; ++i)
+            warp_wait(full(i % G::kStages), (i / G::kStages) & 1u, kGraceNs);
+    if (!ok) gave_up(p);
+}
+
+template <class T, int D, int NT>
+int launch8(const AttnParams& p, cudaStream_t s) {
+    using G = Geo8<D, NT>;
+    CUtensorMap km, vm;
+    const uint32_t slots = p.P < uint32_t(kStep) ? p.P : uint32_t(kStep);
+    if (!encode_codes(&km, p.k_pages, p, p.kp_ss, p.kp_hs, p.kp_ps, slots) ||
+        !encode_codes(&vm, p.v_pages, p, p.vp_ss, p.vp_hs, p.vp_ps, slots))
+        return EINVAL;
+    const auto kernel = attn_decode8_kernel<T, D, NT>;
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return int(e);
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(G::kSmem));
+        if (e != cudaSuccess) return int(e);
+        done.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    const uint32_t sms = sm_count(), most = kMaxCtas * 16 / G::kRows;  // (by the scratch)
+    // (the append before it lets it begin early)
+    return int(launch_after(kernel, sms < most ? sms : most, G::kThreads, G::kSmem, s, p, km, vm));
+}
+template <class T, int D>
+int launch8(const AttnParams& p, cudaStream_t s) {
+    return p.rows <= 8 ? launch8<T, D, 1>(p, s) : p.rows <= 16 ? launch8<T, D, 2>(p, s) : launch8<T, D, 3>(p, s);
+}
+
+}  // namespace
+
+int launch_decode8(const AttnParams& p, uint32_t dtype, cudaStream_t s) {
+    if (p.D == 64) return dtype == LS_B200_BF16 ? launch8<BF16, 64>(p, s) : launch8<F16, 64>(p, s);
+    return dtype == LS_B200_BF16 ? launch8<BF16, 128>(p, s) : launch8<F16, 128>(p, s);
+}
+
+}  // namespace lsb

@@ -72,7 +72,17 @@ template <bool kCall = true>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint64_t ns) {
     return __all_sync(0xffffffffu, bar_wait<kCall>(bar, parity, ns)) != 0;
 }
-// The same for a bound below a try's sleep: polls, and counts SM cycles, two per ns.
+// Whether phase `parity` has completed, without a wait.
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// warp_wait for a bound below a try's sleep: polls, and counts SM cycles, two per ns.
 static __device__ __noinline__ bool warp_wait_short(uint32_t bar, uint32_t parity, uint32_t ns) {
     const uint64_t begin = uint64_t(clock64());
     uint32_t ok;
@@ -212,6 +222,15 @@ __device__ __forceinline__ void st16(uint32_t taddr, const float* v) {
         "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]),
         "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
         : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 
 // Two fp32 values in one 64-bit register: the packed forms of sm_100.
