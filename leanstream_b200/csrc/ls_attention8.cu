@@ -4,9 +4,9 @@
 //
 // An item is a sequence and kv head; its rows are (token, head of the group). Its
 // slots go by in steps of 32 (two blocks); the steps of all items, in order, are
-// cut evenly over one CTA per SM. One warp of a CTA loads: it lays out up to 32
-// steps at a time, a lane each, and fills one ring of stages with what each step
-// needs (first slot, exponents, codes of keys and values). The other warps
+// cut evenly over one CTA per SM. Two warps of a CTA load, keys and values: they
+// lay out up to 32 steps at a time, a lane each, and fill one ring of stages with
+// what each step needs (first slot, exponents, codes). The other warps
 // take the steps in turn, with maxima and sums of their own, and meet at the end of
 // an item's piece; the loads run on into the next piece meanwhile. An item cut over
 // several CTAs is joined, in the order of its pieces, by the CTA that arrives last.
@@ -39,9 +39,8 @@ using namespace tc;
 
 constexpr int kStep = 2 * kBlock;          // slots of a step
 constexpr int kSegCount = 48;              // pieces listed at a time
-constexpr int64_t kItemCost8 = 8;          // steps that beginning and joining an item counts as
+constexpr int64_t kItemCost8 = 16;         // steps that beginning and joining an item counts as
 constexpr int64_t kMinUnits8 = 24;         // steps that a CTA takes at least
-constexpr int kLoadLanes = 8;              // steps that the loading warp waits for at a time
 constexpr uint64_t kGraceNs = 1000000000ull;
 constexpr uint64_t kShortNs = 100000;      // bounds that a barrier's try may sleep over: a load takes less
 
@@ -49,7 +48,7 @@ constexpr uint64_t kShortNs = 100000;      // bounds that a barrier's try may sl
 // shared memory that the warps' sums, half of them at a time, leave.
 template <int D, int NT>
 struct Geo8 {
-    static constexpr int kWarps = NT == 1 ? 11 : NT == 2 ? 10 : 7, kThreads = 32 * (kWarps + 1), kSide = (kWarps + 1) / 2;
+    static constexpr int kWarps = NT <= 2 ? 10 : 6, kThreads = 32 * (kWarps + 2), kSide = (kWarps + 1) / 2;
     static constexpr int kRows = 8 * NT;
     static constexpr uint32_t kHalf = kStep * D, kStage = 2 * kHalf;  // a step's keys, and its values
     // A stage is always the same warp's: then its next round cannot be taken for the
@@ -58,7 +57,7 @@ struct Geo8 {
     static constexpr uint32_t kJoin = kStages * kStage, kSegs = kJoin + kSide * kRows * D * 4;
     static constexpr uint32_t kNotes = kSegs + kSegCount * 64, kBars = kNotes + 8 * kStages;
     static constexpr uint32_t kStat = kBars + 16 * kStages, kScan = kStat + 8 * kWarps * kRows;
-    static constexpr uint32_t kSmem = kScan + 16 * (kWarps + 1) + 16 + 1024;  // + alignment of the swizzled tiles
+    static constexpr uint32_t kSmem = kScan + 16 * (kWarps + 2) + 16 + 1024;  // + alignment of the swizzled tiles
     static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -294,9 +293,11 @@ struct Rows8 {
                 if (lane < 4) sm[row] = m[i][y], sl[row] = sum;
             }
     }
-    // The sums times 2^(own maximum - top(row)) to row at0 + row of `join`, or added there.
+    // The sums times 2^(own maximum - top(row)) (`own`: as they are) to row at0 + row of
+    // `join`, or added there.
     template <class F>
-    __device__ __forceinline__ void sums(float* join, uint32_t at0, int32_t R, bool add, F top, uint32_t lane) const {
+    __device__ __forceinline__ void sums(float* join, uint32_t at0, int32_t R, bool own, bool add, F top,
+                                         uint32_t lane) const {
         const float unit = two_to(max(most - int(F16::kChunkShift), -126));
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -304,8 +305,8 @@ struct Rows8 {
             for (int y = 0; y < 2; ++y) {
                 const uint32_t row = 8 * i + 2 * (lane & 3u) + y, at = at0 + row;
                 if (int32_t(row) >= R) continue;
-                const float mx = top(row);
-                const float f = mx == -INFINITY ? 0.f : ex2(m[i][y] - mx) * unit;
+                const float mx = own ? m[i][y] : top(row);
+                const float f = mx == -INFINITY ? 0.f : own ? unit : ex2(m[i][y] - mx) * unit;
                 float* to = join + at * D;
 #pragma unroll
                 for (int n = 0; n < KS; ++n) {
@@ -345,6 +346,21 @@ __device__ __forceinline__ Pair8 block_scan8(Pair8 v, Pair8* sh, Pair8& before) 
     return total;
 }
 
+// A quotient of two counts, in 32 bits where they fit (nearly always).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return uint64_t(a | b) >> 32 ? a / b : int64_t(uint32_t(a) / uint32_t(b));
+}
+// U units cut over G CTAs: the first U % G take one more than the others.
+struct Cut {
+    int64_t each, more;
+    __device__ __forceinline__ Cut(int64_t U, int64_t G) : each(quotient(U, G)), more(U - each * G) {}
+    __device__ __forceinline__ int64_t begin(int64_t c) const { return c * each + min(c, more); }
+    __device__ __forceinline__ int64_t owner(int64_t u) const {
+        const int64_t head = more * (each + 1);
+        return u < head ? quotient(u, each + 1) : more + quotient(u - head, each);
+    }
+};
+
 template <class T, int D, int NT>
 __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
     attn_decode8_kernel(const AttnParams p, const __grid_constant__ CUtensorMap kmap,
@@ -358,7 +374,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
     Note* const notes = reinterpret_cast<Note*>(smem + G::kNotes);
     float* const join = reinterpret_cast<float*>(smem + G::kJoin);
     Pair8* const scan = reinterpret_cast<Pair8*>(smem + G::kScan);
-    volatile uint32_t* const flag = reinterpret_cast<uint32_t*>(scan + W + 1);
+    volatile uint32_t* const flag = reinterpret_cast<uint32_t*>(scan + W + 2);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t g = int32_t(p.g);
     auto full = [&](uint32_t s) { return sbase + G::kBars + 8 * s; };
@@ -369,7 +385,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
     };
 
     if (warp == W) {
-        for (uint32_t i = lane; i < 2u * G::kStages; i += 32) bar_init(full(i), 1);
+        for (uint32_t i = lane; i < 2u * G::kStages; i += 32) bar_init(full(i), i < uint32_t(G::kStages) ? 2 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (lane < 2) prefetch_map(lane ? &vmap : &kmap);
     }
@@ -386,23 +402,24 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
     SeqRange seq0;
     const Pair8 v0 = units_of(tid, seq0);
     Pair8 before0;
-    const Pair8 total0 = block_scan8<W + 1>(v0, scan, before0);
+    const Pair8 total0 = block_scan8<W + 2>(v0, scan, before0);
     int64_t U = total0.x;
     for (uint32_t b0 = G::kThreads; b0 < p.B; b0 += G::kThreads) {
         SeqRange s;
         Pair8 before;
-        U += block_scan8<W + 1>(units_of(b0 + tid, s), scan, before).x;
+        U += block_scan8<W + 2>(units_of(b0 + tid, s), scan, before).x;
     }
     if (!U) return;
-    const int64_t NC = max(int64_t(1), min(int64_t(gridDim.x), (U + kMinUnits8 - 1) / kMinUnits8));
+    const int64_t NC = max(int64_t(1), min(int64_t(gridDim.x), quotient(U + kMinUnits8 - 1, kMinUnits8)));
     if (int64_t(blockIdx.x) >= NC) return;
-    const int64_t cta = blockIdx.x, u_begin = cut_begin(U, NC, cta), u_end = cut_begin(U, NC, cta + 1);
+    const Cut cut(U, NC);
+    const int64_t cta = blockIdx.x, u_begin = cut.begin(cta), u_end = cut.begin(cta + 1);
     // after a wait that gave up the warp loads and computes no more, and only meets
     // the others
     bool ok = true;
     uint32_t done = 0;                      // steps of the pieces so far
     uint32_t turn = warp, t_stage = warp, t_round = 0;  // this warp's next step, its stage and its round
-    uint32_t loaded = 0, loaded_to = 0;     // steps loaded
+    uint32_t loaded = 0;                    // steps loaded
     static_assert(G::kStages % W == 0, "a stage is always the same warp's");
     Rows8<T, D, NT> rows;
 
@@ -418,17 +435,17 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             Pair8 v = v0, before = before0, total = total0;
             if (b0) {
                 v = units_of(b0 + tid, s);
-                total = block_scan8<W + 1>(v, scan, before);
+                total = block_scan8<W + 2>(v, scan, before);
             }
-            const int64_t at = base + before.x, item_units = v.y ? v.x / p.Hkv : 1;
+            const int64_t at = base + before.x, item_units = v.y ? quotient(v.x, p.Hkv) : 1;
             const int32_t seq = seqs + before.y;
             if (v.y && u >= at && u < at + v.x)
-                flag[1] = uint32_t(seq * int32_t(p.Hkv) + int32_t((u - at) / item_units));
+                flag[1] = uint32_t(seq * int32_t(p.Hkv) + int32_t(quotient(u - at, item_units)));
             __syncthreads();
             const int64_t from = max(u, at), to = min(u_end, at + v.x);
             if (from < to) {
                 const KeyRange kr = key_range<kStep>(p, s, 0, s.nq);
-                int32_t h = int32_t((from - at) / item_units);
+                int32_t h = int32_t(quotient(from - at, item_units));
                 int32_t idx = seq * int32_t(p.Hkv) + h - int32_t(flag[1]);
                 for (; h < int32_t(p.Hkv) && idx < kSegCount; ++h, ++idx) {
                     Seg8 x;
@@ -451,9 +468,11 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
         const uint32_t count = flag[0];
         if (!count) break;  // what is left of the range is the cost of an item
 
-        if (warp == W) {
+        if (warp >= W) {
             // ---- loads: blocks of steps of a piece, a lane and a stage each; the pages of
-            // the block after it are under way
+            // the block after it are under way. The warp of the keys also takes the exponents.
+            const bool keys = warp == W;
+            const CUtensorMap* const map = keys ? &kmap : &vmap;
             constexpr int32_t kBlockSteps = G::kStages < 32 ? G::kStages : 32;
             const bool pairs = p.P >= uint32_t(kStep);  // a step lies in one page
             auto seen = [&](const Seg8& x, int32_t k) { return (k < x.hi && k + kBlock > x.lo) || k < x.sink; };
@@ -468,7 +487,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 auto page = [&](int32_t slot) {
                     const int32_t at = row[slot >> p.pshift];
                     if (uint32_t(at) < p.pages) return at;
-                    if (p.err) atomicOr(p.err, kErrPage);
+                    if (keys && p.err) atomicOr(p.err, kErrPage);
                     return int32_t(p.pages);
                 };
                 if (seen(x, k)) id.x = page(k);
@@ -477,7 +496,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             };
             auto exponents_of = [&](uint32_t c, int32_t step, int2 id) -> uint32_t {
                 uint32_t ex = 0;
-                if (c >= count) return ex;
+                if (!keys || c >= count) return ex;
                 const Seg8& x = segs[c];
                 const int32_t in = step < x.loads() ? x.slot0(step) & int32_t(p.P - 1) : 0;
                 const uint8_t* at = p.ex + int64_t(x.h) * p.ex_hs;
@@ -506,47 +525,34 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 const int32_t k = mine ? x.slot0(at + int32_t(lane)) : 0, in = k & int32_t(p.P - 1);
                 const bool masked = k + kStep - 1 > x.f ||
                                     (p.window && int64_t(k) <= int64_t(x.hi) - 1 - int64_t(p.window));
-                const uint32_t boxes = pairs ? 2u : 2u * uint32_t((id.x >= 0) + (id.y >= 0));
+                const uint32_t bytes = pairs ? G::kHalf : uint32_t((id.x >= 0) + (id.y >= 0)) * (G::kHalf / 2);
                 const uint32_t st = (loaded + lane) % G::kStages, round = (loaded + lane) / G::kStages;
-                const uint32_t dst = sbase + st * G::kStage, bar = full(st);
-                // Lanes load when their stage is free, some at a time (of the first block
-                // all, so that its loads are under way when the exponents are waited for).
-                for (int32_t i0 = 0, size = loaded ? kLoadLanes : 32; ok && i0 < n; i0 += size) {
-                    const bool turn_of = mine && uint32_t(int32_t(lane) - i0) < uint32_t(size);
-                    bool left = turn_of;
-                    const uint64_t begin = now();
-                    for (uint32_t spin = 1;; ++spin) {
-                        if (left && (!round || bar_test(empty(st), (round - 1) & 1u))) {
-                            if (pairs) {
-                                tma4(dst, &kmap, bar, 0, in, h, max(id.x, id.y));
-                                tma4(dst + G::kHalf, &vmap, bar, 0, in, h, max(id.x, id.y));
-                            } else {
-                                if (id.x >= 0) {
-                                    tma4(dst, &kmap, bar, 0, in, h, id.x);
-                                    tma4(dst + G::kHalf, &vmap, bar, 0, in, h, id.x);
-                                }
-                                if (id.y >= 0) {
-                                    tma4(dst + kBlock * D, &kmap, bar, 0, 0, h, id.y);
-                                    tma4(dst + G::kHalf + kBlock * D, &vmap, bar, 0, 0, h, id.y);
-                                }
-                            }
-                            notes[st] = Note{uint32_t(k) | uint32_t(masked), ex};
-                            bar_arrive_tx(bar, boxes * (pairs ? G::kHalf : G::kHalf / 2));
-                            left = false;
+                const uint32_t dst = sbase + st * G::kStage + (keys ? 0 : G::kHalf), bar = full(st);
+                // each lane loads when its stage is free
+                bool left = mine;
+                const uint64_t begin = now();
+                for (uint32_t spin = 1;; ++spin) {
+                    if (left && (!round || bar_test(empty(st), (round - 1) & 1u))) {
+                        if (pairs) {
+                            tma4(dst, map, bar, 0, in, h, max(id.x, id.y));
+                        } else {
+                            if (id.x >= 0) tma4(dst, map, bar, 0, in, h, id.x);
+                            if (id.y >= 0) tma4(dst + kBlock * D, map, bar, 0, 0, h, id.y);
                         }
-                        if (!__any_sync(0xffffffffu, left)) break;
-                        if (spin % 64 == 0 && __any_sync(0xffffffffu, now() - begin > p.timeout_ns)) {
-                            ok = false;  // (what this group has loaded lands before the CTA ends)
-                            if (turn_of && !left) bar_wait(bar, round & 1u, kGraceNs);
-                            break;
-                        }
+                        if (keys) notes[st] = Note{uint32_t(k) | uint32_t(masked), ex};
+                        bar_arrive_tx(bar, bytes);
+                        left = false;
                     }
-                    __syncwarp();
-                    if (i0 == 0) n_ex = exponents_of(n_c, n_at + int32_t(lane), n_id);
-                    if (ok) loaded_to = loaded + uint32_t(min(n, i0 + size));
+                    if (!__any_sync(0xffffffffu, left)) break;
+                    if (spin % 64 == 0 && __any_sync(0xffffffffu, now() - begin > p.timeout_ns)) {
+                        ok = false;  // (what this block has loaded lands before the CTA ends)
+                        if (mine && !left) bar_wait(bar, round & 1u, kGraceNs);
+                        break;
+                    }
                 }
-                if (n <= 0) n_ex = exponents_of(n_c, n_at + int32_t(lane), n_id);
-                loaded = loaded_to;
+                __syncwarp();
+                n_ex = exponents_of(n_c, n_at + int32_t(lane), n_id);
+                if (ok) loaded += uint32_t(max(n, 0));
                 c = n_c, at = n_at, id = n_id, ex = n_ex;
                 after();
                 n_id = pages_of(n_c, n_at + int32_t(lane));
@@ -579,12 +585,18 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                     if (t_stage >= uint32_t(G::kStages)) t_stage -= G::kStages, ++t_round;
                 }
                 done += n;
-                // the warps' sums meet: maxima first, then the rows, half of the warps at a time
+                // the warps' sums meet: where they all fit each as it is; else maxima first,
+                // then half of the warps at a time
+                const bool own = W * R <= G::kSide * MR;
+                const int32_t side = own ? W : G::kSide;
                 rows.stats(sm + warp * MR, sl + warp * MR, lane);
-                meet();
-                if (warp < G::kSide) rows.sums(join, warp * uint32_t(R), R, false, top, lane);
-                meet();
-                if (warp >= G::kSide) rows.sums(join, (warp - G::kSide) * uint32_t(R), R, true, top, lane);
+                if (!own) meet();
+                if (int32_t(warp) < side) rows.sums(join, warp * uint32_t(R), R, own, false, top, lane);
+                if (!own) {
+                    meet();
+                    if (int32_t(warp) >= side)
+                        rows.sums(join, (warp - uint32_t(side)) * uint32_t(R), R, false, true, top, lane);
+                }
                 if (c + 1 < count) rows.queries(p, segs[c + 1], lane);
                 meet();
                 // rows by warps, D / 32 elements of a row per lane
@@ -609,16 +621,16 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                     const float mx = top(uint32_t(row));
                     float sum = 0.f, v[E];
 #pragma unroll
-                    for (int w = 0; w < W; ++w)
-                        sum = fmaf(mx == -INFINITY ? 0.f : ex2(sm[w * MR + row] - mx), sl[w * MR + row], sum);
-#pragma unroll
                     for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll
-                    for (uint32_t w = 0; w < uint32_t(G::kSide); ++w) {
-                        const uint32_t at = w * uint32_t(R) + uint32_t(row);
+                    for (int w = 0; w < W; ++w) {
+                        const float f = mx == -INFINITY ? 0.f : ex2(sm[w * MR + row] - mx);
+                        sum = fmaf(f, sl[w * MR + row], sum);
+                        if (w >= side) continue;
+                        const uint32_t at = uint32_t(w * R + row);
                         const float* from = join + at * D + ((lane * E) ^ (at & 7u) * 8);
 #pragma unroll
-                        for (int e = 0; e < E; ++e) v[e] += from[e];
+                        for (int e = 0; e < E; ++e) v[e] = fmaf(own ? f : 1.f, from[e], v[e]);
                     }
                     if (whole) {
                         finish(row, v, mx, sum);
@@ -629,7 +641,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                     }
                 }
                 if (!whole) {
-                    const int64_t c0 = cut_owner(U, NC, x.item), c1 = cut_owner(U, NC, x.item + x.tiles - 1);
+                    const int64_t c0 = cut.owner(x.item), c1 = cut.owner(x.item + x.tiles - 1);
                     __threadfence();
                     meet();
                     if (tid == 0) {
@@ -641,7 +653,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                     if (flag[2]) {
                         __threadfence();
                         const int32_t pieces = int32_t(c1 - c0) + 1;
-                        const float* const p0 = p.part + (2 * c0 + (cut_begin(U, NC, c0) != x.item)) * kPart;
+                        const float* const p0 = p.part + (2 * c0 + (cut.begin(c0) != x.item)) * kPart;
                         auto piece = [&](int32_t i) { return i ? p.part + 2 * (c0 + i) * kPart : p0; };
                         for (int32_t row = int32_t(warp); row < R; row += W) {
                             float mx = -INFINITY, sum = 0.f, v[E] = {};
@@ -692,7 +704,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
         __syncthreads();  // the list has been read
         u = segs[count - 1].item + segs[count - 1].j0 + segs[count - 1].steps;
     }
-    if (warp == W)  // every load has landed before the CTA ends
+    if (warp >= W)  // every load has landed before the CTA ends
         for (uint32_t i = loaded - min(loaded, uint32_t(G::kStages)); i != loaded; ++i)
             warp_wait(full(i % G::kStages), (i / G::kStages) & 1u, kGraceNs);
     if (!ok) gave_up(p);
