@@ -30,8 +30,8 @@ namespace lsb {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kQueryHeads = 4;   // query heads that a warp has under way
-constexpr int kCtasPerSm = 8;
+constexpr int kHeads = 4;  // heads that a warp has under way
+constexpr int kCtasPerSm = 2;
 constexpr uint32_t kMaxTokens = 1u << 27;  // blocks of 256 sequences count in 32 bits, even of overlapping ones
 
 struct AppendParams {
@@ -51,13 +51,12 @@ struct AppendParams {
     int64_t q_ts, q_hs, qo_ts, qo_hs, kn_ts, kn_hs, vn_ts, vn_hs;
     int64_t kp_ps, kp_ss, kp_hs, vp_ps, vp_ss, vp_hs, ex_ps, ex_hs, table_s, cs_s;
     uint32_t B, Hq, Hkv, P, pshift, pages, tpages, tokens, rotary, angles;
-    uint32_t interleaved, q_tasks;  // query tasks of an item
+    uint32_t interleaved;
+    uint32_t per_task, splits;      // heads of a task, and tasks that share a block's rows
     int32_t lowest, highest;        // exponents that the 16-bit type holds exactly
 };
 
-// A task: up to 16 new tokens of a sequence whose slots lie in one block (the
-// item), and one of: keys of a kv head, values of one, queries of a row group
-// and kQueryHeads heads.
+// An item: up to 16 new tokens of a sequence whose slots lie in one block.
 struct Rows {
     int32_t b, block;
     int32_t token, slot, n;  // first row of q, its slot, rows
@@ -109,26 +108,33 @@ __device__ __forceinline__ uint4 narrow(const float* x) {
     return make_uint4(T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7]));
 }
 
-struct Turn {  // angles of a lane's eight pairs
-    float c[8], s[8];
+// Angles of a lane's eight pairs, two pairs side by side. Products and sums are
+// rounded one by one: x (-s) is -(x s), and no pair of them is fused.
+struct Turn {
+    uint64_t c[4], s[4], n[4];  // cosines, sines, and the sines negated
     __device__ __forceinline__ void load(const float* row, uint32_t i, uint32_t half) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(row + i * 8 + e);
-            *reinterpret_cast<float4*>(s + e) = *reinterpret_cast<const float4*>(row + half + i * 8 + e);
+        for (int e = 0; e < 4; e += 2) {
+            const float4 x = *reinterpret_cast<const float4*>(row + i * 8 + e * 2);
+            const float4 y = *reinterpret_cast<const float4*>(row + half + i * 8 + e * 2);
+            c[e] = tc::pack2(x.x, x.y), c[e + 1] = tc::pack2(x.z, x.w);
+            s[e] = tc::pack2(y.x, y.y), s[e + 1] = tc::pack2(y.z, y.w);
+            n[e] = tc::pack2(-y.x, -y.y), n[e + 1] = tc::pack2(-y.z, -y.w);
         }
     }
-    static __device__ __forceinline__ void pair(float& a, float& b, float c, float s) {
-        const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-        b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
-        a = x;
+    template <int step, int next>  // from a pair's first to its second, and to the next pair
+    __device__ __forceinline__ void pairs(float* x) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float* const y = x + 2 * next * e;
+            const uint64_t a = tc::pack2(y[0], y[next]), b = tc::pack2(y[step], y[step + next]);
+            tc::unpack2(tc::add2(tc::mul2(a, c[e]), tc::mul2(b, n[e])), y[0], y[next]);
+            tc::unpack2(tc::add2(tc::mul2(b, c[e]), tc::mul2(a, s[e])), y[step], y[step + next]);
+        }
     }
     __device__ __forceinline__ void apply(float* x, bool interleaved) const {  // x: pieces a and b
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (interleaved) pair(x[2 * e], x[2 * e + 1], c[e], s[e]);
-            else pair(x[e], x[8 + e], c[e], s[e]);
-        }
+        if (interleaved) pairs<1, 2>(x);
+        else pairs<8, 1>(x);
     }
 };
 
@@ -141,163 +147,189 @@ __device__ __forceinline__ int32_t angle_row(const AppendParams& p, int32_t toke
     return -1;
 }
 
+// Four numbers, of at most 127 units of 1 / inv, to codes: x inv + 1.5 * 2^23 ends in
+// the nearest whole number's low byte (inv is a power of two: one rounding).
 __device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
-    uint32_t r = 0;
+    uint32_t v[4], lo, hi, r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int32_t v = __float2int_rn(fminf(fmaxf(x[e] * inv, -127.f), 127.f));
-        r |= (uint32_t(v) & 0xffu) << (8 * e);
-    }
+    for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(fmaf(x[e], inv, 12582912.f));
+    asm("prmt.b32 %0, %1, %2, 0x0040;" : "=r"(lo) : "r"(v[0]), "r"(v[1]));
+    asm("prmt.b32 %0, %1, %2, 0x0040;" : "=r"(hi) : "r"(v[2]), "r"(v[3]));
+    asm("prmt.b32 %0, %1, %2, 0x5410;" : "=r"(r) : "r"(lo), "r"(hi));
     return r;
 }
 
-// Keys (VALUES false) or values of one kv head.
-template <class T, int D, bool Q8, bool VALUES>
-__device__ __forceinline__ void append_rows(const AppendParams& p, const Rows& t, int32_t h) {
+// Where the rows of a task come from and go to: queries, or keys or values in 16 bits.
+struct Heads {
+    const uint16_t* from;  // of head 0
+    uint16_t* to;
+    int64_t from_ts, from_hs, to_ts, to_hs;
+    uint32_t heads;
+    bool turned;
+};
+
+// kHeads heads at a time, from head0 to head1 - 1, of the rows it0 * kRows .. of a
+// task: a row's angles are read once for them.
+template <class T, int D>
+__device__ __forceinline__ void move_rows(const AppendParams& p, const Rows& t, const Heads& w, int32_t to_row,
+                                          uint32_t head0, uint32_t head1, int32_t it) {
+    const Lane<D> at(threadIdx.x & 31u, w.turned ? p.rotary : 0, p.interleaved);
+    const int32_t r = it * Lane<D>::kRows + int32_t(at.row);
+    if (r >= t.n) return;
+    const int64_t token = t.token + r;
+    const uint16_t* from = w.from + token * w.from_ts;
+    uint16_t* to = w.to + int64_t(to_row + r) * w.to_ts;
+    int32_t angle = 0;
+    Turn turn;
+    for (uint32_t h = head0; h < head1; h += kHeads) {
+        uint4 a[kHeads], b[kHeads];
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            const uint16_t* row = from + int64_t(min(h + i, head1 - 1)) * w.from_hs;
+            a[i] = *reinterpret_cast<const uint4*>(row + at.a);
+            b[i] = *reinterpret_cast<const uint4*>(row + at.b);
+        }
+        if (h == head0) {
+            angle = angle_row(p, int32_t(token), t.slot + r);
+            if (angle >= 0 && at.turned) turn.load(p.cos_sin + int64_t(angle) * p.cs_s, at.i, p.rotary / 2);
+        }
+        if (angle < 0) return;
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            if (h + i >= head1) break;
+            if (at.turned) {
+                float x[16];
+                widen<T>(a[i], x);
+                widen<T>(b[i], x + 8);
+                turn.apply(x, p.interleaved);
+                a[i] = narrow<T>(x);
+                b[i] = narrow<T>(x + 8);
+            }
+            uint16_t* row = to + int64_t(h + i) * w.to_hs;
+            *reinterpret_cast<uint4*>(row + at.a) = a[i];
+            *reinterpret_cast<uint4*>(row + at.b) = b[i];
+        }
+    }
+}
+
+// Page of a task's block; -1 where it has none (no slot, or reported).
+__device__ __forceinline__ int32_t page_of(const AppendParams& p, const Rows& t) {
+    if (t.slot + t.n <= 0) return -1;
+    const int32_t id = p.table[int64_t(t.b) * p.table_s + ((t.block * kBlock) >> p.pshift)];
+    if (uint32_t(id) < p.pages) return id;
+    if ((threadIdx.x & 31u) == 0 && p.err) atomicOr(p.err, kErrPage);
+    return -1;
+}
+
+// Keys (VALUES false) or values of one kv head into a block of codes. The rows stay in
+// registers as they come, all of them under way at a time, and are rotated twice, for
+// the largest value and for the codes: in 32 bits they leave one CTA per SM its place.
+template <class T, int D, bool VALUES>
+__device__ __forceinline__ void append_codes(const AppendParams& p, const Rows& t, int32_t h) {
     const uint32_t lane = threadIdx.x & 31u;
     const Lane<D> at(lane, VALUES ? 0 : p.rotary, p.interleaved);
     constexpr int R = Lane<D>::kRows, N = Lane<D>::kIters;
-    const int32_t id = t.slot + t.n > 0 ? p.table[int64_t(t.b) * p.table_s + ((t.block * kBlock) >> p.pshift)] : 0;
-    const uint16_t* from = VALUES ? p.v_new + int64_t(h) * p.vn_hs : p.k_new + int64_t(h) * p.kn_hs;
-    const int64_t from_s = VALUES ? p.vn_ts : p.kn_ts;
-    float x[N][16];
-    bool on[N];
+    const uint16_t* from = (VALUES ? p.v_new + int64_t(h) * p.vn_hs : p.k_new + int64_t(h) * p.kn_hs) +
+                           int64_t(t.token + int32_t(at.row)) * (VALUES ? p.vn_ts : p.kn_ts);
+    const int64_t from_s = R * (VALUES ? p.vn_ts : p.kn_ts);
+    uint4 a[N], b[N];
+    int32_t angle[N];  // -1: no row
 #pragma unroll
     for (int it = 0; it < N; ++it) {
-        const int32_t r = it * R + int32_t(at.row), slot = t.slot + r;
-        on[it] = r < t.n && slot >= 0;
-        uint4 a{}, b{};
-        int32_t angle = 0;
-        if (on[it]) {
-            const uint16_t* row = from + int64_t(t.token + r) * from_s;
-            a = *reinterpret_cast<const uint4*>(row + at.a);
-            b = *reinterpret_cast<const uint4*>(row + at.b);
-            angle = angle_row(p, t.token + r, slot);
-            on[it] = angle >= 0;
+        const int32_t r = it * R + int32_t(at.row);
+        angle[it] = -1;
+        if (r < t.n && t.slot + r >= 0) {
+            a[it] = *reinterpret_cast<const uint4*>(from + it * from_s + at.a);
+            b[it] = *reinterpret_cast<const uint4*>(from + it * from_s + at.b);
+            angle[it] = angle_row(p, t.token + r, t.slot + r);
         }
-        widen<T>(a, x[it]);
-        widen<T>(b, x[it] + 8);
-        if (!VALUES && on[it] && at.turned) {
+    }
+    const int32_t id = page_of(p, t);
+    if (id < 0) return;
+    auto row_of = [&](int it, float* x) {
+        // (or the compiler keeps the first pass's numbers for the second)
+        asm volatile("" : "+r"(a[it].x), "+r"(a[it].y), "+r"(a[it].z), "+r"(a[it].w));
+        asm volatile("" : "+r"(b[it].x), "+r"(b[it].y), "+r"(b[it].z), "+r"(b[it].w));
+        widen<T>(a[it], x);
+        widen<T>(b[it], x + 8);
+        if (!VALUES && at.turned) {
             Turn turn;
-            turn.load(p.cos_sin + int64_t(angle) * p.cs_s, at.i, p.rotary / 2);
-            turn.apply(x[it], p.interleaved);
-        }
-    }
-    if (t.slot + t.n <= 0) return;
-    if (uint32_t(id) >= p.pages) {
-        if (lane == 0 && p.err) atomicOr(p.err, kErrPage);
-        return;
-    }
-    const int32_t in = (t.block * kBlock) & int32_t(p.P - 1), skip = t.slot - t.block * kBlock;
-    if constexpr (!Q8) {
-        uint16_t* to = VALUES ? static_cast<uint16_t*>(p.v_pages) + int64_t(id) * p.vp_ps + int64_t(h) * p.vp_hs
-                              : static_cast<uint16_t*>(p.k_pages) + int64_t(id) * p.kp_ps + int64_t(h) * p.kp_hs;
-        const int64_t to_s = VALUES ? p.vp_ss : p.kp_ss;
-#pragma unroll
-        for (int it = 0; it < N; ++it) {
-            if (!on[it]) continue;
-            uint16_t* row = to + int64_t(in + skip + it * R + int32_t(at.row)) * to_s;
-            *reinterpret_cast<uint4*>(row + at.a) = narrow<T>(x[it]);
-            *reinterpret_cast<uint4*>(row + at.b) = narrow<T>(x[it] + 8);
-        }
-    } else {
-        int8_t* to = VALUES ? static_cast<int8_t*>(p.v_pages) + int64_t(id) * p.vp_ps + int64_t(h) * p.vp_hs
-                            : static_cast<int8_t*>(p.k_pages) + int64_t(id) * p.kp_ps + int64_t(h) * p.kp_hs;
-        const int64_t to_s = VALUES ? p.vp_ss : p.kp_ss;
-        int8_t* ex = p.exponents + int64_t(id) * p.ex_ps + int64_t(h) * p.ex_hs + (in / kBlock) * 2 + VALUES;
-        const int32_t was = t.fresh ? p.lowest : *ex;
-        uint32_t top = 0;  // bits of the largest |x|: in order, infinities and NaN above every number
-        bool any = false;
-#pragma unroll
-        for (int it = 0; it < N; ++it) {
-            any = any || on[it];
-            if (!on[it]) continue;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[it][e]) & 0x7fffffffu);
-        }
-        if (!__any_sync(0xffffffffu, any)) return;
-        top = __reduce_max_sync(0xffffffffu, top);
-        const bool bad = top >= 0x7f800000u || was == kNoExponent;
-        // 127 = 1.984375 * 2^6 (numbers below 2^-126 only meet the lowest exponent)
-        int32_t e = int32_t(top >> 23) - 127 - 6 + ((top & 0x7fffffu) > 0x7e0000u ? 1 : 0);
-        e = max(min(max(e, p.lowest), p.highest), was);
-        if (!bad && !t.fresh && e > was) {
-            // older rows to the new step, 16 bytes per lane and row
-            constexpr uint32_t kPieces = D / 16;
-            const float shift = two_to(max(was - e, -100));
-            for (int32_t r = int32_t(lane / kPieces); r < skip; r += 32 / int32_t(kPieces)) {
-                uint4* cell = reinterpret_cast<uint4*>(to + int64_t(in + r) * to_s + (lane % kPieces) * 16);
-                uint4 v = *cell;
-                uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    float c[4];
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) c[z] = float(int8_t(w[y] >> (8 * z)));
-                    w[y] = codes4(c, shift);
-                }
-                *cell = v;
-            }
-        }
-        const float inv = bad ? 0.f : two_to(-e);
-#pragma unroll
-        for (int it = 0; it < N; ++it) {
-            if (!on[it]) continue;
-            if (bad)
-#pragma unroll
-                for (int y = 0; y < 16; ++y) x[it][y] = 0.f;
-            int8_t* row = to + int64_t(in + skip + it * R + int32_t(at.row)) * to_s;
-            *reinterpret_cast<uint2*>(row + at.a) = make_uint2(codes4(x[it], inv), codes4(x[it] + 4, inv));
-            *reinterpret_cast<uint2*>(row + at.b) = make_uint2(codes4(x[it] + 8, inv), codes4(x[it] + 12, inv));
-        }
-        if (lane == 0) *ex = int8_t(bad ? kNoExponent : e);
-    }
-}
-
-// Queries: one group of rows, kQueryHeads heads, so that a row's angles are read
-// once for these.
-template <class T, int D>
-__device__ __forceinline__ void rotate_queries(const AppendParams& p, const Rows& t, uint32_t task) {
-    const Lane<D> at(threadIdx.x & 31u, p.rotary, p.interleaved);
-    const uint32_t head0 = task / Lane<D>::kIters * kQueryHeads;
-    const int32_t r = int32_t(task % Lane<D>::kIters * Lane<D>::kRows + at.row);
-    if (r >= t.n) return;
-    const int64_t token = t.token + r;
-    uint4 a[kQueryHeads], b[kQueryHeads];
-#pragma unroll
-    for (int i = 0; i < kQueryHeads; ++i) {
-        if (head0 + i >= p.Hq) break;
-        const uint16_t* row = p.q + token * p.q_ts + int64_t(head0 + i) * p.q_hs;
-        a[i] = *reinterpret_cast<const uint4*>(row + at.a);
-        b[i] = *reinterpret_cast<const uint4*>(row + at.b);
-    }
-    const int32_t angle = angle_row(p, int32_t(token), t.slot + r);
-    if (angle < 0) return;
-    Turn turn;
-    if (at.turned) turn.load(p.cos_sin + int64_t(angle) * p.cs_s, at.i, p.rotary / 2);
-#pragma unroll
-    for (int i = 0; i < kQueryHeads; ++i) {
-        if (head0 + i >= p.Hq) break;
-        if (at.turned) {
-            float x[16];
-            widen<T>(a[i], x);
-            widen<T>(b[i], x + 8);
+            turn.load(p.cos_sin + int64_t(angle[it]) * p.cs_s, at.i, p.rotary / 2);
             turn.apply(x, p.interleaved);
-            a[i] = narrow<T>(x);
-            b[i] = narrow<T>(x + 8);
         }
-        uint16_t* row = p.q_out + token * p.qo_ts + int64_t(head0 + i) * p.qo_hs;
-        *reinterpret_cast<uint4*>(row + at.a) = a[i];
-        *reinterpret_cast<uint4*>(row + at.b) = b[i];
+    };
+    const int32_t in = (t.block * kBlock) & int32_t(p.P - 1), skip = t.slot - t.block * kBlock;
+    int8_t* to = VALUES ? static_cast<int8_t*>(p.v_pages) + int64_t(id) * p.vp_ps + int64_t(h) * p.vp_hs
+                        : static_cast<int8_t*>(p.k_pages) + int64_t(id) * p.kp_ps + int64_t(h) * p.kp_hs;
+    const int64_t to_s = VALUES ? p.vp_ss : p.kp_ss;
+    int8_t* ex = p.exponents + int64_t(id) * p.ex_ps + int64_t(h) * p.ex_hs + (in / kBlock) * 2 + VALUES;
+    const int32_t was = t.fresh ? p.lowest : *ex;
+    float largest = 0.f;  // NaN where one is
+    bool any = false;
+#pragma unroll
+    for (int it = 0; it < N; ++it) {
+        if (angle[it] < 0) continue;
+        any = true;
+        float x[16];
+        row_of(it, x);
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) largest = tc::max3(largest, fabsf(x[e]), fabsf(x[e + 1]));
     }
+    if (!__any_sync(0xffffffffu, any)) return;
+    // as bits they keep their order, infinities and NaN above every number
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest) & 0x7fffffffu);
+    const bool bad = top >= 0x7f800000u || was == kNoExponent;
+    // 127 = 1.984375 * 2^6 (numbers below 2^-126 only meet the lowest exponent)
+    int32_t e = int32_t(top >> 23) - 127 - 6 + ((top & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+    e = max(min(max(e, p.lowest), p.highest), was);
+    if (!bad && !t.fresh && e > was) {
+        // older rows to the new step, 16 bytes per lane and row
+        constexpr uint32_t kPieces = D / 16;
+        const float shift = two_to(max(was - e, -100));
+        for (int32_t r = int32_t(lane / kPieces); r < skip; r += 32 / int32_t(kPieces)) {
+            uint4* cell = reinterpret_cast<uint4*>(to + int64_t(in + r) * to_s + (lane % kPieces) * 16);
+            uint4 v = *cell;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                float c[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) c[z] = float(int8_t(w[y] >> (8 * z)));
+                w[y] = codes4(c, shift);
+            }
+            *cell = v;
+        }
+    }
+    const float inv = two_to(-e);
+    const bool beyond = !bad && __uint_as_float(top) > 127.f * two_to(min(e, 120));  // (of the largest exponent)
+#pragma unroll
+    for (int it = 0; it < N; ++it) {
+        if (angle[it] < 0) continue;
+        float x[16];
+        row_of(it, x);
+        if (bad || beyond) {
+            const float most = bad ? 0.f : 127.f * two_to(e);
+#pragma unroll
+            for (int y = 0; y < 16; ++y) x[y] = bad ? 0.f : fminf(fmaxf(x[y], -most), most);
+        }
+        int8_t* row = to + int64_t(in + skip + it * R + int32_t(at.row)) * to_s;
+        *reinterpret_cast<uint2*>(row + at.a) = make_uint2(codes4(x, inv), codes4(x + 4, inv));
+        *reinterpret_cast<uint2*>(row + at.b) = make_uint2(codes4(x + 8, inv), codes4(x + 12, inv));
+    }
+    if (lane == 0) *ex = int8_t(bad ? kNoExponent : e);
 }
 
 template <class T, int D, bool Q8>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) append_kernel(const AppendParams p) {
     __shared__ int32_t first[kThreads + 1];  // items before each sequence of the batch piece
     __shared__ int32_t sums[kWarps];
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t tasks = 2 * int64_t(p.Hkv) + p.q_tasks;  // of an item
+    // tasks of an item: keys, values (codes: a head each; else groups of heads as the
+    // queries), queries
+    const uint32_t groups = (p.Hkv + p.per_task - 1) / p.per_task;
+    const uint32_t k_tasks = Q8 ? p.Hkv : groups * p.splits;
+    const int64_t tasks = 2 * int64_t(k_tasks) + (p.Hq + p.per_task - 1) / p.per_task * p.splits;
+    const uint32_t period = max(1u, gridDim.x * kWarps / uint32_t(tasks));
     tc::after_wait();
     tc::after_start();
     int64_t base = 0, task = int64_t(blockIdx.x) * kWarps + warp;
@@ -325,7 +357,10 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
         __syncthreads();
         for (; task < (base + total) * tasks; task += int64_t(gridDim.x) * kWarps) {
             const int32_t item = int32_t(task / tasks - base);
-            const uint32_t kind = uint32_t(task - (base + item) * tasks);
+            // (a warp's next task lies about `period` items on: there the kinds go backwards, so
+            // that codes, which take longest, and queries fall to the same warps)
+            const uint32_t at = uint32_t(task - (base + item) * tasks);
+            const uint32_t kind = uint32_t(item) / period & 1u ? uint32_t(tasks) - 1 - at : at;
             uint32_t lo = 0, hi = kThreads;  // the sequence: first[lo] <= item < first[lo + 1]
             while (hi - lo > 1) {
                 const uint32_t mid = (lo + hi) / 2;
@@ -341,9 +376,36 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
             t.n = min(q.n, start + kBlock) - t.slot;
             t.token = q.q0 + t.slot - q.f;
             t.fresh = q.f <= start;
-            if (kind < p.Hkv) append_rows<T, D, Q8, false>(p, t, int32_t(kind));
-            else if (kind < 2 * p.Hkv) append_rows<T, D, Q8, true>(p, t, int32_t(kind - p.Hkv));
-            else rotate_queries<T, D>(p, t, kind - 2 * p.Hkv);
+            if (Q8 && kind < 2 * k_tasks) {
+                if (kind < k_tasks) append_codes<T, D, false>(p, t, int32_t(kind));
+                else append_codes<T, D, true>(p, t, int32_t(kind - k_tasks));
+                continue;
+            }
+            Heads w;
+            uint32_t part = kind;
+            int32_t to_row = t.token;
+            if (kind < 2 * k_tasks) {
+                const bool values = kind >= k_tasks;
+                const int32_t id = page_of(p, t);
+                if (id < 0) continue;
+                // (rows at slots below 0 come before the block's first: none of it)
+                to_row = t.slot & int32_t(p.P - 1);
+                w.from = values ? p.v_new : p.k_new;
+                w.from_ts = values ? p.vn_ts : p.kn_ts, w.from_hs = values ? p.vn_hs : p.kn_hs;
+                w.to = static_cast<uint16_t*>(values ? p.v_pages : p.k_pages) +
+                       int64_t(id) * (values ? p.vp_ps : p.kp_ps);
+                w.to_ts = values ? p.vp_ss : p.kp_ss, w.to_hs = values ? p.vp_hs : p.kp_hs;
+                w.heads = p.Hkv, w.turned = !values;
+                if (values) part -= k_tasks;
+            } else {
+                w.from = p.q, w.from_ts = p.q_ts, w.from_hs = p.q_hs;
+                w.to = p.q_out, w.to_ts = p.qo_ts, w.to_hs = p.qo_hs;
+                w.heads = p.Hq, w.turned = true;
+                part -= 2 * k_tasks;
+            }
+            const uint32_t head0 = part / p.splits * p.per_task, head1 = min(head0 + p.per_task, w.heads);
+            for (int32_t it = int32_t(part % p.splits); it * Lane<D>::kRows < t.n; it += int32_t(p.splits))
+                move_rows<T, D>(p, t, w, to_row, head0, head1, it);
         }
         base += total;
         __syncthreads();  // the counts have been read
@@ -411,12 +473,17 @@ extern "C" int ls_b200_append_cache(const ls_b200_append_args* a, void* stream) 
     while ((1u << p.pshift) < p.P) ++p.pshift;
     p.lowest = a->dtype == LS_B200_FP16 ? -24 : -126;
     p.highest = a->dtype == LS_B200_FP16 ? 9 : 120;
-    const uint32_t groups = a->head_dim == 128 ? Lane<128>::kIters : Lane<64>::kIters;
-    p.q_tasks = (p.Hq + kQueryHeads - 1) / kQueryHeads * groups;
+    // Few tokens: a warp takes all of a block's rows. Many: every row group is a task, of
+    // twice the heads.
+    const bool many = p.tokens > 2 * p.B;
+    p.per_task = many ? 2 * kHeads : kHeads;
+    p.splits = !many ? 1 : a->head_dim == 128 ? Lane<128>::kIters : Lane<64>::kIters;
     // at most tokens / 16 blocks, and two that are cut for each sequence
     uint64_t items = uint64_t(p.tokens) / kBlock + 2ull * p.B;
     items = items < p.tokens ? items : p.tokens;
-    const uint64_t ctas = (items * (2ull * p.Hkv + p.q_tasks) + kWarps - 1) / kWarps;
+    const uint64_t k_tasks = int8 ? p.Hkv : (p.Hkv + p.per_task - 1) / p.per_task * p.splits;
+    const uint64_t tasks = 2 * k_tasks + (p.Hq + p.per_task - 1) / p.per_task * p.splits;
+    const uint64_t ctas = (items * tasks + kWarps - 1) / kWarps;
     const uint64_t most = uint64_t(sm_count()) * kCtasPerSm;
     const uint32_t grid = uint32_t(ctas < most ? ctas : most);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
