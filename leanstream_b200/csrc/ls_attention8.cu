@@ -45,17 +45,19 @@ constexpr uint64_t kGraceNs = 1000000000ull;
 constexpr uint64_t kShortNs = 100000;      // bounds that a barrier's try may sleep over: a load takes less
 
 // NT tiles of eight rows, kWarps that compute. One CTA per SM; the ring takes the
-// shared memory that the warps' sums, half of them at a time, leave.
+// shared memory that the sums of kSide warps at a time leave.
 template <int D, int NT>
 struct Geo8 {
     static constexpr int kWarps = NT <= 2 ? 10 : 6, kThreads = 32 * (kWarps + 2), kSide = (kWarps + 1) / 2;
+    static constexpr bool kSharedQ = NT > 1;  // one tile's queries stay in registers, more in shared memory
     static constexpr int kRows = 8 * NT;
     static constexpr uint32_t kHalf = kStep * D, kStage = 2 * kHalf;  // a step's keys, and its values
     // A stage is always the same warp's: then its next round cannot be taken for the
     // one before, whose load may still be under way.
     static constexpr int kStages = kWarps * (NT == 3 ? 3 : 2) * (128 / D);
     static constexpr uint32_t kJoin = kStages * kStage, kSegs = kJoin + kSide * kRows * D * 4;
-    static constexpr uint32_t kNotes = kSegs + kSegCount * 64, kBars = kNotes + 8 * kStages;
+    static constexpr uint32_t kQ = kSegs + kSegCount * 64, kNotes = kQ + (kSharedQ ? kRows * (D * 2 + 4) : 0);
+    static constexpr uint32_t kBars = kNotes + 8 * kStages;
     static constexpr uint32_t kStat = kBars + 16 * kStages, kScan = kStat + 8 * kWarps * kRows;
     static constexpr uint32_t kSmem = kScan + 16 * (kWarps + 2) + 16 + 1024;  // + alignment of the swizzled tiles
     static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
@@ -104,58 +106,68 @@ constexpr uint32_t kCodes01 = 0x4140, kCodes23 = 0x4342, kCodes02 = 0x4240, kCod
 template <class T, int D, int NT>
 struct Rows8 {
     static constexpr int KS = D / 16;
-    uint2 q[NT][KS];     // row g: elements 4 t .. 4 t + 3 of each 16, as the codes come
+    static constexpr bool kSharedQ = Geo8<D, NT>::kSharedQ;
+    // Row g of a tile: elements 4 t .. 4 t + 3 of each 16, as the codes come. Of the
+    // one tile, or of the tile that this warp puts to shared memory.
+    uint2 q[KS];
     float cq[NT][2];     // scale * log2 e and the rows' own powers of two
     float o[NT][KS][4];  // in units of 2^(most - kChunkShift)
     float m[NT][2], l[NT][2];  // l: of this lane's slots
-    int32_t pos[NT][2];  // slot of the rows' tokens (-1: no row)
     int32_t most;
 
-    __device__ __forceinline__ void queries(const AttnParams& p, const Seg8& x, uint32_t lane) {
-        const int32_t g = int32_t(p.g);
+    __device__ __forceinline__ void queries(const AttnParams& p, const Seg8& x, int tile, uint32_t lane) {
+        const int32_t g = int32_t(p.g), r = int32_t(lane >> 2) + 8 * tile;
+        const bool on = r < x.rows;
+        const uint16_t* at = p.q + int64_t(x.q0 + (on ? r / g : 0)) * p.q_ts +
+                             int64_t(x.h * g + (on ? r % g : 0)) * p.q_hs + (lane & 3u) * 4;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int32_t r = int32_t(lane >> 2) + 8 * i;
-            const bool on = r < x.rows;
-            const uint16_t* at = p.q + int64_t(x.q0 + (on ? r / g : 0)) * p.q_ts +
-                                 int64_t(x.h * g + (on ? r % g : 0)) * p.q_hs + (lane & 3u) * 4;
+        for (int k = 0; k < KS; ++k) q[k] = on ? *reinterpret_cast<const uint2*>(at + k * 16) : make_uint2(0u, 0u);
+    }
+    // To float16; the row's factor of the logits.
+    __device__ __forceinline__ float convert(float c) {
+        if constexpr (std::is_same_v<T, BF16>) {
+            uint32_t top = 0;  // bits of the largest |q| of the row
 #pragma unroll
             for (int k = 0; k < KS; ++k)
-                q[i][k] = on ? *reinterpret_cast<const uint2*>(at + k * 16) : make_uint2(0u, 0u);
+                top = max(max(top, max(q[k].x & 0x7fffu, (q[k].x >> 16) & 0x7fffu)),
+                          max(q[k].y & 0x7fffu, (q[k].y >> 16) & 0x7fffu));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // to [2^14, 2^15); infinities and NaN stay what they are
+            const int32_t e = top >= 0x7f80u ? 0 : max(int32_t(top >> 7) - 127 - 14, -112);
+            const float f = two_to(-e);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                float a, b;
+                BF16::unpack(q[k].x, a, b);
+                q[k].x = F16::pack(a * f, b * f);
+                BF16::unpack(q[k].y, a, b);
+                q[k].y = F16::pack(a * f, b * f);
+            }
+            c *= two_to(e);
         }
+        return c;
     }
-    __device__ __forceinline__ void begin(const AttnParams& p, const Seg8& x, uint32_t lane) {
-        const int32_t g = int32_t(p.g), t = int32_t(lane & 3u);
+    // A tile's queries to shared memory: [tile][D / 32][lane] of two k's, then the factors.
+    __device__ __forceinline__ void share(uint8_t* to, float c, int tile, uint32_t lane) {
+        c = convert(c);
+#pragma unroll
+        for (int k = 0; k < KS; k += 2)
+            *reinterpret_cast<uint4*>(to + ((tile * (KS / 2) + k / 2) * 32 + lane) * 16) =
+                make_uint4(q[k].x, q[k].y, q[k + 1].x, q[k + 1].y);
+        if ((lane & 3u) == 0) reinterpret_cast<float*>(to + NT * KS * 256)[8 * tile + (lane >> 2)] = c;
+    }
+    __device__ __forceinline__ void begin(const uint8_t* shared, float scale, uint32_t lane) {
+        const int32_t t = int32_t(lane & 3u);
+        float c = scale;
+        if constexpr (!kSharedQ) c = convert(scale);
         most = -126;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            float c = p.c;
-            if constexpr (std::is_same_v<T, BF16>) {
-                uint32_t top = 0;  // bits of the largest |q| of the row
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-                    top = max(max(top, max(q[i][k].x & 0x7fffu, (q[i][k].x >> 16) & 0x7fffu)),
-                              max(q[i][k].y & 0x7fffu, (q[i][k].y >> 16) & 0x7fffu));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // to [2^14, 2^15); infinities and NaN stay what they are
-                const int32_t e = top >= 0x7f80u ? 0 : max(int32_t(top >> 7) - 127 - 14, -112);
-                const float f = two_to(-e);
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    float a, b;
-                    BF16::unpack(q[i][k].x, a, b);
-                    q[i][k].x = F16::pack(a * f, b * f);
-                    BF16::unpack(q[i][k].y, a, b);
-                    q[i][k].y = F16::pack(a * f, b * f);
-                }
-                c *= two_to(e);
-            }
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                const int32_t row = 8 * i + 2 * t + y;
-                cq[i][y] = __shfl_sync(0xffffffffu, c, (2 * t + y) * 4);
-                pos[i][y] = row < x.rows ? max(x.f + row / g, -1) : -1;
+                cq[i][y] = kSharedQ ? reinterpret_cast<const float*>(shared + NT * KS * 256)[8 * i + 2 * t + y]
+                                    : __shfl_sync(0xffffffffu, c, (2 * t + y) * 4);
                 m[i][y] = -INFINITY, l[i][y] = 0.f;
             }
 #pragma unroll
@@ -165,11 +177,17 @@ struct Rows8 {
         }
     }
     // 32 slots, codes of their keys and values at ks and vs
-    __device__ __forceinline__ void step(const AttnParams& p, uint32_t ks, uint32_t vs, Note note, uint32_t lane) {
+    __device__ __forceinline__ void step(const AttnParams& p, const Seg8& x, const uint8_t* shared, uint32_t ks,
+                                         uint32_t vs, Note note, uint32_t lane) {
         const int32_t k0 = int32_t(note.k & ~1u);
         float s[2][NT][4] = {};
 #pragma unroll
-        for (int k = 0; k < KS; k += 2)
+        for (int k = 0; k < KS; k += 2) {
+            uint4 qk[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+                qk[i] = kSharedQ ? *reinterpret_cast<const uint4*>(shared + ((i * (KS / 2) + k / 2) * 32 + lane) * 16)
+                                 : make_uint4(q[k].x, q[k].y, q[k + 1].x, q[k + 1].y);
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
                 uint32_t v[4];  // slots 0-7 and 8-15 (v[2], v[3]) of two 16-byte pieces
@@ -181,9 +199,11 @@ struct Rows8 {
                     const uint32_t a[4] = {codes_f16(v[y], kCodes01), codes_f16(v[2 + y], kCodes01),
                                            codes_f16(v[y], kCodes23), codes_f16(v[2 + y], kCodes23)};
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) F16::mma(s[z][i], a, q[i][k + y].x, q[i][k + y].y);
+                    for (int i = 0; i < NT; ++i)
+                        F16::mma(s[z][i], a, y ? qk[i].z : qk[i].x, y ? qk[i].w : qk[i].y);
                 }
             }
+        }
         int32_t ev[2];
         float fk[2];
 #pragma unroll
@@ -200,13 +220,19 @@ struct Rows8 {
                 for (int e = 0; e < 4; ++e) s[z][i][e] *= cq[i][e & 1] * fk[z];
         if (note.k & 1u) {
 #pragma unroll
-            for (int z = 0; z < 2; ++z)
+            for (int i = 0; i < NT; ++i)
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                for (int y = 0; y < 2; ++y) {
+                    // slot of the row's token (-1: no row)
+                    const int32_t row = 8 * i + 2 * int32_t(lane & 3u) + y;
+                    const int32_t pos = row < x.rows ? max(x.f + row / int32_t(p.g), -1) : -1;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!sees(p, pos[i][e & 1], k0 + z * kBlock + int32_t(lane >> 2) + 8 * (e >> 1)))
-                            s[z][i][e] = -INFINITY;
+                    for (int z = 0; z < 2; ++z)
+#pragma unroll
+                        for (int e = y; e < 4; e += 2)
+                            if (!sees(p, pos, k0 + z * kBlock + int32_t(lane >> 2) + 8 * (e >> 1)))
+                                s[z][i][e] = -INFINITY;
+                }
         }
         bool raise = false;
 #pragma unroll
@@ -568,16 +594,22 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 for (int w = 1; w < W; ++w) mx = fmaxf(mx, sm[w * MR + row]);
                 return mx;
             };
-            rows.queries(p, segs[0], lane);
+            uint8_t* const shared = smem + G::kQ;
+            const int tile = G::kSharedQ ? int(warp) : 0;  // of the queries that this warp reads
+            if (tile < NT) rows.queries(p, segs[0], tile, lane);
+            if constexpr (G::kSharedQ) {
+                if (tile < NT) rows.share(shared, p.c, tile, lane);
+                meet();
+            }
             for (uint32_t c = 0; c < count; ++c) {
                 const Seg8& x = segs[c];
                 const int32_t R = x.rows, h = x.h;
                 const uint32_t n = uint32_t(x.loads());
-                rows.begin(p, x, lane);
+                rows.begin(shared, p.c, lane);
                 while (ok && turn - done < n) {
                     if (!(ok = wait(full(t_stage), t_round & 1u))) break;
                     const uint32_t ks = sbase + t_stage * G::kStage;
-                    rows.step(p, ks, ks + G::kHalf, notes[t_stage], lane);
+                    rows.step(p, x, shared, ks, ks + G::kHalf, notes[t_stage], lane);
                     __syncwarp();
                     if (lane == 0) bar_arrive(empty(t_stage));
                     turn += W;
@@ -586,19 +618,18 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 }
                 done += n;
                 // the warps' sums meet: where they all fit each as it is; else maxima first,
-                // then half of the warps at a time
+                // then some of the warps at a time
                 const bool own = W * R <= G::kSide * MR;
                 const int32_t side = own ? W : G::kSide;
                 rows.stats(sm + warp * MR, sl + warp * MR, lane);
                 if (!own) meet();
-                if (int32_t(warp) < side) rows.sums(join, warp * uint32_t(R), R, own, false, top, lane);
-                if (!own) {
+                for (int32_t w0 = 0; w0 < W; w0 += side) {
+                    if (uint32_t(int32_t(warp) - w0) < uint32_t(side))
+                        rows.sums(join, uint32_t((int32_t(warp) - w0) * R), R, own, w0 != 0, top, lane);
+                    if (w0 + side >= W && c + 1 < count && tile < NT) rows.queries(p, segs[c + 1], tile, lane);
                     meet();
-                    if (int32_t(warp) >= side)
-                        rows.sums(join, (warp - uint32_t(side)) * uint32_t(R), R, false, true, top, lane);
                 }
-                if (c + 1 < count) rows.queries(p, segs[c + 1], lane);
-                meet();
+                if (G::kSharedQ && c + 1 < count && tile < NT) rows.share(shared, p.c, tile, lane);
                 // rows by warps, D / 32 elements of a row per lane
                 constexpr int E = D / 32;
                 const bool whole = x.j0 == 0 && x.steps == x.tiles;
