@@ -4,9 +4,11 @@
 //
 // An item is a sequence and kv head; its rows are (token, head of the group). Its
 // slots go by in steps of 32 (two blocks); the steps of all items, in order, are
-// cut evenly over one CTA per SM. Two warps of a CTA load, keys and values: they
-// lay out up to 32 steps at a time, a lane each, and fill one ring of stages with
-// what each step needs (first slot, exponents, codes). The other warps
+// cut evenly over one CTA per SM. Two warps of a CTA load, keys and values (four where
+// a step's blocks lie in two pages: a box takes its warp about 75 cycles to issue, and
+// 32 sequences of pages of 16 slots take 63 us with two): they lay out up to 32 steps
+// at a time, a lane each, and fill one ring of stages with what each step needs (first
+// slot, exponents, codes). The other warps
 // take the steps in turn, with maxima and sums of their own, and meet at the end of
 // an item's piece; the loads run on into the next piece meanwhile. An item cut over
 // several CTAs is joined, in the order of its pieces, by the CTA that arrives last.
@@ -48,18 +50,19 @@ constexpr uint64_t kShortNs = 100000;      // bounds that a barrier's try may sl
 // shared memory that the sums of kSide warps at a time leave.
 template <int D, int NT>
 struct Geo8 {
-    static constexpr int kWarps = NT <= 2 ? 10 : 6, kThreads = 32 * (kWarps + 2), kSide = (kWarps + 1) / 2;
+    static constexpr int kWarps = NT <= 2 ? 8 : 6, kLoaders = NT <= 2 ? 4 : 2, kThreads = 32 * (kWarps + kLoaders);
+    static constexpr int kSide = (kWarps + 1) / 2;
     static constexpr bool kSharedQ = NT > 1;  // one tile's queries stay in registers, more in shared memory
     static constexpr int kRows = 8 * NT;
     static constexpr uint32_t kHalf = kStep * D, kStage = 2 * kHalf;  // a step's keys, and its values
     // A stage is always the same warp's: then its next round cannot be taken for the
     // one before, whose load may still be under way.
-    static constexpr int kStages = kWarps * (NT == 3 ? 3 : 2) * (128 / D);
+    static constexpr int kStages = kWarps * (NT == 2 ? 2 : 3) * (128 / D);
     static constexpr uint32_t kJoin = kStages * kStage, kSegs = kJoin + kSide * kRows * D * 4;
     static constexpr uint32_t kQ = kSegs + kSegCount * 64, kNotes = kQ + (kSharedQ ? kRows * (D * 2 + 4) : 0);
     static constexpr uint32_t kBars = kNotes + 8 * kStages;
     static constexpr uint32_t kStat = kBars + 16 * kStages, kScan = kStat + 8 * kWarps * kRows;
-    static constexpr uint32_t kSmem = kScan + 16 * (kWarps + 2) + 16 + 1024;  // + alignment of the swizzled tiles
+    static constexpr uint32_t kSmem = kScan + 16 * (kWarps + kLoaders + 1) + 1024;  // + alignment of the tiles
     static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -400,7 +403,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
     Note* const notes = reinterpret_cast<Note*>(smem + G::kNotes);
     float* const join = reinterpret_cast<float*>(smem + G::kJoin);
     Pair8* const scan = reinterpret_cast<Pair8*>(smem + G::kScan);
-    volatile uint32_t* const flag = reinterpret_cast<uint32_t*>(scan + W + 2);
+    volatile uint32_t* const flag = reinterpret_cast<uint32_t*>(scan + W + G::kLoaders);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t g = int32_t(p.g);
     auto full = [&](uint32_t s) { return sbase + G::kBars + 8 * s; };
@@ -411,7 +414,8 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
     };
 
     if (warp == W) {
-        for (uint32_t i = lane; i < 2u * G::kStages; i += 32) bar_init(full(i), i < uint32_t(G::kStages) ? 2 : 1);
+        const uint32_t loaders = p.P >= uint32_t(kStep) ? 2 : G::kLoaders;
+        for (uint32_t i = lane; i < 2u * G::kStages; i += 32) bar_init(full(i), i < uint32_t(G::kStages) ? loaders : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (lane < 2) prefetch_map(lane ? &vmap : &kmap);
     }
@@ -428,12 +432,12 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
     SeqRange seq0;
     const Pair8 v0 = units_of(tid, seq0);
     Pair8 before0;
-    const Pair8 total0 = block_scan8<W + 2>(v0, scan, before0);
+    const Pair8 total0 = block_scan8<W + G::kLoaders>(v0, scan, before0);
     int64_t U = total0.x;
     for (uint32_t b0 = G::kThreads; b0 < p.B; b0 += G::kThreads) {
         SeqRange s;
         Pair8 before;
-        U += block_scan8<W + 2>(units_of(b0 + tid, s), scan, before).x;
+        U += block_scan8<W + G::kLoaders>(units_of(b0 + tid, s), scan, before).x;
     }
     if (!U) return;
     const int64_t NC = max(int64_t(1), min(int64_t(gridDim.x), quotient(U + kMinUnits8 - 1, kMinUnits8)));
@@ -461,7 +465,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             Pair8 v = v0, before = before0, total = total0;
             if (b0) {
                 v = units_of(b0 + tid, s);
-                total = block_scan8<W + 2>(v, scan, before);
+                total = block_scan8<W + G::kLoaders>(v, scan, before);
             }
             const int64_t at = base + before.x, item_units = v.y ? quotient(v.x, p.Hkv) : 1;
             const int32_t seq = seqs + before.y;
@@ -494,10 +498,12 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
         const uint32_t count = flag[0];
         if (!count) break;  // what is left of the range is the cost of an item
 
-        if (warp >= W) {
+        if (warp >= W + 2 && p.P >= uint32_t(kStep)) {  // (a step lies in one page: two warps load)
+        } else if (warp >= W) {
             // ---- loads: blocks of steps of a piece, a lane and a stage each; the pages of
-            // the block after it are under way. The warp of the keys also takes the exponents.
-            const bool keys = warp == W;
+            // the block after it are under way. One of the warps also takes the exponents.
+            const bool keys = (warp - W) % 2 == 0, note = warp == W;
+            const bool first = G::kLoaders == 2 || warp < W + 2, second = G::kLoaders == 2 || warp >= W + 2;  // blocks
             const CUtensorMap* const map = keys ? &kmap : &vmap;
             constexpr int32_t kBlockSteps = G::kStages < 32 ? G::kStages : 32;
             const bool pairs = p.P >= uint32_t(kStep);  // a step lies in one page
@@ -513,7 +519,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 auto page = [&](int32_t slot) {
                     const int32_t at = row[slot >> p.pshift];
                     if (uint32_t(at) < p.pages) return at;
-                    if (keys && p.err) atomicOr(p.err, kErrPage);
+                    if (note && p.err) atomicOr(p.err, kErrPage);
                     return int32_t(p.pages);
                 };
                 if (seen(x, k)) id.x = page(k);
@@ -522,7 +528,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             };
             auto exponents_of = [&](uint32_t c, int32_t step, int2 id) -> uint32_t {
                 uint32_t ex = 0;
-                if (!keys || c >= count) return ex;
+                if (!note || c >= count) return ex;
                 const Seg8& x = segs[c];
                 const int32_t in = step < x.loads() ? x.slot0(step) & int32_t(p.P - 1) : 0;
                 const uint8_t* at = p.ex + int64_t(x.h) * p.ex_hs;
@@ -551,7 +557,8 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 const int32_t k = mine ? x.slot0(at + int32_t(lane)) : 0, in = k & int32_t(p.P - 1);
                 const bool masked = k + kStep - 1 > x.f ||
                                     (p.window && int64_t(k) <= int64_t(x.hi) - 1 - int64_t(p.window));
-                const uint32_t bytes = pairs ? G::kHalf : uint32_t((id.x >= 0) + (id.y >= 0)) * (G::kHalf / 2);
+                const uint32_t boxes = (first && id.x >= 0) + (second && id.y >= 0);  // of a block
+                const uint32_t bytes = pairs ? G::kHalf : boxes * (G::kHalf / 2);
                 const uint32_t st = (loaded + lane) % G::kStages, round = (loaded + lane) / G::kStages;
                 const uint32_t dst = sbase + st * G::kStage + (keys ? 0 : G::kHalf), bar = full(st);
                 // each lane loads when its stage is free
@@ -562,10 +569,10 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                         if (pairs) {
                             tma4(dst, map, bar, 0, in, h, max(id.x, id.y));
                         } else {
-                            if (id.x >= 0) tma4(dst, map, bar, 0, in, h, id.x);
-                            if (id.y >= 0) tma4(dst + kBlock * D, map, bar, 0, 0, h, id.y);
+                            if (first && id.x >= 0) tma4(dst, map, bar, 0, in, h, id.x);
+                            if (second && id.y >= 0) tma4(dst + kBlock * D, map, bar, 0, 0, h, id.y);
                         }
-                        if (keys) notes[st] = Note{uint32_t(k) | uint32_t(masked), ex};
+                        if (note) notes[st] = Note{uint32_t(k) | uint32_t(masked), ex};
                         bar_arrive_tx(bar, bytes);
                         left = false;
                     }
