@@ -449,14 +449,15 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
     bool ok = true;
     uint32_t done = 0;                      // steps of the pieces so far
     uint32_t turn = warp, t_stage = warp, t_round = 0;  // this warp's next step, its stage and its round
-    uint32_t loaded = 0;                    // steps loaded
+    uint32_t loaded = 0;                    // steps loaded in whole blocks
+    uint32_t again = 0;                     // lanes of the block that was given up which have loaded
     static_assert(G::kStages % W == 0, "a stage is always the same warp's");
     Rows8<T, D, NT> rows;
 
     for (int64_t u = u_begin; u < u_end;) {
         // the next pieces, listed by the threads of their sequences: items (y
         // counts sequences with rows) from the one that holds unit u
-        if (tid == 0) flag[0] = flag[1] = 0;
+        if (tid == 0) flag[0] = flag[1] = flag[3] = 0;
         __syncthreads();
         int64_t base = 0;
         int32_t seqs = 0;
@@ -561,9 +562,10 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 const uint32_t bytes = pairs ? G::kHalf : boxes * (G::kHalf / 2);
                 const uint32_t st = (loaded + lane) % G::kStages, round = (loaded + lane) / G::kStages;
                 const uint32_t dst = sbase + st * G::kStage + (keys ? 0 : G::kHalf), bar = full(st);
-                // each lane loads when its stage is free
-                bool left = mine;
-                const uint64_t begin = now();
+                // Each lane loads when its stage is free. That ends, as every wait of the warps
+                // that compute does; once they are through, what is free is loaded by every
+                // loading warp and the rest by none, so that each stage's barrier completes.
+                bool left = mine, through = false;
                 for (uint32_t spin = 1;; ++spin) {
                     if (left && (!round || bar_test(empty(st), (round - 1) & 1u))) {
                         if (pairs) {
@@ -577,10 +579,15 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                         left = false;
                     }
                     if (!__any_sync(0xffffffffu, left)) break;
-                    if (spin % 64 == 0 && __any_sync(0xffffffffu, now() - begin > p.timeout_ns)) {
-                        ok = false;  // (what this block has loaded lands before the CTA ends)
+                    if (through) {
+                        ok = false;
+                        again = __ballot_sync(0xffffffffu, mine && !left);
                         if (mine && !left) bar_wait(bar, round & 1u, kGraceNs);
                         break;
+                    }
+                    if (spin % 16 == 0) {
+                        through = __all_sync(0xffffffffu, flag[3] == uint32_t(W));
+                        __threadfence_block();
                     }
                 }
                 __syncwarp();
@@ -738,13 +745,18 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 }
                 meet();  // the joined sums and maxima have been read
             }
+            __threadfence_block();
+            if (lane == 0) atomicAdd(const_cast<uint32_t*>(flag) + 3, 1u);
         }
         __syncthreads();  // the list has been read
         u = segs[count - 1].item + segs[count - 1].j0 + segs[count - 1].steps;
     }
     if (warp >= W)  // every load has landed before the CTA ends
-        for (uint32_t i = loaded - min(loaded, uint32_t(G::kStages)); i != loaded; ++i)
+        for (uint32_t i = loaded - min(loaded, uint32_t(G::kStages)); i != loaded; ++i) {
+            const uint32_t j = i + G::kStages - loaded;  // the lane whose stage this is in the next block
+            if (j < 32 && again >> j & 1u) continue;     // (it landed, and a load after it)
             warp_wait(full(i % G::kStages), (i / G::kStages) & 1u, kGraceNs);
+        }
     if (!ok) gave_up(p);
 }
 

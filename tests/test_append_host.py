@@ -37,8 +37,8 @@ INT8 = dict(cache_dtype=2, exponents=1 << 30, exponents_page_stride=4, exponents
     dict(page_table=None), dict(q_start=None), dict(kv_len=None), dict(cos_sin=None), dict(cos_sin=(1 << 29) + 4),
     dict(exponents=1 << 30), dict(cache_dtype=2), dict(q_token_stride=1020), dict(q_out_head_stride=-128),
     dict(k_slot_stride=260), dict(cos_sin_stride=130), dict(table_stride=-1),
-    dict(cos_sin=None, rotary_dim=0, angles=0), dict(cos_sin=None, rotary_dim=0, angles=0, q=None, q_out=None, q_heads=0,
-                                                     positions=1 << 31),
+    dict(cos_sin=None, rotary_dim=0, angles=0),
+    dict(cos_sin=None, rotary_dim=0, angles=0, q=None, q_out=None, q_heads=0, positions=1 << 31),
     {**INT8, "exponents": (1 << 30) + 1}, {**INT8, "exponents_page_stride": 3}, {**INT8, "exponents_head_stride": -2},
     {**INT8, "k_slot_stride": 264}], ids=str)
 def test_refusals(native_lib, change):
