@@ -2,17 +2,18 @@
 // in 8 bits. The formula is that of ls_attention.cu; a value of the cache is code *
 // 2^e, one e for the 16 slots of a block, kv head, and keys or values.
 //
-// An item is a sequence and kv head; its rows are (token, head of the group). Its
-// slots go by in steps of 32 (two blocks); the steps of all items, in order, are
-// cut evenly over one CTA per SM. Two warps of a CTA load, keys and values (four where
-// a step's blocks lie in two pages: a box takes its warp about 75 cycles to issue, and
-// 32 sequences of pages of 16 slots take 63 us with two): they lay out up to 32 steps
-// at a time, a lane each, and fill one ring of stages with what each step needs (first
-// slot, exponents, codes). The other warps
-// take the steps in turn, with maxima and sums of their own, and meet at the end of
-// an item's piece; the loads run on into the next piece meanwhile. An item cut over
-// several CTAs is joined, in the order of its pieces, by the CTA that arrives last.
-// Which warp takes which step follows from the step, so results do not depend on
+// An item is a sequence and kv head, or some neighbouring kv heads where the codes of
+// one fill less than a line of memory; the rows of a head are (token, head of the
+// group). The slots go by in units of 32 (two blocks), a step for each of the heads;
+// the units of all items, in order, are cut evenly over one CTA per SM. Two warps of a
+// CTA load, keys and values (four where a step's blocks lie in two pages: a box takes
+// its warp about 75 cycles to issue, and 48 sequences in pages of 16 slots take 63 us
+// with two, 58 with four). They lay out up to 32 steps at a time, a lane each, and fill
+// one ring of stages with what each step needs (first slot, exponents, codes). The
+// other warps take the steps in turn, with maxima and sums of their own, and meet at
+// the end of an item's piece; the loads run on into the next piece meanwhile. An item
+// cut over several CTAs is joined, in the order of its pieces, by the CTA that arrives
+// last. Which warp takes which step follows from the step, so results do not depend on
 // timing.
 //
 // Slots and elements are the M dimension of the products and rows their N, so that
@@ -42,7 +43,7 @@ using namespace tc;
 constexpr int kStep = 2 * kBlock;          // slots of a step
 constexpr int kSegCount = 48;              // pieces listed at a time
 constexpr int64_t kItemCost8 = 16;         // steps that beginning and joining an item counts as
-constexpr int64_t kMinUnits8 = 24;         // steps that a CTA takes at least
+constexpr int64_t kMinSteps8 = 24;         // steps that a CTA takes at least
 constexpr uint64_t kGraceNs = 1000000000ull;
 constexpr uint64_t kShortNs = 100000;      // bounds that a barrier's try may sleep over: a load takes less
 
@@ -51,7 +52,12 @@ constexpr uint64_t kShortNs = 100000;      // bounds that a barrier's try may sl
 template <int D, int NT>
 struct Geo8 {
     static constexpr int kWarps = NT <= 2 ? 8 : 6, kLoaders = NT <= 2 ? 4 : 2, kThreads = 32 * (kWarps + kLoaders);
-    static constexpr int kSide = (kWarps + 1) / 2;
+    static constexpr int kSide = NT == 3 && D == 64 ? 4 : (kWarps + 1) / 2;
+    // kv heads of an item, at most: the codes of 64 elements take half a line of 128 bytes
+    // (48 sequences of up to 5000 slots, 16 kv heads: 98 us with one, 72 with two, 68 with
+    // four; of 128 elements no gain)
+    static constexpr int kHeads = D == 128 ? 1 : NT == 1 ? 4 : 2;
+    static_assert(kWarps % kHeads == 0 && kSide % kHeads == 0, "a warp takes one of them");
     static constexpr bool kSharedQ = NT > 1;  // one tile's queries stay in registers, more in shared memory
     static constexpr int kRows = 8 * NT;
     static constexpr uint32_t kHalf = kStep * D, kStage = 2 * kHalf;  // a step's keys, and its values
@@ -59,25 +65,27 @@ struct Geo8 {
     // one before, whose load may still be under way.
     static constexpr int kStages = kWarps * (NT == 2 ? 2 : 3) * (128 / D);
     static constexpr uint32_t kJoin = kStages * kStage, kSegs = kJoin + kSide * kRows * D * 4;
-    static constexpr uint32_t kQ = kSegs + kSegCount * 64, kNotes = kQ + (kSharedQ ? kRows * (D * 2 + 4) : 0);
+    static constexpr uint32_t kQ = kSegs + kSegCount * 64, kQBytes = kSharedQ ? kRows * (D * 2 + 4) : 0;  // of a head
+    static constexpr uint32_t kNotes = kQ + kHeads * kQBytes;
     static constexpr uint32_t kBars = kNotes + 8 * kStages;
     static constexpr uint32_t kStat = kBars + 16 * kStages, kScan = kStat + 8 * kWarps * kRows;
     static constexpr uint32_t kSmem = kScan + 16 * (kWarps + kLoaders + 1) + 1024;  // + alignment of the tiles
     static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 };
 
-// A piece of an item: `steps` steps from step j0 of a sequence and kv head.
+// A piece of an item: `units` units from unit j0 of a sequence and its kv heads from h.
 struct Seg8 {
     int32_t b, h, q0, rows;
     int32_t f, hi, lo, sink;  // as SeqRange, KeyRange
-    int32_t ns, first, j0, steps;
-    int32_t tiles, own;       // steps of the item; own: it does not begin the CTA's range
+    int32_t ns, first, j0, units;
+    int32_t tiles, own;       // units of the item; own: it does not begin the CTA's range
     int64_t item;             // first unit of the item
-    __device__ __forceinline__ int32_t slot0(int32_t step) const {
-        const int32_t j = j0 + step;
+    __device__ __forceinline__ int32_t slot0(int32_t unit) const {
+        const int32_t j = j0 + unit;
         return (j < ns ? j : first + j - ns) * kStep;
     }
-    __device__ __forceinline__ int32_t loads() const { return hi ? steps : 0; }  // (rows that see nothing have a step)
+    // steps of 2^hs heads (rows that see nothing have a unit, but no step)
+    __device__ __forceinline__ int32_t steps(uint32_t hs) const { return hi ? units << hs : 0; }
 };
 static_assert(sizeof(Seg8) == 64, "list entries");
 
@@ -118,11 +126,12 @@ struct Rows8 {
     float m[NT][2], l[NT][2];  // l: of this lane's slots
     int32_t most;
 
-    __device__ __forceinline__ void queries(const AttnParams& p, const Seg8& x, int tile, uint32_t lane) {
+    __device__ __forceinline__ void queries(const AttnParams& p, const Seg8& x, int32_t h, int tile,
+                                            uint32_t lane) {
         const int32_t g = int32_t(p.g), r = int32_t(lane >> 2) + 8 * tile;
         const bool on = r < x.rows;
         const uint16_t* at = p.q + int64_t(x.q0 + (on ? r / g : 0)) * p.q_ts +
-                             int64_t(x.h * g + (on ? r % g : 0)) * p.q_hs + (lane & 3u) * 4;
+                             int64_t(h * g + (on ? r % g : 0)) * p.q_hs + (lane & 3u) * 4;
 #pragma unroll
         for (int k = 0; k < KS; ++k) q[k] = on ? *reinterpret_cast<const uint2*>(at + k * 16) : make_uint2(0u, 0u);
     }
@@ -421,26 +430,36 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
     }
     after_start();
     after_wait();
-    // units of this thread's sequence (of the first kThreads), and of the call; y: 1
+    // tiles of this thread's sequence (of the first kThreads), and of the call; y: 1
     // where the sequence has rows
-    auto units_of = [&](uint32_t b, SeqRange& s) -> Pair8 {
+    auto tiles_of = [&](uint32_t b, SeqRange& s) -> Pair8 {
         s = SeqRange{0, 0, 0, 0};
         if (b < p.B) s = load_seq(p, b);
         if (!s.nq) return Pair8{0, 0};
-        return Pair8{(key_range<kStep>(p, s, 0, s.nq).tiles + kItemCost8) * p.Hkv, 1};
+        return Pair8{key_range<kStep>(p, s, 0, s.nq).tiles, 1};
     };
     SeqRange seq0;
-    const Pair8 v0 = units_of(tid, seq0);
+    const Pair8 v0 = tiles_of(tid, seq0);
     Pair8 before0;
     const Pair8 total0 = block_scan8<W + G::kLoaders>(v0, scan, before0);
-    int64_t U = total0.x;
+    Pair8 all = total0;
     for (uint32_t b0 = G::kThreads; b0 < p.B; b0 += G::kThreads) {
         SeqRange s;
         Pair8 before;
-        U += block_scan8<W + G::kLoaders>(units_of(b0 + tid, s), scan, before).x;
+        const Pair8 more = block_scan8<W + G::kLoaders>(tiles_of(b0 + tid, s), scan, before);
+        all.x += more.x, all.y += more.y;
     }
-    if (!U) return;
-    const int64_t NC = max(int64_t(1), min(int64_t(gridDim.x), quotient(U + kMinUnits8 - 1, kMinUnits8)));
+    if (!all.y) return;
+    // heads of an item: 2^hs, as many as leave items for half of the CTAs (fewer items
+    // are cut into more parts, which one CTA joins)
+    uint32_t hs = 0;
+    for (uint32_t more = 1; 1 << more <= G::kHeads; ++more)
+        if (p.Hkv % (1u << more) == 0 && int64_t(all.y) * (p.Hkv >> more) * 2 >= gridDim.x) hs = more;
+    const uint32_t side_by = (1u << hs) - 1;
+    const int64_t Hi = p.Hkv >> hs, item_cost = kItemCost8 >> hs, min_units = kMinSteps8 >> hs;
+    auto units = [&](Pair8 v) { return (v.x + v.y * item_cost) * Hi; };
+    const int64_t U = units(all);
+    const int64_t NC = max(int64_t(1), min(int64_t(gridDim.x), quotient(U + min_units - 1, min_units)));
     if (int64_t(blockIdx.x) >= NC) return;
     const Cut cut(U, NC);
     const int64_t cta = blockIdx.x, u_begin = cut.begin(cta), u_end = cut.begin(cta + 1);
@@ -465,34 +484,34 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             SeqRange s = seq0;
             Pair8 v = v0, before = before0, total = total0;
             if (b0) {
-                v = units_of(b0 + tid, s);
+                v = tiles_of(b0 + tid, s);
                 total = block_scan8<W + G::kLoaders>(v, scan, before);
             }
-            const int64_t at = base + before.x, item_units = v.y ? quotient(v.x, p.Hkv) : 1;
+            const int64_t at = base + units(before), item_units = v.y ? v.x + item_cost : 1, end = at + units(v);
             const int32_t seq = seqs + before.y;
-            if (v.y && u >= at && u < at + v.x)
-                flag[1] = uint32_t(seq * int32_t(p.Hkv) + int32_t(quotient(u - at, item_units)));
+            if (v.y && u >= at && u < end)
+                flag[1] = uint32_t(seq * int32_t(Hi) + int32_t(quotient(u - at, item_units)));
             __syncthreads();
-            const int64_t from = max(u, at), to = min(u_end, at + v.x);
+            const int64_t from = max(u, at), to = min(u_end, end);
             if (from < to) {
                 const KeyRange kr = key_range<kStep>(p, s, 0, s.nq);
                 int32_t h = int32_t(quotient(from - at, item_units));
-                int32_t idx = seq * int32_t(p.Hkv) + h - int32_t(flag[1]);
-                for (; h < int32_t(p.Hkv) && idx < kSegCount; ++h, ++idx) {
+                int32_t idx = seq * int32_t(Hi) + h - int32_t(flag[1]);
+                for (; h < int32_t(Hi) && idx < kSegCount; ++h, ++idx) {
                     Seg8 x;
-                    x.item = at + h * item_units + kItemCost8;
+                    x.item = at + h * item_units + item_cost;
                     const int64_t a = max(x.item, u), e = min(x.item + kr.tiles, u_end);
                     if (a >= e) break;  // only the item's cost lies in the range
-                    x.b = int32_t(b0 + tid), x.h = h, x.q0 = s.q0, x.rows = s.nq * g;
+                    x.b = int32_t(b0 + tid), x.h = h << hs, x.q0 = s.q0, x.rows = s.nq * g;
                     x.f = s.f, x.hi = kr.hi, x.lo = kr.lo, x.sink = kr.sink, x.ns = kr.ns, x.first = kr.first;
                     x.tiles = kr.tiles;
-                    x.j0 = int32_t(a - x.item), x.steps = int32_t(e - a);
+                    x.j0 = int32_t(a - x.item), x.units = int32_t(e - a);
                     x.own = a != u_begin;
                     segs[idx] = x;
                     atomicMax(const_cast<uint32_t*>(flag), uint32_t(idx + 1));
                 }
             }
-            base += total.x;
+            base += units(total);
             seqs += total.y;
         }
         __syncthreads();
@@ -507,6 +526,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             const bool first = G::kLoaders == 2 || warp < W + 2, second = G::kLoaders == 2 || warp >= W + 2;  // blocks
             const CUtensorMap* const map = keys ? &kmap : &vmap;
             constexpr int32_t kBlockSteps = G::kStages < 32 ? G::kStages : 32;
+            static_assert(kBlockSteps % G::kHeads == 0, "a unit's steps stay together");
             const bool pairs = p.P >= uint32_t(kStep);  // a step lies in one page
             auto seen = [&](const Seg8& x, int32_t k) { return (k < x.hi && k + kBlock > x.lo) || k < x.sink; };
             // pages of both blocks of a step (-1: no row sees the block)
@@ -514,8 +534,8 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 int2 id = make_int2(-1, -1);
                 if (c >= count) return id;
                 const Seg8& x = segs[c];
-                if (step >= x.loads()) return id;
-                const int32_t k = x.slot0(step);
+                if (step >= x.steps(hs)) return id;
+                const int32_t k = x.slot0(step >> hs);
                 const int32_t* row = p.table + int64_t(x.b) * p.table_s;
                 auto page = [&](int32_t slot) {
                     const int32_t at = row[slot >> p.pshift];
@@ -531,8 +551,8 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 uint32_t ex = 0;
                 if (!note || c >= count) return ex;
                 const Seg8& x = segs[c];
-                const int32_t in = step < x.loads() ? x.slot0(step) & int32_t(p.P - 1) : 0;
-                const uint8_t* at = p.ex + int64_t(x.h) * p.ex_hs;
+                const int32_t in = step < x.steps(hs) ? x.slot0(step >> hs) & int32_t(p.P - 1) : 0;
+                const uint8_t* at = p.ex + int64_t(x.h + int32_t(uint32_t(step) & side_by)) * p.ex_hs;
                 if (uint32_t(id.x) < p.pages)
                     ex = *reinterpret_cast<const uint16_t*>(at + int64_t(id.x) * p.ex_ps + (in >> 3));
                 if (uint32_t(id.y) < p.pages)
@@ -545,7 +565,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             int32_t at = 0, n_at = 0;
             auto after = [&]() {
                 n_at += kBlockSteps;
-                if (n_c < count && n_at >= segs[n_c].loads()) ++n_c, n_at = 0;
+                if (n_c < count && n_at >= segs[n_c].steps(hs)) ++n_c, n_at = 0;
             };
             int2 id = pages_of(0, int32_t(lane)), n_id;
             uint32_t ex = exponents_of(0, int32_t(lane), id), n_ex = 0;
@@ -553,9 +573,9 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             n_id = pages_of(n_c, n_at + int32_t(lane));
             while (ok && c < count) {
                 const Seg8& x = segs[c];
-                const int32_t n = min(kBlockSteps, x.loads() - at), h = x.h;
+                const int32_t n = min(kBlockSteps, x.steps(hs) - at), h = x.h + int32_t(lane & side_by);
                 const bool mine = int32_t(lane) < n;
-                const int32_t k = mine ? x.slot0(at + int32_t(lane)) : 0, in = k & int32_t(p.P - 1);
+                const int32_t k = mine ? x.slot0((at + int32_t(lane)) >> hs) : 0, in = k & int32_t(p.P - 1);
                 const bool masked = k + kStep - 1 > x.f ||
                                     (p.window && int64_t(k) <= int64_t(x.hi) - 1 - int64_t(p.window));
                 const uint32_t boxes = (first && id.x >= 0) + (second && id.y >= 0);  // of a block
@@ -602,23 +622,26 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             float* const sm = reinterpret_cast<float*>(smem + G::kStat);  // [W][MR]
             float* const sl = sm + W * MR;
             auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory"); };
-            auto top = [&](uint32_t row) {
-                float mx = sm[row];
+            const uint32_t mine = warp & side_by;  // the head of an item that this warp takes
+            auto top_of = [&](uint32_t of, uint32_t row) {
+                float mx = sm[of * MR + row];
 #pragma unroll
-                for (int w = 1; w < W; ++w) mx = fmaxf(mx, sm[w * MR + row]);
+                for (uint32_t w = 1; w < uint32_t(W); ++w)
+                    if ((w & side_by) == of) mx = fmaxf(mx, sm[w * MR + row]);
                 return mx;
             };
-            uint8_t* const shared = smem + G::kQ;
-            const int tile = G::kSharedQ ? int(warp) : 0;  // of the queries that this warp reads
-            if (tile < NT) rows.queries(p, segs[0], tile, lane);
+            auto top = [&](uint32_t row) { return top_of(mine, row); };
+            uint8_t* const shared = smem + G::kQ + mine * G::kQBytes;
+            const int tile = G::kSharedQ ? int(warp >> hs) : 0;  // of the queries that this warp reads
+            if (tile < NT) rows.queries(p, segs[0], segs[0].h + int32_t(mine), tile, lane);
             if constexpr (G::kSharedQ) {
                 if (tile < NT) rows.share(shared, p.c, tile, lane);
                 meet();
             }
             for (uint32_t c = 0; c < count; ++c) {
                 const Seg8& x = segs[c];
-                const int32_t R = x.rows, h = x.h;
-                const uint32_t n = uint32_t(x.loads());
+                const int32_t R = x.rows;
+                const uint32_t n = uint32_t(x.steps(hs));
                 rows.begin(shared, p.c, lane);
                 while (ok && turn - done < n) {
                     if (!(ok = wait(full(t_stage), t_round & 1u))) break;
@@ -640,18 +663,19 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 for (int32_t w0 = 0; w0 < W; w0 += side) {
                     if (uint32_t(int32_t(warp) - w0) < uint32_t(side))
                         rows.sums(join, uint32_t((int32_t(warp) - w0) * R), R, own, w0 != 0, top, lane);
-                    if (w0 + side >= W && c + 1 < count && tile < NT) rows.queries(p, segs[c + 1], tile, lane);
+                    if (w0 + side >= W && c + 1 < count && tile < NT)
+                        rows.queries(p, segs[c + 1], segs[c + 1].h + int32_t(mine), tile, lane);
                     meet();
                 }
                 if (G::kSharedQ && c + 1 < count && tile < NT) rows.share(shared, p.c, tile, lane);
                 // rows by warps, D / 32 elements of a row per lane
                 constexpr int E = D / 32;
-                const bool whole = x.j0 == 0 && x.steps == x.tiles;
-                constexpr int64_t kPart = MR * (D + 2);
-                float* const slot = p.part + (2 * cta + x.own) * kPart;
-                auto finish = [&](int32_t row, const float (&v)[E], float mx, float sum) {
+                const bool whole = x.j0 == 0 && x.units == x.tiles;
+                constexpr int64_t kPart = MR * (D + 2);  // of a head
+                float* const slot = p.part + ((2 * cta + x.own) << hs) * kPart;
+                auto finish = [&](int32_t of, int32_t row, const float (&v)[E], float mx, float sum) {
                     const int32_t token = x.q0 + row / g;
-                    const int64_t head = h * g + row % g;
+                    const int64_t head = (x.h + of) * g + row % g;
                     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
                     uint16_t* out = p.out + int64_t(token) * p.o_ts + head * p.o_hs + lane * E;
                     if constexpr (E == 4)
@@ -662,13 +686,15 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                     if (lane == 0 && p.lse)
                         p.lse[int64_t(token) * p.Hq + head] = sum == 0.f ? -INFINITY : (mx + lg2(sum)) * kLn2;
                 };
-                for (int32_t row = int32_t(warp); row < R; row += W) {
-                    const float mx = top(uint32_t(row));
+                for (int32_t i = int32_t(warp); i < R << hs; i += W) {
+                    const int32_t of = hs ? i / R : 0, row = i - of * R;  // head of the item
+                    const float mx = top_of(uint32_t(of), uint32_t(row));
                     float sum = 0.f, v[E];
 #pragma unroll
                     for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
+                        if ((uint32_t(w) & side_by) != uint32_t(of)) continue;
                         const float f = mx == -INFINITY ? 0.f : ex2(sm[w * MR + row] - mx);
                         sum = fmaf(f, sl[w * MR + row], sum);
                         if (w >= side) continue;
@@ -678,11 +704,12 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                         for (int e = 0; e < E; ++e) v[e] = fmaf(own ? f : 1.f, from[e], v[e]);
                     }
                     if (whole) {
-                        finish(row, v, mx, sum);
+                        finish(of, row, v, mx, sum);
                     } else {
+                        float* const to = slot + of * kPart;
 #pragma unroll
-                        for (int e = 0; e < E; ++e) slot[row * D + lane * E + e] = v[e];
-                        if (lane == 0) slot[MR * D + row] = mx, slot[MR * D + MR + row] = sum;
+                        for (int e = 0; e < E; ++e) to[row * D + lane * E + e] = v[e];
+                        if (lane == 0) to[MR * D + row] = mx, to[MR * D + MR + row] = sum;
                     }
                 }
                 if (!whole) {
@@ -698,9 +725,12 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                     if (flag[2]) {
                         __threadfence();
                         const int32_t pieces = int32_t(c1 - c0) + 1;
-                        const float* const p0 = p.part + (2 * c0 + (cut.begin(c0) != x.item)) * kPart;
-                        auto piece = [&](int32_t i) { return i ? p.part + 2 * (c0 + i) * kPart : p0; };
-                        for (int32_t row = int32_t(warp); row < R; row += W) {
+                        const int64_t first = 2 * c0 + (cut.begin(c0) != x.item);
+                        for (int32_t j = int32_t(warp); j < R << hs; j += W) {
+                            const int32_t of = hs ? j / R : 0, row = j - of * R;
+                            auto piece = [&](int32_t i) {
+                                return p.part + (((i ? 2 * (c0 + i) : first) << hs) + of) * kPart;
+                            };
                             float mx = -INFINITY, sum = 0.f, v[E] = {};
                             for (int32_t i0 = 0; i0 < pieces; i0 += 32) {
                                 const int32_t i = i0 + int32_t(lane), n = min(32, pieces - i0);
@@ -739,7 +769,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                             }
 #pragma unroll
                             for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                            finish(row, v, mx, sum);
+                            finish(of, row, v, mx, sum);
                         }
                     }
                 }
@@ -749,7 +779,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             if (lane == 0) atomicAdd(const_cast<uint32_t*>(flag) + 3, 1u);
         }
         __syncthreads();  // the list has been read
-        u = segs[count - 1].item + segs[count - 1].j0 + segs[count - 1].steps;
+        u = segs[count - 1].item + segs[count - 1].j0 + segs[count - 1].units;
     }
     if (warp >= W)  // every load has landed before the CTA ends
         for (uint32_t i = loaded - min(loaded, uint32_t(G::kStages)); i != loaded; ++i) {
@@ -779,7 +809,7 @@ int launch8(const AttnParams& p, cudaStream_t s) {
         if (e != cudaSuccess) return int(e);
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
-    const uint32_t sms = sm_count(), most = kMaxCtas * 16 / G::kRows;  // (by the scratch)
+    const uint32_t sms = sm_count(), most = kMaxCtas * 16 / (G::kRows * G::kHeads);  // (by the scratch)
     // (the append before it lets it begin early)
     return int(launch_after(kernel, sms < most ? sms : most, G::kThreads, G::kSmem, s, p, km, vm));
 }
