@@ -113,13 +113,13 @@ def test_layouts_long_caches_and_reuse(cuda_device, native_lib, q):
 
 
 @pytest.mark.parametrize("q", [1, 2, 3])
-@pytest.mark.parametrize("heads", [(16, 16, 64), (48, 6, 64), (24, 3, 64), (32, 4, 64), (16, 8, 128), (64, 8, 128)])
+@pytest.mark.parametrize("heads", [(16, 16, 64), (12, 6, 64), (24, 3, 64), (16, 4, 128)])
 def test_many_sequences(cuda_device, native_lib, heads, q):
     """Items of one, two and four kv heads, more than one list of pieces per CTA, windows among them."""
-    lengths = [(1 + i % q, 5 + 13 * i % 700) for i in range(90)] + [(0, 3), (q, 1), (q, 0)]
+    lengths = [(1 + i % q, 5 + 13 * i % 700) for i in range(80)] + [(0, 3), (q, 1), (q, 0)]
     Call8(lengths, *heads, page=16, q_scale=2.0).run()
     Call8(lengths, *heads, page=64, dtype=torch.bfloat16, layout="hnd", window=100, sinks=3).run()
-    Call8([(q, 7 + i % 60) for i in range(600)], heads[0], heads[1], heads[2], page=32).run()
+    Call8([(q, 7 + i % 60) for i in range(500)], heads[0] // heads[1], 1, heads[2], page=32).run()
 
 
 @pytest.mark.parametrize("q", [1, 60])
