@@ -108,28 +108,24 @@ __device__ __forceinline__ uint4 narrow(const float* x) {
     return make_uint4(T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7]));
 }
 
-// Angles of a lane's eight pairs, two pairs side by side. Products and sums are
-// rounded one by one: x (-s) is -(x s), and no pair of them is fused.
+// Angles of a lane's eight pairs. (Scalar products: the packed ones of two pairs come
+// out fused with the sums.)
 struct Turn {
-    uint64_t c[4], s[4], n[4];  // cosines, sines, and the sines negated
+    float c[8], s[8];
     __device__ __forceinline__ void load(const float* row, uint32_t i, uint32_t half) {
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-            const float4 x = *reinterpret_cast<const float4*>(row + i * 8 + e * 2);
-            const float4 y = *reinterpret_cast<const float4*>(row + half + i * 8 + e * 2);
-            c[e] = tc::pack2(x.x, x.y), c[e + 1] = tc::pack2(x.z, x.w);
-            s[e] = tc::pack2(y.x, y.y), s[e + 1] = tc::pack2(y.z, y.w);
-            n[e] = tc::pack2(-y.x, -y.y), n[e + 1] = tc::pack2(-y.z, -y.w);
+        for (int e = 0; e < 8; e += 4) {
+            *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(row + i * 8 + e);
+            *reinterpret_cast<float4*>(s + e) = *reinterpret_cast<const float4*>(row + half + i * 8 + e);
         }
     }
     template <int step, int next>  // from a pair's first to its second, and to the next pair
     __device__ __forceinline__ void pairs(float* x) const {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float* const y = x + 2 * next * e;
-            const uint64_t a = tc::pack2(y[0], y[next]), b = tc::pack2(y[step], y[step + next]);
-            tc::unpack2(tc::add2(tc::mul2(a, c[e]), tc::mul2(b, n[e])), y[0], y[next]);
-            tc::unpack2(tc::add2(tc::mul2(b, c[e]), tc::mul2(a, s[e])), y[step], y[step + next]);
+        for (int e = 0; e < 8; ++e) {
+            const float a = x[next * e], b = x[next * e + step];
+            x[next * e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
+            x[next * e + step] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
         }
     }
     __device__ __forceinline__ void apply(float* x, bool interleaved) const {  // x: pieces a and b
