@@ -196,6 +196,58 @@ def test_layouts_positions_and_rows_behind(cuda_device, native_lib, int8):
 
 
 @pytest.mark.parametrize("int8", [False, True])
+def test_keys_alone_large_pages_and_slices(cuda_device, native_lib, int8):
+    """No queries; pages of 256 slots; pools that are one layer's part of all layers'; a key head for all."""
+    from leanstream_b200 import append_cache
+
+    for dim in (64, 128):
+        c = Case(LENGTHS[2], dim=dim, page=256, int8=int8)
+        for name in ("k_pages", "v_pages", "exponents")[:3 if int8 else 2]:
+            t = getattr(c, name)
+            layers = torch.zeros(t.shape[0], 3, *t.shape[1:], dtype=t.dtype, device="cuda")
+            layers[:, 1] = t
+            setattr(c, name, layers[:, 1])
+        c.k_new = c.k_new[:, :1].expand(-1, 2, -1)
+        c.keep()
+        append_cache(**{**c.kwargs(), "q": None, "q_out": None})
+        torch.cuda.synchronize()
+        assert (c.q_out == 7).all()
+        append_cache(**c.kwargs())
+        torch.cuda.synchronize()
+        assert c.error.item() == 0
+        c.check()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_many_sequences_and_tokens(cuda_device, native_lib, int8):
+    """Against the same rows appended sequence by sequence: more tasks than warps, and
+    more sequences than a CTA counts at a time."""
+    from leanstream_b200 import append_cache
+
+    for lengths in ([(700 + 37 * i, 900 + 41 * i) for i in range(9)], [(1 + i % 5, 9 + i % 40) for i in range(700)]):
+        c = Case(lengths, 12, 4, 128, 32, torch.bfloat16, int8, 48, positions=True)
+        append_cache(**c.kwargs())
+        torch.cuda.synchronize()
+        assert c.error.item() == 0
+        got = [t.clone() for t in (c.k_pages, c.v_pages, c.q_out)] + ([c.exponents.clone()] if int8 else [])
+        for now, was in zip((c.k_pages, c.v_pages, c.exponents), c.before):
+            if now is not None:
+                now.copy_(was)
+        c.q_out.fill_(7)
+        at = 0
+        for b, (q, n) in enumerate(lengths):
+            part = slice(at, at + q)
+            append_cache(**{**c.kwargs(), "k_new": c.k_new[part], "v_new": c.v_new[part], "q": c.q[part],
+                            "q_out": c.q_out[part], "positions": c.positions[part], "kv_len": c.kv_len[b:b + 1],
+                            "page_table": c.page_table[b:b + 1],
+                            "q_start": torch.tensor([0, q], dtype=torch.int32, device="cuda")})
+            at += q
+        torch.cuda.synchronize()
+        for a, b in zip(got, (c.k_pages, c.v_pages, c.q_out, c.exponents)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("int8", [False, True])
 def test_queries_in_place_and_streams(cuda_device, native_lib, int8):
     c = Case(LENGTHS[2], int8=int8)
     same = c.q.clone()

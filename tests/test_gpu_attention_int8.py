@@ -236,6 +236,51 @@ def test_offsets_past_32_bits(cuda_device, native_lib, q):
     c.run()
 
 
+@pytest.mark.parametrize("q", [1, 5, 60])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_pages_of_256_and_slices_of_a_pool(cuda_device, native_lib, q, dim):
+    """The largest pages; pools and exponents that are one layer's part of all layers'."""
+    c = Call8([(q, 900), (q, 256), (q, 257)], 8, 2, dim, page=256)
+    c.run()
+    for name in ("k_pages", "v_pages", "exponents"):
+        t = getattr(c, name)
+        layers = torch.randint(-128, 128, (t.shape[0], 3, *t.shape[1:]), device="cuda").to(torch.int8)
+        layers[:, 1] = t
+        setattr(c, name, layers[:, 1])
+    c.run()
+
+
+@pytest.mark.parametrize("q", [1, 60])
+def test_two_engines_at_once(cuda_device, native_lib, q):
+    calls = [Call8([(q, 5000), (q, 300)], seed=i, page=32) for i in range(2)]
+    engines, streams = [c.engine() for c in calls], [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, engine, stream in zip(calls, engines, streams):
+            engine.run(stream=stream, **c.kwargs())
+    torch.cuda.synchronize()
+    for c, engine in zip(calls, engines):
+        assert engine.error() == 0
+        c.check()
+
+
+@pytest.mark.parametrize("bound", [3, 64, 1 << 16])
+@pytest.mark.parametrize("batch", [3, 1 << 13])
+def test_loose_bound(cuda_device, native_lib, batch, bound):
+    """max_q far above the new tokens, most sequences without any."""
+    from leanstream_b200 import PagedAttention
+
+    lengths = [(0, 9), (3, 300), (1, 77)] + [(0, 0)] * (batch - 3)
+    lengths[-1] = lengths[-1] if batch == 3 else (2, 50)
+    c = Call8(lengths, 8, 2, 64, page=32)
+    engine = PagedAttention(8, 2, 64, page_size=32, cache_dtype="int8", max_sequences=batch,
+                            max_tokens=c.q.shape[0], max_queries=bound)
+    engine.run(**{**c.kwargs(), "max_q": bound})
+    torch.cuda.synchronize()
+    assert engine.error() == 0
+    c.check()
+
+
 @pytest.mark.parametrize("q", [1, 50])
 def test_bad_lengths_and_pages_are_reported(cuda_device, native_lib, q):
     from leanstream_b200 import _native as N
