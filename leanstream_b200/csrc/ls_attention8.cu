@@ -784,7 +784,8 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             __threadfence_block();
             if (lane == 0) atomicAdd(const_cast<uint32_t*>(flag) + 3, 1u);
         }
-        __syncthreads();  // the list has been read
+        if (count < uint32_t(kSegCount)) break;  // the list was the whole range
+        __syncthreads();                         // it has been read
         u = segs[count - 1].item + segs[count - 1].j0 + segs[count - 1].units;
     }
     if (warp >= W)  // every load has landed before the CTA ends
