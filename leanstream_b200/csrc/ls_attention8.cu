@@ -434,6 +434,7 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (lane < 2) prefetch_map(lane ? &vmap : &kmap);
     }
+    if (tid == 0) flag[0] = flag[1] = flag[3] = 0;
     after_start();
     after_wait();
     // tiles of this thread's sequence (of the first kThreads), and of the call; y: 1
@@ -482,8 +483,10 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
     for (int64_t u = u_begin; u < u_end;) {
         // the next pieces, listed by the threads of their sequences: items (y
         // counts sequences with rows) from the one that holds unit u
-        if (tid == 0) flag[0] = flag[1] = flag[3] = 0;
-        __syncthreads();
+        if (u != u_begin) {
+            if (tid == 0) flag[0] = flag[1] = flag[3] = 0;
+            __syncthreads();
+        }
         int64_t base = 0;
         int32_t seqs = 0;
         for (uint32_t b0 = 0; b0 < p.B && base < u_end; b0 += G::kThreads) {
@@ -575,8 +578,8 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
             };
             int2 id = pages_of(0, int32_t(lane)), n_id;
             uint32_t ex = exponents_of(0, int32_t(lane), id), n_ex = 0;
+            bool known = false;  // the next block's pages: of the second looked up when the first loads
             after();
-            n_id = pages_of(n_c, n_at + int32_t(lane));
             while (ok && c < count) {
                 const Seg8& x = segs[c];
                 const int32_t n = min(kBlockSteps, x.steps(hs) - at), h = x.h + int32_t(lane & side_by);
@@ -617,6 +620,8 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                     }
                 }
                 __syncwarp();
+                if (!known) n_id = pages_of(n_c, n_at + int32_t(lane));
+                known = true;
                 n_ex = exponents_of(n_c, n_at + int32_t(lane), n_id);
                 if (ok) loaded += uint32_t(max(n, 0));
                 c = n_c, at = n_at, id = n_id, ex = n_ex;
