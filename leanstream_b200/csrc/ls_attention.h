@@ -88,7 +88,7 @@ bool encode_codes(CUtensorMap* map, const void* base, const AttnParams& p, int64
                   uint32_t slots);
 uint32_t sm_count();  // of the current device
 // Few rows over a cache in 8 bits (ls_attention8.cu).
-constexpr uint32_t kMaxRows8 = 24;
+constexpr uint32_t kMaxRows8 = 32;
 int launch_decode8(const AttnParams& p, uint32_t dtype, cudaStream_t stream);
 int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream);
 

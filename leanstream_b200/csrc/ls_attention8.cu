@@ -49,7 +49,7 @@ using namespace tc;
 constexpr int kStep = 2 * kBlock;          // slots of a step
 constexpr int kSegCount = 48;              // pieces listed at a time
 constexpr int64_t kItemCost8 = 16;         // steps that beginning and joining an item counts as
-constexpr int64_t kMinSteps8 = 24;         // steps that a CTA takes at least
+constexpr int64_t kMinSteps8 = 16;         // steps that a CTA takes at least
 constexpr uint64_t kGraceNs = 1000000000ull;
 constexpr uint64_t kShortNs = 100000;      // bounds that a barrier's try may sleep over: a load takes less
 
@@ -58,11 +58,11 @@ constexpr uint64_t kShortNs = 100000;      // bounds that a barrier's try may sl
 template <int D, int NT>
 struct Geo8 {
     static constexpr int kWarps = NT <= 2 ? 8 : 6, kLoaders = NT <= 2 ? 4 : 2, kThreads = 32 * (kWarps + kLoaders);
-    static constexpr int kSide = NT == 3 && D == 64 ? 4 : (kWarps + 1) / 2;
+    static constexpr int kSide = NT >= 3 && D == 64 ? 4 : (kWarps + 1) / 2;
     // kv heads of an item, at most: the codes of 64 elements take half a line of 128 bytes
     // (48 sequences of up to 5000 slots, 16 kv heads: 98 us with one, 72 with two, 68 with
     // four; of 128 elements no gain)
-    static constexpr int kHeads = D == 128 ? 1 : NT == 1 ? 4 : 2;
+    static constexpr int kHeads = D == 128 || NT == 4 ? 1 : NT == 1 ? 4 : 2;
     static_assert(kWarps % kHeads == 0 && kSide % kHeads == 0, "a warp takes one of them");
     static constexpr bool kSharedQ = NT > 1;  // one tile's queries stay in registers, more in shared memory
     static constexpr int kRows = 8 * NT;
@@ -827,7 +827,10 @@ int launch8(const AttnParams& p, cudaStream_t s) {
 }
 template <class T, int D>
 int launch8(const AttnParams& p, cudaStream_t s) {
-    return p.rows <= 8 ? launch8<T, D, 1>(p, s) : p.rows <= 16 ? launch8<T, D, 2>(p, s) : launch8<T, D, 3>(p, s);
+    return p.rows <= 8    ? launch8<T, D, 1>(p, s)
+           : p.rows <= 16 ? launch8<T, D, 2>(p, s)
+           : p.rows <= 24 ? launch8<T, D, 3>(p, s)
+                          : launch8<T, D, 4>(p, s);
 }
 
 }  // namespace
