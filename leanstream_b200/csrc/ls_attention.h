@@ -87,7 +87,7 @@ bool encode_map(CUtensorMap* map, bool bf16, const void* base, uint32_t rank, co
 bool encode_codes(CUtensorMap* map, const void* base, const AttnParams& p, int64_t ss, int64_t hs, int64_t ps,
                   uint32_t slots);
 uint32_t sm_count();  // of the current device
-// Few rows over a cache in 8 bits (ls_attention8.cu).
+// Few rows of a kv head over a cache in 8 bits (ls_attention8.cu).
 constexpr uint32_t kMaxRows8 = 32;
 int launch_decode8(const AttnParams& p, uint32_t dtype, cudaStream_t stream);
 int launch_chunk(const AttnParams& p, uint32_t dtype, const ChunkScratch& s, uint32_t sms, cudaStream_t stream);

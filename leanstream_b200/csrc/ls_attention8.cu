@@ -28,9 +28,9 @@
 // passes it by 2^kRaise. P is rounded once, to float16, times 2^kChunkShift.
 //
 // Bound by the read of the cache: two sequences of up to 150000 slots, 64 heads of 128
-// over 8, take 98 to 105 us, of which 90 stream at 5.9 TB/s; 48 of up to 5000 slots, 32
-// heads, 59 us; 12 of up to 9000 slots with up to 5 tokens (20 rows, six warps) 58 us; one
-// of 130 slots 7.5 us. Rows as the M dimension, one CTA of four warps that load for
+// over 8, take 97 to 104 us, of which 90 stream at 5.9 TB/s; 48 of up to 5000 slots, 32
+// heads, 58 us; 12 of up to 9000 slots with up to 5 tokens (20 rows, six warps) 57 us; one
+// of 130 slots 6.8 us. Rows as the M dimension, one CTA of four warps that load for
 // themselves: 163, 90 and (on the chunk kernel) 80 us.
 #include <stdint.h>
 
@@ -48,8 +48,10 @@ using namespace tc;
 
 constexpr int kStep = 2 * kBlock;          // slots of a step
 constexpr int kSegCount = 48;              // pieces listed at a time
-constexpr int64_t kItemCost8 = 16;         // steps that beginning and joining an item counts as
-constexpr int64_t kMinSteps8 = 16;         // steps that a CTA takes at least
+// Steps that beginning and joining an item counts as, and that a CTA takes at least.
+// (With 10 and 24 as the cost 48 sequences of up to 5000 slots take 59.0 us, with 16
+// 57.6; with 40 as the least, or a cost of 10, one of 130 slots is cut: 9.7 against 6.9.)
+constexpr int64_t kItemCost8 = 16, kMinSteps8 = 16;
 constexpr uint64_t kGraceNs = 1000000000ull;
 constexpr uint64_t kShortNs = 100000;      // bounds that a barrier's try may sleep over: a load takes less
 
