@@ -352,3 +352,65 @@ def test_append_and_attend(cuda_device, native_lib, dtype, q):
             c.keys[b] = kp[where, i % page].double() * size[..., 0][..., None]
             c.values[b] = vp[where, i % page].double() * size[..., 1][..., None]
         c.check()
+
+
+@pytest.mark.parametrize("q", [1, 40])
+def test_step_in_a_graph_between_other_work(cuda_device, native_lib, q):
+    """Append and attention captured after copies, fills and another stream's work,
+    before some; replayed step after step with lengths that grow on the device."""
+    from leanstream_b200 import PagedAttention, append_cache
+    from test_gpu_append import angles
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    heads, hk, dim, page, batch, steps = 8, 2, 64, 16, 2, 4
+    int8, int32 = dict(dtype=torch.int8, device="cuda"), dict(dtype=torch.int32, device="cuda")
+    half = dict(dtype=torch.float16, device="cuda")
+    table = torch.randperm(40, generator=g, device="cuda")[:batch * 15].int().reshape(batch, 15)
+    pages, exponents = [torch.zeros(40, page, hk, dim, **int8) for _ in range(2)], torch.zeros(40, hk, 1, 2, **int8)
+    kv_len, more = torch.zeros(batch, **int32), torch.full((batch,), q, **int32)
+    x, given = (torch.empty(batch * q, heads + 2 * hk, dim, **half) for _ in range(2))
+    out, last = torch.empty(batch * q, heads, dim, **half), torch.empty(batch * q, heads, dim, **half)
+    lse = torch.empty(batch * q, heads, device="cuda")
+    starts, cos_sin = (torch.arange(batch + 1, device="cuda") * q).int(), angles(200, dim)
+    engine = PagedAttention(heads, hk, dim, page_size=page, cache_dtype="int8", max_sequences=batch,
+                            max_tokens=batch * q, max_queries=q)
+    other = torch.cuda.Stream()
+
+    def step():
+        main = torch.cuda.current_stream()
+        other.wait_stream(main)
+        with torch.cuda.stream(other):
+            kv_len.add_(more)
+        x.copy_(given)
+        main.wait_stream(other)
+        append_cache(q=x[:, :heads], q_out=x[:, :heads], k_new=x[:, heads:heads + hk], v_new=x[:, heads + hk:],
+                     k_pages=pages[0], v_pages=pages[1], exponents=exponents, page_table=table, q_start=starts,
+                     kv_len=kv_len, cos_sin=cos_sin)
+        out.zero_()
+        engine.run(q=x[:, :heads], output=out, k_pages=pages[0], v_pages=pages[1], exponents=exponents,
+                   page_table=table, q_start=starts, kv_len=kv_len, max_q=q, lse=lse)
+        last.copy_(out)
+
+    given.copy_(torch.randn(given.shape, generator=g, device="cuda"))
+    step()  # (sets kernel attributes)
+    torch.cuda.synchronize()
+    kv_len.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(steps):
+        given.copy_(torch.randn(given.shape, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        n = (i + 1) * q
+        assert engine.error() == 0 and kv_len.tolist() == [n] * batch
+        c = Call8([(q, n)] * batch, heads, hk, dim, page)
+        c.q, c.output, c.lse = x[:, :heads].clone(), last, lse
+        c.k_pages, c.v_pages, c.exponents = pages[0], pages[1], exponents
+        at = torch.arange(n, device="cuda")
+        for b in range(batch):
+            where = table[b].long()[at // page]
+            size = 2.0 ** exponents[where, :, 0].double()
+            c.keys[b] = pages[0][where, at % page].double() * size[..., 0][..., None]
+            c.values[b] = pages[1][where, at % page].double() * size[..., 1][..., None]
+        c.check()
