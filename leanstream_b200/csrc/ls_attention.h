@@ -13,10 +13,12 @@ constexpr uint32_t kErrPage = 1u << 2;    // a visible slot's page index is outs
 
 constexpr uint32_t kMaxSlots = 0x7fff0000u;  // of a sequence: a tile past the last slot still counts in 32 bits
 
-// The cache in 8 bits: slots that share an exponent, and the exponent of a block
-// with a value that is not finite (it reads as NaN).
+// The cache in 8 bits: slots that share an exponent, the exponent of a block with a
+// value that is not finite (it reads as NaN), and what the attention takes for a block
+// that is not read: below every other, so that it is never the largest of a sequence.
 constexpr int kBlockShift = 4, kBlock = 1 << kBlockShift;
-constexpr int32_t kNoExponent = -128;
+constexpr int32_t kNoExponent = -128, kNeutral = -127;
+constexpr uint32_t kNeutral2 = 0x101u * uint8_t(kNeutral);  // of keys and values
 static_assert(kBlock == LS_B200_CACHE_BLOCK, "public block size");
 
 // ls_b200_attention_args in the kernels' units. Strides are in elements.

@@ -98,7 +98,8 @@ struct Seg8 {
 static_assert(sizeof(Seg8) == 64, "list entries");
 
 // What a stage's step needs beside its codes: its first slot, 1 where a row does
-// not see all of it; the exponents of both blocks (key's, value's).
+// not see all of it; the exponents of both blocks (key's, value's), kNeutral where no
+// row sees the block or its page is outside the pool.
 struct Note {
     uint32_t k, ex;
 };
@@ -558,19 +559,19 @@ __global__ void __launch_bounds__(Geo8<D, NT>::kThreads, 1)
                 if (seen(x, k + kBlock)) id.y = pairs && id.x >= 0 ? id.x : page(k + kBlock);
                 return id;
             };
+            // (blocks without any stay neutral: they leave the unit of the sums as it is)
             auto exponents_of = [&](uint32_t c, int32_t step, int2 id) -> uint32_t {
-                uint32_t ex = 0;
-                if (!note || c >= count) return ex;
+                uint32_t x0 = kNeutral2, x1 = kNeutral2;
+                if (!note || c >= count) return 0;
                 const Seg8& x = segs[c];
                 const int32_t in = step < x.steps(hs) ? x.slot0(step >> hs) & int32_t(p.P - 1) : 0;
                 const uint8_t* at = p.ex + int64_t(x.h + int32_t(uint32_t(step) & side_by)) * p.ex_hs;
                 if (uint32_t(id.x) < p.pages)
-                    ex = *reinterpret_cast<const uint16_t*>(at + int64_t(id.x) * p.ex_ps + (in >> 3));
+                    x0 = *reinterpret_cast<const uint16_t*>(at + int64_t(id.x) * p.ex_ps + (in >> 3));
                 if (uint32_t(id.y) < p.pages)
-                    ex |= uint32_t(*reinterpret_cast<const uint16_t*>(at + int64_t(id.y) * p.ex_ps +
-                                                                      (((in + kBlock) & int32_t(p.P - 1)) >> 3)))
-                          << 16;
-                return ex;
+                    x1 = *reinterpret_cast<const uint16_t*>(at + int64_t(id.y) * p.ex_ps +
+                                                            (((in + kBlock) & int32_t(p.P - 1)) >> 3));
+                return x0 | x1 << 16;
             };
             uint32_t c = 0, n_c = 0;
             int32_t at = 0, n_at = 0;

@@ -417,18 +417,18 @@ __global__ void __launch_bounds__(Q8 ? kThreads8 : kThreads, 1)
             const int32_t* trow = p.table + int64_t(w.b) * p.table_s;
             const uint8_t* eh = p.ex + int64_t(w.h) * p.ex_hs;
             // lanes 0 and 1: where the exponents of their block of a step lie; blocks that no
-            // row sees are zeros (-127)
+            // row sees are zeros (kNeutral)
             auto page_of = [&](int32_t step) -> int32_t {
                 if (step >= w.steps || lane >= 2) return -1;
                 const int32_t k0 = w.slot0(step) + int32_t(mine + lane * 16), k1 = k0 + 16;
                 return (k0 < w.hi && k1 > w.lo) || k0 < w.sink ? trow[k0 >> p.pshift] : -1;
             };
             auto exponents_of = [&](int32_t step, int32_t id) -> uint32_t {
-                if (uint32_t(id) >= p.pages) return 0x8181u;
+                if (uint32_t(id) >= p.pages) return kNeutral2;
                 const int32_t in = (w.slot0(step) + int32_t(mine + lane * 16)) & int32_t(p.P - 1);
                 return *reinterpret_cast<const uint16_t*>(eh + int64_t(id) * p.ex_ps + (in >> 3));
             };
-            uint32_t ex = exponents_of(0, page_of(0)), next_ex = 0x8181u;
+            uint32_t ex = exponents_of(0, page_of(0)), next_ex = kNeutral2;
             for (int32_t j = 0; j < w.steps; ++j) {
                 const int32_t next_id = page_of(j + 1);
                 for (int kv = 0; kv < 2; ++kv, ++slot) {
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(Q8 ? kThreads8 : kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int32_t e = int8_t(__shfl_sync(0xffffffffu, ex, i) >> (8 * kv));
-                        step[i] = e == -127 ? 0u : step_of<T>(e);
+                        step[i] = e == kNeutral ? 0u : step_of<T>(e);
                     }
                     if (kv) next_ex = exponents_of(j + 1, next_id);
                     if (!(ok = warp_wait<!Q8>(bar.codes_full(cs), cn & 1u, p.timeout_ns))) break;
