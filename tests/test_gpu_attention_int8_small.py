@@ -97,3 +97,19 @@ def test_pages_outside_the_pool(cuda_device, native_lib, dtype, shift, q):
         torch.cuda.synchronize()
         assert engine.error() == N.ATTN_PAGE
         c.check()
+
+
+@pytest.mark.parametrize("q", [1, 4, 6, 8])
+@pytest.mark.parametrize("shift", [-111, -115, -117, -118])
+def test_the_lowest_exponents(cuda_device, native_lib, shift, q):
+    """bfloat16 down to -126."""
+    for page in (16, 32):
+        Small([(min(q, n), n) for n in SHORT], shift, dtype=torch.bfloat16, page=page).run()
+        c = Small([(q, 500), (q, 2000)], shift, dtype=torch.bfloat16, page=page, heads=16, kv_heads=8, dim=64)
+        for b, n in enumerate((500, 2000)):  # every block at the lowest one
+            i = torch.arange(n, device="cuda")
+            where = c.page_table[b].long()[i // page]
+            c.exponents[where, :, i // 16 % (page // 16), 1] = -126
+            c.values[b] = c.v_pages[where, i % page].double() * 2.0 ** -126
+        c.largest = -126
+        c.run()
