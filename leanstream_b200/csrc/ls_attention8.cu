@@ -281,7 +281,7 @@ struct Rows8 {
         }
         if (max(ev[0], ev[1]) > most) {
             const int32_t top = max(ev[0], ev[1]);
-            const float f = two_to(max(most - top, -126));
+            const float f = most - top < -126 ? 0.f : two_to(most - top);
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll

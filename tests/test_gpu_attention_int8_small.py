@@ -113,3 +113,25 @@ def test_the_lowest_exponents(cuda_device, native_lib, shift, q):
             c.values[b] = c.v_pages[where, i % page].double() * 2.0 ** -126
         c.largest = -126
         c.run()
+
+
+@pytest.mark.parametrize("q", [1, 6])
+def test_values_of_no_weight_and_a_large_exponent(cuda_device, native_lib, q):
+    """A block 2^226 above the others whose probabilities are far below 2^-226: the others may count as 0,
+    and for no more than themselves."""
+    c = Small([(q, 600)], -118, dtype=torch.bfloat16, page=16, spread=1, marked=False)
+    where = int(c.page_table[0, 16])  # slots 256 to 271, of a warp that has taken earlier ones
+    # logits near -570, against the others' few tens
+    c.k_pages[where] = -127
+    c.q.abs_()
+    c.exponents[where, :, 0, 0], c.exponents[where, :, 0, 1] = -1, 100
+    c.keys[0][256:272] = -63.5
+    c.values[0][256:272] = c.v_pages[where].double() * 2.0 ** 100
+    engine = c.engine()
+    engine.run(**c.kwargs())
+    torch.cuda.synchronize()
+    assert engine.error() == 0
+    _, area, lse, _, _ = c.expected()
+    # area + u (area + ..), with the probabilities' own rounding
+    assert (c.output.double().abs() <= area * (1 + 2.0 ** -8) * (1 + 2.0 ** -10) + SMALLEST[torch.bfloat16] / 2).all()
+    assert (c.lse.double() - lse).abs().max().item() <= 2e-5
