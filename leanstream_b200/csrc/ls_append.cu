@@ -431,12 +431,10 @@ extern "C" int ls_b200_append_cache(const ls_b200_append_args* a, void* stream) 
         a->interleaved > 1 || a->reserved)
         return EINVAL;
     const bool int8 = a->cache_dtype == LS_B200_INT8;
-    if (a->cos_sin ? !a->rotary_dim || a->rotary_dim % 16 || a->rotary_dim > a->head_dim || !a->angles ||
-                         a->angles > 0x7fffffffu
-                   : a->rotary_dim || a->positions || a->q)
-        return EINVAL;
+    if (a->rotary_dim % 16 || a->rotary_dim > a->head_dim || a->angles > 0x7fffffffu) return EINVAL;
+    if (!a->batch || !a->tokens) return 0;  // (an empty tensor's address may be NULL)
+    if (a->cos_sin ? !a->rotary_dim || !a->angles : a->rotary_dim || a->positions || a->q) return EINVAL;
     if ((!a->q) != (!a->q_out) || (!a->q) != (!a->q_heads)) return EINVAL;
-    if (!a->batch || !a->tokens) return 0;
     if (!a->k_new || !a->v_new || !a->k_pages || !a->v_pages || !a->page_table || !a->q_start || !a->kv_len ||
         !a->pages || !a->table_pages || int8 != (a->exponents != nullptr))
         return EINVAL;

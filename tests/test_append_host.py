@@ -112,3 +112,31 @@ def test_tensors_are_checked(calls):  # noqa: F811
             with pytest.raises(ValueError, match=name):
                 append_cache(**good(0, True, **{name: twice}))
     assert not calls
+
+
+@pytest.mark.parametrize("change", [
+    dict(), dict(q=None, q_out=None), dict(q=None, q_out=None, k_new=None, v_new=None, positions=None),
+    dict(q=None, q_out=None, k_new=None, v_new=None, cos_sin=None, angles=0),
+    {**INT8, "q": None, "q_out": None, "k_new": None, "v_new": None}], ids=str)
+def test_no_new_tokens(native_lib, change):
+    """Tensors without elements have no address."""
+    for empty in (dict(tokens=0), dict(tokens=0, batch=0)):
+        assert native_lib.ls_b200_append_cache(C.byref(_args(**{**change, **empty})), None) == 0
+    for wrong in (dict(rotary_dim=24), dict(rotary_dim=144), dict(head_dim=96), dict(interleaved=2)):
+        assert native_lib.ls_b200_append_cache(C.byref(_args(**{**change, **wrong, "tokens": 0})), None) == errno.EINVAL
+
+
+def test_no_new_tokens_by_the_entry_point(native_lib, monkeypatch):
+    from leanstream_b200 import append_cache, attention
+
+    monkeypatch.setattr(attention, "_current_device", lambda: 0)
+    monkeypatch.setattr(attention, "_raw_stream", lambda index: 0)
+    i32 = dict(dtype=torch.int32)
+    empty = dict(k_new=on(0, 0, 2, 128), v_new=on(0, 0, 2, 128), q=on(0, 0, 8, 128), q_out=on(0, 0, 8, 128),
+                 positions=on(0, 0, **i32))
+    assert empty["q"].data_ptr() == 0
+    for int8 in (False, True):
+        append_cache(**good(0, int8, **empty))
+        append_cache(**good(0, int8, **{**empty, "q": None, "q_out": None}))
+        append_cache(**good(0, int8, **empty, kv_len=on(0, 0, **i32), q_start=on(0, 1, **i32),
+                            page_table=on(0, 0, 4, **i32)))
