@@ -431,7 +431,9 @@ enum {
                                      * new token's slot holds its key and value, or what it held before */
     LS_B200_ATTN_LENGTH = 1u << 1,  /* q_start / kv_len of a sequence do not fit the call: skipped */
     LS_B200_ATTN_PAGE = 1u << 2,    /* a page index of a visible slot is outside the pool */
-    LS_B200_ATTN_POSITION = 1u << 3 /* a token's position has no angles: skipped */
+    LS_B200_ATTN_POSITION = 1u << 3, /* a token's position has no angles: skipped */
+    LS_B200_ATTN_EXPONENT = 1u << 4 /* an exponent of a visible block is outside the range of the attention's type:
+                                     * the block reads as NaN */
 };
 
 /* Attention of the new tokens of `batch` sequences over their cache. Token t of
@@ -506,7 +508,9 @@ enum { LS_B200_CACHE_BLOCK = 16 };
  * output; no k_new, v_new, weights. Everything else, the scratch too, is as for
  * ls_b200_paged_attention, but that for both types a probability times 2^(its
  * block's exponent - the largest of the sequence's values) below 2^-32 of the row's
- * largest may count as 0. Blocks without a visible slot are not read. */
+ * largest may count as 0. Blocks without a visible slot are not read. The others'
+ * exponents lie in the range of dtype that ls_b200_append_cache gives below, as they
+ * do where the cache was filled from that type, or from float16 for bfloat16 queries. */
 typedef struct ls_b200_cache_exponents {
     const int8_t* exponents;        /* [pages][kv_heads][page_size / LS_B200_CACHE_BLOCK][2] */
     int64_t page_stride, head_stride; /* even */

@@ -133,7 +133,7 @@ class BatchArgs(C.Structure):
                 ("timeout_ns", C.c_uint64)]
 
 FP16, BF16, INT8 = 0, 1, 2
-ATTN_TIMEOUT, ATTN_LENGTH, ATTN_PAGE, ATTN_POSITION = 1, 2, 4, 8
+ATTN_TIMEOUT, ATTN_LENGTH, ATTN_PAGE, ATTN_POSITION, ATTN_EXPONENT = 1, 2, 4, 8, 16
 CACHE_BLOCK = 16  # slots of a cache in 8 bits that share an exponent
 
 

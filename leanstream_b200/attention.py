@@ -98,7 +98,10 @@ class PagedAttention:
     overlap. `scratch` = (pointer, bytes) supplies caller-owned, zeroed device
     memory instead; `error` is then the device address of a caller-owned, zeroed
     32-bit error word (or None). cache_dtype "int8": the cache is in 8 bits, as
-    append_cache fills it (no weights; the call does not append)."""
+    append_cache fills it (no weights; the call does not append). Its exponents
+    then lie in the range of `dtype`, -24 to 9 for float16 and -126 to 120 for
+    bfloat16, as they do where it was filled from that type: a visible block
+    outside reads as NaN and sets N.ATTN_EXPONENT."""
 
     def __init__(self, q_heads: int, kv_heads: int, head_dim: int, *, page_size: int, dtype="float16",
                  max_sequences: int, max_tokens: int, max_queries: int = 1, max_weights_length: int = 0, device=None,

@@ -470,8 +470,8 @@ extern "C" int ls_b200_append_cache(const ls_b200_append_args* a, void* stream) 
     p.tpages = a->table_pages, p.tokens = a->tokens, p.rotary = a->rotary_dim, p.angles = a->angles;
     p.interleaved = a->interleaved;
     while ((1u << p.pshift) < p.P) ++p.pshift;
-    p.lowest = a->dtype == LS_B200_FP16 ? -24 : -126;
-    p.highest = a->dtype == LS_B200_FP16 ? 9 : 120;
+    p.lowest = a->dtype == LS_B200_FP16 ? F16::kLowest : BF16::kLowest;
+    p.highest = a->dtype == LS_B200_FP16 ? F16::kHighest : BF16::kHighest;
     // Few tokens: a warp takes all of a block's rows. Many: every row group is a task, of
     // twice the heads.
     const bool many = p.tokens > 2 * p.B;

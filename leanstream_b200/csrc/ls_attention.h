@@ -18,7 +18,6 @@ constexpr uint32_t kMaxSlots = 0x7fff0000u;  // of a sequence: a tile past the l
 // that is not read: below every other, so that it is never the largest of a sequence.
 constexpr int kBlockShift = 4, kBlock = 1 << kBlockShift;
 constexpr int32_t kNoExponent = -128, kNeutral = -127;
-constexpr uint32_t kNeutral2 = 0x101u * uint8_t(kNeutral);  // of keys and values
 static_assert(kBlock == LS_B200_CACHE_BLOCK, "public block size");
 
 // ls_b200_attention_args in the kernels' units. Strides are in elements.
@@ -186,8 +185,10 @@ constexpr float kLog2e = 1.44269504088896341f;
 // 2^15 in both; what rounds to zero is below 2^-40, or 2^-32, of the row's largest.
 // (kRaise 4 and kChunkShift 11: 273 -> 296 us for 2048 tokens over 8192 slots, 32
 // heads of 128, with logits of deviation 4, whose maxima grow often.)
+// kLowest to kHighest: exponents of a cache in 8 bits that the type holds with any code.
 struct F16 {
     static constexpr uint32_t kUmmaFormat = 0;
+    static constexpr int32_t kLowest = -24, kHighest = 9;
     static constexpr float kShift = 15.f, kRaise = 8.f, kChunkShift = 7.f;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
@@ -207,6 +208,7 @@ struct F16 {
 };
 struct BF16 {  // (the exponents of 32-bit numbers)
     static constexpr uint32_t kUmmaFormat = 1;
+    static constexpr int32_t kLowest = -126, kHighest = 120;
     static constexpr float kShift = 0.f, kRaise = 8.f, kChunkShift = 0.f;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
@@ -224,6 +226,19 @@ struct BF16 {  // (the exponents of 32-bit numbers)
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 };
+
+// Exponents of blocks as the products take them, four bytes of v: those that are
+// `held` (bytes of ones) as they are, but outside T's range they are reported and read
+// as NaN; the others are kNeutral.
+template <class T>
+__device__ __forceinline__ uint32_t known_exponents(uint32_t v, uint32_t held, uint32_t* err) {
+    constexpr uint32_t kAll = 0x01010101u;
+    const uint32_t above = __vsub4(v, kAll * uint8_t(T::kLowest));  // the lowest
+    const uint32_t bad = __vcmpgtu4(above, kAll * uint32_t(T::kHighest - T::kLowest)) &
+                         ~__vcmpeq4(v, kAll * uint8_t(kNoExponent)) & held;
+    if (bad && err) atomicOr(err, uint32_t(LS_B200_ATTN_EXPONENT));
+    return (v & held & ~bad) | (kAll * uint8_t(kNoExponent) & bad) | (kAll * uint8_t(kNeutral) & ~held);
+}
 
 // First unit of CTA c when U units are cut evenly over G CTAs, and the CTA of a unit.
 __device__ __forceinline__ int64_t cut_begin(int64_t U, int64_t G, int64_t c) { return c * U / G; }
