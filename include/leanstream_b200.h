@@ -536,7 +536,10 @@ int ls_b200_paged_attention_int8(const ls_b200_attention_args* args, const ls_b2
  *
  * A token whose position has no angles is skipped: its slot, and its row of
  * q_out, are left as they were; so is everything behind the last sequence, and
- * the slots behind the last token. Pages that the call writes must be listed
+ * the slots behind the last token. In 8 bits that is their codes: they read with
+ * the exponent that their block gets from the rows that are written. A block none
+ * of whose new rows is written keeps its own, and begins anew no more than a block
+ * that the call does not touch. Pages that the call writes must be listed
  * once. Strides are in elements, non-negative multiples of 8 (pages in 8 bits:
  * 16; exponents: 2; cos_sin: 4); q_out may be q. */
 typedef struct ls_b200_append_args {

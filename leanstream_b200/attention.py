@@ -336,7 +336,8 @@ def append_cache(*, k_new, v_new, k_pages, v_pages, page_table, q_start, kv_len,
 
     error: an optional int32 device tensor, N.ATTN_* bits are ORed in (lengths,
     pages and positions that do not fit: what they would have touched is left as
-    it was). `stream` as in PagedAttention.run."""
+    it was, in 8 bits the codes, which read with the exponent of their block's
+    other new rows). `stream` as in PagedAttention.run."""
     new, pool, table, lengths = k_new.shape, k_pages.shape, page_table.shape, kv_len.shape
     e, cached, dev = k_new.dtype, k_pages.dtype, kv_len.get_device()
     qp = op = hq = q0 = q1 = o0 = o1 = ps = cs = rotary = angles = cs0 = ex = ex0 = ex1 = er = 0
