@@ -8,6 +8,7 @@ snapshot; nothing is JIT-compiled at import time.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -22,6 +23,10 @@ SOURCES = ("ls_kernel.cu", "ls_kernel_traced.cu", "ls_backend.cu", "ls_aux.cu", 
            "ls_append.cu", "ls_evict.cu")
 HEADERS = ("ls_internal.h", "ls_attention.h", "ls_tc.h")
 ARCH = ("-gencode", "arch=compute_100a,code=sm_100a")
+# Kernels that split the registers of their launch between their warps count on as many
+# as the compiler was told (a part of the mangled name, registers per thread); the
+# launch refuses any other number with ENOTSUP.
+REGISTERS = {"ls_attention_chunk.cu": (r"chunk_attn_kernelI\w*Lb1E", 128)}
 
 
 def nvcc() -> str:
@@ -42,6 +47,15 @@ def needs_build(target: Path = LIBRARY) -> bool:
 def _flags():
     return [*ARCH, "-O3", "-std=c++17", "-lineinfo", "-Xptxas", "-v", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
             "-I", str(ROOT / "include")]
+
+
+def check_registers(src: str, log: str) -> None:
+    """Raises where a kernel of REGISTERS got another number, by the assembler's report."""
+    name, want = REGISTERS.get(src, (None, 0))
+    for kernel, used in re.findall(r"Compiling entry function '(\w+)'(?:(?!Compiling).)*?Used (\d+) registers", log,
+                                   re.DOTALL):
+        if name and re.search(name, kernel) and int(used) != want:
+            raise RuntimeError(f"{src}: {kernel} has {used} registers per thread, its split counts on {want}")
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -66,6 +80,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
                               capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"nvcc failed on {src}:\n" + proc.stdout + proc.stderr)
+        check_registers(src, proc.stderr)
         os.replace(str(obj) + ".tmp", obj)
         return obj, proc.stderr
 
