@@ -13,11 +13,10 @@ constexpr uint32_t kErrPage = 1u << 2;    // a visible slot's page index is outs
 
 constexpr uint32_t kMaxSlots = 0x7fff0000u;  // of a sequence: a tile past the last slot still counts in 32 bits
 
-// The cache in 8 bits: slots that share an exponent, the exponent of a block with a
-// value that is not finite (it reads as NaN), and what the attention takes for a block
-// that is not read: below every other, so that it is never the largest of a sequence.
+// The cache in 8 bits: slots that share an exponent, and the exponent of a block
+// with a value that is not finite (it reads as NaN).
 constexpr int kBlockShift = 4, kBlock = 1 << kBlockShift;
-constexpr int32_t kNoExponent = -128, kNeutral = -127;
+constexpr int32_t kNoExponent = -128;
 static_assert(kBlock == LS_B200_CACHE_BLOCK, "public block size");
 
 // ls_b200_attention_args in the kernels' units. Strides are in elements.
@@ -226,19 +225,6 @@ struct BF16 {  // (the exponents of 32-bit numbers)
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 };
-
-// Exponents of blocks as the products take them, four bytes of v: those that are
-// `held` (bytes of ones) as they are, but outside T's range they are reported and read
-// as NaN; the others are kNeutral.
-template <class T>
-__device__ __forceinline__ uint32_t known_exponents(uint32_t v, uint32_t held, uint32_t* err) {
-    constexpr uint32_t kAll = 0x01010101u;
-    const uint32_t above = __vsub4(v, kAll * uint8_t(T::kLowest));  // the lowest
-    const uint32_t bad = __vcmpgtu4(above, kAll * uint32_t(T::kHighest - T::kLowest)) &
-                         ~__vcmpeq4(v, kAll * uint8_t(kNoExponent)) & held;
-    if (bad && err) atomicOr(err, uint32_t(LS_B200_ATTN_EXPONENT));
-    return (v & held & ~bad) | (kAll * uint8_t(kNoExponent) & bad) | (kAll * uint8_t(kNeutral) & ~held);
-}
 
 // First unit of CTA c when U units are cut evenly over G CTAs, and the CTA of a unit.
 __device__ __forceinline__ int64_t cut_begin(int64_t U, int64_t G, int64_t c) { return c * U / G; }

@@ -104,6 +104,29 @@ struct Note {
     uint32_t k, ex;
 };
 
+// The exponent of a block that is not read: below every other, so that it is never the
+// largest of a sequence.
+constexpr int32_t kNeutral = -127;
+// Exponents of blocks as the products take them, four bytes of v: those that are
+// `held` (bytes of ones) as they are, but outside T's range they are reported and read
+// as NaN; the others are kNeutral.
+template <class T>
+__device__ __forceinline__ uint32_t known_exponents(uint32_t v, uint32_t held, uint32_t* err) {
+    constexpr uint32_t kAll = 0x01010101u, kLow = 0x7f * kAll, kTop = 0x80 * kAll;
+    constexpr uint32_t kSpan = uint32_t(T::kHighest - T::kLowest);
+    // byte by byte, without a carry: above the lowest; then the top bit where that passes kSpan
+    const uint32_t above = ((v & kLow) + kAll * uint32_t(-T::kLowest)) ^ (v & kTop);
+    const uint32_t over = (above & kLow) + kAll * ((kSpan < 128 ? 127 : 255) - kSpan);
+    const uint32_t wrong = (kSpan < 128 ? over | above : over & above) & held & kTop;
+    if (wrong) {
+        const uint32_t bytes = (wrong >> 7) * 0xffu;
+        if (err && (bytes & ~__vcmpeq4(v, kAll * uint8_t(kNoExponent))))
+            atomicOr(err, uint32_t(LS_B200_ATTN_EXPONENT));
+        v = (v & ~bytes) | (kAll * uint8_t(kNoExponent) & bytes);
+    }
+    return (v & held) | (kAll * uint8_t(kNeutral) & ~held);
+}
+
 // 16-byte piece of a row in a tile of codes, rows of D bytes, as the TMA's swizzle
 // lays them, so that the eight rows of an ldmatrix lie in different banks.
 template <int D>

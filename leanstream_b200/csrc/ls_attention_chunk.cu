@@ -85,14 +85,15 @@ __device__ __forceinline__ uint32_t permute(uint32_t v, uint32_t with, uint32_t 
     return r;
 }
 template <class T>
-__device__ __forceinline__ uint32_t step_of(int32_t e) {  // a pair of 2^e; NaN for a marked block, 0 for kNeutral
-    uint32_t one;
-    if constexpr (std::is_same_v<T, F16>)
-        one = e == kNoExponent ? 0x7e00u : e >= -14 ? uint32_t(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
-    else
-        one = e == kNoExponent ? 0x7fc0u : uint32_t(e + 127) << 7;
-    return one * 0x10001u;
-}
+struct Step {
+    static constexpr uint32_t kNan = (std::is_same_v<T, F16> ? 0x7e00u : 0x7fc0u) * 0x10001u;
+    // a pair of 2^e; NaN for a marked block and outside the type's range
+    static __device__ __forceinline__ uint32_t of(int32_t e) {
+        if (uint32_t(e - T::kLowest) > uint32_t(T::kHighest - T::kLowest)) return kNan;
+        if constexpr (std::is_same_v<T, F16>) return (e >= -14 ? uint32_t(e + 15) << 10 : 1u << (e + 24)) * 0x10001u;
+        return (uint32_t(e + 127) << 7) * 0x10001u;
+    }
+};
 template <class T>
 __device__ __forceinline__ uint2 values4(uint32_t v, uint32_t step) {
     uint2 r;
@@ -416,21 +417,20 @@ __global__ void __launch_bounds__(Q8 ? kThreads8 : kThreads, 1)
             const Seg w = segs[sg % kSegs];
             const int32_t* trow = p.table + int64_t(w.b) * p.table_s;
             const uint8_t* eh = p.ex + int64_t(w.h) * p.ex_hs;
-            constexpr uint32_t kHeld = 1u << 16;  // beside exponents that were read
             // lanes 0 and 1: where the exponents of their block of a step lie; blocks that no
-            // row sees are zeros (kNeutral)
+            // row sees are zeros
+            constexpr uint32_t kZeros = 1u << 16;  // in the place of exponents
             auto page_of = [&](int32_t step) -> int32_t {
                 if (step >= w.steps || lane >= 2) return -1;
                 const int32_t k0 = w.slot0(step) + int32_t(mine + lane * 16), k1 = k0 + 16;
                 return (k0 < w.hi && k1 > w.lo) || k0 < w.sink ? trow[k0 >> p.pshift] : -1;
             };
             auto exponents_of = [&](int32_t step, int32_t id) -> uint32_t {
-                if (uint32_t(id) >= p.pages) return 0;
+                if (uint32_t(id) >= p.pages) return kZeros;
                 const int32_t in = (w.slot0(step) + int32_t(mine + lane * 16)) & int32_t(p.P - 1);
-                return kHeld | *reinterpret_cast<const uint16_t*>(eh + int64_t(id) * p.ex_ps + (in >> 3));
+                return *reinterpret_cast<const uint16_t*>(eh + int64_t(id) * p.ex_ps + (in >> 3));
             };
-            auto known = [&](uint32_t v) { return known_exponents<T>(v, v & kHeld ? 0xffffu : 0u, p.err); };
-            uint32_t ex = known(exponents_of(0, page_of(0))), next_ex = 0;
+            uint32_t ex = exponents_of(0, page_of(0)), next_ex = kZeros;
             for (int32_t j = 0; j < w.steps; ++j) {
                 const int32_t next_id = page_of(j + 1);
                 for (int kv = 0; kv < 2; ++kv, ++slot) {
@@ -439,8 +439,11 @@ __global__ void __launch_bounds__(Q8 ? kThreads8 : kThreads, 1)
                     uint32_t step[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const int32_t e = int8_t(__shfl_sync(0xffffffffu, ex, i) >> (8 * kv));
-                        step[i] = step_of<T>(e);
+                        const uint32_t v = __shfl_sync(0xffffffffu, ex, i);
+                        const int32_t e = int8_t(v >> (8 * kv));
+                        step[i] = v & kZeros ? 0u : Step<T>::of(e);
+                        if (step[i] == Step<T>::kNan && e != kNoExponent && lane == 0 && p.err)
+                            atomicOr(p.err, uint32_t(LS_B200_ATTN_EXPONENT));
                     }
                     if (kv) next_ex = exponents_of(j + 1, next_id);
                     if (!(ok = warp_wait<!Q8>(bar.codes_full(cs), cn & 1u, p.timeout_ns))) break;
@@ -479,7 +482,7 @@ __global__ void __launch_bounds__(Q8 ? kThreads8 : kThreads, 1)
                     if (lane == 0) bar_arrive(bar.full(s));
                 }
                 if (!ok) break;
-                ex = known(next_ex);
+                ex = next_ex;
             }
             release();
         }
