@@ -99,7 +99,7 @@ def test_pages_outside_the_pool(cuda_device, native_lib, dtype, shift, q):
         c.check()
 
 
-@pytest.mark.parametrize("q", [1, 4, 6, 8])
+@pytest.mark.parametrize("q", [1, 4, 6, 8, 40, 100])
 @pytest.mark.parametrize("shift", [-111, -115, -117, -118])
 def test_the_lowest_exponents(cuda_device, native_lib, shift, q):
     """bfloat16 down to -126."""
@@ -135,3 +135,33 @@ def test_values_of_no_weight_and_a_large_exponent(cuda_device, native_lib, q):
     # area + u (area + ..), with the probabilities' own rounding
     assert (c.output.double().abs() <= area * (1 + 2.0 ** -8) * (1 + 2.0 ** -10) + SMALLEST[torch.bfloat16] / 2).all()
     assert (c.lse.double() - lse).abs().max().item() <= 2e-5
+
+
+@pytest.mark.parametrize("dtype,scale", [(torch.float16, 2.0 ** -13), (torch.bfloat16, 2.0 ** -40), (torch.bfloat16, 2.0 ** -112)])
+def test_decoding_with_small_values(cuda_device, native_lib, dtype, scale):
+    """Token after token through append_cache and the attention, past the ends of blocks and steps."""
+    from leanstream_b200 import append_cache
+
+    c = Small([(1, 70)], 0, dtype=dtype, page=32)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    k, v = (torch.randn(70, 2, 128, generator=g, device="cuda") for _ in range(2))
+    k, v = k.to(dtype), (v * scale).to(dtype)
+    c.exponents.zero_()
+    starts, engine, got = torch.tensor([0, 1], dtype=torch.int32, device="cuda"), c.engine(), []
+    for n in range(1, 71):
+        c.kv_len.fill_(n)
+        append_cache(k_new=k[n - 1:n], v_new=v[n - 1:n], k_pages=c.k_pages, v_pages=c.v_pages, exponents=c.exponents,
+                     page_table=c.page_table, q_start=starts, kv_len=c.kv_len)
+        engine.run(**c.kwargs())
+        got.append([t.clone() for t in (c.output, c.lse, c.k_pages, c.v_pages, c.exponents)])
+    torch.cuda.synchronize()
+    assert engine.error() == 0
+    for n, (output, lse, k_pages, v_pages, exponents) in enumerate(got, 1):
+        i = torch.arange(n, device="cuda")
+        where = c.page_table[0].long()[i // 32]
+        size = exponents[where, :, i // 16 % 2].double()
+        c.lengths, c.largest, c.output, c.lse = [(1, n)], float(size[..., 1].max()), output, lse
+        c.keys, c.values = ([p[where, i % 32].double() * (2.0 ** size[..., j])[..., None]]
+                            for j, p in enumerate((k_pages, v_pages)))
+        c.check()
+        assert (c.values[0] - v[:n].double()).abs().max() < 2.0 ** c.largest
