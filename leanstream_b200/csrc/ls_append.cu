@@ -20,7 +20,7 @@
 //
 // Bound by memory, queries in and out, keys and values in, rows out, and by its
 // latency: 4096 tokens with 32 query heads of 128 over 8 into 16-bit pages (103 MB) take
-// 22 us, 4.7 TB/s; four prompts' chunks of up to 900 tokens into codes 24 us; one token 3.7.
+// 22 us, 4.7 TB/s; four prompts' chunks of up to 900 tokens into codes 25 us; one token 3.8.
 #include <stdint.h>
 
 #include <cerrno>
@@ -224,7 +224,7 @@ __device__ __forceinline__ int32_t page_of(const AppendParams& p, const Rows& t)
 // Keys (VALUES false) or values of one kv head into a block of codes. The rows stay in
 // registers as they come, all of them under way at a time, and are rotated twice, for
 // the largest value and for the codes: kept in 32 bits they take 172 registers, one CTA
-// per SM (33 us for four prompts' chunks, where this takes 24).
+// per SM (33 us for four prompts' chunks, where this takes 25).
 template <class T, int D, bool VALUES>
 __device__ __forceinline__ void append_codes(const AppendParams& p, const Rows& t, int32_t h) {
     const uint32_t lane = threadIdx.x & 31u;

@@ -28,9 +28,9 @@
 // passes it by 2^kRaise. P is rounded once, to float16, times 2^kChunkShift.
 //
 // Bound by the read of the cache: two sequences of up to 150000 slots, 64 heads of 128
-// over 8, take 97 to 104 us, of which 90 stream at 5.9 TB/s; 48 of up to 5000 slots, 32
-// heads, 58 us; 12 of up to 9000 slots with up to 5 tokens (20 rows, six warps) 57 us; one
-// of 130 slots 6.8 us. Rows as the M dimension, one CTA of four warps that load for
+// over 8, take 99 to 104 us, of which 90 stream at 5.9 TB/s; 48 of up to 5000 slots, 32
+// heads, 59 us; 12 of up to 9000 slots with up to 5 tokens (20 rows, six warps) 57 us; one
+// of 130 slots 7.2 us. Rows as the M dimension, one CTA of four warps that load for
 // themselves: 163, 90 and (on the chunk kernel) 80 us.
 #include <stdint.h>
 
