@@ -165,7 +165,7 @@ class PagedAttention:
             if k_new is not None or weights is not None:
                 raise ValueError("a cache in 8 bits is filled by append_cache, and keeps no weights")
             _want("exponents", exponents, _BYTE, (k_pages.shape[0], hk, size // N.CACHE_BLOCK, 2), on)
-            if exponents.stride(2) != 2:
+            if exponents.stride(2) != 2 and exponents.shape[2] != 1:
                 raise ValueError("exponents: contiguous last dimensions expected")
         _want("kv_len", kv_len, _INT, (-1,), on)
         _want("page_table", page_table, _INT, (kv_len.shape[0], -1), on)
@@ -234,7 +234,7 @@ class PagedAttention:
                 exponents.get_device() == dev
             if good:
                 ex0, ex1, a, b = exponents.stride()
-                good = a == 2 and b == 1 or not pool[0]
+                good = (a == 2 or self.page_size == 16) and b == 1 or not pool[0]
         elif good:
             good = not self._int8
         if good and lse is not None:
@@ -298,7 +298,7 @@ def _refuse_append(k_new, v_new, k_pages, v_pages, page_table, q_start, kv_len, 
     _want("q_start", q_start, _INT, (kv_len.shape[0] + 1,), on, contiguous=True)
     if exponents is not None:
         _want("exponents", exponents, _BYTE, (k_pages.shape[0], hk, k_pages.shape[1] // N.CACHE_BLOCK, 2), on)
-        if exponents.stride(2) != 2:
+        if exponents.stride(2) != 2 and exponents.shape[2] != 1:
             raise ValueError("exponents: contiguous last dimensions expected")
     if (q is None) != (q_out is None):
         raise ValueError("q and q_out come together")
@@ -356,7 +356,7 @@ def append_cache(*, k_new, v_new, k_pages, v_pages, page_table, q_start, kv_len,
         if good:
             ex = exponents.data_ptr()
             ex0, ex1, a, b = exponents.stride()
-            good = (a == 2 and b == 1) or not exponents.numel()
+            good = ((a == 2 or pool[1] == 16) and b == 1) or not exponents.numel()
     if good and q is not None:
         wide = q.shape
         good = q_out is not None and len(wide) == 3 and q_out.shape == wide and wide[0] == new[0] and \
